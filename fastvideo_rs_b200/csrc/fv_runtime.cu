@@ -191,13 +191,20 @@ extern "C" int fv_device_status(void* stream, int* code_out) {
     int* w;
     rc = fvrt::status_word(dev, &w);
     if (rc != FV_RAN) return rc;
-    int code = 0;
-    FV_CUDA(cudaMemcpyAsync(&code, w, sizeof(int), cudaMemcpyDeviceToHost, (cudaStream_t)stream));
+    int words[2] = {0, 0};
+    FV_CUDA(cudaMemcpyAsync(words, w, sizeof(words), cudaMemcpyDeviceToHost, (cudaStream_t)stream));
     FV_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+    const int code = words[0] ? words[0] : words[1];
     if (code_out) *code_out = code;
     if (code != 0) {
-        FV_CUDA(cudaMemsetAsync(w, 0, sizeof(int), (cudaStream_t)stream));
+        FV_CUDA(cudaMemsetAsync(w, 0, sizeof(words), (cudaStream_t)stream));
         FV_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+        if (words[0] == 0)
+            return fvrt::fail(FV_ERR_DEVICE_STATUS, "paged cache: %s (status %d)",
+                              code == 200   ? "a page that a call needed lies outside the pool or the table"
+                              : code == 201 ? "cu_q or the lengths of a batch are outside its bounds"
+                                            : "a position lies outside the rotation tables",
+                              code);
         return fvrt::fail(FV_ERR_DEVICE_STATUS, "a kernel gave up a bounded wait (status %d: role %d)", code, code - 100);
     }
     return FV_RAN;

@@ -14,8 +14,9 @@ int fail(int code, const char* fmt, ...);   // sets the error text, returns code
 void clear_error();
 // FV_RAN when the current device is sm_100 / sm_103; else FV_ERR_NO_DEVICE (text set).
 int require_sm100(int* device_out);
-// Device pointer of the current device's status word.  The word lives in a file-scope __device__
-// array of the library (zero when the module loads), so asking for it never allocates.
+// Device pointer of the current device's status words: [0] a bounded wait that ran out, [1] tables of a paged cache that
+// lead outside of it (paged.cuh).  The words live in a file-scope __device__
+// array of the library (zero when the module loads), so asking for them never allocates.
 int status_word(int device, int** ptr_out);
 // Number of SMs of `device` (cached).
 int sm_count(int device, int* out);
@@ -25,7 +26,7 @@ int take_spare_sms();
 // process, like the reference's rt::log::info_once one-liners that name the kernel a call ran
 // (crates/fastvideo-cudarc/src/rt/attn.rs:306-310).  FV_LOG=0 silences them.  The text of the last
 // line of each thread is also kept for fv_last_kernel().
-enum LogKey { kLogDense = 0, kLogCausal, kLogSplitKv, kLogPrep, kLogVsa, kLogSp, kLogGlue, kLogKeys };
+enum LogKey { kLogDense = 0, kLogCausal, kLogSplitKv, kLogPrep, kLogVsa, kLogSp, kLogGlue, kLogPaged, kLogPagedAttn, kLogKeys };
 void ran(LogKey key, const char* fmt, ...);
 
 // 4-D bf16 tensor map, dims innermost first, strides in bytes for dims 1..3,

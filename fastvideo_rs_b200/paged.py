@@ -1,0 +1,244 @@
+"""A paged K/V cache for streaming generation: appending a ragged batch's keys and values (rotated on the way) to pages of
+bf16 or of 4 bits, reading rows back, and attention over the pages with a sliding window and sink tokens.
+
+`wan.CausalKvCache` keeps one contiguous buffer per sequence and rolls it by copying; here a sequence is a list of pages, so
+a window slides by handing pages back, sequences of any lengths share one pool, query heads may share K/V heads, and
+4-bit pages take little more than a quarter of the memory.  One `PagedKv` is one layer's pool; one `PagedBatch` says where
+the sequences of a call lie in it and serves every layer that uses the same tables."""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .sdpa import BlockCausal
+
+FORMATS = ("bf16", "q4")
+PAIRINGS = {"interleaved": 0, "half": 1}
+D = 128
+_vp, _ll, _int = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
+
+
+class _KvC(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("format", _int), ("pages", _int),
+                ("page_rows", _int), ("kv_heads", _int)]
+
+
+class _BatchC(ctypes.Structure):
+    _fields_ = [("page_table", _vp), ("kv_len", _vp), ("cu_q", _vp), ("seqs", _int), ("table_width", _int),
+                ("max_q", _int), ("max_kv", _int)]
+
+
+_fns = None
+
+
+def _entries():
+    """The C entries with their argument types declared once: a decode step calls them for every layer, and untyped
+    ctypes arguments cost more than the launch."""
+    global _fns
+    if _fns is None:
+        L = _lib.lib()
+        L.fv_paged_append_bf16.argtypes = [_vp, _vp, _vp, _int, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _int, _vp, _vp, _vp,
+                                           _int, _vp, _int]
+        L.fv_paged_read_bf16.argtypes = [_vp, _vp, _vp, _vp, _vp, _int, _vp, _vp]
+        L.fv_paged_attn_workspace_bytes.argtypes = [_vp, _vp, _int, _int, _int, _int, _int, _int]
+        L.fv_paged_attn_workspace_bytes.restype = ctypes.c_size_t
+        L.fv_paged_attn_bf16.argtypes = [_vp, _vp, _vp, _int, _vp, _ll, _ll, _int, _int, _int, _int, _int, ctypes.c_float, _vp, _vp,
+                                         ctypes.c_size_t]
+        _fns = (L.fv_paged_append_bf16, L.fv_paged_read_bf16, L.fv_paged_attn_workspace_bytes, L.fv_paged_attn_bf16)
+    return _fns
+
+
+def _index(name: str, t: torch.Tensor, shape: Tuple[int, ...], device) -> torch.Tensor:
+    if not t.is_cuda or t.device != device or t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be a contiguous int32 tensor {list(shape)} on {device}")
+    return t
+
+
+class PagedKv:
+    """The pool of one layer.  bf16 pages: k, v [pages, kv_heads, page_rows, 128] bf16.  4-bit pages: k, v [pages, kv_heads,
+    page_rows, 64] uint8 (value 2 i in the low half of byte i, as code + 8) and k_scale, v_scale [pages, kv_heads,
+    page_rows, 2] bf16 = (step, zero): a row stands for zero + step * code.  page_rows 16, 32, 64, 128 or 256."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+                 v_scale: Optional[torch.Tensor] = None):
+        if k.dim() != 4 or k.dtype not in (torch.bfloat16, torch.uint8):
+            raise ValueError("PagedKv: k must be [pages, kv_heads, page_rows, 128] bf16 or [.., 64] uint8")
+        q4 = k.dtype == torch.uint8
+        if k.shape[3] != (D // 2 if q4 else D) or v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError("PagedKv: k and v must be [pages, kv_heads, page_rows, 128] bf16 or [.., 64] uint8")
+        if k.shape[2] not in (16, 32, 64, 128, 256):
+            raise ValueError(f"PagedKv: pages of {k.shape[2]} rows (16, 32, 64, 128 or 256)")
+        if q4 != (k_scale is not None) or q4 != (v_scale is not None):
+            raise ValueError("PagedKv: 4-bit pages have scales, bf16 pages have none")
+        for name, t in (("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale)):
+            if t is None:
+                continue
+            if not t.is_cuda or t.device != k.device or not t.is_contiguous():
+                raise ValueError(f"PagedKv: {name} must be a contiguous CUDA tensor on one device: this package has no CPU path")
+            if name.endswith("scale") and (t.dtype != torch.bfloat16 or t.shape != (*k.shape[:3], 2)):
+                raise ValueError(f"PagedKv: {name} must be bf16 [pages, kv_heads, page_rows, 2]")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.format = "q4" if q4 else "bf16"
+        self.pages, self.kv_heads, self.page_rows = k.shape[:3]
+        self.device = k.device
+        ptr = lambda t: t.data_ptr() if t is not None else None
+        self._c = _KvC(ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), int(q4), self.pages, self.page_rows, self.kv_heads)
+        self._ref = ctypes.addressof(self._c)
+
+    @staticmethod
+    def empty(pages: int, page_rows: int, kv_heads: int, format: str = "bf16", device="cuda") -> "PagedKv":
+        """A pool of its own; the memory is not cleared (rows are read only after they were appended)."""
+        if format not in FORMATS:
+            raise ValueError(f"PagedKv: unknown format {format!r} {FORMATS}")
+        mk = lambda width, dtype: torch.empty((pages, kv_heads, page_rows, width), dtype=dtype, device=device)
+        if format == "bf16":
+            return PagedKv(mk(D, torch.bfloat16), mk(D, torch.bfloat16))
+        return PagedKv(mk(D // 2, torch.uint8), mk(D // 2, torch.uint8), mk(2, torch.bfloat16), mk(2, torch.bfloat16))
+
+
+class PagedBatch:
+    """The sequences of a call.  page_table [seqs, width] int32: the page of rows i * page_rows .. of each sequence (entries
+    that the call does not need may be -1).  kv_len [seqs] int32: tokens of each sequence, those of this call included.
+    cu_q [seqs + 1] int32, ascending from 0: rows cu_q[s] .. cu_q[s + 1] of the packed operands are the last tokens of
+    sequence s.  max_q and max_kv bound the tokens and lengths; the tensors may change under a captured graph as long as they
+    keep to them.  Rows of an operand from cu_q[seqs] on belong to no sequence: outputs leave them as they were."""
+
+    def __init__(self, page_table: torch.Tensor, kv_len: torch.Tensor, cu_q: torch.Tensor, *, max_q: int, max_kv: int):
+        if page_table.dim() != 2:
+            raise ValueError("PagedBatch: page_table must be [seqs, width]")
+        seqs, width = page_table.shape
+        dev = page_table.device
+        self.page_table = _index("PagedBatch: page_table", page_table, (seqs, width), dev)
+        self.kv_len = _index("PagedBatch: kv_len", kv_len, (seqs,), dev)
+        self.cu_q = _index("PagedBatch: cu_q", cu_q, (seqs + 1,), dev)
+        if max_q < 0 or max_kv < 0:
+            raise ValueError("PagedBatch: max_q and max_kv must not be negative")
+        self.seqs, self.max_q, self.max_kv, self.device = seqs, int(max_q), int(max_kv), dev
+        self._c = _BatchC(page_table.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), seqs, width, self.max_q, self.max_kv)
+        self._ref = ctypes.addressof(self._c)
+
+
+def _heads_in(name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int], device) -> None:
+    if not t.is_cuda or t.device != device:
+        raise ValueError(f"{name} must be a CUDA tensor on {device}: this package has no CPU path")
+    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[2] != D or (t.stride(2) != 1 and t.numel() > 0):
+        raise ValueError(f"{name} must be bfloat16 [tokens, heads, 128] with adjacent values")
+    if (tokens is not None and t.shape[0] != tokens) or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} is {list(t.shape)}: {tokens} tokens of {heads} heads are wanted")
+
+
+def _on(kv: PagedKv, batch: PagedBatch):
+    if kv.device != batch.device:
+        raise ValueError(f"the cache is on {kv.device}, the batch on {batch.device}")
+    return torch.cuda.device(kv.device)
+
+
+def append(kv: PagedKv, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, *, q: Optional[torch.Tensor] = None,
+           cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+           pairing: str = "interleaved", q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Writes the call's tokens into the cache: k, v [tokens, kv_heads, 128] bf16 (any strides of tokens and heads that are
+    multiples of 8: slices of a fused projection are read in place), K rotated on the way when cos / sin f32 [rows, 128] are
+    given: token t with row positions[t] (int32), by default its position in its sequence.  pairing "interleaved": values
+    2 i and 2 i + 1 (the tables of wan.wan_rope_tables), "half": values i and i + 64.  q [tokens, heads, 128], if given, is
+    rotated too and returned as [tokens, heads, 128].  Two tokens of a call must not fall on the same cache row."""
+    tokens = k.shape[0]
+    _heads_in("append: k", k, None, kv.kv_heads, kv.device)
+    _heads_in("append: v", v, tokens, kv.kv_heads, kv.device)
+    if (cos is None) != (sin is None) or (positions is not None and cos is None):
+        raise ValueError("append: cos, sin and positions go together")
+    if pairing not in PAIRINGS:
+        raise ValueError(f"append: unknown pairing {pairing!r} {tuple(PAIRINGS)}")
+    rows = 0
+    if cos is not None:
+        rows = cos.shape[0]
+        for name, t in (("cos", cos), ("sin", sin)):
+            if t.dtype != torch.float32 or not t.is_cuda or t.device != kv.device or not t.is_contiguous() or tuple(t.shape) != (rows, D):
+                raise ValueError(f"append: {name} must be a contiguous CUDA float32 [rows, 128] tensor")
+        if positions is not None:
+            _index("append: positions", positions, (tokens,), kv.device)
+    heads = qt = qh = 0
+    if q is not None:
+        _heads_in("append: q", q, tokens, None, kv.device)
+        heads, qt, qh = q.shape[1], q.stride(0), q.stride(1)
+        if q_out is None:
+            q_out = torch.empty((tokens, heads, D), dtype=torch.bfloat16, device=kv.device)
+        else:
+            _heads_in("append: q_out", q_out, tokens, heads, kv.device)
+            if not q_out.is_contiguous():
+                raise ValueError("append: q_out must be contiguous")
+    elif q_out is not None:
+        raise ValueError("append: q_out without q")
+    if tokens == 0 or batch.seqs == 0 or batch.max_q == 0 or heads + kv.kv_heads == 0:
+        return q_out
+    fn = _entries()[0]
+    with _on(kv, batch):
+        rc = fn(torch.cuda.current_stream().cuda_stream, kv._ref, batch._ref, tokens, k.data_ptr(), k.stride(0), k.stride(1),
+                v.data_ptr(), v.stride(0), v.stride(1), q.data_ptr() if q is not None else None, qt, qh, heads,
+                q_out.data_ptr() if q is not None else None, cos.data_ptr() if cos is not None else None,
+                sin.data_ptr() if cos is not None else None, rows, positions.data_ptr() if positions is not None else None,
+                PAIRINGS[pairing])
+    if rc:
+        _lib.check(rc, "paged append")
+    return q_out
+
+
+def read(kv: PagedKv, batch: PagedBatch, *, rows: int, cu_rows: Optional[torch.Tensor] = None,
+         first: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows of the sequences as packed (k, v) [rows, kv_heads, 128] bf16, 4-bit rows as the values they stand for: sequence s
+    gives rows cu_rows[s] .. cu_rows[s + 1] (int32 [seqs + 1]; default: the batch's own tokens), beginning with its token
+    first[s] (int32 [seqs]; default: its last ones).  Rows from cu_rows[seqs] on are zero, as are rows that a sequence does
+    not hold; rows below cu_rows[seqs] gives the first ones.  What dense attention, an exchange or a copy of a cache starts from."""
+    if rows < 0:
+        raise ValueError("read: rows must not be negative")
+    cu = batch.cu_q if cu_rows is None else _index("read: cu_rows", cu_rows, (batch.seqs + 1,), kv.device)
+    if first is not None:
+        _index("read: first", first, (batch.seqs,), kv.device)
+    k, v = (torch.empty((rows, kv.kv_heads, D), dtype=torch.bfloat16, device=kv.device) for _ in range(2))
+    if rows == 0:
+        return k, v
+    if batch.seqs == 0:
+        return k.zero_(), v.zero_()
+    fn = _entries()[1]
+    with _on(kv, batch):
+        rc = fn(torch.cuda.current_stream().cuda_stream, kv._ref, batch._ref, cu.data_ptr(),
+                first.data_ptr() if first is not None else None, rows, k.data_ptr(), v.data_ptr())
+    if rc:
+        _lib.check(rc, "paged read")
+    return k, v
+
+
+def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[BlockCausal] = None, *,
+           scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q [tokens, heads, 128] bf16 (the batch's tokens, rotated; strides as in append) over the cache, in place:
+    returns [tokens, heads, 128] bf16.  heads is a multiple of kv_heads; head h reads K/V head h // (heads // kv_heads).
+    mask None: every key of the sequence.  BlockCausal(block_tokens, window, sink): key j is visible to position p iff
+    t_j <= t_p and (window == 0 or t_p - t_j < window or t_j < sink), t = index // block_tokens -- block_tokens 1: causal
+    by token, a window of `window` tokens, the first `sink` tokens always visible; block_tokens of a frame: the streaming
+    form of the block-causal mask.  A row that sees no key is zero.  Pages of which no row sees a key need not exist.
+    With `out`, rows that belong to no sequence keep what they hold."""
+    _heads_in("attend: q", q, None, None, kv.device)
+    tokens, heads = q.shape[:2]
+    if heads < 1 or heads % kv.kv_heads:
+        raise ValueError(f"attend: {heads} heads over {kv.kv_heads} K/V heads")
+    if out is None:
+        out = torch.empty((tokens, heads, D), dtype=torch.bfloat16, device=kv.device)
+    else:
+        _heads_in("attend: out", out, tokens, heads, kv.device)
+        if not out.is_contiguous():
+            raise ValueError("attend: out must be contiguous")
+    if tokens == 0 or batch.seqs == 0 or batch.max_q == 0:
+        return out
+    mode, bt, win, sink = (1, mask.block_tokens, mask.window, mask.sink) if mask is not None else (0, 0, 0, 0)
+    _, _, need_fn, fn = _entries()
+    with _on(kv, batch):
+        need = need_fn(kv._ref, batch._ref, tokens, heads, mode, bt, win, sink)
+        # (scratch of this call alone, from the stream's own pool: calls on other streams and captured graphs share nothing)
+        ws = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None
+        rc = fn(torch.cuda.current_stream().cuda_stream, kv._ref, batch._ref, tokens, q.data_ptr(), q.stride(0), q.stride(1),
+                heads, mode, bt, win, sink, D ** -0.5 if scale is None else float(scale), out.data_ptr(), ws.data_ptr() if need else None, need)
+    if rc:
+        _lib.check(rc, "paged attention")
+    return out

@@ -52,9 +52,10 @@ FV_API const char* fv_last_error(void);
 /* Library version string (host pointer). */
 FV_API const char* fv_version(void);
 
-/* Reads and clears the current device's kernel status word.  Synchronises `stream`.
+/* Reads and clears the current device's kernel status.  Synchronises `stream`.
  * Returns FV_RAN when every kernel finished its waits, FV_ERR_DEVICE_STATUS when one
- * gave up (code in *code_out: 100 + role), FV_ERR_CUDA on a CUDA error.
+ * gave up (code in *code_out: 100 + role) or met tables of a paged cache that lead outside of it (200 .. 202, see there;
+ * unlike a wait that ran out these do not keep later launches from running), FV_ERR_CUDA on a CUDA error.
  * The word is part of the library's module image (a file-scope __device__ array, zero at load): every
  * kernel of the library reports there, the two-pass call on built-in scratch included, and neither this
  * call nor any launch allocates for it. */
@@ -261,6 +262,72 @@ FV_API int fv_kv_roll(void* stream, void* cache, int elem_bytes, int planes, int
 FV_API int fv_sdpa_window_bf16(void* stream, const void* q, const void* k_cache, const void* v_cache, void* out,
                                int out_is_bf16, int bh, int sq, int cache_rows, int window_start, int window_len, int d,
                                float scale, int out_heads);
+
+/* ---- paged K/V cache: append, read back, attention with a sliding window and sinks --------------------------------
+ * The causal cache above is one contiguous buffer per sequence, which rolls by copying its rows down past the sink and
+ * holds bf16 (crates/fastvideo-cudarc/src/wan/causal.rs:541-628).  Over pages a window slides by giving pages back, a
+ * batch may hold sequences of any lengths, query heads may share K/V heads, and a page may hold 4 bits a value.  No
+ * counterpart in the reference.
+ *
+ * fv_paged_kv: the pool of one layer.  FV_PAGE_BF16: k, v [pages, kv_heads, page_rows, 128] bf16, scales null.
+ *   FV_PAGE_Q4: k, v [pages, kv_heads, page_rows, 64] bytes, value 2 i in the low and 2 i + 1 in the high half of byte i,
+ *   stored as code + 8; k_scale, v_scale [pages, kv_heads, page_rows, 2] bf16 = (step, zero): a row stands for
+ *   zero + step * code, code in -8 .. 7.  page_rows 16, 32, 64, 128 or 256.  16-byte aligned.
+ * fv_paged_batch: page_table [seqs, table_width] i32: page of rows i * page_rows .. of each sequence; entries that no row
+ *   of the call reads or writes may hold anything (-1).  kv_len [seqs] i32: tokens of each sequence, those of this call
+ *   included.  cu_q [seqs + 1] i32, ascending from 0: the call's tokens of sequence s are rows cu_q[s] .. cu_q[s + 1] of
+ *   the packed operands, the LAST ones of the sequence: row i has position kv_len[s] - nq + i.  All three are device
+ *   pointers and may change between launches of a captured graph; the host gives bounds only: tokens >= cu_q[seqs], the rows
+ *   of the packed operands (rows from cu_q[seqs] on belong to no sequence: q_out and out keep what they hold there), max_q >= every nq, max_kv >=
+ *   every kv_len, table_width * page_rows >= max_kv.  Numbers in device memory that break these bounds, a page outside
+ *   the pool and a position outside the tables are never followed: the rows concerned come out unspecified (a sequence
+ *   with broken numbers counts as empty) and fv_device_status answers FV_ERR_DEVICE_STATUS with code 200 (page), 201 (batch)
+ *   or 202 (position).
+ *
+ * fv_paged_append_bf16: k, v [tokens, kv_heads, 128] bf16 and, unless null, q [tokens, q_heads, 128]; *_tok and *_head are
+ *   strides in values (multiples of 8), so slices of a fused projection are read in place.  cosv, sinv (both or neither)
+ *   f32 [table_rows, 128]: token t is rotated with row positions[t] (i32; null: its position in the sequence), pairing
+ *   FV_ROPE_INTERLEAVED (values 2 i, 2 i + 1; each factor stored twice, as fv_wan_rope_tables writes them) or FV_ROPE_HALF
+ *   (values i, i + 64; factors i and i + 64 equal).  K, rotated, and V go to the tokens' rows in the pages; q, rotated, to
+ *   q_out [tokens, q_heads, 128].  f32 arithmetic, products and sums rounded separately, one rounding to bf16 (or from f32
+ *   to 4 bits: step = bf16((max - min) / 15), zero = bf16(min + 8 step), code = clamp(rint((x - zero) / step), -8, 7)).
+ *   Tokens before the start of their sequence (nq > kv_len) are stored nowhere and their q_out is zero.  Two tokens of one
+ *   call must not fall on the same row.
+ * fv_paged_read_bf16: rows first[s] .. first[s] + (cu_rows[s + 1] - cu_rows[s]) of each sequence as packed
+ *   k_out, v_out [rows, kv_heads, 128] bf16 (4-bit rows as the values they stand for); first null: the last rows of each
+ *   sequence.  Rows that a sequence does not hold, and rows from cu_rows[seqs] on, are zero.  Uses the batch's table and kv_len only.
+ * fv_paged_attn_bf16: q [tokens, heads, 128] bf16 by strides (heads a multiple of kv_heads; head h reads K/V head
+ *   h / (heads / kv_heads)) -> out [tokens, heads, 128] bf16.  mask_mode FV_MASK_NONE: every key below kv_len.
+ *   FV_MASK_BLOCK_CAUSAL: key j is visible to position p iff t_j <= t_p and (window == 0 or t_p - t_j < window or
+ *   t_j < sink), t = index / block_tokens: block_tokens 1 is causal by token.  (The mask of fv_sdpa_dense_bf16 but that the
+ *   sinks stay causal too: what a cache can hold.)  Rows that see no key give zeros.  Keys that no row of a tile of rows may see have
+ *   no influence whatever their memory holds; a key that some row sees must be finite (a NaN in it may reach other
+ *   rows of the call).  The workspace is scratch of this call alone (fv_paged_attn_workspace_bytes, may be 0; same arguments).
+ * Declines: empty batches, more than 2^31 - 1 blocks of work. */
+#define FV_PAGE_BF16 0
+#define FV_PAGE_Q4 1
+#define FV_ROPE_INTERLEAVED 0
+#define FV_ROPE_HALF 1
+typedef struct fv_paged_kv {
+    void *k, *v;
+    void *k_scale, *v_scale;
+    int format, pages, page_rows, kv_heads;
+} fv_paged_kv;
+typedef struct fv_paged_batch {
+    const int *page_table, *kv_len, *cu_q;
+    int seqs, table_width, max_q, max_kv;
+} fv_paged_batch;
+FV_API int fv_paged_append_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* batch, int tokens, const void* k, long long k_tok,
+                                long long k_head, const void* v, long long v_tok, long long v_head, const void* q,
+                                long long q_tok, long long q_head, int q_heads, void* q_out, const float* cosv,
+                                const float* sinv, int table_rows, const int* positions, int pairing);
+FV_API int fv_paged_read_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* batch, const int* cu_rows,
+                              const int* first, int rows, void* k_out, void* v_out);
+FV_API size_t fv_paged_attn_workspace_bytes(const fv_paged_kv* kv, const fv_paged_batch* batch, int tokens, int heads, int mask_mode,
+                                            int block_tokens, int window, int sink);
+FV_API int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* batch, int tokens, const void* q, long long q_tok,
+                              long long q_head, int heads, int mask_mode, int block_tokens, int window, int sink,
+                              float scale, void* out, void* workspace, size_t workspace_bytes);
 
 /* ---- operand rounding for f32-stored activations ------------------------------------------------
  * The reference rounds q, k, v to bf16 before its attention kernels under bf16 activations and rounds the
