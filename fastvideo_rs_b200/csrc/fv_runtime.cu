@@ -110,8 +110,7 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 static EncodeTiledFn g_encode = nullptr;
 
-int encode_map4(CUtensorMap* map, const void* base, const uint64_t dims[4], const uint64_t strides[3],
-                uint32_t box_rows) {
+int encode_map4_box(CUtensorMap* map, const void* base, const uint64_t dims[4], const uint64_t strides[3], const uint32_t box4[4]) {
     if (!g_encode) {
         std::lock_guard<std::mutex> lk(g_mu);
         void* fn = nullptr;
@@ -123,7 +122,7 @@ int encode_map4(CUtensorMap* map, const void* base, const uint64_t dims[4], cons
     }
     cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
     cuuint64_t s[3] = {strides[0], strides[1], strides[2]};
-    cuuint32_t box[4] = {64, box_rows, 1, 1};
+    cuuint32_t box[4] = {box4[0], box4[1], box4[2], box4[3]};
     cuuint32_t es[4] = {1, 1, 1, 1};
     CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, s, box, es,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -133,6 +132,12 @@ int encode_map4(CUtensorMap* map, const void* base, const uint64_t dims[4], cons
                     (unsigned long long)d[0], (unsigned long long)d[1], (unsigned long long)d[2], (unsigned long long)d[3],
                     (unsigned long long)s[0], (unsigned long long)s[1], (unsigned long long)s[2]);
     return FV_RAN;
+}
+
+int encode_map4(CUtensorMap* map, const void* base, const uint64_t dims[4], const uint64_t strides[3],
+                uint32_t box_rows) {
+    const uint32_t box[4] = {64, box_rows, 1, 1};
+    return encode_map4_box(map, base, dims, strides, box);
 }
 
 struct MapKey {

@@ -26,14 +26,16 @@ int take_spare_sms();
 // process, like the reference's rt::log::info_once one-liners that name the kernel a call ran
 // (crates/fastvideo-cudarc/src/rt/attn.rs:306-310).  FV_LOG=0 silences them.  The text of the last
 // line of each thread is also kept for fv_last_kernel().
-enum LogKey { kLogDense = 0, kLogCausal, kLogSplitKv, kLogPrep, kLogVsa, kLogSp, kLogGlue, kLogPaged, kLogPagedAttn, kLogKeys };
+enum LogKey { kLogDense = 0, kLogCausal, kLogSplitKv, kLogPrep, kLogVsa, kLogSp, kLogGlue, kLogPaged, kLogPagedAttn, kLogPagedChunk, kLogKeys };
 void ran(LogKey key, const char* fmt, ...);
 
 // 4-D bf16 tensor map, dims innermost first, strides in bytes for dims 1..3,
 // box (64, box_rows, 1, 1), 128-byte swizzle, out-of-range reads as zero.
 int encode_map4(CUtensorMap* map, const void* base, const uint64_t dims[4], const uint64_t strides[3],
                 uint32_t box_rows);
-// The same through a small per-process cache keyed by (base, dims, strides, box_rows): a denoising
+// The same with any box (its inner extent 64 values).
+int encode_map4_box(CUtensorMap* map, const void* base, const uint64_t dims[4], const uint64_t strides[3], const uint32_t box[4]);
+// encode_map4 through a small per-process cache keyed by (base, dims, strides, box_rows): a denoising
 // loop calls with the same buffers every step, and the reference re-encodes three maps per call
 // (crates/fastvideo-cudarc/src/rt/attn_dc.rs:242-246).
 int encode_map4_cached(CUtensorMap* map, const void* base, const uint64_t dims[4], const uint64_t strides[3],

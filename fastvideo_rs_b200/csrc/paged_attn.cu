@@ -6,8 +6,10 @@
 // kv_heads): one pass over the keys serves all of them.
 #include "fv_runtime.h"
 #include "paged.cuh"
+#include "paged_fwd.cuh"
 #include "paged_host.h"
 #include <math.h>
+#include <mutex>
 
 namespace fvpg {
 
@@ -28,7 +30,8 @@ struct AttnArgs {
     float sl2;
 };
 
-FV_DEV float neg_inf() { return __int_as_float(0xff800000); }
+
+using fvattn::neg_inf;
 
 // The key tiles a block of rows visits: those of [0, sink), then those of [lo, hi), each tile once.
 struct Tiles {
@@ -485,16 +488,55 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_merge_kernel(const Attn
         make_uint2(fvp::pack_bf16x2(acc.x, acc.y), fvp::pack_bf16x2(acc.z, acc.w));
 }
 
+template <bool Q4>
+__global__ void __launch_bounds__(Roles<Q4>::kThreads, 1)
+fv_paged_chunk_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                      const __grid_constant__ ChunkJob jb) {
+#if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM103_ALL)
+    extern __shared__ __align__(1024) unsigned char fv_smem[];
+    chunk_persistent<Q4>(&mq, &mk, &mv, jb, fv_smem);
+#endif
+}
+
 // ---- host --------------------------------------------------------------------------------------------------------------
 
 struct Shape {
-    int splits, row_blocks, nt;
+    bool chunk;  // the tensor-core kernel for long chunks
+    int splits, row_blocks, nt, tile_tokens;
 };
-// How a call is cut: rows of 8 or 16 per CTA, and the keys in `splits` ranges so that all SMs have work.
+// How a call is cut.  Few rows per kv head: blocks of 8 or 16 rows, and the keys in `splits` ranges so that all SMs have
+// work.  From kChunkFrom rows on: items of 2 x 128 rows, the keys cut where that evens out the waves.
+constexpr int kChunkFrom = 33;
 static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads, const Mask& m, int sms) {
     Shape s;
     const int group = heads / kv->kv_heads;
     const long long rows = (long long)b->max_q * group;
+    s.chunk = rows >= kChunkFrom && group <= kChunkRows;
+    s.tile_tokens = s.chunk ? kChunkRows / group : 0;
+    if (s.chunk) {
+        long long seen = b->max_kv;
+        if (m.block > 0 && m.window > 0) {
+            const long long some = ((long long)m.window + m.sink + 1) * m.block + 2 * s.tile_tokens;
+            seen = some < seen ? some : seen;
+        }
+        const int tiles = (int)((seen + kChunkTile - 1) / kChunkTile);
+        s.nt = 0;
+        s.row_blocks = (b->max_q + 2 * s.tile_tokens - 1) / (2 * s.tile_tokens);
+        const long long items = (long long)b->seqs * kv->kv_heads * s.row_blocks;
+        // Time of a cut, in key tiles of a CTA: whole waves of equal items, each with a fixed cost of about four tiles,
+        // and the merge's traffic (a part is 516 bytes a row; a key tile takes about 1.5 us, 7.5 MB at 5 TB/s).
+        double best = 0;
+        s.splits = 1;
+        for (int n = 1; n <= 16 && (n == 1 || tiles >= 4 * n); n++) {
+            const long long waves = (items * n + sms - 1) / sms;
+            const double cost = (double)waves * ((tiles + n - 1) / n + 4) + (n > 1 ? 2.0 + (double)b->max_q * b->seqs * heads * n * 1032.0 / 7.5e6 : 0.0);
+            if (n == 1 || cost < 0.95 * best) {
+                best = cost;
+                s.splits = n;
+            }
+        }
+        return s;
+    }
     s.nt = rows > 8 ? 2 : 1;
     s.row_blocks = (int)((rows + 8 * s.nt - 1) / (8 * s.nt));
     long long keys = b->max_kv;
@@ -508,6 +550,65 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads,
     long long n = want < most ? want : most;
     s.splits = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
     return s;
+}
+
+static int launch_chunk(cudaStream_t st, const fv_paged_kv* kv, const AttnArgs& a, const Shape& s, int dev, int sms) {
+    const bool q4 = kv->format == FV_PAGE_Q4;
+    ChunkJob jb{};
+    jb.pool = a.pool;
+    jb.batch = a.batch;
+    jb.mask = a.mask;
+    jb.q = a.q;
+    jb.q_tok = a.q_tok;
+    jb.q_head = a.q_head;
+    jb.out = a.out;
+    jb.part_o = a.part_o;
+    jb.part_lse = a.part_lse;
+    jb.wait_status = a.batch.status - 1;
+    jb.wait_cycles = FV_WAIT_CYCLES;
+    jb.heads = a.heads;
+    jb.group = a.group;
+    jb.tile_tokens = s.tile_tokens;
+    jb.splits = s.splits;
+    jb.planes = a.batch.seqs * a.pool.kv_heads;
+    jb.q_blocks = s.row_blocks;
+    const long long items = (long long)jb.planes * s.row_blocks * s.splits;
+    if (items > 0x3fffffffll) return FV_DECLINED;
+    jb.items = (int)items;
+    jb.box_rows = kv->page_rows < kChunkTile ? kv->page_rows : kChunkTile;
+    jb.sl2 = a.sl2;
+    CUtensorMap mq{}, mk{}, mv{};
+    if (!q4) {
+        const uint64_t dq[4] = {128, (uint64_t)a.heads, (uint64_t)a.batch.tokens, 1};
+        const uint64_t sq[3] = {(uint64_t)a.q_head * 2, (uint64_t)a.q_tok * 2, (uint64_t)a.q_tok * 2};
+        const uint32_t bq[4] = {64, (uint32_t)a.group, (uint32_t)s.tile_tokens, 1};
+        int rc = fvrt::encode_map4_box(&mq, a.q, dq, sq, bq);
+        if (rc != FV_RAN) return rc;
+        const uint64_t row = 256, head = row * kv->page_rows, page = head * kv->kv_heads;
+        const uint64_t dk[4] = {128, (uint64_t)kv->page_rows, (uint64_t)kv->kv_heads, (uint64_t)kv->pages};
+        const uint64_t sk[3] = {row, head, page};
+        rc = fvrt::encode_map4_cached(&mk, kv->k, dk, sk, (uint32_t)jb.box_rows);
+        if (rc != FV_RAN) return rc;
+        rc = fvrt::encode_map4_cached(&mv, kv->v, dk, sk, (uint32_t)jb.box_rows);
+        if (rc != FV_RAN) return rc;
+    }
+    {
+        static bool attr_set[64][2] = {};
+        static std::mutex attr_mu;
+        std::lock_guard<std::mutex> lock(attr_mu);
+        if (!attr_set[dev][q4]) {
+            if (q4) FV_CUDA(cudaFuncSetAttribute(fv_paged_chunk_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kChunkSmem));
+            else FV_CUDA(cudaFuncSetAttribute(fv_paged_chunk_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kChunkSmem));
+            attr_set[dev][q4] = true;
+        }
+    }
+    const unsigned grid = (unsigned)(items < sms ? items : sms);
+    if (q4) fv_paged_chunk_kernel<true><<<grid, Roles<true>::kThreads, kChunkSmem, st>>>(mq, mk, mv, jb);
+    else fv_paged_chunk_kernel<false><<<grid, Roles<false>::kThreads, kChunkSmem, st>>>(mq, mk, mv, jb);
+    FV_CUDA(cudaGetLastError());
+    fvrt::ran(fvrt::kLogPagedChunk, "paged attention: fv_paged_chunk_kernel<%s> (sm_100a tcgen05, persistent, %u CTAs) %d sequences x %d heads / %d, %d key ranges",
+              q4 ? "4 bits" : "bf16", grid, a.batch.seqs, a.heads, a.pool.kv_heads, s.splits);
+    return FV_RAN;
 }
 
 static int check_mask(int mask_mode, int block_tokens, int window, int sink, Mask* m) {
@@ -578,6 +679,15 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
     const long long grid = (long long)b->seqs * kv->kv_heads * s.row_blocks * s.splits;
     if (grid > 0x7fffffffll || (long long)rows > 0x7fffffffll) return FV_DECLINED;
     cudaStream_t st = (cudaStream_t)stream;
+    if (s.chunk) {
+        rc = launch_chunk(st, kv, a, s, dev, sms);
+        if (rc != FV_RAN) return rc;
+        if (s.splits > 1) {
+            fv_paged_merge_kernel<<<(unsigned)((rows + kWarps - 1) / kWarps), kAttnThreads, 0, st>>>(a);
+            FV_CUDA(cudaGetLastError());
+        }
+        return FV_RAN;
+    }
     const bool q4 = kv->format == FV_PAGE_Q4;
     if (q4 && s.nt == 1) fv_paged_decode_kernel<true, 1><<<(unsigned)grid, kAttnThreads, 0, st>>>(a);
     else if (q4) fv_paged_decode_kernel<true, 2><<<(unsigned)grid, kAttnThreads, 0, st>>>(a);

@@ -1,0 +1,740 @@
+// Attention of long chunks over a paged K/V cache on the tensor cores (tcgen05), head dim 128.
+//
+// The skeleton is that of the dense kernel (attn_fwd.cuh): persistent CTAs, work items of two 128-row tiles dealt in snake
+// order, the K/V ring in pairs [V(j-1) | K(j)], one issuing thread, one query row per softmax thread, a softmax without a
+// maximum pass whose row sum guards the reference.  What differs:
+//   * A work item is (sequence, kv head, rows, key range).  A row tile holds 128 / g tokens of the g heads that share the
+//     kv head, so shared heads cost no extra pass over the keys; lengths, rows and the page table are read on the device.
+//   * Key tiles are 128 keys at multiples of 128: those of the sinks, then those of the window.  Pages outside are not
+//     touched.
+//   * bf16 pages: one lane of the loader warp per page (or half a page of 256 rows) issues that page's TMA boxes; boxes
+//     of which the item sees nothing take a page coordinate past the pool, which reads as zeros.  In the few tiles that
+//     the item's visible keys only cover in part, one warp ("fixer") then zeroes V's rows that no row of the item sees: a P of
+//     zero times whatever memory holds there must be zero.
+//   * 4-bit pages: four more warps expand the codes to f16, one key row a thread, into the swizzled tiles that TMA would
+//     have written, and bring Q as f16.  Both products then run in f16: a value zero + step code is rounded once, by
+//     2^-11 at most (in bf16 the roundings of K and V, 2^-8 each, would be of the size of the output's own), P by 2^-11.
+//     f16's range is the price: values beyond 65 504 saturate, below 2^-14 they lose relative precision.  Against that,
+//     P's reference is set 2^6 below the first maximum found: P up to 2^15 fits, and P is zero only 2^30 below the maximum.
+#pragma once
+#include "attn_fwd.cuh"
+#include "paged.cuh"
+
+namespace fvpg {
+
+constexpr int kChunkTile = 128;  // keys
+constexpr int kChunkRows = 128;  // query rows of a row tile; an item has two
+
+struct ChunkJob {
+    Pool pool;
+    Batch batch;
+    Mask mask;
+    const uint16_t* q;
+    long long q_tok, q_head;
+    uint16_t* out;
+    float *part_o, *part_lse;  // splits > 1: [splits, tokens * heads, 128] and [splits, tokens * heads]
+    int* wait_status;          // the first status word
+    long long wait_cycles;
+    int heads, group, tile_tokens, splits, planes, q_blocks, items, box_rows;
+    float sl2;
+};
+
+#if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM103_ALL) || !defined(__CUDA_ARCH__)
+
+using fvattn::as_f;
+using fvattn::as_u;
+using fvattn::Cols;
+using fvattn::RowState;
+using fvattn::Smem;
+using fvattn::neg_inf;
+using namespace fvp;
+
+constexpr uint32_t kVFixed = Smem::total;  // a barrier for each pair slot: V's invisible rows are zeroed
+constexpr uint32_t kChunkSmem = kVFixed + 8 * fvattn::kKvPairs;
+static_assert(kVFixed % 8 == 0 && kChunkSmem <= 232448, "shared memory");
+static_assert(fvattn::kKvPairs == 2 && fvattn::kEarlyKeys == 128, "P is handed over whole");
+
+template <bool Q4>
+struct Roles {
+    static constexpr int kWarps = Q4 ? 16 : 12;
+    static constexpr int kThreads = 32 * kWarps;
+    static constexpr int kLoader = 8, kIssuer = 9, kFixer = 10;  // (bf16: loader and fixer)
+    static constexpr int kExpander = 12;                         // 4 bits: warps 12-15
+};
+
+// What an item covers; every role works it out for itself, from the same numbers.
+struct Work {
+    Seq seq;
+    Span span;
+    int s, head, split, tok0;  // first token of the item inside the call's tokens of the sequence
+    int sinks, first, u0, n;   // its key tiles: number u0 + j of the row of sink tiles, then window tiles
+    FV_DEV int pos0() const { return seq.len - seq.nq; }
+    FV_DEV int key(int j) const {
+        const int u = u0 + j;
+        return (u < sinks ? u : first + (u - sinks)) * kChunkTile;
+    }
+    FV_DEV bool sees(int j) const { return (j >= span.lo && j < span.hi) || j < span.sink; }
+    FV_DEV bool whole(int k0) const { return (k0 >= span.lo && k0 + kChunkTile <= span.hi) || k0 + kChunkTile <= span.sink; }
+};
+// False: item i has no rows.
+FV_DEV bool work_at(const ChunkJob& jb, int i, Work& w) {
+    const int per = jb.planes * jb.splits;
+    const int qb = jb.q_blocks - 1 - i / per, rest = i % per;  // (the last rows see the most keys: heaviest first)
+    w.split = rest % jb.splits;
+    const int plane = rest / jb.splits;
+    w.head = plane % jb.pool.kv_heads;
+    w.s = plane / jb.pool.kv_heads;
+    w.seq = seq_of(jb.batch, w.s);
+    w.tok0 = qb * 2 * jb.tile_tokens;
+    if (w.tok0 >= w.seq.nq) return false;
+    const int last = min(w.tok0 + 2 * jb.tile_tokens, w.seq.nq) - 1;
+    w.span = span_of(jb.mask, w.pos0() + w.tok0, w.pos0() + last, w.seq.len);
+    w.sinks = (w.span.sink + kChunkTile - 1) / kChunkTile;
+    w.first = max(w.span.lo / kChunkTile, w.sinks);
+    const int count = w.sinks + max(0, (w.span.hi + kChunkTile - 1) / kChunkTile - w.first);
+    w.u0 = (int)((long long)count * w.split / jb.splits);
+    w.n = (int)((long long)count * (w.split + 1) / jb.splits) - w.u0;
+    return true;
+}
+// The next item of this CTA that has rows (and, unless `empty` is allowed, keys).
+struct ChunkDeal {
+    int round = 0;
+    FV_DEV bool next(const ChunkJob& jb, Work& w, bool empty) {
+        const int g = (int)gridDim.x, c = (int)blockIdx.x;
+        for (;;) {
+            const int i = round * g + ((round & 1) ? g - 1 - c : c);
+            if (round * g >= jb.items) return false;
+            round++;
+            if (i < jb.items && work_at(jb, i, w) && (empty || w.n > 0)) return true;
+        }
+    }
+};
+
+struct ChunkWait {
+    uint32_t sbase;
+    int* status;
+    long long cycles;
+    int role;
+    FV_DEV bool operator()(uint32_t bar, uint32_t parity) const {
+        if (mbar_try(bar, parity)) return true;
+        const long long t0 = clock64();
+        uint32_t n = 0;
+        while (!mbar_try(bar, parity)) {
+            if (((++n) & 63u) == 0u) {
+                uint32_t gone;
+                asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(gone) : "r"(sbase + Smem::abort_flag) : "memory");
+                if (gone) return false;
+                if (clock64() - t0 > cycles) {
+                    asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(sbase + Smem::abort_flag), "r"(1u) : "memory");
+                    atomicCAS(status, FV_ST_OK, FV_ST_TIMEOUT_BASE + role);
+                    return false;
+                }
+            }
+        }
+        return true;
+    }
+};
+
+// ------------------------------------------------------------------------------------------------- products
+// kind::f16 with both operands bf16 (as umma_idesc_bf16) or both f16 (type fields 0).
+template <bool F16>
+__host__ __device__ constexpr uint32_t chunk_idesc(uint32_t b_mn_major) {
+    return F16 ? (1u << 4) | (b_mn_major << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24) : umma_idesc_bf16(128, 128, b_mn_major);
+}
+template <bool F16>
+FV_DEV void chunk_scores(uint32_t tS, uint64_t qd, uint64_t kd) {
+    constexpr uint32_t idesc = chunk_idesc<F16>(0);
+    asm volatile(
+        "{\n\t.reg .pred pt, pf;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 pf, %3, %3;\n\tsetp.eq.b32 pt, %3, %3;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, pf;\n\t"
+        FV_QK_STEP(2) FV_QK_STEP(4) FV_QK_STEP(6) FV_QK_STEP(1024) FV_QK_STEP(1026) FV_QK_STEP(1028) FV_QK_STEP(1030)
+        "}"
+        ::"r"(tS), "l"(qd), "l"(kd), "r"(idesc)
+        : "memory");
+}
+template <bool F16>
+FV_DEV void chunk_output(uint32_t tO, uint32_t tP, uint64_t vd, bool fresh) {
+    constexpr uint32_t idesc = chunk_idesc<F16>(1);
+    asm volatile(
+        "{\n\t.reg .pred pt, p0;\n\t.reg .b64 b;\n\t.reg .b32 t;\n\t"
+        "setp.eq.b32 p0, %4, 0;\n\tsetp.eq.b32 pt, %3, %3;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p0;\n\t"
+        FV_PV_STEP(8, 128) FV_PV_STEP(16, 256) FV_PV_STEP(24, 384) FV_PV_STEP(32, 512) FV_PV_STEP(40, 640)
+        FV_PV_STEP(48, 768) FV_PV_STEP(56, 896)
+        "}"
+        ::"r"(tO), "r"(tP), "l"(vd), "r"(idesc), "r"(fresh ? 1u : 0u)
+        : "memory");
+}
+
+// -------------------------------------------------------------------------------------------------- softmax
+FV_DEV uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <bool F16>
+FV_DEV uint32_t pack_p(float lo, float hi) {
+    return F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+}
+// As fvattn::exp32: 2^(u sl2 + noff) of 32 columns to packed pairs, every fourth pair on the FMA pipe (POLY).
+template <bool F16, bool POLY>
+FV_DEV void chunk_exp32(const uint32_t (&u)[32], uint32_t* pw, uint64_t s2, uint64_t nf, uint64_t& acc0, uint64_t& acc1, float& top) {
+#pragma unroll
+    for (int w = 0; w < 16; w++) {
+        float t0, t1, p0, p1;
+        unpack_f32x2(fma_f32x2(pack_f32x2(as_f(u[2 * w]), as_f(u[2 * w + 1])), s2, nf), t0, t1);
+        if (POLY && (w & 3) == 3) {
+            top = max3(top, t0, t1);
+            ex2_poly_x2(t0, t1, p0, p1);
+        } else {
+            p0 = ex2(t0);
+            p1 = ex2(t1);
+        }
+        const uint64_t pp = pack_f32x2(p0, p1);
+        if (w & 1) acc1 = add_f32x2(acc1, pp);
+        else acc0 = add_f32x2(acc0, pp);
+        pw[w] = pack_p<F16>(p0, p1);
+    }
+}
+
+// A tile with invisible columns, or whose sum tripped the guard: exact maxima, the reference moved, O and the sum
+// rescaled (as fvattn::careful_tile, whose comment gives the reasons for keeping it out of line).
+template <bool F16>
+static __device__ __noinline__ void chunk_careful(uint32_t tS, uint32_t tO, uint32_t bt, Cols cols, float sl2, bool have_o, int lane,
+                                                  RowState* rs) {
+    float m = rs->m, l = rs->l;
+    float mx = neg_inf();
+#pragma unroll 1
+    for (int c = 0; c < 4; c++) {
+        uint32_t u[32];
+        fvattn::load_chunk(tS, c, u);
+        fvattn::land_chunk(u);
+        cols.hide(u, 32 * c);
+        mx = fmaxf(mx, fvattn::max32(u));
+    }
+    const float cand = mx * sl2;
+    float a = 1.f;
+    if (cand > m + 8.f) {
+        a = ex2(m - cand);
+        m = cand;
+        l *= a;
+    }
+    if (have_o && __any_sync(kFullWarp, a != 1.f)) {
+#pragma unroll 1
+        for (int q = 0; q < 4; q++) {
+            uint32_t o[32];
+            tmem_ld32_issue(tO + 32u * q, o);
+            tmem_ld_wait();
+            tmem_pin(o);
+#pragma unroll
+            for (int c = 0; c < 32; c++) o[c] = as_u(as_f(o[c]) * a);
+            tmem_st32(tO + 32u * q, o);
+        }
+    }
+    const float noff = (m == neg_inf()) ? 0.f : -m;
+    const uint64_t s2 = pack_f32x2(sl2, sl2), nf = pack_f32x2(noff, noff);
+#pragma unroll 1
+    for (int c = 0; c < 4; c++) {
+        uint32_t u[32], pw[16];
+        fvattn::load_chunk(tS, c, u);
+        fvattn::land_chunk(u);
+        cols.hide(u, 32 * c);
+        uint64_t acc0 = pack_f32x2(0.f, 0.f), acc1 = acc0;
+        float top = 0.f;
+        chunk_exp32<F16, false>(u, pw, s2, nf, acc0, acc1, top);
+        l += fvattn::part_sum<false>(acc0, acc1, top);
+        tmem_st16(tS + 16u * (uint32_t)c, pw);
+    }
+    fvattn::publish(bt + Smem::p_ready, lane);
+    rs->m = m;
+    rs->l = l;
+}
+
+// Columns 32 q .. 32 q + 31 of the warp's 32 rows; `row` is this lane's output row or -1.  The 16-byte pieces are transposed
+// between neighbouring lanes first, so that a store covers whole runs of a row (fvattn::store_cols32).
+template <bool F32>
+FV_DEV void chunk_store32(void* base, const uint32_t (&o)[32], float inv, int row, int q, int lane) {
+    constexpr int G = F32 ? 8 : 4;
+    uint4 p[G];
+    float f[32];
+#pragma unroll
+    for (int c = 0; c < 32; c++) f[c] = as_f(o[c]) * inv;
+#pragma unroll
+    for (int c = 0; c < G; c++) {
+        if (F32) p[c] = make_uint4(as_u(f[4 * c]), as_u(f[4 * c + 1]), as_u(f[4 * c + 2]), as_u(f[4 * c + 3]));
+        else p[c] = make_uint4(pack_bf16x2(f[(8 * c) & 31], f[(8 * c + 1) & 31]), pack_bf16x2(f[(8 * c + 2) & 31], f[(8 * c + 3) & 31]),
+                               pack_bf16x2(f[(8 * c + 4) & 31], f[(8 * c + 5) & 31]), pack_bf16x2(f[(8 * c + 6) & 31], f[(8 * c + 7) & 31]));
+    }
+    fvattn::transpose_pieces<G>(p, lane);
+    const int l = lane & (G - 1);
+#pragma unroll
+    for (int k = 0; k < G; k++) {
+        const int r = __shfl_sync(kFullWarp, row, (lane & ~(G - 1)) + k);
+        if (r >= 0) {
+            if (F32) *reinterpret_cast<uint4*>(static_cast<float*>(base) + (size_t)r * kD + 32 * q + 4 * l) = p[k];
+            else *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + (size_t)r * kD + 32 * q + 8 * l) = p[k];
+        }
+    }
+}
+template <bool F32>
+static __device__ __noinline__ void chunk_write(void* base, uint32_t tO, float inv, int row, bool have_o, int lane) {
+#pragma unroll 1
+    for (int q = 0; q < 4; q++) {
+        uint32_t o[32];
+        if (have_o) {
+            tmem_ld32_issue(tO + 32u * q, o);
+            tmem_ld_wait();
+            tmem_pin(o);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 32; c++) o[c] = 0u;
+        }
+        chunk_store32<F32>(base, o, inv, row, q, lane);
+    }
+}
+
+template <bool Q4>
+FV_DEV void chunk_softmax(const ChunkJob& jb, uint32_t sbase, uint32_t tmem, int warp, int lane, const ChunkWait& wait) {
+    constexpr float kChunkGuard = Q4 ? 32768.f : fvattn::kGuard;  // a row sum of P above this could leave P's type
+    constexpr float kBelow = Q4 ? 6.f : 0.f;                      // the reference starts 2^kBelow below the first maximum
+    const int tile = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+    const uint32_t tS = lanes + fvattn::tmem_scores((uint32_t)tile), tO = lanes + fvattn::tmem_output((uint32_t)tile);
+    const uint32_t bt = sbase + 8u * (uint32_t)tile;
+    const float sl2 = jb.sl2;
+    const int row_tok = row / jb.group, row_head = row - row_tok * jb.group;
+    uint32_t s_count = 0, o_count = 0;
+    ChunkDeal deal;
+    Work w;
+    bool more = deal.next(jb, w, true);
+    while (more) {
+        const int tok = w.tok0 + tile * jb.tile_tokens + row_tok;
+        const bool live = row_tok < jb.tile_tokens && tok < w.seq.nq;
+        const int pos = w.pos0() + tok;
+        const Span rsp = span_of(jb.mask, pos, pos, w.seq.len);
+        RowState rs{neg_inf(), 0.f};
+        for (int j = 0; j < w.n; j++) {
+            if (!__all_sync(kFullWarp, wait(bt + Smem::s_ready, s_count & 1u))) return;
+            s_count++;
+            tc_fence_after();
+            const int k0 = w.key(j);
+            Cols cols{0, 0, 0, false};  // (a row that is none: nothing visible, and no say in the votes)
+            if (live) {
+                cols.lo = rsp.lo - k0;
+                cols.hi = min(rsp.hi - k0, kChunkTile);
+                cols.sink = min(rsp.sink - k0, kChunkTile);
+                cols.whole = (cols.lo <= 0 && cols.hi >= kChunkTile) || cols.sink >= kChunkTile;
+            }
+            bool hot = __all_sync(kFullWarp, cols.whole || !live);
+            if (hot) {
+                uint32_t u0[32], u1[32], pw[64];
+                fvattn::load_chunk(tS, 0, u0);
+                fvattn::land_chunk(u0);
+                if (rs.m == neg_inf()) rs.m = live ? fvattn::max32(u0) * sl2 - kBelow : 0.f;
+                const uint64_t s2 = pack_f32x2(sl2, sl2), nf = pack_f32x2(-rs.m, -rs.m);
+                uint64_t acc0 = pack_f32x2(0.f, 0.f), acc1 = acc0;
+                float top = 0.f;
+                fvattn::load_chunk(tS, 1, u1);
+                chunk_exp32<Q4, true>(u0, pw, s2, nf, acc0, acc1, top);
+                fvattn::land_chunk(u1);
+                fvattn::load_chunk(tS, 2, u0);
+                chunk_exp32<Q4, true>(u1, pw + 16, s2, nf, acc0, acc1, top);
+                fvattn::land_chunk(u0);
+                fvattn::load_chunk(tS, 3, u1);
+                chunk_exp32<Q4, true>(u0, pw + 32, s2, nf, acc0, acc1, top);
+                fvattn::land_chunk(u1);
+                chunk_exp32<Q4, true>(u1, pw + 48, s2, nf, acc0, acc1, top);
+                const float sum = fvattn::part_sum<true>(acc0, acc1, top);
+                if (__any_sync(kFullWarp, live && !(sum <= kChunkGuard))) {
+                    hot = false;  // nothing of this tile is stored
+                } else {
+                    fvattn::store_early(tS, pw);
+                    fvattn::publish(bt + Smem::p_ready, lane);
+                    rs.l += sum;
+                }
+            }
+            if (!hot) chunk_careful<Q4>(tS, tO, bt, cols, sl2, j > 0, lane, &rs);
+        }
+        const bool have_o = w.n > 0;
+        const int split = w.split;
+        const int out_row = live ? (w.seq.q0 + tok) * jb.heads + w.head * jb.group + row_head : -1;
+        more = deal.next(jb, w, true);  // (looked up while the last product runs)
+        if (have_o) {
+            if (!__all_sync(kFullWarp, wait(bt + Smem::o_ready, o_count & 1u))) return;
+            o_count++;
+            tc_fence_after();
+        }
+        const float inv = rs.l > 0.f ? 1.f / rs.l : 0.f;
+        if (jb.splits == 1) {
+            chunk_write<false>(jb.out, tO, inv, out_row, have_o, lane);
+        } else {
+            const size_t rows = (size_t)jb.batch.tokens * jb.heads;
+            chunk_write<true>(jb.part_o + (size_t)split * rows * kD, tO, inv, out_row, have_o, lane);
+            if (out_row >= 0) jb.part_lse[(size_t)split * rows + out_row] = rs.l > 0.f ? rs.m + log2f(rs.l) : neg_inf();
+        }
+    }
+}
+
+// --------------------------------------------------------------------------------- loader and fixer (bf16 pages)
+FV_DEV void chunk_loader(const CUtensorMap* mq, const CUtensorMap* mk, const CUtensorMap* mv, const ChunkJob& jb, uint32_t sbase,
+                         int lane, const ChunkWait& wait) {
+    using namespace fvattn;
+    uint32_t qn = 0, kvn = 0;
+    if (lane == 0) {
+        tma_prefetch_desc(mq);
+        tma_prefetch_desc(mk);
+        tma_prefetch_desc(mv);
+    }
+    const uint32_t q_bytes = (uint32_t)(jb.tile_tokens * jb.group) * 128u;  // of one 64-column panel
+    auto ok_all = [&](uint32_t bar, uint32_t parity) { return __all_sync(fvpg::kFullWarp, wait(bar, parity)) != 0; };
+    auto load_q = [&](const Work& w, int tile) -> bool {
+        const uint32_t slot = qn % kQSlots, use = qn / kQSlots;
+        if (use > 0 && !ok_all(sbase + Smem::q_free + 8u * slot, (use - 1u) & 1u)) return false;
+        const uint32_t dst = sbase + Smem::q + slot * kSlotBytes, bar = sbase + Smem::q_full + 8u * slot;
+        if (lane == 0) {
+            const int tok = w.seq.q0 + w.tok0 + tile * jb.tile_tokens;  // rows of other sequences or past the end: never stored
+            mbar_expect_tx(bar, 2 * q_bytes);
+            tma_load4(dst, mq, bar, 0, w.head * jb.group, tok, 0);
+            tma_load4(dst + kPanelBytes, mq, bar, 64, w.head * jb.group, tok, 0);
+        }
+        qn++;
+        return true;
+    };
+    const int boxes = kChunkTile / jb.box_rows;
+    // Page of this lane's box of the key tile at k0; past the pool (zeros) where the item sees nothing of it.
+    auto box_page = [&](const Work& w, int k0) -> int {
+        if (lane >= boxes) return jb.pool.pages;
+        const int a = k0 + lane * jb.box_rows, b = a + jb.box_rows;
+        if (!((a < w.span.hi && b > w.span.lo) || a < w.span.sink)) return jb.pool.pages;
+        const int page = page_of(jb.pool, jb.batch, w.s, a);
+        return page < 0 ? jb.pool.pages : page;
+    };
+    auto load_tile = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, int k0, int page, int head) {
+        const int row = (k0 + lane * jb.box_rows) & ((1 << jb.pool.log_rows) - 1);
+        const uint32_t at = dst + (uint32_t)(lane * jb.box_rows) * 128u;
+        tma_load4(at, map, bar, 0, row, head, page);
+        tma_load4(at + kPanelBytes, map, bar, 64, row, head, page);
+    };
+    ChunkDeal deal;
+    Work w, nw;
+    bool ok = true;
+    bool have = deal.next(jb, w, false);
+    if (have) ok = load_q(w, 0) && load_q(w, 1);
+    while (ok && have) {
+        const bool more = deal.next(jb, nw, false);
+        if (more) ok = load_q(nw, 0);
+        int page = box_page(w, w.key(0)), prev = 0;
+        for (int j = 0; ok && j <= w.n; j++) {
+            const int ahead = j + 1 < w.n ? box_page(w, w.key(j + 1)) : 0;  // (the look-up's latency runs under the wait)
+            const uint32_t slot = kvn % kKvPairs, use = kvn / kKvPairs;
+            if (use > 0 && !ok_all(sbase + Smem::kv_free + 8u * slot, (use - 1u) & 1u)) { ok = false; break; }
+            const uint32_t dst = sbase + Smem::kv + slot * 2u * kSlotBytes, bar = sbase + Smem::kv_full + 8u * slot;
+            if (lane == 0) mbar_expect_tx(bar, (j > 0 ? kSlotBytes : 0u) + (j < w.n ? kSlotBytes : 0u));
+            __syncwarp();
+            if (lane < boxes) {
+                if (j > 0) load_tile(mv, dst, bar, w.key(j - 1), prev, w.head);
+                if (j < w.n) load_tile(mk, dst + kSlotBytes, bar, w.key(j), page, w.head);
+            }
+            kvn++;
+            prev = page;
+            page = ahead;
+        }
+        if (ok && more) ok = load_q(nw, 1);
+        w = nw;
+        have = more;
+    }
+    __syncwarp();
+    if (lane == 0) {  // copies in flight must land before the CTA's shared memory goes away
+        for (uint32_t s = 0; s < (uint32_t)kQSlots && s < qn; s++) {
+            const uint32_t last = ((qn - 1u - s) / kQSlots) * kQSlots + s;
+            mbar_drain(sbase + Smem::q_full + 8u * s, (last / kQSlots) & 1u);
+        }
+        for (uint32_t s = 0; s < (uint32_t)kKvPairs && s < kvn; s++) {
+            const uint32_t last = ((kvn - 1u - s) / kKvPairs) * kKvPairs + s;
+            mbar_drain(sbase + Smem::kv_full + 8u * s, (last / kKvPairs) & 1u);
+        }
+    }
+}
+
+// Follows the pairs one by one (it has a share in kv_free, so it can neither run ahead of a phase nor miss one).
+FV_DEV void chunk_fixer(const ChunkJob& jb, uint32_t sbase, int lane, const ChunkWait& wait) {
+    using namespace fvattn;
+    uint32_t pn = 0;
+    ChunkDeal deal;
+    Work w;
+    while (deal.next(jb, w, false)) {
+        for (int j = 0; j <= w.n; j++) {
+            const uint32_t slot = pn % kKvPairs;
+            if (!__all_sync(fvpg::kFullWarp, wait(sbase + Smem::kv_full + 8u * slot, (pn / kKvPairs) & 1u))) return;
+            if (j > 0 && !w.whole(w.key(j - 1))) {
+                const int k0 = w.key(j - 1);
+                const uint32_t v = sbase + Smem::kv + slot * 2u * kSlotBytes;
+                for (int r = lane; r < kChunkTile; r += 32) {
+                    if (w.sees(k0 + r)) continue;
+#pragma unroll
+                    for (int c = 0; c < 8; c++) {
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + 128u * r + 16u * c), "r"(0) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + kPanelBytes + 128u * r + 16u * c), "r"(0) : "memory");
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor cores read the rows
+                warp_arrive(sbase + kVFixed + 8u * slot, lane);
+            }
+            warp_arrive(sbase + Smem::kv_free + 8u * slot, lane);
+            pn++;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------ expander (4-bit pages)
+struct CodeRow {
+    uint4 c[4];
+    uint32_t sz;
+};
+FV_DEV void load_codes(CodeRow& r, const uint8_t* codes, const uint32_t* scale, const ChunkJob& jb, int page, int head, int key) {
+    if (page < 0) {  // a key that the item does not see, or without a page: zeros
+#pragma unroll
+        for (int i = 0; i < 4; i++) r.c[i] = make_uint4(0, 0, 0, 0);
+        r.sz = 0u;
+        return;
+    }
+    const size_t row = pool_row(jb.pool, page, head, key);
+    const uint4* p = reinterpret_cast<const uint4*>(codes + row * kQ4Bytes);
+#pragma unroll
+    for (int i = 0; i < 4; i++) asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.c[i].x), "=r"(r.c[i].y), "=r"(r.c[i].z), "=r"(r.c[i].w) : "l"(p + i));
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r.sz) : "l"(scale + row));
+}
+FV_DEV uint32_t add_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+FV_DEV uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+// 16-byte piece c (8 values) of row r of a 128 x 128 tile in two 64-column panels with the 128-byte swizzle.
+FV_DEV uint32_t swizzled(uint32_t tile, int r, int c) {
+    return tile + (uint32_t)(c >> 3) * fvattn::kPanelBytes + 128u * (uint32_t)r + 16u * (uint32_t)((c ^ r) & 7);
+}
+FV_DEV void store_piece(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// One row of codes as f16 values zero + step code: a code n goes into the mantissa of 1024 (unit 1), 1032 off is n - 8
+// exactly, and one fused multiply-add rounds once.
+FV_DEV void expand_row(const CodeRow& r, uint32_t tile, int row) {
+    const float step = __uint_as_float(r.sz << 16), zero = __uint_as_float(r.sz & 0xffff0000u);
+    const uint32_t s2 = pack_f16x2(step, step), z2 = pack_f16x2(zero, zero);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t word[4] = {r.c[i].x, r.c[i].y, r.c[i].z, r.c[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t even = word[j], odd = word[j] >> 4;
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {  // bytes k of both: values 2 k and 2 k + 1 of this piece
+                const uint32_t pair = __byte_perm(even, odd, (uint32_t)(k | (k << 4) | ((4 + k) << 8) | ((4 + k) << 12)));
+                h[k] = fma_f16x2(add_f16x2((pair & 0x000f000fu) | 0x64006400u, 0xe408e408u), s2, z2);
+            }
+            store_piece(swizzled(tile, row, 4 * i + j), h[0], h[1], h[2], h[3]);
+        }
+    }
+}
+FV_DEV void chunk_expander(const ChunkJob& jb, uint32_t sbase, int row, int lane, const ChunkWait& wait) {
+    using namespace fvattn;
+    uint32_t qn = 0, kvn = 0;
+    const int row_tok = row / jb.group, row_head = row - row_tok * jb.group;
+    auto ok_all = [&](uint32_t bar, uint32_t parity) { return __all_sync(fvpg::kFullWarp, wait(bar, parity)) != 0; };
+    auto arrive = [&](uint32_t bar) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor cores read what was stored
+        warp_arrive(bar, lane);
+    };
+    auto load_q = [&](const Work& w, int tile) -> bool {
+        const uint32_t slot = qn % kQSlots, use = qn / kQSlots;
+        if (use > 0 && !ok_all(sbase + Smem::q_free + 8u * slot, (use - 1u) & 1u)) return false;
+        const uint32_t dst = sbase + Smem::q + slot * kSlotBytes;
+        const int tok = w.tok0 + tile * jb.tile_tokens + row_tok;
+        const bool live = row_tok < jb.tile_tokens && tok < w.seq.nq;
+        const uint16_t* p = jb.q + (long long)(w.seq.q0 + (live ? tok : 0)) * jb.q_tok + (long long)(w.head * jb.group + row_head) * jb.q_head;
+#pragma unroll 4
+        for (int c = 0; c < 16; c++) {
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (live) u = __ldg(reinterpret_cast<const uint4*>(p) + c);
+            auto half2 = [](uint32_t x) { return pack_f16x2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); };
+            store_piece(swizzled(dst, row, c), half2(u.x), half2(u.y), half2(u.z), half2(u.w));
+        }
+        arrive(sbase + Smem::q_full + 8u * slot);
+        qn++;
+        return true;
+    };
+    auto key_page = [&](const Work& w, int j) -> int {
+        const int key = w.key(j) + row;
+        return w.sees(key) ? page_of(jb.pool, jb.batch, w.s, key) : -1;
+    };
+    ChunkDeal deal;
+    Work w, nw;
+    bool ok = true;
+    bool have = deal.next(jb, w, false);
+    if (have) ok = load_q(w, 0) && load_q(w, 1);
+    while (ok && have) {
+        const bool more = deal.next(jb, nw, false);
+        if (more) ok = load_q(nw, 0);
+        CodeRow kc, vc;
+        int page = key_page(w, 0), ahead = w.n > 1 ? key_page(w, 1) : -1;
+        load_codes(kc, jb.pool.k, jb.pool.k_scale, jb, page, w.head, w.key(0) + row);
+        for (int j = 0; ok && j <= w.n; j++) {
+            const uint32_t slot = kvn % kKvPairs, use = kvn / kKvPairs;
+            if (use > 0 && !ok_all(sbase + Smem::kv_free + 8u * slot, (use - 1u) & 1u)) { ok = false; break; }
+            const uint32_t dst = sbase + Smem::kv + slot * 2u * kSlotBytes;
+            // K(j) out of registers, then the loads of K(j + 1); V(j - 1) likewise, then those of V(j).
+            if (j < w.n) {
+                expand_row(kc, dst + kSlotBytes, row);
+                if (j + 1 < w.n) load_codes(kc, jb.pool.k, jb.pool.k_scale, jb, ahead, w.head, w.key(j + 1) + row);
+            }
+            if (j > 0) expand_row(vc, dst, row);
+            arrive(sbase + Smem::kv_full + 8u * slot);
+            kvn++;
+            if (j < w.n) {
+                load_codes(vc, jb.pool.v, jb.pool.v_scale, jb, page, w.head, w.key(j) + row);
+                page = ahead;
+                ahead = j + 2 < w.n ? key_page(w, j + 2) : -1;
+            }
+        }
+        if (ok && more) ok = load_q(nw, 1);
+        w = nw;
+        have = more;
+    }
+}
+
+// --------------------------------------------------------------------------------------------------- issuer
+// Step j of an item: O_t += P_t(j-1) . V(j-1) for j > 0, then S_t = Q_t . K(j)^T for j < n, t = A then B, strictly in order
+// (fvattn::issuer_thread).
+template <bool Q4>
+FV_DEV void chunk_issuer(const ChunkJob& jb, uint32_t sbase, uint32_t tmem, const ChunkWait& wait) {
+    using namespace fvattn;
+    uint32_t qn = 0, pn = 0, pc = 0;
+    uint32_t fixed[kKvPairs] = {};  // V tiles of each slot that the fixer had to touch so far
+    ChunkDeal deal;
+    Work w;
+    bool ok = true;
+    while (ok && deal.next(jb, w, false)) {
+        const uint32_t qa = qn % kQSlots, qb = (qn + 1u) % kQSlots;
+        const uint32_t qa_par = (qn / kQSlots) & 1u, qb_par = ((qn + 1u) / kQSlots) & 1u;
+        qn += 2;
+        const uint64_t qd_a = umma_desc_sw128(sbase + Smem::q + qa * kSlotBytes, 16, 1024);
+        const uint64_t qd_b = umma_desc_sw128(sbase + Smem::q + qb * kSlotBytes, 16, 1024);
+#pragma unroll 1
+        for (int j = 0; j <= w.n; j++) {
+            const uint32_t slot = pn % kKvPairs;
+            const uint32_t pair = sbase + Smem::kv + slot * 2u * kSlotBytes;
+            if (!wait(sbase + Smem::kv_full + 8u * slot, (pn / kKvPairs) & 1u)) { ok = false; break; }
+            if (!Q4 && j > 0 && !w.whole(w.key(j - 1))) {
+                uint32_t& count = slot ? fixed[1] : fixed[0];
+                if (!wait(sbase + kVFixed + 8u * slot, count & 1u)) { ok = false; break; }
+                count++;
+            }
+            tc_fence_after();
+            const uint64_t vd = umma_desc_sw128(pair, kPanelBytes, 1024);
+            const uint64_t kd = umma_desc_sw128(pair + kSlotBytes, 16, 1024);
+#pragma unroll
+            for (uint32_t t = 0; t < 2; t++) {
+                if (j > 0) {
+                    if (!wait(sbase + 8u * t + Smem::p_ready, pc & 1u)) { ok = false; break; }
+                    tc_fence_after();
+                    chunk_output<Q4>(tmem + tmem_output(t), tmem + tmem_scores(t), vd, j == 1);
+                }
+                if (j == w.n) {
+                    umma_commit(sbase + Smem::o_ready + 8u * t);
+                    continue;
+                }
+                if (j == 0) {
+                    if (!wait(sbase + Smem::q_full + 8u * (t ? qb : qa), t ? qb_par : qa_par)) { ok = false; break; }
+                    tc_fence_after();
+                }
+                chunk_scores<Q4>(tmem + tmem_scores(t), t ? qd_b : qd_a, kd);
+                umma_commit(sbase + Smem::s_ready + 8u * t);
+                if (j == w.n - 1) umma_commit(sbase + Smem::q_free + 8u * (t ? qb : qa));
+            }
+            if (!ok) break;
+            umma_commit(sbase + Smem::kv_free + 8u * slot);
+            pn++;
+            if (j > 0) pc++;
+        }
+    }
+    umma_commit(sbase + Smem::drain);
+    mbar_drain(sbase + Smem::drain, 0);
+}
+
+template <bool Q4>
+FV_DEV void chunk_persistent(const CUtensorMap* mq, const CUtensorMap* mk, const CUtensorMap* mv, const ChunkJob& jb, unsigned char* smem) {
+    using namespace fvattn;
+    using R = Roles<Q4>;
+    const uint32_t sbase = smem_u32(smem);
+    const int warp = (int)(threadIdx.x >> 5), lane = (int)(threadIdx.x & 31);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Smem::abort_flag);
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + Smem::tmem_slot);
+    if (threadIdx.x == 0) {
+        const uint32_t producers = Q4 ? 4 : 1;  // the expander's four warps, or one transaction count
+        for (int s = 0; s < kQSlots; s++) {
+            mbar_init(sbase + Smem::q_full + 8u * s, producers);
+            mbar_init(sbase + Smem::q_free + 8u * s, 1);
+        }
+        for (int s = 0; s < kKvPairs; s++) {
+            mbar_init(sbase + Smem::kv_full + 8u * s, producers);
+            mbar_init(sbase + Smem::kv_free + 8u * s, Q4 ? 1 : 2);  // the issuer's commit (and the fixer)
+            mbar_init(sbase + kVFixed + 8u * s, 1);
+        }
+        for (int t = 0; t < 2; t++) {
+            mbar_init(sbase + Smem::s_ready + 8u * t, 1);
+            mbar_init(sbase + Smem::p_ready + 8u * t, 4);
+            mbar_init(sbase + Smem::o_ready + 8u * t, 1);
+        }
+        mbar_init(sbase + Smem::drain, 1);
+        int bad = (*(volatile int*)jb.wait_status != FV_ST_OK) ? 1 : 0;  // a CTA that starts after another one gave up does nothing
+        if (sbase & 1023u) {
+            atomicCAS(jb.wait_status, FV_ST_OK, FV_ST_BAD_SMEM);
+            bad = 1;
+        }
+        *abort_flag = bad;
+        mbar_init_fence();
+    }
+    __syncthreads();
+    if (*abort_flag) return;  // CTA-uniform
+    if (warp == R::kIssuer) tmem_alloc(sbase + Smem::tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    auto waiter = [&](int role) { return ChunkWait{sbase, jb.wait_status, jb.wait_cycles, role}; };
+    // Registers: 384 x 168 = 256 x 216 + 128 x 72; 512 x 128 = 256 x 184 + 256 x 72.
+    if (warp < kSoftmaxWarps) {
+        if (Q4) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;" ::: "memory");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;" ::: "memory");
+        chunk_softmax<Q4>(jb, sbase, tmem, warp, lane, waiter(3));
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
+        if (warp == R::kIssuer) {
+            if (lane == 0) chunk_issuer<Q4>(jb, sbase, tmem, waiter(2));
+        } else if (Q4) {
+            if (warp >= R::kExpander) chunk_expander(jb, sbase, 32 * (warp - R::kExpander) + lane, lane, waiter(1));
+        } else if (warp == R::kLoader) {
+            chunk_loader(mq, mk, mv, jb, sbase, lane, waiter(1));
+        } else if (warp == R::kFixer) {
+            chunk_fixer(jb, sbase, lane, waiter(4));
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == R::kIssuer) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+#endif  // sm_100a / host pass
+
+}  // namespace fvpg
