@@ -8,13 +8,18 @@
 #include "paged.cuh"
 #include "paged_fwd.cuh"
 #include "paged_host.h"
+#include <cooperative_groups.h>
 #include <math.h>
+#include <stdlib.h>
 #include <mutex>
 
 namespace fvpg {
 
+namespace cg = cooperative_groups;
+
 constexpr int kWarps = 4;
 constexpr int kAttnThreads = 32 * kWarps;
+constexpr int kMaxCluster = 8;  // CTAs of a portable cluster
 constexpr int kTile = 16;  // keys a warp takes at a time (one page holds them: page_rows is a multiple of 16)
 
 struct AttnArgs {
@@ -27,6 +32,7 @@ struct AttnArgs {
     float* part_o;            // [splits, tokens * heads, 128] normalised, when splits > 1
     float* part_lse;          // [splits, tokens * heads], base 2
     int heads, group, splits, row_blocks;
+    int cluster;              // the key ranges of a block of rows are one cluster, which joins them itself
     float sl2;
 };
 
@@ -59,84 +65,102 @@ FV_DEV uint32_t ld_stream1(const void* p) {
     asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r) : "l"(p));
     return r;
 }
-// D (16 x 8 f32) += A (16 x 16 bf16) . B (16 x 8 bf16).  Lane 4 g + t holds of A rows g (a0, a2) and g + 8 (a1, a3), of B
-// column g, of D rows g (c0, c1) and g + 8 (c2, c3), columns 2 t and 2 t + 1.
+// D (16 x 8 f32) += A (16 x 16) . B (16 x 8), both bf16 or both f16.  Lane 4 g + t holds of A rows g (a0, a2) and g + 8
+// (a1, a3), of B column g, of D rows g (c0, c1) and g + 8 (c2, c3), columns 2 t and 2 t + 1.
+template <bool F16>
 FV_DEV void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if (F16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Transpose of an 8 x 8 tile of bf16 held one row per quad of lanes.
+// Transpose of an 8 x 8 tile of 16-bit values held one row per quad of lanes.
 FV_DEV uint32_t transpose8(uint32_t x) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
 FV_DEV uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
-// Codes n of nibbles i and i + 4 of x as the bf16 pair (128 + n): 128 has a unit in its last place of one, so or-ing the
-// code into the mantissa is exact.
-FV_DEV uint32_t codes128(uint32_t x, int i) { return ((x >> (4 * i)) & 0x000f000fu) | 0x43004300u; }
-FV_DEV uint32_t sub136(uint32_t x) {  // (128 + n) - 136 = n - 8, exact
-    uint32_t r;
-    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0xc308c308u));
-    return r;
+// The eight codes of a word as four f16 pairs code = n - 8, pair i from nibbles i and i + 4.  A nibble at bits 0-3 or 4-7 of a
+// half word is or-ed into the mantissa of 1024 (unit 1) as it lies: 1024 + n or 1024 + 16 n, exact, and one addition or
+// multiply-add takes the 1024 off, exact as well: one shift and four three-input logic operations a word (the logic pipe
+// is what bounds this kernel), the rest on the otherwise idle FMA pipe.
+FV_DEV void codes_f16(uint32_t w, uint32_t (&h)[4]) {
+    const uint32_t v = w >> 8;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(h[0]) : "r"(w), "r"(0x000f000fu), "r"(0x64006400u));
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(h[1]) : "r"(w), "r"(0x00f000f0u), "r"(0x64006400u));
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(h[2]) : "r"(v), "r"(0x000f000fu), "r"(0x64006400u));
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(h[3]) : "r"(v), "r"(0x00f000f0u), "r"(0x64006400u));
+    h[0] = add_f16x2(h[0], 0xe408e408u);               // - 1032
+    h[1] = fma_f16x2(h[1], 0x2c002c00u, 0xd480d480u);  // / 16 - 72
+    h[2] = add_f16x2(h[2], 0xe408e408u);
+    h[3] = fma_f16x2(h[3], 0x2c002c00u, 0xd480d480u);
 }
 FV_DEV float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
 FV_DEV float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
-// One tile of 16 keys in registers, as lane 4 g + t holds it.
+FV_DEV uint32_t word(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
+
+// One tile of 16 keys in registers, as lane 4 g + t holds it; `row` is the pool row of the tile's first key, or kNoRow.
 //   bf16  k0 / k1: keys g and g + 8, 16-byte pieces 4 n + t of their rows; v: keys 2t, 2t+1, 2t+8, 2t+9, pieces g and
 //         g + 8 of their rows.
-//   4 bit k0[0] / k1[0]: values 32 t .. 32 t + 31 of keys g and g + 8; v4: values 16 g .. 16 g + 15 of the four keys;
-//         ks / vs: (step, zero) of keys g and g + 8.
+//   4 bit k0 / k1: values 32 t .. 32 t + 31 of keys g and g + 8; v: values 16 g .. 16 g + 15 of the four keys; s0 / s1:
+//         (step, zero) of keys g and g + 8.
+constexpr uint32_t kNoRow = 0xffffffffu;
 template <bool Q4>
 struct Keys;
 template <>
 struct Keys<false> {
     uint4 k0[4], k1[4];
-    FV_DEV void load(const Pool& p, int page, int head, int key, int g, int t) {
-        if (page < 0) {
+    FV_DEV void load(const uint8_t* lane_k, const uint32_t*, uint32_t row) {
+        if (row == kNoRow) {
 #pragma unroll
             for (int n = 0; n < 4; n++) k0[n] = k1[n] = make_uint4(0, 0, 0, 0);
             return;
         }
-        const uint8_t* r = p.k + pool_row(p, page, head, key) * 256 + (size_t)g * 256 + 16 * t;
+        const uint8_t* r = lane_k + (size_t)row * 256;
 #pragma unroll
         for (int n = 0; n < 4; n++) {
             k0[n] = ld_stream(r + 64 * n);
             k1[n] = ld_stream(r + 8 * 256 + 64 * n);
         }
     }
+    static FV_DEV size_t lane_offset(int g, int t) { return (size_t)g * 256 + 16 * t; }
 };
 template <>
 struct Keys<true> {
-    uint4 k0[1], k1[1];
+    uint4 k0, k1;
     uint32_t s0, s1;
-    FV_DEV void load(const Pool& p, int page, int head, int key, int g, int t) {
-        if (page < 0) {
-            k0[0] = k1[0] = make_uint4(0, 0, 0, 0);
+    FV_DEV void load(const uint8_t* lane_k, const uint32_t* lane_s, uint32_t row) {
+        if (row == kNoRow) {
+            k0 = k1 = make_uint4(0, 0, 0, 0);
             s0 = s1 = 0;
             return;
         }
-        const size_t row = pool_row(p, page, head, key) + g;
-        k0[0] = ld_stream(p.k + row * kQ4Bytes + 16 * t);
-        k1[0] = ld_stream(p.k + (row + 8) * kQ4Bytes + 16 * t);
-        s0 = ld_stream1(p.k_scale + row);
-        s1 = ld_stream1(p.k_scale + row + 8);
+        const uint8_t* r = lane_k + (size_t)row * kQ4Bytes;
+        k0 = ld_stream(r);
+        k1 = ld_stream(r + 8 * kQ4Bytes);
+        s0 = ld_stream1(lane_s + row);
+        s1 = ld_stream1(lane_s + row + 8);
     }
+    static FV_DEV size_t lane_offset(int g, int t) { return (size_t)g * kQ4Bytes + 16 * t; }
 };
 template <bool Q4>
 struct Values;
 template <>
 struct Values<false> {
     uint4 a[4], b[4];  // pieces g and g + 8 of keys 2t, 2t+1, 2t+8, 2t+9
-    FV_DEV void load(const Pool& p, int page, int head, int key, int g, int t) {
-        if (page < 0) {
+    FV_DEV void load(const uint8_t* lane_v, const uint32_t*, uint32_t row) {
+        if (row == kNoRow) {
 #pragma unroll
             for (int i = 0; i < 4; i++) a[i] = b[i] = make_uint4(0, 0, 0, 0);
             return;
         }
-        const uint8_t* r = p.v + pool_row(p, page, head, key) * 256 + (size_t)(2 * t) * 256 + 16 * g;
+        const uint8_t* r = lane_v + (size_t)row * 256;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int o = ((i & 1) + 8 * (i >> 1)) * 256;
@@ -144,36 +168,40 @@ struct Values<false> {
             b[i] = ld_stream(r + o + 128);
         }
     }
-    FV_DEV void clear(int i) { a[i] = b[i] = make_uint4(0, 0, 0, 0); }
+    static FV_DEV size_t lane_offset(int g, int t) { return (size_t)(2 * t) * 256 + 16 * g; }
 };
 template <>
 struct Values<true> {
     uint2 a[4];
     uint32_t s0, s1;
-    FV_DEV void load(const Pool& p, int page, int head, int key, int g, int t) {
-        if (page < 0) {
+    FV_DEV void load(const uint8_t* lane_v, const uint32_t* lane_s, uint32_t row) {
+        if (row == kNoRow) {
 #pragma unroll
             for (int i = 0; i < 4; i++) a[i] = make_uint2(0, 0);
             s0 = s1 = 0;
             return;
         }
-        const size_t row = pool_row(p, page, head, key);
+        const uint8_t* r = lane_v + (size_t)row * kQ4Bytes;
 #pragma unroll
-        for (int i = 0; i < 4; i++) a[i] = ld_stream2(p.v + (row + 2 * t + (i & 1) + 8 * (i >> 1)) * kQ4Bytes + 8 * g);
-        s0 = ld_stream1(p.v_scale + row + g);
-        s1 = ld_stream1(p.v_scale + row + g + 8);
+        for (int i = 0; i < 4; i++) a[i] = ld_stream2(r + ((i & 1) + 8 * (i >> 1)) * kQ4Bytes);
+        s0 = ld_stream1(lane_s + row);
+        s1 = ld_stream1(lane_s + row + 8);
     }
+    static FV_DEV size_t lane_offset(int g, int t) { return (size_t)(2 * t) * kQ4Bytes + 8 * g; }
 };
-
-FV_DEV uint32_t word(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
 
 // NT groups of 8 query rows.  The transposed products S^T = K . Q^T and O^T = V^T . P^T keep keys and head dim on the
 // 16-wide side of the matrix instruction and the (few) query rows on the 8-wide one; the sums of either product may run
 // in any order of d or key, so every lane's operands are whole 16-byte pieces as they lie in memory and no shared
 // memory is needed on the way.
+//
+// A warp takes a run of tiles of its own.  Their pool rows are looked up 32 at a time, one tile a lane, a batch ahead; a tile's
+// K registers are loaded anew as soon as its scores are done and V's as soon as its product is, so that memory is always
+// being read while the warp computes.
 template <bool Q4, int NT>
 __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const AttnArgs a) {
     constexpr int kRows = 8 * NT;
+    constexpr int SUB = Q4 ? 2 : 1;  // tiles at a time (4 bits: 16 keys are too few bytes in flight)
     __shared__ float sh_o[kWarps][kRows][kD + 4];
     __shared__ float sh_m[kWarps][kRows], sh_l[kWarps][kRows];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -185,20 +213,57 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
     const int head = b % a.pool.kv_heads, s = b / a.pool.kv_heads;
     const Seq seq = seq_of(a.batch, s);
     const int row0 = rb * kRows, rows = min(kRows, seq.nq * a.group - row0);
-    if (rows <= 0) return;
+    if (rows <= 0) return;  // (the same for all key ranges of these rows)
     const int pos0 = seq.len - seq.nq;  // position of the sequence's first token of this call
     const int first = pos0 + row0 / a.group, last = pos0 + (row0 + rows - 1) / a.group;
     const Span span = span_of(a.mask, first, last, seq.len);
-    const Span lowest = span_of(a.mask, first, first, seq.len), highest = span_of(a.mask, last, last, seq.len);
     const Tiles tiles(span);
-    // (every row sees the whole tile: inside the first row's end and the last row's start, or inside the sinks)
-    const int whole_lo = highest.lo, whole_hi = lowest.hi;
-    const int whole_sink = min(lowest.lo == 0 ? lowest.hi : lowest.sink, highest.lo == 0 ? highest.hi : highest.sink);
     const int u0 = (int)((long long)tiles.count * split / a.splits), u1 = (int)((long long)tiles.count * (split + 1) / a.splits);
+    const int w0 = u0 + (u1 - u0) * warp / kWarps, n_tiles = u0 + (u1 - u0) * (warp + 1) / kWarps - w0;
 
-    // Q^T: column g of each group of 8 rows, in the order of d that the keys' lanes hold.
+    // Tiles of which every row sees every key: inside the first row's end and the last row's start, or inside the sinks.
+    int whole_lo, whole_hi, whole_sink;
+    {
+        const Span lowest = span_of(a.mask, first, first, seq.len), highest = span_of(a.mask, last, last, seq.len);
+        whole_lo = highest.lo;
+        whole_hi = lowest.hi;
+        whole_sink = min(lowest.lo == 0 ? lowest.hi : lowest.sink, highest.lo == 0 ? highest.hi : highest.sink);
+    }
+    struct Feed {
+        uint32_t row, whole;  // this lane's tile's pool row; bit i: tile i of the batch is whole
+    };
+    auto lookup = [&](int base) {
+        Feed f{kNoRow, 0u};
+        bool whole = false;
+        if (base + lane < n_tiles) {
+            const int key = tiles.key(w0 + base + lane);
+            const int page = page_of(a.pool, a.batch, s, key);
+            if (page >= 0) {
+                f.row = (uint32_t)pool_row(a.pool, page, head, key);
+                whole = (key >= whole_lo && key + kTile <= whole_hi) || key + kTile <= whole_sink;
+            }
+        }
+        f.whole = __ballot_sync(kFullWarp, whole);
+        return f;
+    };
+    Feed cur = lookup(0), nxt = lookup(32);
+    const uint8_t* lane_k = a.pool.k + Keys<Q4>::lane_offset(g, t);
+    const uint8_t* lane_v = a.pool.v + Values<Q4>::lane_offset(g, t);
+    const uint32_t *lane_ks = a.pool.k_scale + g, *lane_vs = a.pool.v_scale + g;
+    Keys<Q4> kt[SUB];
+    Values<Q4> vt[SUB];
+#pragma unroll
+    for (int i = 0; i < SUB; i++) {
+        const uint32_t row = __shfl_sync(kFullWarp, cur.row, i);
+        kt[i].load(lane_k, lane_ks, row);
+        vt[i].load(lane_v, lane_vs, row);
+    }
+
+    // Q^T: column g of each group of 8 rows, in the order of d that the keys' lanes hold.  4 bits: as f16, scaled by a power
+    // of two that brings the row's largest value to 2^8 .. 2^9 (what falls below f16's range is 2^-32 of that), which goes into
+    // the row's softmax scale; qsum: the row's sum in the same units.
     uint32_t qf[NT][16];
-    float qsum[NT][2];
+    float qsum[NT][2], sl2[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const int r = row0 + 8 * n + g;
@@ -211,26 +276,47 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
 #pragma unroll
             for (int i = 0; i < 4; i++) u[i] = make_uint4(0, 0, 0, 0);
         }
-        float sum = 0.f;
+        if constexpr (Q4) {
+            float top = 0.f, sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (Q4) {  // pairs (d, d + 4) of eight values: the nibbles that one shift and mask give
-                qf[n][4 * i + 0] = prmt(u[i].x, u[i].z, 0x5410);
-                qf[n][4 * i + 1] = prmt(u[i].x, u[i].z, 0x7632);
-                qf[n][4 * i + 2] = prmt(u[i].y, u[i].w, 0x5410);
-                qf[n][4 * i + 3] = prmt(u[i].y, u[i].w, 0x7632);
-            } else {
+            for (int i = 0; i < 4; i++) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float x = lo_f(word(u[i], j)), y = hi_f(word(u[i], j));
+                    top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
+                    sum += x + y;
+                }
+            }
+            top = fmaxf(top, __shfl_xor_sync(kFullWarp, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(kFullWarp, top, 2));
+            sum += __shfl_xor_sync(kFullWarp, sum, 1);
+            sum += __shfl_xor_sync(kFullWarp, sum, 2);
+            // 2^(8 - floor(log2 top)) and its inverse, from the exponent field (kept inside the normal numbers)
+            const int e = min(max((int)(__float_as_uint(top) >> 23), 16), 246);
+            const float up = __uint_as_float((uint32_t)(262 - e) << 23), down = __uint_as_float((uint32_t)(e - 8) << 23);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {  // pairs (d, d + 4) of eight values: the nibbles that one mask gives
+                auto pair = [&](uint32_t x, uint32_t y, bool high) {
+                    return high ? pack_f16x2(hi_f(x) * up, hi_f(y) * up) : pack_f16x2(lo_f(x) * up, lo_f(y) * up);
+                };
+                qf[n][4 * i + 0] = pair(u[i].x, u[i].z, false);
+                qf[n][4 * i + 1] = pair(u[i].x, u[i].z, true);
+                qf[n][4 * i + 2] = pair(u[i].y, u[i].w, false);
+                qf[n][4 * i + 3] = pair(u[i].y, u[i].w, true);
+            }
+            const float scaled = sum * up, back = a.sl2 * down;
+            qsum[n][0] = __shfl_sync(kFullWarp, scaled, 8 * t);      // of row 2 t, which the lanes 4 (2 t) .. hold
+            qsum[n][1] = __shfl_sync(kFullWarp, scaled, 8 * t + 4);  // of row 2 t + 1
+            sl2[n][0] = __shfl_sync(kFullWarp, back, 8 * t);
+            sl2[n][1] = __shfl_sync(kFullWarp, back, 8 * t + 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) qf[n][4 * i + j] = word(u[i], j);
             }
-#pragma unroll
-            for (int j = 0; j < 4; j++) sum += lo_f(word(u[i], j)) + hi_f(word(u[i], j));
-        }
-        if (Q4) {
-            sum += __shfl_xor_sync(kFullWarp, sum, 1);
-            sum += __shfl_xor_sync(kFullWarp, sum, 2);
-            qsum[n][0] = __shfl_sync(kFullWarp, sum, 8 * t);      // of row 2 t, which the lanes 4 (2 t) .. hold
-            qsum[n][1] = __shfl_sync(kFullWarp, sum, 8 * t + 4);  // of row 2 t + 1
+            qsum[n][0] = qsum[n][1] = 0.f;
+            sl2[n][0] = sl2[n][1] = a.sl2;
         }
     }
 
@@ -244,99 +330,135 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
         l[n][0] = l[n][1] = z[n][0] = z[n][1] = 0.f;
     }
 
-    auto lookup = [&](int u) { return u < u1 ? page_of(a.pool, a.batch, s, tiles.key(u)) : -1; };
-    Keys<Q4> kt;
-    Values<Q4> vt;
-    int u = u0 + warp;
-    int page = lookup(u), page_next = lookup(u + kWarps);
-    if (u < u1) {
-        kt.load(a.pool, page, head, tiles.key(u), g, t);
-        vt.load(a.pool, page, head, tiles.key(u), g, t);
-    }
-    while (u < u1) {
-        const int key0 = tiles.key(u), un = u + kWarps;
-        const int page_after = lookup(un + kWarps);
-        float c[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    if (Q4) {
-                        const uint32_t w0 = word(kt.k0[0], i), w1 = word(kt.k1[0], i);
-                        mma(c[n], codes128(w0, 2 * j), codes128(w1, 2 * j), codes128(w0, 2 * j + 1), codes128(w1, 2 * j + 1),
-                            qf[n][4 * i + 2 * j], qf[n][4 * i + 2 * j + 1]);
-                    } else {
-                        mma(c[n], word(kt.k0[Q4 ? 0 : i], 2 * j), word(kt.k1[Q4 ? 0 : i], 2 * j), word(kt.k0[Q4 ? 0 : i], 2 * j + 1),
-                            word(kt.k1[Q4 ? 0 : i], 2 * j + 1), qf[n][4 * i + 2 * j], qf[n][4 * i + 2 * j + 1]);
-                    }
-                }
-            }
+    for (int v = 0; v < n_tiles; v += SUB) {
+        const int i0 = v & 31;
+        if (v > 0 && i0 == 0) {
+            cur = nxt;
+            nxt = lookup(v + 32);
         }
-        if constexpr (Q4) {
-            // q . (zero + step code) = step (q . (128 + n)) + (zero - 136 step) sum(q)
-            const float s0 = lo_f(kt.s0), s1 = lo_f(kt.s1);
-            const float z0 = fmaf(-136.f, s0, hi_f(kt.s0)), z1 = fmaf(-136.f, s1, hi_f(kt.s1));
+        uint32_t next_row[SUB];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                c[n][0] = fmaf(c[n][0], s0, z0 * qsum[n][0]);
-                c[n][1] = fmaf(c[n][1], s0, z0 * qsum[n][1]);
-                c[n][2] = fmaf(c[n][2], s1, z1 * qsum[n][0]);
-                c[n][3] = fmaf(c[n][3], s1, z1 * qsum[n][1]);
-            }
-        }
-        if (un < u1) kt.load(a.pool, page_next, head, tiles.key(un), g, t);
+        for (int i = 0; i < SUB; i++) next_row[i] = __shfl_sync(kFullWarp, i0 + SUB < 32 ? cur.row : nxt.row, (i0 + SUB + i) & 31);
+        const bool more = v + SUB < n_tiles;
 
         // c0, c1: key g, rows 2 t and 2 t + 1; c2, c3: key g + 8.
-        const bool whole = page >= 0 && ((key0 >= whole_lo && key0 + kTile <= whole_hi) || key0 + kTile <= whole_sink);
-        if (!whole) {
+        float c[SUB][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
+        for (int i = 0; i < SUB; i++) {
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int r = row0 + 8 * n + 2 * t + e, p = pos0 + r / a.group;
-                    const Span sp = span_of(a.mask, p, p, seq.len);
+            for (int n = 0; n < NT; n++) c[i][n][0] = c[i][n][1] = c[i][n][2] = c[i][n][3] = 0.f;
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int j = key0 + g + 8 * h;
-                        if (page < 0 || !((j >= sp.lo && j < sp.hi) || j < sp.sink)) c[n][2 * h + e] = neg_inf();
+            for (int w = 0; w < 4; w++) {
+                uint32_t x0[4], x1[4];
+                if constexpr (Q4) {
+                    codes_f16(word(kt[i].k0, w), x0);
+                    codes_f16(word(kt[i].k1, w), x1);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        x0[j] = word(kt[i].k0[w], j);
+                        x1[j] = word(kt[i].k1[w], j);
                     }
                 }
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) mma<Q4>(c[i][n], x0[j], x1[j], x0[j + 1], x1[j + 1], qf[n][4 * w + j], qf[n][4 * w + j + 1]);
+                }
             }
-            // Values that no row of this block may see count as zero whatever they hold (0 times NaN is NaN).
-            auto seen = [&](int j) { return (j >= span.lo && j < span.hi) || j < span.sink; };
+            if constexpr (Q4) {  // q . (zero + step code) = step (q . code) + zero sum(q)
+                const float s0 = lo_f(kt[i].s0), s1 = lo_f(kt[i].s1), z0 = hi_f(kt[i].s0), z1 = hi_f(kt[i].s1);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    c[i][n][0] = fmaf(c[i][n][0], s0, z0 * qsum[n][0]);
+                    c[i][n][1] = fmaf(c[i][n][1], s0, z0 * qsum[n][1]);
+                    c[i][n][2] = fmaf(c[i][n][2], s1, z1 * qsum[n][0]);
+                    c[i][n][3] = fmaf(c[i][n][3], s1, z1 * qsum[n][1]);
+                }
+            }
+            if (more) kt[i].load(lane_k, lane_ks, next_row[i]);
+        }
+
+        constexpr uint32_t kAll = (1u << SUB) - 1u;
+        if (((cur.whole >> i0) & kAll) != kAll) {
+#pragma unroll
+            for (int i = 0; i < SUB; i++) {
+                const bool none = __shfl_sync(kFullWarp, cur.row, i0 + i) == kNoRow;
+                const int key0 = none ? 0 : tiles.key(w0 + v + i);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int r = row0 + 8 * n + 2 * t + e, p = pos0 + r / a.group;
+                        const Span sp = span_of(a.mask, p, p, seq.len);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int j = key0 + g + 8 * h;
+                            if (none || !((j >= sp.lo && j < sp.hi) || j < sp.sink)) c[i][n][2 * h + e] = neg_inf();
+                        }
+                    }
+                }
+                // Values that no row of this block may see count as zero whatever they hold (0 times NaN is NaN).
+                auto seen = [&](int j) { return !none && ((j >= span.lo && j < span.hi) || j < span.sink); };
+                if constexpr (Q4) {
+                    if (!seen(key0 + g)) vt[i].s0 = 0u;
+                    if (!seen(key0 + g + 8)) vt[i].s1 = 0u;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (!seen(key0 + 2 * t + (k & 1) + 8 * (k >> 1))) vt[i].a[k] = vt[i].b[k] = make_uint4(0, 0, 0, 0);
+                }
+            }
+        }
+        // Streaming softmax: P against the reference the row has; exact maxima are taken only where there is none yet, or
+        // where a sum comes out above its guard (the reference cancels in O / l).  bf16: P itself must fit bf16 and the f32
+        // sums, 2^40.  4 bits: V's step goes into P (the zeros are summed apart), so that both operands of the product are
+        // exact but for P step, which is rounded to f16 and must fit it: 2^14; a reference bounds P step by 2^8, so that only
+        // what is 2^32 below the largest is lost at f16's lower end.
+        constexpr float kGuard = Q4 ? 16384.f : 1099511627776.f, kGuardP = 1.2676506e30f;  // 2^100
+        float p[SUB][NT][4], ps[SUB][NT][4], sum = 0.f, sum_s = 0.f;
+        auto weigh = [&vt, &p, &ps](int i, int n) {
             if constexpr (Q4) {
-                if (!seen(key0 + g)) vt.s0 = 0u;
-                if (!seen(key0 + g + 8)) vt.s1 = 0u;
+                const float s0 = lo_f(vt[i].s0), s1 = lo_f(vt[i].s1);
+                ps[i][n][0] = p[i][n][0] * s0;
+                ps[i][n][1] = p[i][n][1] * s0;
+                ps[i][n][2] = p[i][n][2] * s1;
+                ps[i][n][3] = p[i][n][3] * s1;
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (!seen(key0 + 2 * t + (i & 1) + 8 * (i >> 1))) vt.clear(i);
+                for (int e = 0; e < 4; e++) ps[i][n][e] = p[i][n][e];
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < SUB; i++) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) p[i][n][e] = fvp::ex2(fmaf(c[i][n][e], sl2[n][e & 1], -m[n][e & 1]));
+                weigh(i, n);
+                if (Q4) sum += (p[i][n][0] + p[i][n][1]) + (p[i][n][2] + p[i][n][3]);
+                sum_s += (ps[i][n][0] + ps[i][n][1]) + (ps[i][n][2] + ps[i][n][3]);
             }
         }
-        // Streaming softmax: P against the reference the row has; the exact maximum is taken only where there is none
-        // yet, or where a P comes out above 2^40 (bf16 and the f32 sums hold that; the reference cancels in O / l).
-        float p[NT][4];
-        bool trip = false;
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                p[n][e] = fvp::ex2(fmaf(c[n][e], a.sl2, -m[n][e & 1]));
-                trip |= !(p[n][e] <= 1099511627776.f);
-            }
-        }
-        if (__any_sync(kFullWarp, trip)) {
+        if (__any_sync(kFullWarp, !(sum_s <= kGuard) || (Q4 && !(sum <= kGuardP)))) {
 #pragma unroll
             for (int n = 0; n < NT; n++) {
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    float mx = fmaxf(c[n][e], c[n][2 + e]) * a.sl2;
+                    float mx = neg_inf();
+#pragma unroll
+                    for (int i = 0; i < SUB; i++) {
+                        const float t0 = c[i][n][e] * sl2[n][e], t1 = c[i][n][2 + e] * sl2[n][e];
+                        if constexpr (Q4) {  // (a key whose values are all equal has step 0)
+                            mx = fmaxf(mx, fmaxf(t0 + fmaxf(log2f(lo_f(vt[i].s0)), -60.f), t1 + fmaxf(log2f(lo_f(vt[i].s1)), -60.f)));
+                        } else {
+                            mx = fmaxf(mx, fmaxf(t0, t1));
+                        }
+                    }
                     mx = fmaxf(mx, __shfl_xor_sync(kFullWarp, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(kFullWarp, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(kFullWarp, mx, 16));
+                    if (Q4) mx -= 8.f;
                     if (mx > m[n][e]) {
                         const float f = fvp::ex2(m[n][e] - mx);  // 0 when there was no reference
                         m[n][e] = mx;
@@ -349,58 +471,63 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
                         }
                     }
                     const float ref = m[n][e] == neg_inf() ? 0.f : m[n][e];  // (a row that has seen nothing yet: P = 0)
-                    p[n][e] = fvp::ex2(fmaf(c[n][e], a.sl2, -ref));
-                    p[n][2 + e] = fvp::ex2(fmaf(c[n][2 + e], a.sl2, -ref));
+#pragma unroll
+                    for (int i = 0; i < SUB; i++) {
+                        p[i][n][e] = fvp::ex2(fmaf(c[i][n][e], sl2[n][e], -ref));
+                        p[i][n][2 + e] = fvp::ex2(fmaf(c[i][n][2 + e], sl2[n][e], -ref));
+                    }
                 }
+#pragma unroll
+                for (int i = 0; i < SUB; i++) weigh(i, n);
             }
         }
-        uint32_t pb[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            l[n][0] += p[n][0] + p[n][2];
-            l[n][1] += p[n][1] + p[n][3];
-            if constexpr (Q4) {  // sum P (zero + step (n - 8)): the step goes into P, the zeros are summed apart
-                const float s0 = lo_f(vt.s0), s1 = lo_f(vt.s1), z0 = hi_f(vt.s0), z1 = hi_f(vt.s1);
-                z[n][0] += p[n][0] * z0 + p[n][2] * z1;
-                z[n][1] += p[n][1] * z0 + p[n][3] * z1;
-                pb[n][0] = transpose8(fvp::pack_bf16x2(p[n][0] * s0, p[n][1] * s0));
-                pb[n][1] = transpose8(fvp::pack_bf16x2(p[n][2] * s1, p[n][3] * s1));
+        for (int i = 0; i < SUB; i++) {
+            uint32_t pb[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                l[n][0] += p[i][n][0] + p[i][n][2];
+                l[n][1] += p[i][n][1] + p[i][n][3];
+                if constexpr (Q4) {
+                    const float z0 = hi_f(vt[i].s0), z1 = hi_f(vt[i].s1);
+                    z[n][0] = fmaf(p[i][n][0], z0, fmaf(p[i][n][2], z1, z[n][0]));
+                    z[n][1] = fmaf(p[i][n][1], z0, fmaf(p[i][n][3], z1, z[n][1]));
+                }
+                pb[n][0] = transpose8(pack_p<Q4>(ps[i][n][0], ps[i][n][1]));
+                pb[n][1] = transpose8(pack_p<Q4>(ps[i][n][2], ps[i][n][3]));
+            }
+            // O^T += V^T . P^T: the pair of one d and two neighbouring keys comes out of two keys' words.
+            if constexpr (Q4) {
+                // Words of both keys' nibbles 0-3 (h = 0) and 4-7, key by key in the halves: codes_f16 would pair nibble k
+                // with k + 4 of one key's word; here the two halves are the two keys.
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t sel = h ? 0x7632 : 0x5410;
+                    uint32_t x0[4], x1[4], x2[4], x3[4];
+                    codes_f16(prmt(vt[i].a[0].x, vt[i].a[1].x, sel), x0);
+                    codes_f16(prmt(vt[i].a[0].y, vt[i].a[1].y, sel), x1);
+                    codes_f16(prmt(vt[i].a[2].x, vt[i].a[3].x, sel), x2);
+                    codes_f16(prmt(vt[i].a[2].y, vt[i].a[3].y, sel), x3);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+#pragma unroll
+                        for (int n = 0; n < NT; n++) mma<true>(o[n][4 * h + k], x0[k], x1[k], x2[k], x3[k], pb[n][0], pb[n][1]);
+                    }
+                }
             } else {
-                pb[n][0] = transpose8(fvp::pack_bf16x2(p[n][0], p[n][1]));
-                pb[n][1] = transpose8(fvp::pack_bf16x2(p[n][2], p[n][3]));
-            }
-        }
-        // O^T += V^T . P^T: the pair of one d and two neighbouring keys comes out of two keys' words.
-        if constexpr (Q4) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {  // the low and the high half of each word: its nibbles 4 h .. 4 h + 3
-                const uint32_t sel = h ? 0x7632 : 0x5410;
-                const uint32_t x0 = prmt(vt.a[0].x, vt.a[1].x, sel), x1 = prmt(vt.a[0].y, vt.a[1].y, sel);
-                const uint32_t x2 = prmt(vt.a[2].x, vt.a[3].x, sel), x3 = prmt(vt.a[2].y, vt.a[3].y, sel);
+                for (int k = 0; k < 8; k++) {
+                    const uint32_t sel = (k & 1) ? 0x7632 : 0x5410;
+                    const uint32_t a0 = prmt(word(vt[i].a[0], k / 2), word(vt[i].a[1], k / 2), sel);
+                    const uint32_t a1 = prmt(word(vt[i].b[0], k / 2), word(vt[i].b[1], k / 2), sel);
+                    const uint32_t a2 = prmt(word(vt[i].a[2], k / 2), word(vt[i].a[3], k / 2), sel);
+                    const uint32_t a3 = prmt(word(vt[i].b[2], k / 2), word(vt[i].b[3], k / 2), sel);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t a0 = sub136(codes128(x0, i)), a1 = sub136(codes128(x1, i));
-                    const uint32_t a2 = sub136(codes128(x2, i)), a3 = sub136(codes128(x3, i));
-#pragma unroll
-                    for (int n = 0; n < NT; n++) mma(o[n][4 * h + i], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+                    for (int n = 0; n < NT; n++) mma<false>(o[n][k], a0, a1, a2, a3, pb[n][0], pb[n][1]);
                 }
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const uint32_t sel = (i & 1) ? 0x7632 : 0x5410;
-                const uint32_t a0 = prmt(word(vt.a[0], i / 2), word(vt.a[1], i / 2), sel);
-                const uint32_t a1 = prmt(word(vt.b[0], i / 2), word(vt.b[1], i / 2), sel);
-                const uint32_t a2 = prmt(word(vt.a[2], i / 2), word(vt.a[3], i / 2), sel);
-                const uint32_t a3 = prmt(word(vt.b[2], i / 2), word(vt.b[3], i / 2), sel);
-#pragma unroll
-                for (int n = 0; n < NT; n++) mma(o[n][i], a0, a1, a2, a3, pb[n][0], pb[n][1]);
-            }
+            if (more) vt[i].load(lane_v, lane_vs, next_row[i]);
         }
-        if (un < u1) vt.load(a.pool, page_next, head, tiles.key(un), g, t);
-        u = un;
-        page = page_next;
-        page_next = page_after;
     }
 
     // The four warps' results side by side, then joined.
@@ -427,26 +554,67 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
     }
     __syncthreads();
     const int d = threadIdx.x;  // kAttnThreads == kD
-#pragma unroll
-    for (int r = 0; r < kRows; r++) {
-        if (r >= rows) break;
-        float top = sh_m[0][r];
+    auto out_row = [&](int r) { return (size_t)(seq.q0 + (row0 + r) / a.group) * a.heads + head * a.group + (row0 + r) % a.group; };
+    // Row r of this CTA: value d against the row's reference, and the sum of P.
+    auto join = [&](int r, float& top, float& sum) {
+        top = sh_m[0][r];
 #pragma unroll
         for (int w = 1; w < kWarps; w++) top = fmaxf(top, sh_m[w][r]);
-        float sum = 0.f, acc = 0.f;
+        float acc = 0.f;
+        sum = 0.f;
         if (top != neg_inf()) {
 #pragma unroll
             for (int w = 0; w < kWarps; w++) {
                 const float f = fvp::ex2(sh_m[w][r] - top);
-                sum += f * sh_l[w][r];
-                if (f != 0.f) acc += f * sh_o[w][r][d];
+                sum = fmaf(f, sh_l[w][r], sum);
+                if (f != 0.f) acc = fmaf(f, sh_o[w][r][d], acc);
             }
-            acc /= sum;
         }
-        const int rr = row0 + r;
-        const size_t oi = (size_t)(seq.q0 + rr / a.group) * a.heads + head * a.group + rr % a.group;
+        return acc;
+    };
+    if (a.cluster) {
+        // The key ranges of these rows are the CTAs of one cluster: each joins its own warps, then the rows are dealt to
+        // the CTAs, which read each other's parts over distributed shared memory, in the order of the ranges.
+        cg::cluster_group cluster = cg::this_cluster();
+        float part[kRows], tops[kRows], sums[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; r++) part[r] = r < rows ? join(r, tops[r], sums[r]) : 0.f;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kRows; r++) {
+            if (r >= rows) break;
+            sh_o[0][r][d] = part[r];
+            if (d == 0) {
+                sh_m[0][r] = tops[r];
+                sh_l[0][r] = sums[r];
+            }
+        }
+        cluster.sync();
+        for (int r = split; r < rows; r += a.splits) {
+            float top = neg_inf();
+            for (int i = 0; i < a.splits; i++) top = fmaxf(top, *cluster.map_shared_rank(&sh_m[0][r], i));
+            float acc = 0.f, sum = 0.f;
+            for (int i = 0; i < a.splits; i++) {
+                const float mi = *cluster.map_shared_rank(&sh_m[0][r], i);
+                const float f = mi == neg_inf() ? 0.f : fvp::ex2(mi - top);
+                if (f == 0.f) continue;
+                sum = fmaf(f, *cluster.map_shared_rank(&sh_l[0][r], i), sum);
+                acc = fmaf(f, *cluster.map_shared_rank(&sh_o[0][r][d], i), acc);
+            }
+            a.out[out_row(r) * kD + d] = (uint16_t)fvp::pack_bf16x2(top == neg_inf() ? 0.f : acc / sum, 0.f);
+        }
+        cluster.sync();  // (no CTA leaves while another one still reads its part)
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; r++) {
+        if (r >= rows) break;
+        float top, sum;
+        float acc = join(r, top, sum);
+        if (top != neg_inf()) acc /= sum;
+        const size_t oi = out_row(r);
         if (a.splits == 1) {
-            a.out[oi * kD + d] = (uint16_t)(fvp::pack_bf16x2(acc, 0.f));
+            a.out[oi * kD + d] = (uint16_t)fvp::pack_bf16x2(acc, 0.f);
         } else {
             const size_t pi = (size_t)split * a.batch.tokens * a.heads + oi;
             a.part_o[pi * kD + d] = acc;
@@ -503,6 +671,7 @@ fv_paged_chunk_kernel(const __grid_constant__ CUtensorMap mq, const __grid_const
 struct Shape {
     bool chunk;  // the tensor-core kernel for long chunks
     int splits, row_blocks, nt, tile_tokens;
+    bool cluster;
 };
 // How a call is cut.  Few rows per kv head: blocks of 8 or 16 rows, and the keys in `splits` ranges so that all SMs have
 // work.  From kChunkFrom rows on: items of 2 x 128 rows, the keys cut where that evens out the waves.
@@ -513,6 +682,7 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads,
     const long long rows = (long long)b->max_q * group;
     s.chunk = rows >= kChunkFrom && group <= kChunkRows;
     s.tile_tokens = s.chunk ? kChunkRows / group : 0;
+    s.cluster = false;
     if (s.chunk) {
         long long seen = b->max_kv;
         if (m.block > 0 && m.window > 0) {
@@ -545,10 +715,17 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads,
         keys = most < keys ? most : keys;
     }
     const long long ctas = (long long)b->seqs * kv->kv_heads * s.row_blocks;
-    const long long want = (6ll * sms + ctas - 1) / ctas;      // CTAs of about two waves of three per SM
-    const long long most = (keys + 4 * kTile * kWarps - 1) / (4 * kTile * kWarps);  // at least four tiles per warp
-    long long n = want < most ? want : most;
+    // Key ranges: as many as fill the SMs once; where the rows alone nearly do, three times over, so that ragged ends even
+    // out.  Up to kMaxCluster ranges are one cluster, which joins its parts itself; the merge kernel behind more of them takes
+    // about 5 us, so more need enough tiles a warp (0.75 us each) to be worth it.
+    const int resident = sms * (s.nt == 1 ? 3 : 2);  // CTAs that run at a time
+    const long long tiles = (keys + kTile - 1) / kTile, most = (tiles + 2 * kWarps - 1) / (2 * kWarps);  // at least two tiles per warp
+    long long n = resident / ctas;
+    if (n < 2) n = (3ll * resident + ctas - 1) / ctas;
+    if (n > kMaxCluster && (n < 12 || tiles < 16 * kWarps * kMaxCluster)) n = kMaxCluster;
+    n = n < most ? n : most;
     s.splits = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+    s.cluster = s.splits > 1 && s.splits <= kMaxCluster;
     return s;
 }
 
@@ -636,7 +813,7 @@ extern "C" size_t fv_paged_attn_workspace_bytes(const fv_paged_kv* kv, const fv_
         fvrt::sm_count(dev, &sms) != FV_RAN)
         return 0;
     const Shape s = shape_of(kv, b, heads, m, sms);
-    return s.splits > 1 ? (size_t)s.splits * tokens * heads * (kD + 1) * sizeof(float) : 0;
+    return s.splits > 1 && !s.cluster ? (size_t)s.splits * tokens * heads * (kD + 1) * sizeof(float) : 0;
 }
 
 extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* b, int tokens, const void* q, long long q_tok,
@@ -662,7 +839,7 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
     if (rc != FV_RAN) return rc;
     const Shape s = shape_of(kv, b, heads, a.mask, sms);
     const size_t rows = (size_t)tokens * heads;
-    if (s.splits > 1 && (!workspace || workspace_bytes < s.splits * rows * (kD + 1) * sizeof(float)))
+    if (s.splits > 1 && !s.cluster && (!workspace || workspace_bytes < s.splits * rows * (kD + 1) * sizeof(float)))
         return fvrt::fail(FV_ERR_INVALID, "paged attention: workspace of %zu bytes, %zu needed", workspace_bytes,
                           s.splits * rows * (kD + 1) * sizeof(float));
     a.q = (const uint16_t*)q;
@@ -675,6 +852,7 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
     a.group = heads / kv->kv_heads;
     a.splits = s.splits;
     a.row_blocks = s.row_blocks;
+    a.cluster = s.cluster;
     a.sl2 = scale * 1.4426950408889634f;
     const long long grid = (long long)b->seqs * kv->kv_heads * s.row_blocks * s.splits;
     if (grid > 0x7fffffffll || (long long)rows > 0x7fffffffll) return FV_DECLINED;
@@ -689,12 +867,20 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
         return FV_RAN;
     }
     const bool q4 = kv->format == FV_PAGE_Q4;
-    if (q4 && s.nt == 1) fv_paged_decode_kernel<true, 1><<<(unsigned)grid, kAttnThreads, 0, st>>>(a);
-    else if (q4) fv_paged_decode_kernel<true, 2><<<(unsigned)grid, kAttnThreads, 0, st>>>(a);
-    else if (s.nt == 1) fv_paged_decode_kernel<false, 1><<<(unsigned)grid, kAttnThreads, 0, st>>>(a);
-    else fv_paged_decode_kernel<false, 2><<<(unsigned)grid, kAttnThreads, 0, st>>>(a);
-    FV_CUDA(cudaGetLastError());
-    if (s.splits > 1) {
+    const auto fn = q4 ? (s.nt == 1 ? fv_paged_decode_kernel<true, 1> : fv_paged_decode_kernel<true, 2>)
+                       : (s.nt == 1 ? fv_paged_decode_kernel<false, 1> : fv_paged_decode_kernel<false, 2>);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kAttnThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)s.splits;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = s.cluster ? 1 : 0;
+    FV_CUDA(cudaLaunchKernelEx(&cfg, fn, a));
+    if (s.splits > 1 && !s.cluster) {
         fv_paged_merge_kernel<<<(unsigned)((rows + kWarps - 1) / kWarps), kAttnThreads, 0, st>>>(a);
         FV_CUDA(cudaGetLastError());
     }

@@ -10,8 +10,9 @@
 // the f32 rotation, not from its bf16 rounding.  One scale for the whole row because its factor then leaves the
 // attention's products (q . k = step (q . code) + zero sum(q)), so that these run on exact codes.
 //
-// HBM-bound: 8 lanes hold one row of one head (16 values a lane: 8 from each half, so both kinds of pairs are inside a
-// lane), a CTA works on one token and keeps its cosines and sines in registers over the heads it takes.
+// HBM-bound: 8 lanes hold one row of one head (16 values a lane), a warp the same head of 4 neighbouring tokens, a CTA
+// of 16: their rows lie side by side in a page, each lane keeps its token's cosines and sines in registers over all heads,
+// and q's, K's and V's heads are loops of their own without a branch inside, four rows in flight per lane.
 #include "fv_runtime.h"
 #include "paged.cuh"
 #include "paged_host.h"
@@ -19,7 +20,7 @@
 namespace fvpg {
 
 constexpr int kThreads = 128;
-constexpr int kRowsAtOnce = kThreads / 8;  // rows (of one head each) that a CTA has in hand at a time
+constexpr int kTokens = kThreads / 8;  // of a CTA
 
 struct AppendArgs {
     Pool pool;
@@ -29,7 +30,7 @@ struct AppendArgs {
     long long q_tok, q_head, k_tok, k_head, v_tok, v_head;  // strides in values
     const float *cosv, *sinv;
     const int* positions;
-    int table_rows, q_heads, parts, half;
+    int table_rows, q_heads, parts;
 };
 
 FV_DEV void widen8(const uint4 u, float* x) {
@@ -58,19 +59,38 @@ FV_DEV float max_nan(float a, float b) {
     return r;
 }
 
+// seq_of_token for the warp's four tokens (one per 8 lanes) at once.
+FV_DEV int seq_of_slot(const int* cu, int seqs, int t, int lane) {
+    int s = 0;
+    for (int base = 0; base < seqs; base += 32) {
+        const int end = base + lane < seqs ? __ldg(cu + base + lane + 1) : 0x7fffffff;
+        bool more = false;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int n = __popc(__ballot_sync(kFullWarp, end <= __shfl_sync(kFullWarp, t, 8 * k)));
+            if ((lane >> 3) == k) s += n;
+            more |= n == 32;
+        }
+        if (!more) break;
+    }
+    return s;
+}
+
 // x[0 .. 7] are values 8 c .. 8 c + 7 of a row, x[8 .. 15] are 64 values further on; cs / sn the factors of its 8 pairs.
-FV_DEV void rotate16(float (&x)[16], const float (&cs)[8], const float (&sn)[8], bool half) {
+template <bool HALF>
+FV_DEV void rotate16(float (&x)[16], const float (&cs)[8], const float (&sn)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const int a = half ? i : 2 * i, b = half ? i + 8 : 2 * i + 1;
+        const int a = HALF ? i : 2 * i, b = HALF ? i + 8 : 2 * i + 1;
         const float xa = x[a], xb = x[b];
         x[a] = __fsub_rn(__fmul_rn(xa, cs[i]), __fmul_rn(xb, sn[i]));
         x[b] = __fadd_rn(__fmul_rn(xa, sn[i]), __fmul_rn(xb, cs[i]));
     }
 }
 // The same row in 4 bits: codes of this lane's 16 values as two words (8 values each), (step, zero) as one.  Collective
-// over the row's 8 lanes (the callers' lanes of a row are live or not together).
-FV_DEV void quantize16(const float (&x)[16], uint32_t& lo, uint32_t& hi, uint32_t& scale, uint32_t lanes) {
+// over the warp.  (A row of one value has step 0 and codes 0.  A row with a value that is not finite has a step that is
+// not: its codes say nothing, the row stands for NaN.)
+FV_DEV void quantize16(const float (&x)[16], uint32_t& lo, uint32_t& hi, uint32_t& scale) {
     float mn = x[0], mx = x[0];
 #pragma unroll
     for (int i = 1; i < 16; i++) {
@@ -79,38 +99,83 @@ FV_DEV void quantize16(const float (&x)[16], uint32_t& lo, uint32_t& hi, uint32_
     }
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) {
-        mn = min_nan(mn, __shfl_xor_sync(lanes, mn, d));
-        mx = max_nan(mx, __shfl_xor_sync(lanes, mx, d));
+        mn = min_nan(mn, __shfl_xor_sync(kFullWarp, mn, d));
+        mx = max_nan(mx, __shfl_xor_sync(kFullWarp, mx, d));
     }
     const float step = bf16_of(__fdiv_rn(__fsub_rn(mx, mn), 15.f));
     const float zero = bf16_of(__fadd_rn(mn, __fmul_rn(8.f, step)));
     scale = fvp::pack_bf16x2(step, zero);
-    lo = hi = 0;
+    lo = hi = 0x88888888u;
+    if (!(step > 0.f)) return;
+    // A quotient by the reciprocal is off by a few units in the last place, which moves a code only where it lies at the
+    // middle between two: a lane that meets such a value (one in 10^4 lanes on ordinary data; a reciprocal that overflows is
+    // caught as well) takes true divisions.  Rounding to the nearest even code is the addition of 1.5 2^23 + 8, whose sum
+    // carries code + 8 in its lowest bits.
+    constexpr float kRound = 12582912.f + 8.f;
+    const float inv = __frcp_rn(step);
+    bool middle = !(inv <= 3e38f);
+    uint32_t n[16];
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-        // (a row of one value has step 0: code 0.  A row with a value that is not finite has a step that is not: its
-        // codes say nothing, the row stands for NaN.)
-        float c = step > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[i], zero), step)) : 0.f;
-        c = fminf(fmaxf(c, -8.f), 7.f);
-        const uint32_t n = (uint32_t)((int)c + 8) & 15u;
-        if (i < 8) lo |= n << (4 * i);
-        else hi |= n << (4 * (i - 8));
+        const float raw = __fmul_rn(__fsub_rn(x[i], zero), inv);
+        const float c = fminf(fmaxf(raw, -8.f), 7.f);
+        const float t = __fadd_rn(c, kRound);
+        middle |= !(fabsf(__fsub_rn(c, __fsub_rn(t, kRound))) <= 0.49998f) || raw != raw;
+        n[i] = __float_as_uint(t) & 15u;
+    }
+    if (middle) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], zero), step)), -8.f), 7.f);
+            n[i] = (uint32_t)((int)c + 8) & 15u;
+        }
+    }
+    lo = hi = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        lo |= n[i] << (4 * i);
+        hi |= n[8 + i] << (4 * i);
     }
 }
 
-template <bool Q4>
+// Rows of `count` heads from head `first` on, UNROLL at a time: raw bits in, `use(head, u0, u1)` gets 16 values.
+template <int UNROLL, class Use>
+FV_DEV void for_heads(const uint16_t* src, long long stride, int first, int last, const Use& use) {
+    int h = first;
+    for (; h + UNROLL <= last; h += UNROLL) {
+        uint4 u[UNROLL][2];
+#pragma unroll
+        for (int i = 0; i < UNROLL; i++) {
+            const uint4* p = reinterpret_cast<const uint4*>(src + (long long)(h + i) * stride);
+            u[i][0] = __ldg(p);
+            u[i][1] = __ldg(p + 8);
+        }
+#pragma unroll
+        for (int i = 0; i < UNROLL; i++) use(h + i, u[i][0], u[i][1]);
+    }
+    for (; h < last; h++) {
+        const uint4* p = reinterpret_cast<const uint4*>(src + (long long)h * stride);
+        use(h, __ldg(p), __ldg(p + 8));
+    }
+}
+
+template <bool Q4, bool HALF>
 __global__ void __launch_bounds__(kThreads) fv_paged_append_kernel(const AppendArgs a) {
-    const int lane = threadIdx.x & 31, part = threadIdx.x & 7, slot = threadIdx.x >> 3;
-    const uint32_t lanes = 0xffu << (lane & 24);
-    const int t = blockIdx.x / a.parts, block = blockIdx.x - t * a.parts;
-    const int s = seq_of_token(a.batch.cu_q, a.batch.seqs, t, lane);
-    if (s >= a.batch.seqs) return;  // behind the last sequence
-    const Seq seq = seq_of(a.batch, s);
-    const int at = t - seq.q0;
-    if (at < 0 || at >= seq.nq) return;
-    const int key = seq.len - seq.nq + at;  // the token's index in its sequence
-    int page = -1;
-    if (key >= 0) page = page_of(a.pool, a.batch, s, key);
+    const int lane = threadIdx.x & 31, part = threadIdx.x & 7;
+    const int block = blockIdx.x / a.parts, share = blockIdx.x - block * a.parts;
+    const int t = min(block * kTokens + (int)(threadIdx.x >> 3), a.batch.tokens - 1);  // (a lane past the end repeats the last
+    bool mine = block * kTokens + (int)(threadIdx.x >> 3) < a.batch.tokens;            // token's loads and stores nothing)
+    const int s = seq_of_slot(a.batch.cu_q, a.batch.seqs, t, lane);
+    int key = -1, page = -1;
+    if (mine && s < a.batch.seqs) {
+        const Seq seq = seq_of(a.batch, s);
+        const int at = t - seq.q0;
+        mine = at >= 0 && at < seq.nq;
+        key = mine ? seq.len - seq.nq + at : -1;  // the token's index in its sequence
+        if (key >= 0) page = page_of(a.pool, a.batch, s, key);
+    } else {
+        mine = false;  // behind the last sequence
+    }
     const bool turn = a.cosv != nullptr;
     bool placed = key >= 0;
     float cs[8], sn[8];
@@ -121,7 +186,7 @@ __global__ void __launch_bounds__(kThreads) fv_paged_append_kernel(const AppendA
             placed = false;
         }
         const size_t row = (size_t)(placed ? pos : 0) * kD;
-        if (a.half) {  // pairs (i, i + 64): this lane's are 8 part .. 8 part + 7
+        if (HALF) {  // pairs (i, i + 64): this lane's are 8 part .. 8 part + 7
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const float4 c = __ldg(reinterpret_cast<const float4*>(a.cosv + row + 8 * part) + i);
@@ -140,48 +205,67 @@ __global__ void __launch_bounds__(kThreads) fv_paged_append_kernel(const AppendA
             }
         }
     }
-    // Rows of this token: q's heads, then K's, then V's; dealt to the parts in runs of kRowsAtOnce.
+    // This CTA's share of the token's rows: q's heads, then K's, then V's.
     const int hk = a.pool.kv_heads, rows = a.q_heads + 2 * hk;
-    for (int r = block * kRowsAtOnce + slot; r < rows; r += a.parts * kRowsAtOnce) {
-        const bool is_q = r < a.q_heads, is_k = !is_q && r < a.q_heads + hk;
-        const int head = is_q ? r : is_k ? r - a.q_heads : r - a.q_heads - hk;
-        if (!is_q && page < 0) continue;
-        const uint16_t* src = is_q ? a.q + t * a.q_tok + head * a.q_head : is_k ? a.k + t * a.k_tok + head * a.k_head
-                                                                                : a.v + t * a.v_tok + head * a.v_head;
-        const uint4 u0 = *reinterpret_cast<const uint4*>(src + 8 * part), u1 = *reinterpret_cast<const uint4*>(src + 64 + 8 * part);
-        float x[16];
-        widen8(u0, x);
-        widen8(u1, x + 8);
-        if (turn && (is_q || is_k)) rotate16(x, cs, sn, a.half);
-        if (is_q) {
-            uint16_t* o = a.q_out + ((size_t)t * a.q_heads + head) * kD + 8 * part;
-            if (!placed) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[i] = 0.f;
+    const int r0 = (int)((long long)rows * share / a.parts), r1 = (int)((long long)rows * (share + 1) / a.parts);
+    auto clip = [](int r, int n) { return min(max(r, 0), n); };
+    for_heads<4>(a.q + t * a.q_tok + 8 * part, a.q_head, clip(r0, a.q_heads), clip(r1, a.q_heads), [&](int h, uint4 u0, uint4 u1) {
+        if (!mine) return;
+        if (!placed) {
+            u0 = u1 = make_uint4(0, 0, 0, 0);
+        } else if (turn) {
+            float x[16];
+            widen8(u0, x);
+            widen8(u1, x + 8);
+            rotate16<HALF>(x, cs, sn);
+            u0 = narrow8(x);
+            u1 = narrow8(x + 8);
+        }
+        uint4* o = reinterpret_cast<uint4*>(a.q_out + ((size_t)t * a.q_heads + h) * kD + 8 * part);
+        o[0] = u0;
+        o[8] = u1;
+    });
+    const bool store = placed && page >= 0;
+    const size_t first = store ? pool_row(a.pool, page, 0, key) : 0;  // head h: h << log_rows rows further on
+    auto put = [&](const uint8_t* pool, const uint32_t* scales, bool rotated) {
+        return [=, &cs, &sn](int h, uint4 u0, uint4 u1) {
+            const size_t row = first + ((size_t)h << a.pool.log_rows);
+            if (Q4 || rotated) {
+                float x[16];
+                widen8(u0, x);
+                widen8(u1, x + 8);
+                if (rotated) rotate16<HALF>(x, cs, sn);
+                if (Q4) {
+                    uint32_t lo, hi, scale;
+                    quantize16(x, lo, hi, scale);
+                    if (!store) return;
+                    uint32_t* o = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(pool) + row * kQ4Bytes);
+                    o[part] = lo;
+                    o[8 + part] = hi;
+                    if (part == 0) const_cast<uint32_t*>(scales)[row] = scale;
+                    return;
+                }
+                u0 = narrow8(x);
+                u1 = narrow8(x + 8);
             }
-            *reinterpret_cast<uint4*>(o) = narrow8(x);
-            *reinterpret_cast<uint4*>(o + 64) = narrow8(x + 8);
-            continue;
-        }
-        if (!placed) continue;
-        const size_t row = pool_row(a.pool, page, head, key);
-        uint8_t* base = const_cast<uint8_t*>(is_k ? a.pool.k : a.pool.v);
-        if (Q4) {
-            uint32_t lo, hi, scale;
-            quantize16(x, lo, hi, scale, lanes);
-            *reinterpret_cast<uint32_t*>(base + row * kQ4Bytes + 4 * part) = lo;
-            *reinterpret_cast<uint32_t*>(base + row * kQ4Bytes + 32 + 4 * part) = hi;
-            if (part == 0) const_cast<uint32_t*>(is_k ? a.pool.k_scale : a.pool.v_scale)[row] = scale;
-        } else {
-            uint16_t* o = reinterpret_cast<uint16_t*>(base) + row * kD + 8 * part;
-            *reinterpret_cast<uint4*>(o) = narrow8(x);
-            *reinterpret_cast<uint4*>(o + 64) = narrow8(x + 8);
-        }
-    }
+            if (!store) return;
+            uint4* o = reinterpret_cast<uint4*>(const_cast<uint8_t*>(pool) + row * (2 * kD)) + part;
+            o[0] = u0;
+            o[8] = u1;
+        };
+    };
+    const int k0 = clip(r0 - a.q_heads, hk), k1 = clip(r1 - a.q_heads, hk);
+    if (turn) for_heads<Q4 ? 2 : 4>(a.k + t * a.k_tok + 8 * part, a.k_head, k0, k1, put(a.pool.k, a.pool.k_scale, true));
+    else for_heads<Q4 ? 2 : 4>(a.k + t * a.k_tok + 8 * part, a.k_head, k0, k1, put(a.pool.k, a.pool.k_scale, false));
+    for_heads<Q4 ? 2 : 4>(a.v + t * a.v_tok + 8 * part, a.v_head, clip(r0 - a.q_heads - hk, hk), clip(r1 - a.q_heads - hk, hk),
+                          put(a.pool.v, a.pool.v_scale, false));
 }
 
 // Read: row r of the packed result is key first[s] + (r - cu_rows[s]) of sequence s, K and V, as bf16 (4-bit rows as the
 // values they stand for, rounded once).  Keys that the sequence does not hold and rows behind the last one give zeros.
+// The append's split: 8 lanes a row, a CTA 16 neighbouring rows of its share of the heads.  (Lane i holds values 8 i .. 8 i + 7 and
+// 64 + 8 i ..: with 16 values side by side its two stores would each fill half of a 32-byte sector, 60 against 45 us for
+// 32 760 rows x 12 heads of 4 bits.)
 struct ReadArgs {
     Pool pool;
     Batch batch;
@@ -190,11 +274,29 @@ struct ReadArgs {
     int rows, parts;
 };
 
+// 8 codes as bf16 values zero + step code: 128 + n by or-ing the code into 128's mantissa, 136 off is code exactly, and
+// one fused multiply-add rounds once.
+FV_DEV uint4 expand8(uint32_t w, uint32_t step2, uint32_t zero2) {
+    const uint32_t odd = w >> 4;
+    uint32_t h[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t pair = __byte_perm(w, odd, (uint32_t)(k | (k << 4) | ((4 + k) << 8) | ((4 + k) << 12)));
+        uint32_t c = (pair & 0x000f000fu) | 0x43004300u;
+        asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(c) : "r"(0xc308c308u));
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(h[k]) : "r"(c), "r"(step2), "r"(zero2));
+    }
+    return make_uint4(h[0], h[1], h[2], h[3]);
+}
+
 template <bool Q4>
 __global__ void __launch_bounds__(kThreads) fv_paged_read_kernel(const ReadArgs a) {
-    const int lane = threadIdx.x & 31, part = threadIdx.x & 7, slot = threadIdx.x >> 3;
-    const int t = blockIdx.x / a.parts, block = blockIdx.x - t * a.parts;
-    const int s = seq_of_token(a.cu_rows, a.batch.seqs, t, lane);
+    constexpr int UNROLL = 4;
+    const int lane = threadIdx.x & 31, part = threadIdx.x & 7;
+    const int block = blockIdx.x / a.parts, share = blockIdx.x - block * a.parts;
+    const int t = block * kTokens + (int)(threadIdx.x >> 3);
+    const int s = seq_of_slot(a.cu_rows, a.batch.seqs, min(t, a.rows - 1), lane);
+    if (t >= a.rows) return;
     long long key = -1;
     int page = -1;
     if (s < a.batch.seqs) {
@@ -207,35 +309,43 @@ __global__ void __launch_bounds__(kThreads) fv_paged_read_kernel(const ReadArgs 
         }
     }
     const int hk = a.pool.kv_heads;
-    for (int r = block * kRowsAtOnce + slot; r < 2 * hk; r += a.parts * kRowsAtOnce) {
-        const bool is_k = r < hk;
-        const int head = is_k ? r : r - hk;
-        uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
-        if (page >= 0) {
-            const size_t row = pool_row(a.pool, page, head, (int)key);
+    const size_t first = page >= 0 ? pool_row(a.pool, page, 0, (int)key) : 0;
+    const int r0 = (int)((long long)2 * hk * share / a.parts), r1 = (int)((long long)2 * hk * (share + 1) / a.parts);
+    for (int r = r0; r < r1; r += UNROLL) {
+        uint4 u[UNROLL][2];
+        uint32_t sc[UNROLL];
+#pragma unroll
+        for (int i = 0; i < UNROLL; i++) {
+            u[i][0] = u[i][1] = make_uint4(0, 0, 0, 0);
+            sc[i] = 0;
+            if (r + i >= r1 || page < 0) continue;
+            const bool is_k = r + i < hk;
+            const size_t row = first + ((size_t)(is_k ? r + i : r + i - hk) << a.pool.log_rows);
             const uint8_t* base = is_k ? a.pool.k : a.pool.v;
             if (Q4) {
-                const uint32_t sc = __ldg((is_k ? a.pool.k_scale : a.pool.v_scale) + row);
-                const uint32_t lo = __ldg(reinterpret_cast<const uint32_t*>(base + row * kQ4Bytes + 4 * part));
-                const uint32_t hi = __ldg(reinterpret_cast<const uint32_t*>(base + row * kQ4Bytes + 32 + 4 * part));
-                const float step = __uint_as_float(sc << 16), zero = __uint_as_float(sc & 0xffff0000u);
-                float x[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) {  // (step * code is exact in f32: 8 bits by 4)
-                    const uint32_t n = ((i < 8 ? lo >> (4 * i) : hi >> (4 * (i - 8))) & 15u);
-                    x[i] = fmaf(step, (float)((int)n - 8), zero);
-                }
-                u0 = narrow8(x);
-                u1 = narrow8(x + 8);
+                const uint32_t* p = reinterpret_cast<const uint32_t*>(base + row * kQ4Bytes) + part;
+                u[i][0].x = __ldg(p);
+                u[i][0].y = __ldg(p + 8);
+                sc[i] = __ldg((is_k ? a.pool.k_scale : a.pool.v_scale) + row);
             } else {
-                const uint4* p = reinterpret_cast<const uint4*>(base + row * 2 * kD);
-                u0 = __ldg(p + part);
-                u1 = __ldg(p + 8 + part);
+                const uint4* p = reinterpret_cast<const uint4*>(base + row * (2 * kD)) + part;
+                u[i][0] = __ldg(p);
+                u[i][1] = __ldg(p + 8);
             }
         }
-        uint16_t* o = (is_k ? a.k_out : a.v_out) + ((size_t)t * hk + head) * kD + 8 * part;
-        *reinterpret_cast<uint4*>(o) = u0;
-        *reinterpret_cast<uint4*>(o + 64) = u1;
+#pragma unroll
+        for (int i = 0; i < UNROLL; i++) {
+            if (r + i >= r1) continue;
+            if (Q4 && page >= 0) {
+                const uint32_t step2 = __byte_perm(sc[i], 0, 0x1010), zero2 = __byte_perm(sc[i], 0, 0x3232);
+                u[i][1] = expand8(u[i][0].y, step2, zero2);
+                u[i][0] = expand8(u[i][0].x, step2, zero2);
+            }
+            const bool is_k = r + i < hk;
+            uint4* o = reinterpret_cast<uint4*>((is_k ? a.k_out : a.v_out) + ((size_t)t * hk + (is_k ? r + i : r + i - hk)) * kD) + part;
+            o[0] = u[i][0];
+            o[8] = u[i][1];
+        }
     }
 }
 
@@ -253,6 +363,8 @@ int check_paged(const char* what, const fv_paged_kv* kv, const fv_paged_batch* b
     if ((long long)b->table_width * kv->page_rows < b->max_kv)
         return fvrt::fail(FV_ERR_INVALID, "%s: a table of %d pages of %d rows does not hold %d keys", what, b->table_width, kv->page_rows, b->max_kv);
     if (b->max_kv > 0x3fffffff) return fvrt::fail(FV_ERR_INVALID, "%s: sequences of %d keys", what, b->max_kv);
+    if ((long long)kv->pages * kv->kv_heads * kv->page_rows > 0xfffffff0ll)  // (the kernels number the pool's rows in 32 bits)
+        return fvrt::fail(FV_ERR_INVALID, "%s: a pool of %d pages x %d heads x %d rows", what, kv->pages, kv->kv_heads, kv->page_rows);
     if (b->seqs == 0 || rows == 0) return FV_DECLINED;
     const int rc = fvrt::require_sm100(dev);
     if (rc != FV_RAN) return rc;
@@ -276,12 +388,12 @@ int check_paged(const char* what, const fv_paged_kv* kv, const fv_paged_batch* b
     return FV_RAN;
 }
 
-// CTAs per token: as many as keep the GPU busy when there are few tokens, as few as possible (one reads the tables'
-// row once for all heads) when there are many.
+// CTAs that share the heads of the same 16 tokens: as many as keep the GPU busy when there are few tokens, as few as
+// possible (one reads the tables' rows once for all heads) when there are many.
 static int parts_for(int tokens, int rows, int sms) {
-    const int most = (rows + kRowsAtOnce - 1) / kRowsAtOnce;
-    const long long want = (16ll * sms + tokens - 1) / tokens;
-    return (int)(want < 1 ? 1 : want > most ? most : want);
+    const int blocks = (tokens + kTokens - 1) / kTokens;
+    const long long want = (8ll * sms + blocks - 1) / blocks;
+    return (int)(want < 1 ? 1 : want > rows ? rows : want);
 }
 
 }  // namespace fvpg
@@ -317,17 +429,18 @@ extern "C" int fv_paged_append_bf16(void* stream, const fv_paged_kv* kv, const f
     a.positions = positions;
     a.table_rows = table_rows;
     a.q_heads = q ? q_heads : 0;
-    a.half = pairing == FV_ROPE_HALF;
     int sms;
     const int rc2 = fvrt::sm_count(dev, &sms);
     if (rc2 != FV_RAN) return rc2;
     a.parts = parts_for(tokens, a.q_heads + 2 * kv->kv_heads, sms);
-    const long long grid = (long long)tokens * a.parts;
+    const long long grid = (((long long)tokens + kTokens - 1) / kTokens) * a.parts;
     if (grid > 0x7fffffffll) return FV_DECLINED;
-    if (kv->format == FV_PAGE_Q4) fv_paged_append_kernel<true><<<(unsigned)grid, kThreads, 0, (cudaStream_t)stream>>>(a);
-    else fv_paged_append_kernel<false><<<(unsigned)grid, kThreads, 0, (cudaStream_t)stream>>>(a);
+    const bool q4 = kv->format == FV_PAGE_Q4, half = pairing == FV_ROPE_HALF;
+    const auto fn = q4 ? (half ? fv_paged_append_kernel<true, true> : fv_paged_append_kernel<true, false>)
+                       : (half ? fv_paged_append_kernel<false, true> : fv_paged_append_kernel<false, false>);
+    fn<<<(unsigned)grid, kThreads, 0, (cudaStream_t)stream>>>(a);
     FV_CUDA(cudaGetLastError());
-    fvrt::ran(fvrt::kLogPaged, "paged append: fv_paged_append_kernel<%s> %d tokens x (%d + 2 x %d) heads", kv->format == FV_PAGE_Q4 ? "4 bits" : "bf16",
+    fvrt::ran(fvrt::kLogPaged, "paged append: fv_paged_append_kernel<%s> %d tokens x (%d + 2 x %d) heads", q4 ? "4 bits" : "bf16",
               tokens, a.q_heads, kv->kv_heads);
     return FV_RAN;
 }
@@ -352,7 +465,7 @@ extern "C" int fv_paged_read_bf16(void* stream, const fv_paged_kv* kv, const fv_
     const int rc2 = fvrt::sm_count(dev, &sms);
     if (rc2 != FV_RAN) return rc2;
     a.parts = parts_for(rows, 2 * kv->kv_heads, sms);
-    const long long grid = (long long)rows * a.parts;
+    const long long grid = (((long long)rows + kTokens - 1) / kTokens) * a.parts;
     if (grid > 0x7fffffffll) return FV_DECLINED;
     if (kv->format == FV_PAGE_Q4) fv_paged_read_kernel<true><<<(unsigned)grid, kThreads, 0, (cudaStream_t)stream>>>(a);
     else fv_paged_read_kernel<false><<<(unsigned)grid, kThreads, 0, (cudaStream_t)stream>>>(a);

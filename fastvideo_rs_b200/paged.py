@@ -31,6 +31,8 @@ class _BatchC(ctypes.Structure):
                 ("max_q", _int), ("max_kv", _int)]
 
 
+# (the handle of the current stream without building a Stream object around it, where torch offers that)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _fns = None
 
 
@@ -83,7 +85,7 @@ class PagedKv:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.format = "q4" if q4 else "bf16"
         self.pages, self.kv_heads, self.page_rows = k.shape[:3]
-        self.device = k.device
+        self.device, self.index = k.device, k.get_device()
         ptr = lambda t: t.data_ptr() if t is not None else None
         self._c = _KvC(ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), int(q4), self.pages, self.page_rows, self.kv_heads)
         self._ref = ctypes.addressof(self._c)
@@ -116,24 +118,45 @@ class PagedBatch:
         self.cu_q = _index("PagedBatch: cu_q", cu_q, (seqs + 1,), dev)
         if max_q < 0 or max_kv < 0:
             raise ValueError("PagedBatch: max_q and max_kv must not be negative")
-        self.seqs, self.max_q, self.max_kv, self.device = seqs, int(max_q), int(max_kv), dev
+        self.seqs, self.max_q, self.max_kv, self.device, self.index = seqs, int(max_q), int(max_kv), dev, page_table.get_device()
+        self._need = {}  # scratch bytes of a token by how the call is cut: a decode step asks for every layer
         self._c = _BatchC(page_table.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), seqs, width, self.max_q, self.max_kv)
         self._ref = ctypes.addressof(self._c)
 
 
-def _heads_in(name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int], device) -> None:
-    if not t.is_cuda or t.device != device:
-        raise ValueError(f"{name} must be a CUDA tensor on {device}: this package has no CPU path")
-    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[2] != D or (t.stride(2) != 1 and t.numel() > 0):
+_bf16, _f32, _SCALE = torch.bfloat16, torch.float32, D ** -0.5
+
+
+def _heads_in(name: str, t: torch.Tensor, tokens: int, heads: int, index: int) -> None:
+    """t is bf16 [tokens, heads, 128] on device `index` (-1: any number of tokens or heads)."""
+    shape = t.shape
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be a CUDA tensor on cuda:{index}: this package has no CPU path")
+    if t.dtype != _bf16 or len(shape) != 3 or shape[2] != D or (t.stride(2) != 1 and t.numel() > 0):
         raise ValueError(f"{name} must be bfloat16 [tokens, heads, 128] with adjacent values")
-    if (tokens is not None and t.shape[0] != tokens) or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} is {list(t.shape)}: {tokens} tokens of {heads} heads are wanted")
+    if (tokens >= 0 and shape[0] != tokens) or (heads >= 0 and shape[1] != heads):
+        raise ValueError(f"{name} is {list(shape)}: {tokens} tokens of {heads} heads are wanted")
 
 
-def _on(kv: PagedKv, batch: PagedBatch):
-    if kv.device != batch.device:
-        raise ValueError(f"the cache is on {kv.device}, the batch on {batch.device}")
-    return torch.cuda.device(kv.device)
+def _strides(t: torch.Tensor) -> Tuple[int, int]:
+    """Strides of tokens and heads; those of an extent of one mean nothing and count as a row's."""
+    a, b, _ = t.stride()
+    n, h, _ = t.shape
+    return (a if n > 1 else D), (b if h > 1 else D)
+
+
+def _call(kv: PagedKv, batch: PagedBatch, what: str, fn, *args) -> None:
+    """One C entry on the current stream of the cache's device."""
+    index = kv.index
+    if batch.index != index:
+        raise ValueError(f"the cache is on cuda:{index}, the batch on cuda:{batch.index}")
+    if torch.cuda.current_device() == index:
+        rc = fn(_raw_stream(index), kv._ref, batch._ref, *args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(_raw_stream(index), kv._ref, batch._ref, *args)
+    if rc:
+        _lib.check(rc, what)
 
 
 def append(kv: PagedKv, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, *, q: Optional[torch.Tensor] = None,
@@ -144,44 +167,45 @@ def append(kv: PagedKv, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, *, 
     given: token t with row positions[t] (int32), by default its position in its sequence.  pairing "interleaved": values
     2 i and 2 i + 1 (the tables of wan.wan_rope_tables), "half": values i and i + 64.  q [tokens, heads, 128], if given, is
     rotated too and returned as [tokens, heads, 128].  Two tokens of a call must not fall on the same cache row."""
-    tokens = k.shape[0]
-    _heads_in("append: k", k, None, kv.kv_heads, kv.device)
-    _heads_in("append: v", v, tokens, kv.kv_heads, kv.device)
-    if (cos is None) != (sin is None) or (positions is not None and cos is None):
-        raise ValueError("append: cos, sin and positions go together")
+    tokens, index = k.shape[0], kv.index
+    _heads_in("append: k", k, -1, kv.kv_heads, index)
+    _heads_in("append: v", v, tokens, kv.kv_heads, index)
     if pairing not in PAIRINGS:
         raise ValueError(f"append: unknown pairing {pairing!r} {tuple(PAIRINGS)}")
+    cp = sp = pp = None
     rows = 0
-    if cos is not None:
+    if cos is not None and sin is not None:
         rows = cos.shape[0]
         for name, t in (("cos", cos), ("sin", sin)):
-            if t.dtype != torch.float32 or not t.is_cuda or t.device != kv.device or not t.is_contiguous() or tuple(t.shape) != (rows, D):
-                raise ValueError(f"append: {name} must be a contiguous CUDA float32 [rows, 128] tensor")
+            if t.dtype != _f32 or t.get_device() != index or not t.is_contiguous() or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != D:
+                raise ValueError(f"append: {name} must be a contiguous CUDA float32 [rows, 128] tensor on cuda:{index}")
+        cp, sp = cos.data_ptr(), sin.data_ptr()
         if positions is not None:
-            _index("append: positions", positions, (tokens,), kv.device)
+            pp = _index("append: positions", positions, (tokens,), kv.device).data_ptr()
+    elif cos is not None or sin is not None or positions is not None:
+        raise ValueError("append: cos, sin and positions go together")
     heads = qt = qh = 0
+    qp = op = None
     if q is not None:
-        _heads_in("append: q", q, tokens, None, kv.device)
-        heads, qt, qh = q.shape[1], q.stride(0), q.stride(1)
+        _heads_in("append: q", q, tokens, -1, index)
+        heads, qp, (qt, qh) = q.shape[1], q.data_ptr(), _strides(q)
         if q_out is None:
-            q_out = torch.empty((tokens, heads, D), dtype=torch.bfloat16, device=kv.device)
+            q_out = q.new_empty((tokens, heads, D))
         else:
-            _heads_in("append: q_out", q_out, tokens, heads, kv.device)
+            _heads_in("append: q_out", q_out, tokens, heads, index)
             if not q_out.is_contiguous():
                 raise ValueError("append: q_out must be contiguous")
+        op = q_out.data_ptr()
+        if heads == 0:
+            qp = op = None
     elif q_out is not None:
         raise ValueError("append: q_out without q")
-    if tokens == 0 or batch.seqs == 0 or batch.max_q == 0 or heads + kv.kv_heads == 0:
+    if tokens == 0 or batch.seqs == 0 or batch.max_q == 0:
         return q_out
-    fn = _entries()[0]
-    with _on(kv, batch):
-        rc = fn(torch.cuda.current_stream().cuda_stream, kv._ref, batch._ref, tokens, k.data_ptr(), k.stride(0), k.stride(1),
-                v.data_ptr(), v.stride(0), v.stride(1), q.data_ptr() if q is not None else None, qt, qh, heads,
-                q_out.data_ptr() if q is not None else None, cos.data_ptr() if cos is not None else None,
-                sin.data_ptr() if cos is not None else None, rows, positions.data_ptr() if positions is not None else None,
-                PAIRINGS[pairing])
-    if rc:
-        _lib.check(rc, "paged append")
+    kt, kh = _strides(k)
+    vt, vh = _strides(v)
+    _call(kv, batch, "paged append", (_fns or _entries())[0], tokens, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, qp, qt, qh, heads, op,
+          cp, sp, rows, pp, PAIRINGS[pairing])
     return q_out
 
 
@@ -196,17 +220,13 @@ def read(kv: PagedKv, batch: PagedBatch, *, rows: int, cu_rows: Optional[torch.T
     cu = batch.cu_q if cu_rows is None else _index("read: cu_rows", cu_rows, (batch.seqs + 1,), kv.device)
     if first is not None:
         _index("read: first", first, (batch.seqs,), kv.device)
-    k, v = (torch.empty((rows, kv.kv_heads, D), dtype=torch.bfloat16, device=kv.device) for _ in range(2))
+    k, v = torch.empty((2, rows, kv.kv_heads, D), dtype=_bf16, device=kv.device).unbind(0)
     if rows == 0:
         return k, v
     if batch.seqs == 0:
         return k.zero_(), v.zero_()
-    fn = _entries()[1]
-    with _on(kv, batch):
-        rc = fn(torch.cuda.current_stream().cuda_stream, kv._ref, batch._ref, cu.data_ptr(),
-                first.data_ptr() if first is not None else None, rows, k.data_ptr(), v.data_ptr())
-    if rc:
-        _lib.check(rc, "paged read")
+    _call(kv, batch, "paged read", (_fns or _entries())[1], cu.data_ptr(), first.data_ptr() if first is not None else None, rows,
+          k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -219,26 +239,31 @@ def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[Block
     by token, a window of `window` tokens, the first `sink` tokens always visible; block_tokens of a frame: the streaming
     form of the block-causal mask.  A row that sees no key is zero.  Pages of which no row sees a key need not exist.
     With `out`, rows that belong to no sequence keep what they hold."""
-    _heads_in("attend: q", q, None, None, kv.device)
-    tokens, heads = q.shape[:2]
+    _heads_in("attend: q", q, -1, -1, kv.index)
+    tokens, heads, _ = q.shape
     if heads < 1 or heads % kv.kv_heads:
         raise ValueError(f"attend: {heads} heads over {kv.kv_heads} K/V heads")
     if out is None:
-        out = torch.empty((tokens, heads, D), dtype=torch.bfloat16, device=kv.device)
+        out = q.new_empty((tokens, heads, D))
     else:
-        _heads_in("attend: out", out, tokens, heads, kv.device)
+        _heads_in("attend: out", out, tokens, heads, kv.index)
         if not out.is_contiguous():
             raise ValueError("attend: out must be contiguous")
     if tokens == 0 or batch.seqs == 0 or batch.max_q == 0:
         return out
-    mode, bt, win, sink = (1, mask.block_tokens, mask.window, mask.sink) if mask is not None else (0, 0, 0, 0)
-    _, _, need_fn, fn = _entries()
-    with _on(kv, batch):
-        need = need_fn(kv._ref, batch._ref, tokens, heads, mode, bt, win, sink)
-        # (scratch of this call alone, from the stream's own pool: calls on other streams and captured graphs share nothing)
-        ws = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None
-        rc = fn(torch.cuda.current_stream().cuda_stream, kv._ref, batch._ref, tokens, q.data_ptr(), q.stride(0), q.stride(1),
-                heads, mode, bt, win, sink, D ** -0.5 if scale is None else float(scale), out.data_ptr(), ws.data_ptr() if need else None, need)
-    if rc:
-        _lib.check(rc, "paged attention")
+    how = (1, mask.block_tokens, mask.window, mask.sink) if mask is not None else (0, 0, 0, 0)
+    fns = _fns or _entries()
+    key = (how, heads, kv.kv_heads)
+    need = batch._need.get(key)
+    if need is None:
+        need = 0
+        if kv.index >= 0:
+            with torch.cuda.device(kv.index):
+                need = batch._need[key] = fns[2](kv._ref, batch._ref, 1, heads, *how)
+    need *= tokens
+    # (scratch of this call alone, from the stream's own pool: calls on other streams and captured graphs share nothing)
+    ws = q.new_empty((need // 2,)) if need else None
+    qt, qh = _strides(q)
+    _call(kv, batch, "paged attention", fns[3], tokens, q.data_ptr(), qt, qh, heads, *how, _SCALE if scale is None else float(scale),
+          out.data_ptr(), ws.data_ptr() if need else None, need)
     return out
