@@ -20,7 +20,9 @@ namespace cg = cooperative_groups;
 constexpr int kWarps = 4;
 constexpr int kAttnThreads = 32 * kWarps;
 constexpr int kMaxCluster = 8;  // CTAs of a portable cluster
-constexpr int kTile = 16;  // keys a warp takes at a time (one page holds them: page_rows is a multiple of 16)
+// Keys a warp takes at a time: 16 are in one page (page_rows is a multiple of 16), 32 in one or two.
+template <bool Q4>
+constexpr int kTile = Q4 ? 32 : 16;
 
 struct AttnArgs {
     Pool pool;
@@ -34,20 +36,22 @@ struct AttnArgs {
     int heads, group, splits, row_blocks;
     int cluster;              // the key ranges of a block of rows are one cluster, which joins them itself
     float sl2;
+    long long wait_cycles;
 };
 
 
 using fvattn::neg_inf;
 
 // The key tiles a block of rows visits: those of [0, sink), then those of [lo, hi), each tile once.
+template <int TILE>
 struct Tiles {
     int sinks, first, count;
     FV_DEV explicit Tiles(const Span& s) {
-        sinks = (s.sink + kTile - 1) / kTile;
-        first = max(s.lo / kTile, sinks);
-        count = sinks + max(0, (s.hi + kTile - 1) / kTile - first);
+        sinks = (s.sink + TILE - 1) / TILE;
+        first = max(s.lo / TILE, sinks);
+        count = sinks + max(0, (s.hi + TILE - 1) / TILE - first);
     }
-    FV_DEV int key(int u) const { return (u < sinks ? u : first + (u - sinks)) * kTile; }
+    FV_DEV int key(int u) const { return (u < sinks ? u : first + (u - sinks)) * TILE; }
 };
 
 FV_DEV uint4 ld_stream(const void* p) {
@@ -85,21 +89,19 @@ FV_DEV uint32_t transpose8(uint32_t x) {
     return r;
 }
 FV_DEV uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
-// The eight codes of a word as four f16 pairs code = n - 8, pair i from nibbles i and i + 4.  A nibble at bits 0-3 or 4-7 of a
-// half word is or-ed into the mantissa of 1024 (unit 1) as it lies: 1024 + n or 1024 + 16 n, exact, and one addition or
-// multiply-add takes the 1024 off, exact as well: one shift and four three-input logic operations a word (the logic pipe
-// is what bounds this kernel), the rest on the otherwise idle FMA pipe.
+// The eight codes of a word as four f16 pairs, pair i from nibbles i and i + 4: a nibble n at bits 0-3 of a half word is the
+// f16 number n 2^-24 as it stands (below f16's normal numbers, which the matrix unit multiplies exactly), at bits 4-7
+// 16 n 2^-24.  One shift and four masks a word and nothing else: expanding the codes is what bounds this kernel (with the
+// codes or-ed into 1024's mantissa and the 1024 taken off again by an addition it took 160 instead of 112 us for 32 sequences of
+// 20 011 keys).  The factors, and the 8 between n and the code, are taken out of the products' results.
 FV_DEV void codes_f16(uint32_t w, uint32_t (&h)[4]) {
     const uint32_t v = w >> 8;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(h[0]) : "r"(w), "r"(0x000f000fu), "r"(0x64006400u));
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(h[1]) : "r"(w), "r"(0x00f000f0u), "r"(0x64006400u));
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(h[2]) : "r"(v), "r"(0x000f000fu), "r"(0x64006400u));
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(h[3]) : "r"(v), "r"(0x00f000f0u), "r"(0x64006400u));
-    h[0] = add_f16x2(h[0], 0xe408e408u);               // - 1032
-    h[1] = fma_f16x2(h[1], 0x2c002c00u, 0xd480d480u);  // / 16 - 72
-    h[2] = add_f16x2(h[2], 0xe408e408u);
-    h[3] = fma_f16x2(h[3], 0x2c002c00u, 0xd480d480u);
+    h[0] = w & 0x000f000fu;
+    h[1] = w & 0x00f000f0u;
+    h[2] = v & 0x000f000fu;
+    h[3] = v & 0x00f000f0u;
 }
+constexpr float kCodeUnit = 16777216.f;  // 2^24
 FV_DEV float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
 FV_DEV float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
@@ -107,16 +109,19 @@ FV_DEV uint32_t word(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y
 
 // One tile of 16 keys in registers, as lane 4 g + t holds it; `row` is the pool row of the tile's first key, or kNoRow.
 //   bf16  k0 / k1: keys g and g + 8, 16-byte pieces 4 n + t of their rows; v: keys 2t, 2t+1, 2t+8, 2t+9, pieces g and
-//         g + 8 of their rows.
-//   4 bit k0 / k1: values 32 t .. 32 t + 31 of keys g and g + 8; v: values 16 g .. 16 g + 15 of the four keys; s0 / s1:
-//         (step, zero) of keys g and g + 8.
+//         g + 8 of their rows.  Straight from memory.
+//   4 bit k0 / k1: values 32 t .. 32 t + 31 of keys g' and g' + 8; v: values 16 g .. 16 g + 15 of four keys; s0 / s1:
+//         (step, zero) of keys g' and g' + 8.  Out of the warp's ring in shared memory.
 constexpr uint32_t kNoRow = 0xffffffffu;
+// The key of a 4-bit tile that stands in row g of the product: every second pair is swapped, so that the lanes that read V's
+// rows 2 t side by side meet both halves of the banks.
+FV_DEV int key_of_row(int g) { return g ^ ((g >> 1) & 1); }
 template <bool Q4>
 struct Keys;
 template <>
 struct Keys<false> {
     uint4 k0[4], k1[4];
-    FV_DEV void load(const uint8_t* lane_k, const uint32_t*, uint32_t row) {
+    FV_DEV void load(const uint8_t* lane_k, uint32_t row) {
         if (row == kNoRow) {
 #pragma unroll
             for (int n = 0; n < 4; n++) k0[n] = k1[n] = make_uint4(0, 0, 0, 0);
@@ -135,26 +140,13 @@ template <>
 struct Keys<true> {
     uint4 k0, k1;
     uint32_t s0, s1;
-    FV_DEV void load(const uint8_t* lane_k, const uint32_t* lane_s, uint32_t row) {
-        if (row == kNoRow) {
-            k0 = k1 = make_uint4(0, 0, 0, 0);
-            s0 = s1 = 0;
-            return;
-        }
-        const uint8_t* r = lane_k + (size_t)row * kQ4Bytes;
-        k0 = ld_stream(r);
-        k1 = ld_stream(r + 8 * kQ4Bytes);
-        s0 = ld_stream1(lane_s + row);
-        s1 = ld_stream1(lane_s + row + 8);
-    }
-    static FV_DEV size_t lane_offset(int g, int t) { return (size_t)g * kQ4Bytes + 16 * t; }
 };
 template <bool Q4>
 struct Values;
 template <>
 struct Values<false> {
     uint4 a[4], b[4];  // pieces g and g + 8 of keys 2t, 2t+1, 2t+8, 2t+9
-    FV_DEV void load(const uint8_t* lane_v, const uint32_t*, uint32_t row) {
+    FV_DEV void load(const uint8_t* lane_v, uint32_t row) {
         if (row == kNoRow) {
 #pragma unroll
             for (int i = 0; i < 4; i++) a[i] = b[i] = make_uint4(0, 0, 0, 0);
@@ -174,36 +166,79 @@ template <>
 struct Values<true> {
     uint2 a[4];
     uint32_t s0, s1;
-    FV_DEV void load(const uint8_t* lane_v, const uint32_t* lane_s, uint32_t row) {
-        if (row == kNoRow) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) a[i] = make_uint2(0, 0);
-            s0 = s1 = 0;
-            return;
-        }
-        const uint8_t* r = lane_v + (size_t)row * kQ4Bytes;
-#pragma unroll
-        for (int i = 0; i < 4; i++) a[i] = ld_stream2(r + ((i & 1) + 8 * (i >> 1)) * kQ4Bytes);
-        s0 = ld_stream1(lane_s + row);
-        s1 = ld_stream1(lane_s + row + 8);
-    }
-    static FV_DEV size_t lane_offset(int g, int t) { return (size_t)(2 * t) * kQ4Bytes + 8 * g; }
 };
+
+// The ring of a warp (4 bits): a stage is a tile of 32 keys, K codes | V codes | K scales | V scales, brought by bulk copies (in
+// pages of 32 rows and more one run of each array, in pages of 16 two), one mbarrier a stage.  A warp fills and waits for
+// its own stages only.
+struct Ring {
+    static constexpr uint32_t kHalfBytes = 2 * 1024 + 2 * 64, kStageBytes = 2 * kHalfBytes;
+    static constexpr uint32_t kV = 2048, kKs = 4096, kVs = 4224;
+    static constexpr int kStages = 3;
+    static constexpr uint32_t kWarpBytes = kStages * kStageBytes;
+};
+template <bool Q4, int NT>
+struct DecodeSmem {
+    static constexpr uint32_t kJoin = kWarps * 8 * NT * (kD + 4) * 4 + 2 * kWarps * 8 * NT * 4;  // the warps' results side by side
+    static constexpr uint32_t kRing = Q4 ? kWarps * Ring::kWarpBytes : 0;                        // (the join comes after the ring)
+    static constexpr uint32_t kBars = kRing > kJoin ? kRing : kJoin;
+    static constexpr uint32_t kTotal = kBars + (Q4 ? kWarps * Ring::kStages * 8 : 0);
+};
+// Bounded wait for a stage; false after a timeout, which is reported.
+struct WaitStage {
+    int* status;
+    long long cycles;
+    FV_DEV bool operator()(uint32_t bar, uint32_t parity) const {
+        if (fvp::mbar_try(bar, parity)) return true;
+        const long long t0 = clock64();
+        while (!fvp::mbar_try(bar, parity)) {
+            if (clock64() - t0 > cycles) {
+                atomicCAS(status, FV_ST_OK, FV_ST_TIMEOUT_BASE + 5);
+                return false;
+            }
+        }
+        return true;
+    }
+};
+FV_DEV bool elect_one() {  // one lane of the converged warp
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
+FV_DEV uint4 lds128(uint32_t a) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+    return r;
+}
+FV_DEV uint2 lds64(uint32_t a) {
+    uint2 r;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
+    return r;
+}
+FV_DEV uint32_t lds32(uint32_t a) {
+    uint32_t r;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(a) : "memory");
+    return r;
+}
 
 // NT groups of 8 query rows.  The transposed products S^T = K . Q^T and O^T = V^T . P^T keep keys and head dim on the
 // 16-wide side of the matrix instruction and the (few) query rows on the 8-wide one; the sums of either product may run
 // in any order of d or key, so every lane's operands are whole 16-byte pieces as they lie in memory and no shared
 // memory is needed on the way.
 //
-// A warp takes a run of tiles of its own.  Their pool rows are looked up 32 at a time, one tile a lane, a batch ahead; a tile's
-// K registers are loaded anew as soon as its scores are done and V's as soon as its product is, so that memory is always
-// being read while the warp computes.
+// A warp takes a run of tiles of its own.  Their pool rows are looked up 32 at a time, one tile a lane, a batch ahead.
+// bf16: a tile's K registers are loaded anew as soon as its scores are done and V's as soon as its product is, so that
+// memory is always being read while the warp computes.  4 bits: 16 keys are too few bytes for that (and the registers are
+// needed for more warps: expanding the codes is what bounds this form), so a ring in shared memory runs three stages ahead.
 template <bool Q4, int NT>
-__global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_paged_decode_kernel(const AttnArgs a) {
     constexpr int kRows = 8 * NT;
-    constexpr int SUB = Q4 ? 2 : 1;  // tiles at a time (4 bits: 16 keys are too few bytes in flight)
-    __shared__ float sh_o[kWarps][kRows][kD + 4];
-    __shared__ float sh_m[kWarps][kRows], sh_l[kWarps][kRows];
+    constexpr int SUB = kTile<Q4> / 16;  // products of 16 keys in a tile
+    using Sm = DecodeSmem<Q4, NT>;
+    extern __shared__ __align__(128) unsigned char decode_smem[];
+    float (*sh_o)[kRows][kD + 4] = reinterpret_cast<float (*)[kRows][kD + 4]>(decode_smem);
+    float (*sh_m)[kRows] = reinterpret_cast<float (*)[kRows]>(decode_smem + kWarps * kRows * (kD + 4) * 4);
+    float (*sh_l)[kRows] = sh_m + kWarps;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     int b = blockIdx.x;
     const int split = b % a.splits;
@@ -217,7 +252,7 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
     const int pos0 = seq.len - seq.nq;  // position of the sequence's first token of this call
     const int first = pos0 + row0 / a.group, last = pos0 + (row0 + rows - 1) / a.group;
     const Span span = span_of(a.mask, first, last, seq.len);
-    const Tiles tiles(span);
+    const Tiles<kTile<Q4>> tiles(span);
     const int u0 = (int)((long long)tiles.count * split / a.splits), u1 = (int)((long long)tiles.count * (split + 1) / a.splits);
     const int w0 = u0 + (u1 - u0) * warp / kWarps, n_tiles = u0 + (u1 - u0) * (warp + 1) / kWarps - w0;
 
@@ -230,33 +265,75 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
         whole_sink = min(lowest.lo == 0 ? lowest.hi : lowest.sink, highest.lo == 0 ? highest.hi : highest.sink);
     }
     struct Feed {
-        uint32_t row, whole;  // this lane's tile's pool row; bit i: tile i of the batch is whole
+        uint32_t row[SUB], whole;  // pool rows of this lane's tile (of its halves); bit i: tile i of the batch is whole
     };
     auto lookup = [&](int base) {
-        Feed f{kNoRow, 0u};
+        Feed f;
         bool whole = false;
+#pragma unroll
+        for (int i = 0; i < SUB; i++) f.row[i] = kNoRow;
         if (base + lane < n_tiles) {
             const int key = tiles.key(w0 + base + lane);
-            const int page = page_of(a.pool, a.batch, s, key);
-            if (page >= 0) {
-                f.row = (uint32_t)pool_row(a.pool, page, head, key);
-                whole = (key >= whole_lo && key + kTile <= whole_hi) || key + kTile <= whole_sink;
+#pragma unroll
+            for (int i = 0; i < SUB; i++) {
+                const int k = key + 16 * i;
+                if (i > 0 && a.pool.log_rows > 4) {  // (the same page)
+                    if (f.row[0] != kNoRow) f.row[i] = f.row[0] + 16;
+                } else if (SUB == 1 || a.pool.log_rows > 4 || (k < span.hi && k + 16 > span.lo) || k < span.sink) {
+                    const int page = page_of(a.pool, a.batch, s, k);
+                    if (page >= 0) f.row[i] = (uint32_t)pool_row(a.pool, page, head, k);
+                }
             }
+            whole = f.row[0] != kNoRow && f.row[SUB - 1] != kNoRow &&
+                    ((key >= whole_lo && key + kTile<Q4> <= whole_hi) || key + kTile<Q4> <= whole_sink);
         }
         f.whole = __ballot_sync(kFullWarp, whole);
         return f;
     };
     Feed cur = lookup(0), nxt = lookup(32);
-    const uint8_t* lane_k = a.pool.k + Keys<Q4>::lane_offset(g, t);
-    const uint8_t* lane_v = a.pool.v + Values<Q4>::lane_offset(g, t);
-    const uint32_t *lane_ks = a.pool.k_scale + g, *lane_vs = a.pool.v_scale + g;
     Keys<Q4> kt[SUB];
     Values<Q4> vt[SUB];
-#pragma unroll
-    for (int i = 0; i < SUB; i++) {
-        const uint32_t row = __shfl_sync(kFullWarp, cur.row, i);
-        kt[i].load(lane_k, lane_ks, row);
-        vt[i].load(lane_v, lane_vs, row);
+    const uint8_t *lane_k = a.pool.k, *lane_v = a.pool.v;
+    const uint32_t ring = fvp::smem_u32(decode_smem) + warp * Ring::kWarpBytes;
+    const uint32_t bars = fvp::smem_u32(decode_smem) + Sm::kBars + warp * Ring::kStages * 8;
+    // 4 bits: tile j of the batch that `cur` (j >= 32: `nxt`) holds into stage st.
+    auto fill_stage = [&](int j, int st) {
+        const uint32_t r0 = __shfl_sync(kFullWarp, j < 32 ? cur.row[0] : nxt.row[0], j & 31);
+        const uint32_t r1 = __shfl_sync(kFullWarp, j < 32 ? cur.row[SUB - 1] : nxt.row[SUB - 1], j & 31);
+        if (!elect_one()) return;
+        const uint32_t bar = bars + 8 * st, dst = ring + st * Ring::kStageBytes;
+        if (r0 != kNoRow && r1 == r0 + 16) {
+            fvp::mbar_expect_tx(bar, Ring::kStageBytes);
+            fvp::bulk_load(dst, a.pool.k + (size_t)r0 * kQ4Bytes, 2048, bar);
+            fvp::bulk_load(dst + Ring::kV, a.pool.v + (size_t)r0 * kQ4Bytes, 2048, bar);
+            fvp::bulk_load(dst + Ring::kKs, a.pool.k_scale + r0, 128, bar);
+            fvp::bulk_load(dst + Ring::kVs, a.pool.v_scale + r0, 128, bar);
+        } else {  // two pages, or a half without one
+            fvp::mbar_expect_tx(bar, ((r0 != kNoRow) + (r1 != kNoRow)) * Ring::kHalfBytes);
+#pragma unroll 1
+            for (uint32_t i = 0; i < 2; i++) {
+                const uint32_t row = i ? r1 : r0;
+                if (row == kNoRow) continue;
+                fvp::bulk_load(dst + 1024 * i, a.pool.k + (size_t)row * kQ4Bytes, 1024, bar);
+                fvp::bulk_load(dst + Ring::kV + 1024 * i, a.pool.v + (size_t)row * kQ4Bytes, 1024, bar);
+                fvp::bulk_load(dst + Ring::kKs + 64 * i, a.pool.k_scale + row, 64, bar);
+                fvp::bulk_load(dst + Ring::kVs + 64 * i, a.pool.v_scale + row, 64, bar);
+            }
+        }
+    };
+    if constexpr (Q4) {
+        if (lane == 0) {
+            for (int st = 0; st < Ring::kStages; st++) fvp::mbar_init(bars + 8 * st, 1);
+            fvp::mbar_init_fence();
+        }
+        __syncwarp();
+        for (int st = 0; st < Ring::kStages && st < n_tiles; st++) fill_stage(st, st);
+    } else {
+        lane_k += Keys<false>::lane_offset(g, t);
+        lane_v += Values<false>::lane_offset(g, t);
+        const uint32_t row = __shfl_sync(kFullWarp, cur.row[0], 0);
+        kt[0].load(lane_k, row);
+        vt[0].load(lane_v, row);
     }
 
     // Q^T: column g of each group of 8 rows, in the order of d that the keys' lanes hold.  4 bits: as f16, scaled by a power
@@ -296,15 +373,13 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
             const float up = __uint_as_float((uint32_t)(262 - e) << 23), down = __uint_as_float((uint32_t)(e - 8) << 23);
 #pragma unroll
             for (int i = 0; i < 4; i++) {  // pairs (d, d + 4) of eight values: the nibbles that one mask gives
-                auto pair = [&](uint32_t x, uint32_t y, bool high) {
-                    return high ? pack_f16x2(hi_f(x) * up, hi_f(y) * up) : pack_f16x2(lo_f(x) * up, lo_f(y) * up);
-                };
-                qf[n][4 * i + 0] = pair(u[i].x, u[i].z, false);
-                qf[n][4 * i + 1] = pair(u[i].x, u[i].z, true);
-                qf[n][4 * i + 2] = pair(u[i].y, u[i].w, false);
-                qf[n][4 * i + 3] = pair(u[i].y, u[i].w, true);
+                const float up16 = up * 0.0625f;  // (the second and fourth pair meet codes that stand for 16 n)
+                qf[n][4 * i + 0] = pack_f16x2(lo_f(u[i].x) * up, lo_f(u[i].z) * up);
+                qf[n][4 * i + 1] = pack_f16x2(hi_f(u[i].x) * up16, hi_f(u[i].z) * up16);
+                qf[n][4 * i + 2] = pack_f16x2(lo_f(u[i].y) * up, lo_f(u[i].w) * up);
+                qf[n][4 * i + 3] = pack_f16x2(hi_f(u[i].y) * up16, hi_f(u[i].w) * up16);
             }
-            const float scaled = sum * up, back = a.sl2 * down;
+            const float scaled = sum * up * (1.f / kCodeUnit), back = a.sl2 * down * kCodeUnit;
             qsum[n][0] = __shfl_sync(kFullWarp, scaled, 8 * t);      // of row 2 t, which the lanes 4 (2 t) .. hold
             qsum[n][1] = __shfl_sync(kFullWarp, scaled, 8 * t + 4);  // of row 2 t + 1
             sl2[n][0] = __shfl_sync(kFullWarp, back, 8 * t);
@@ -330,16 +405,37 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
         l[n][0] = l[n][1] = z[n][0] = z[n][1] = 0.f;
     }
 
-    for (int v = 0; v < n_tiles; v += SUB) {
+    int st = 0;  // 4 bits: the stage of this step and the phase of its barrier
+    uint32_t phase = 0;
+    const WaitStage wait_stage{a.batch.status - 1, a.wait_cycles};
+    for (int v = 0; v < n_tiles; v++) {
         const int i0 = v & 31;
         if (v > 0 && i0 == 0) {
             cur = nxt;
             nxt = lookup(v + 32);
         }
-        uint32_t next_row[SUB];
+        const bool more = v + 1 < n_tiles;
+        uint32_t next_row = kNoRow, stage = 0;
+        if constexpr (Q4) {
+            stage = ring + st * Ring::kStageBytes;
+            if (!__all_sync(kFullWarp, wait_stage(bars + 8 * st, phase))) {  // (given up and reported: what was asked for must land)
+                for (int k = 0; k < Ring::kStages && v + k < n_tiles; k++) {
+                    fvp::mbar_drain(bars + 8 * st, phase);
+                    st = st + 1 == Ring::kStages ? 0 : st + 1;
+                    phase ^= st == 0;
+                }
+                break;
+            }
 #pragma unroll
-        for (int i = 0; i < SUB; i++) next_row[i] = __shfl_sync(kFullWarp, i0 + SUB < 32 ? cur.row : nxt.row, (i0 + SUB + i) & 31);
-        const bool more = v + SUB < n_tiles;
+            for (int i = 0; i < SUB; i++) {
+                kt[i].k0 = lds128(stage + 1024 * i + 64 * key_of_row(g) + 16 * t);
+                kt[i].k1 = lds128(stage + 1024 * i + 64 * key_of_row(g) + 512 + 16 * t);
+                kt[i].s0 = lds32(stage + Ring::kKs + 64 * i + 4 * key_of_row(g));
+                kt[i].s1 = lds32(stage + Ring::kKs + 64 * i + 4 * key_of_row(g) + 32);
+            }
+        } else {
+            next_row = __shfl_sync(kFullWarp, i0 + 1 < 32 ? cur.row[0] : nxt.row[0], (i0 + 1) & 31);
+        }
 
         // c0, c1: key g, rows 2 t and 2 t + 1; c2, c3: key g + 8.
         float c[SUB][NT][4];
@@ -366,8 +462,9 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
                     for (int n = 0; n < NT; n++) mma<Q4>(c[i][n], x0[j], x1[j], x0[j + 1], x1[j + 1], qf[n][4 * w + j], qf[n][4 * w + j + 1]);
                 }
             }
-            if constexpr (Q4) {  // q . (zero + step code) = step (q . code) + zero sum(q)
-                const float s0 = lo_f(kt[i].s0), s1 = lo_f(kt[i].s1), z0 = hi_f(kt[i].s0), z1 = hi_f(kt[i].s1);
+            if constexpr (Q4) {  // q . (zero + step code) = step (q . n) + (zero - 8 step) sum(q), all by 2^-24
+                const float s0 = lo_f(kt[i].s0), s1 = lo_f(kt[i].s1);
+                const float z0 = fmaf(-8.f, s0, hi_f(kt[i].s0)), z1 = fmaf(-8.f, s1, hi_f(kt[i].s1));
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     c[i][n][0] = fmaf(c[i][n][0], s0, z0 * qsum[n][0]);
@@ -376,15 +473,21 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
                     c[i][n][3] = fmaf(c[i][n][3], s1, z1 * qsum[n][1]);
                 }
             }
-            if (more) kt[i].load(lane_k, lane_ks, next_row[i]);
+            if constexpr (!Q4) {
+                if (more) kt[i].load(lane_k, next_row);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++) vt[i].a[k] = lds64(stage + Ring::kV + 1024 * i + 64 * (key_of_row(2 * t + (k & 1)) + 8 * (k >> 1)) + 8 * g);
+                vt[i].s0 = lds32(stage + Ring::kVs + 64 * i + 4 * key_of_row(g));
+                vt[i].s1 = lds32(stage + Ring::kVs + 64 * i + 4 * key_of_row(g) + 32);
+            }
         }
 
-        constexpr uint32_t kAll = (1u << SUB) - 1u;
-        if (((cur.whole >> i0) & kAll) != kAll) {
+        if (!((cur.whole >> i0) & 1u)) {
 #pragma unroll
             for (int i = 0; i < SUB; i++) {
-                const bool none = __shfl_sync(kFullWarp, cur.row, i0 + i) == kNoRow;
-                const int key0 = none ? 0 : tiles.key(w0 + v + i);
+                const bool none = __shfl_sync(kFullWarp, cur.row[i], i0) == kNoRow;
+                const int key0 = tiles.key(w0 + v) + 16 * i;
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -393,7 +496,7 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
                         const Span sp = span_of(a.mask, p, p, seq.len);
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const int j = key0 + g + 8 * h;
+                            const int j = key0 + (Q4 ? key_of_row(g) : g) + 8 * h;
                             if (none || !((j >= sp.lo && j < sp.hi) || j < sp.sink)) c[i][n][2 * h + e] = neg_inf();
                         }
                     }
@@ -401,8 +504,8 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
                 // Values that no row of this block may see count as zero whatever they hold (0 times NaN is NaN).
                 auto seen = [&](int j) { return !none && ((j >= span.lo && j < span.hi) || j < span.sink); };
                 if constexpr (Q4) {
-                    if (!seen(key0 + g)) vt[i].s0 = 0u;
-                    if (!seen(key0 + g + 8)) vt[i].s1 = 0u;
+                    if (!seen(key0 + key_of_row(g))) vt[i].s0 = 0u;
+                    if (!seen(key0 + key_of_row(g) + 8)) vt[i].s1 = 0u;
                 } else {
 #pragma unroll
                     for (int k = 0; k < 4; k++)
@@ -416,7 +519,7 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
         // exact but for P step, which is rounded to f16 and must fit it: 2^14; a reference bounds P step by 2^8, so that only
         // what is 2^32 below the largest is lost at f16's lower end.
         constexpr float kGuard = Q4 ? 16384.f : 1099511627776.f, kGuardP = 1.2676506e30f;  // 2^100
-        float p[SUB][NT][4], ps[SUB][NT][4], sum = 0.f, sum_s = 0.f;
+        float p[SUB][NT][4] = {}, ps[SUB][NT][4], sum = 0.f, sum_s = 0.f;
         auto weigh = [&vt, &p, &ps](int i, int n) {
             if constexpr (Q4) {
                 const float s0 = lo_f(vt[i].s0), s1 = lo_f(vt[i].s1);
@@ -489,7 +592,7 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
                 l[n][0] += p[i][n][0] + p[i][n][2];
                 l[n][1] += p[i][n][1] + p[i][n][3];
                 if constexpr (Q4) {
-                    const float z0 = hi_f(vt[i].s0), z1 = hi_f(vt[i].s1);
+                    const float z0 = fmaf(-8.f, lo_f(vt[i].s0), hi_f(vt[i].s0)), z1 = fmaf(-8.f, lo_f(vt[i].s1), hi_f(vt[i].s1));
                     z[n][0] = fmaf(p[i][n][0], z0, fmaf(p[i][n][2], z1, z[n][0]));
                     z[n][1] = fmaf(p[i][n][1], z0, fmaf(p[i][n][3], z1, z[n][1]));
                 }
@@ -526,10 +629,37 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
                     for (int n = 0; n < NT; n++) mma<false>(o[n][k], a0, a1, a2, a3, pb[n][0], pb[n][1]);
                 }
             }
-            if (more) vt[i].load(lane_v, lane_vs, next_row[i]);
+            if constexpr (!Q4) {
+                if (more) vt[i].load(lane_v, next_row);
+            }
+        }
+        if constexpr (Q4) {
+            __syncwarp();  // every lane has its operands out of the stage: fill it again
+            if (v + Ring::kStages < n_tiles) fill_stage(i0 + Ring::kStages, st);
+            st = st + 1 == Ring::kStages ? 0 : st + 1;
+            phase ^= st == 0;
+            // O holds sum P step n and z the sum of P (zero - 8 step): both grow with every key, their sum does not.  Every 256
+            // keys z goes into O, so that f32 (whose sums the matrix unit truncates) never carries more than those keys' offset.
+            if ((v & 7) == 7) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) z[n][e] += __shfl_xor_sync(kFullWarp, z[n][e], d);
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            o[n][k][e] = fmaf(z[n][e], ((k & 1) ? 16.f : 1.f) / kCodeUnit, o[n][k][e]);
+                            o[n][k][2 + e] = fmaf(z[n][e], ((k & 1) ? 16.f : 1.f) / kCodeUnit, o[n][k][2 + e]);
+                        }
+                        z[n][e] = 0.f;
+                    }
+                }
+            }
         }
     }
 
+    if (Q4) __syncthreads();  // (the join's memory is the ring's)
     // The four warps' results side by side, then joined.
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -547,8 +677,9 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_decode_kernel(const Att
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                sh_o[warp][r][Q4 ? 16 * g + i : 8 * g + i] = o[n][i][e] + z[n][e];
-                sh_o[warp][r][Q4 ? 16 * g + 8 + i : 64 + 8 * g + i] = o[n][i][2 + e] + z[n][e];
+                const float unit = Q4 ? ((i & 1) ? kCodeUnit / 16.f : kCodeUnit) : 1.f;
+                sh_o[warp][r][Q4 ? 16 * g + i : 8 * g + i] = fmaf(o[n][i][e], unit, z[n][e]);
+                sh_o[warp][r][Q4 ? 16 * g + 8 + i : 64 + 8 * g + i] = fmaf(o[n][i][2 + e], unit, z[n][e]);
             }
         }
     }
@@ -718,11 +849,11 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads,
     // Key ranges: as many as fill the SMs once; where the rows alone nearly do, three times over, so that ragged ends even
     // out.  Up to kMaxCluster ranges are one cluster, which joins its parts itself; the merge kernel behind more of them takes
     // about 5 us, so more need enough tiles a warp (0.75 us each) to be worth it.
-    const int resident = sms * (s.nt == 1 ? 3 : 2);  // CTAs that run at a time
-    const long long tiles = (keys + kTile - 1) / kTile, most = (tiles + 2 * kWarps - 1) / (2 * kWarps);  // at least two tiles per warp
+    const int resident = sms * (s.nt == 1 ? (kv->format == FV_PAGE_Q4 ? 4 : 3) : 2);  // CTAs that run at a time
+    const long long tiles = (keys + 15) / 16, most = (tiles + 2 * kWarps - 1) / (2 * kWarps);  // at least 32 keys per warp
     long long n = resident / ctas;
     if (n < 2) n = (3ll * resident + ctas - 1) / ctas;
-    if (n > kMaxCluster && (n < 12 || tiles < 16 * kWarps * kMaxCluster)) n = kMaxCluster;
+    if (n > kMaxCluster && (n < 16 || tiles < 16 * kWarps * kMaxCluster)) n = kMaxCluster;
     n = n < most ? n : most;
     s.splits = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
     s.cluster = s.splits > 1 && s.splits <= kMaxCluster;
@@ -854,6 +985,7 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
     a.row_blocks = s.row_blocks;
     a.cluster = s.cluster;
     a.sl2 = scale * 1.4426950408889634f;
+    a.wait_cycles = FV_WAIT_CYCLES;
     const long long grid = (long long)b->seqs * kv->kv_heads * s.row_blocks * s.splits;
     if (grid > 0x7fffffffll || (long long)rows > 0x7fffffffll) return FV_DECLINED;
     cudaStream_t st = (cudaStream_t)stream;
@@ -867,11 +999,29 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
         return FV_RAN;
     }
     const bool q4 = kv->format == FV_PAGE_Q4;
-    const auto fn = q4 ? (s.nt == 1 ? fv_paged_decode_kernel<true, 1> : fv_paged_decode_kernel<true, 2>)
-                       : (s.nt == 1 ? fv_paged_decode_kernel<false, 1> : fv_paged_decode_kernel<false, 2>);
+    void (*fn)(AttnArgs);
+    uint32_t smem;
+    auto pick = [&](auto f, uint32_t bytes) {
+        fn = f;
+        smem = bytes;
+    };
+    if (q4 && s.nt == 1) pick(fv_paged_decode_kernel<true, 1>, DecodeSmem<true, 1>::kTotal);
+    else if (q4) pick(fv_paged_decode_kernel<true, 2>, DecodeSmem<true, 2>::kTotal);
+    else if (s.nt == 1) pick(fv_paged_decode_kernel<false, 1>, DecodeSmem<false, 1>::kTotal);
+    else pick(fv_paged_decode_kernel<false, 2>, DecodeSmem<false, 2>::kTotal);
+    if (q4) {  // (more shared memory than a launch gets unasked)
+        static bool attr_set[64][3] = {};
+        static std::mutex attr_mu;
+        std::lock_guard<std::mutex> lock(attr_mu);
+        if (!attr_set[dev][s.nt]) {
+            FV_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            attr_set[dev][s.nt] = true;
+        }
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kAttnThreads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
