@@ -11,8 +11,8 @@
 //     of which the item sees nothing take a page coordinate past the pool, which reads as zeros.  In the few tiles that
 //     the item's visible keys only cover in part, one warp ("fixer") then zeroes V's rows that no row of the item sees: a P of
 //     zero times whatever memory holds there must be zero.
-//   * 4-bit pages: four more warps expand the codes to f16, one key row a thread, into the swizzled tiles that TMA would
-//     have written, and bring Q as f16.  Both products then run in f16: a value zero + step code is rounded once, by
+//   * 4-bit pages: the loader brings the packed codes by bulk copies, six more warps expand them to f16 into the swizzled
+//     tiles that TMA would have written, and bring Q as f16.  Both products then run in f16: a value zero + step code is rounded once, by
 //     2^-11 at most (in bf16 the roundings of K and V, 2^-8 each, would be of the size of the output's own), P by 2^-11.
 //     f16's range is the price: values beyond 65 504 saturate, below 2^-14 they lose relative precision.  Against that,
 //     P's reference is set 2^6 below the first maximum found: P up to 2^15 fits, and P is zero only 2^30 below the maximum.
@@ -49,17 +49,24 @@ using fvattn::Smem;
 using fvattn::neg_inf;
 using namespace fvp;
 
-constexpr uint32_t kVFixed = Smem::total;  // a barrier for each pair slot: V's invisible rows are zeroed
-constexpr uint32_t kChunkSmem = kVFixed + 8 * fvattn::kKvPairs;
-static_assert(kVFixed % 8 == 0 && kChunkSmem <= 232448, "shared memory");
-static_assert(fvattn::kKvPairs == 2 && fvattn::kEarlyKeys == 128, "P is handed over whole");
+// Shared memory: the dense kernel's map.  After its barriers, bf16: a barrier for each pair slot, "V's invisible rows are
+// zeroed".  4 bits: two stages of packed codes, [V(j-1) | K(j)] as they lie in the pages, take the place of the third Q slot;
+// their barriers and scales come last.
+constexpr uint32_t kVFixed = Smem::total;
+constexpr uint32_t kCodeFull = kVFixed + 8 * fvattn::kKvPairs, kCodeFree = kCodeFull + 16;
+constexpr uint32_t kScales = (kCodeFree + 16 + 15) & ~15u;      // [stage][V | K][128 keys] (step, zero)
+constexpr uint32_t kChunkSmem = kScales + 2 * 1024;
+constexpr uint32_t kCodes = Smem::q + 2 * fvattn::kSlotBytes;   // [stage][V | K][128 keys][64 bytes]
+static_assert(kVFixed % 8 == 0 && kChunkSmem <= 232448 && fvattn::kQSlots == 3 && fvattn::kSlotBytes == 32768, "shared memory");
+static_assert(fvattn::kKvPairs == 2 && fvattn::kEarlyKeys == 128, "the ring in pairs, P handed over whole");
 
 template <bool Q4>
 struct Roles {
     static constexpr int kWarps = Q4 ? 16 : 12;
     static constexpr int kThreads = 32 * kWarps;
-    static constexpr int kLoader = 8, kIssuer = 9, kFixer = 10;  // (bf16: loader and fixer)
-    static constexpr int kExpander = 12;                         // 4 bits: warps 12-15
+    static constexpr int kLoader = 8, kIssuer = 9, kFixer = 10;  // (fixer: bf16)
+    static constexpr int kExpander = 10, kExpanders = 6;         // 4 bits: warps 10-15
+    static constexpr uint32_t kQ = Q4 ? 2 : fvattn::kQSlots;     // Q slots
 };
 
 // What an item covers; every role works it out for itself, from the same numbers.
@@ -253,13 +260,13 @@ static __device__ __noinline__ void chunk_careful(uint32_t tS, uint32_t tO, uint
 
 // Columns 32 q .. 32 q + 31 of the warp's 32 rows; `row` is this lane's output row or -1.  The 16-byte pieces are transposed
 // between neighbouring lanes first, so that a store covers whole runs of a row (fvattn::store_cols32).
-template <bool F32>
+template <bool Q4, bool F32>
 FV_DEV void chunk_store32(void* base, const uint32_t (&o)[32], float inv, int row, int q, int lane) {
     constexpr int G = F32 ? 8 : 4;
     uint4 p[G];
     float f[32];
 #pragma unroll
-    for (int c = 0; c < 32; c++) f[c] = as_f(o[c]) * inv;
+    for (int c = 0; c < 32; c++) f[Q4 ? (c & 24) + ((c & 7) >> 1) + 4 * (c & 1) : c] = as_f(o[c]) * inv;  // (4 bits: see expand_unit)
 #pragma unroll
     for (int c = 0; c < G; c++) {
         if (F32) p[c] = make_uint4(as_u(f[4 * c]), as_u(f[4 * c + 1]), as_u(f[4 * c + 2]), as_u(f[4 * c + 3]));
@@ -277,7 +284,7 @@ FV_DEV void chunk_store32(void* base, const uint32_t (&o)[32], float inv, int ro
         }
     }
 }
-template <bool F32>
+template <bool Q4, bool F32>
 static __device__ __noinline__ void chunk_write(void* base, uint32_t tO, float inv, int row, bool have_o, int lane) {
 #pragma unroll 1
     for (int q = 0; q < 4; q++) {
@@ -290,7 +297,7 @@ static __device__ __noinline__ void chunk_write(void* base, uint32_t tO, float i
 #pragma unroll
             for (int c = 0; c < 32; c++) o[c] = 0u;
         }
-        chunk_store32<F32>(base, o, inv, row, q, lane);
+        chunk_store32<Q4, F32>(base, o, inv, row, q, lane);
     }
 }
 
@@ -367,10 +374,10 @@ FV_DEV void chunk_softmax(const ChunkJob& jb, uint32_t sbase, uint32_t tmem, int
         }
         const float inv = rs.l > 0.f ? 1.f / rs.l : 0.f;
         if (jb.splits == 1) {
-            chunk_write<false>(jb.out, tO, inv, out_row, have_o, lane);
+            chunk_write<Q4, false>(jb.out, tO, inv, out_row, have_o, lane);
         } else {
             const size_t rows = (size_t)jb.batch.tokens * jb.heads;
-            chunk_write<true>(jb.part_o + (size_t)split * rows * kD, tO, inv, out_row, have_o, lane);
+            chunk_write<Q4, true>(jb.part_o + (size_t)split * rows * kD, tO, inv, out_row, have_o, lane);
             if (out_row >= 0) jb.part_lse[(size_t)split * rows + out_row] = rs.l > 0.f ? rs.m + log2f(rs.l) : neg_inf();
         }
     }
@@ -488,23 +495,6 @@ FV_DEV void chunk_fixer(const ChunkJob& jb, uint32_t sbase, int lane, const Chun
 }
 
 // ------------------------------------------------------------------------------------ expander (4-bit pages)
-struct CodeRow {
-    uint4 c[4];
-    uint32_t sz;
-};
-FV_DEV void load_codes(CodeRow& r, const uint8_t* codes, const uint32_t* scale, const ChunkJob& jb, int page, int head, int key) {
-    if (page < 0) {  // a key that the item does not see, or without a page: zeros
-#pragma unroll
-        for (int i = 0; i < 4; i++) r.c[i] = make_uint4(0, 0, 0, 0);
-        r.sz = 0u;
-        return;
-    }
-    const size_t row = pool_row(jb.pool, page, head, key);
-    const uint4* p = reinterpret_cast<const uint4*>(codes + row * kQ4Bytes);
-#pragma unroll
-    for (int i = 0; i < 4; i++) asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.c[i].x), "=r"(r.c[i].y), "=r"(r.c[i].z), "=r"(r.c[i].w) : "l"(p + i));
-    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r.sz) : "l"(scale + row));
-}
 FV_DEV uint32_t add_f16x2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -515,97 +505,159 @@ FV_DEV uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
-// 16-byte piece c (8 values) of row r of a 128 x 128 tile in two 64-column panels with the 128-byte swizzle.
-FV_DEV uint32_t swizzled(uint32_t tile, int r, int c) {
-    return tile + (uint32_t)(c >> 3) * fvattn::kPanelBytes + 128u * (uint32_t)r + 16u * (uint32_t)((c ^ r) & 7);
+FV_DEV uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
+    return r;
 }
 FV_DEV void store_piece(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-// One row of codes as f16 values zero + step code: a code n goes into the mantissa of 1024 (unit 1), 1032 off is n - 8
-// exactly, and one fused multiply-add rounds once.
-FV_DEV void expand_row(const CodeRow& r, uint32_t tile, int row) {
-    const float step = __uint_as_float(r.sz << 16), zero = __uint_as_float(r.sz & 0xffff0000u);
+// The unit of the expander's work: 8 neighbouring rows, a quarter (32 values, one 16-byte load) a lane.  Piece j (8 values) of
+// quarter q of a row goes to piece_base(...) ^ (j << 4): the 128 x 128 tile has two 64-column panels, and the 128-byte
+// swizzle puts piece c of row r into slot (c ^ r) & 7 of its panel's row.
+FV_DEV uint32_t piece_base(uint32_t tile, int row, int q) {
+    return tile + (uint32_t)(q >> 1) * fvattn::kPanelBytes + 128u * (uint32_t)row + 16u * (uint32_t)(((4 * (q & 1)) ^ row) & 7);
+}
+// Eight values of a word stand in a piece in the order 0 4 1 5 2 6 3 7: the pairs that one mask gives.  Q's pieces get the
+// same order (the sum over d does not care), and the output's columns are put back when they are stored.
+// f16 values zero + step code: a nibble is or-ed into 1024's mantissa (unit 1) where it lies, 1024 + n or 1024 + 16 n, an
+// addition or multiply-add makes it n - 8 exactly, and one more multiply-add rounds once.
+FV_DEV void expand_unit(uint4 c, uint32_t sz, uint32_t base, int q) {
+    const float step = __uint_as_float(sz << 16), zero = __uint_as_float(sz & 0xffff0000u);
     const uint32_t s2 = pack_f16x2(step, step), z2 = pack_f16x2(zero, zero);
+    // (Quarters 0 and 2, 1 and 3 meet in the same banks, in different panels: the upper two take their words in the order 2 3 0 1.)
+    const bool swap = q >= 2;
+    const uint32_t word[4] = {swap ? c.z : c.x, swap ? c.w : c.y, swap ? c.x : c.z, swap ? c.y : c.w};
+    base ^= swap ? 32u : 0u;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t word[4] = {r.c[i].x, r.c[i].y, r.c[i].z, r.c[i].w};
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t even = word[j], odd = word[j] >> 4;
-            uint32_t h[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {  // bytes k of both: values 2 k and 2 k + 1 of this piece
-                const uint32_t pair = __byte_perm(even, odd, (uint32_t)(k | (k << 4) | ((4 + k) << 8) | ((4 + k) << 12)));
-                h[k] = fma_f16x2(add_f16x2((pair & 0x000f000fu) | 0x64006400u, 0xe408e408u), s2, z2);
-            }
-            store_piece(swizzled(tile, row, 4 * i + j), h[0], h[1], h[2], h[3]);
-        }
+    for (int j = 0; j < 4; j++) {
+        const uint32_t w = word[j], v = w >> 8;
+        const uint32_t h0 = add_f16x2(and_or(w, 0x000f000fu, 0x64006400u), 0xe408e408u);               // - 1032
+        const uint32_t h1 = fma_f16x2(and_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd480d480u);  // / 16 - 72
+        const uint32_t h2 = add_f16x2(and_or(v, 0x000f000fu, 0x64006400u), 0xe408e408u);
+        const uint32_t h3 = fma_f16x2(and_or(v, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd480d480u);
+        store_piece(base ^ (16u * j), fma_f16x2(h0, s2, z2), fma_f16x2(h1, s2, z2), fma_f16x2(h2, s2, z2), fma_f16x2(h3, s2, z2));
     }
 }
-FV_DEV void chunk_expander(const ChunkJob& jb, uint32_t sbase, int row, int lane, const ChunkWait& wait) {
+// Six warps, a pair's 32 units dealt in turn.  (With one key row a lane in four warps, page look-ups and loads of their own, the expansion
+// took as long as one and a half tiles' products: block of 4 680 rows x 12 heads over 28 080 keys 1 294 us against 958 us with bf16
+// pages; look-ups and loads are the loader's since.)
+FV_DEV void chunk_expander(const ChunkJob& jb, uint32_t sbase, int wid, int lane, const ChunkWait& wait) {
     using namespace fvattn;
+    using R = Roles<true>;
+    constexpr int kW = R::kExpanders;
     uint32_t qn = 0, kvn = 0;
-    const int row_tok = row / jb.group, row_head = row - row_tok * jb.group;
+    const int r8 = lane >> 2, q = lane & 3;  // this lane's row of a unit and its quarter
     auto ok_all = [&](uint32_t bar, uint32_t parity) { return __all_sync(fvpg::kFullWarp, wait(bar, parity)) != 0; };
     auto arrive = [&](uint32_t bar) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor cores read what was stored
         warp_arrive(bar, lane);
     };
     auto load_q = [&](const Work& w, int tile) -> bool {
-        const uint32_t slot = qn % kQSlots, use = qn / kQSlots;
+        const uint32_t slot = qn % R::kQ, use = qn / R::kQ;
         if (use > 0 && !ok_all(sbase + Smem::q_free + 8u * slot, (use - 1u) & 1u)) return false;
         const uint32_t dst = sbase + Smem::q + slot * kSlotBytes;
-        const int tok = w.tok0 + tile * jb.tile_tokens + row_tok;
-        const bool live = row_tok < jb.tile_tokens && tok < w.seq.nq;
-        const uint16_t* p = jb.q + (long long)(w.seq.q0 + (live ? tok : 0)) * jb.q_tok + (long long)(w.head * jb.group + row_head) * jb.q_head;
-#pragma unroll 4
-        for (int c = 0; c < 16; c++) {
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (live) u = __ldg(reinterpret_cast<const uint4*>(p) + c);
-            auto half2 = [](uint32_t x) { return pack_f16x2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); };
-            store_piece(swizzled(dst, row, c), half2(u.x), half2(u.y), half2(u.z), half2(u.w));
+#pragma unroll 1
+        for (int u = wid; u < 16; u += kW) {
+            const int row = 8 * u + r8, row_tok = row / jb.group, tok = w.tok0 + tile * jb.tile_tokens + row_tok;
+            const bool live = row_tok < jb.tile_tokens && tok < w.seq.nq;
+            const uint16_t* p = jb.q + (long long)(w.seq.q0 + (live ? tok : 0)) * jb.q_tok +
+                                (long long)(w.head * jb.group + (live ? row - row_tok * jb.group : 0)) * jb.q_head + 32 * q;
+            const uint32_t base = piece_base(dst, row, q);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (live) x = __ldg(reinterpret_cast<const uint4*>(p) + j);
+                auto low = [](uint32_t a, uint32_t b) { return pack_f16x2(__uint_as_float(a << 16), __uint_as_float(b << 16)); };
+                auto high = [](uint32_t a, uint32_t b) { return pack_f16x2(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u)); };
+                store_piece(base ^ (16u * j), low(x.x, x.z), high(x.x, x.z), low(x.y, x.w), high(x.y, x.w));
+            }
         }
         arrive(sbase + Smem::q_full + 8u * slot);
         qn++;
         return true;
     };
-    auto key_page = [&](const Work& w, int j) -> int {
-        const int key = w.key(j) + row;
-        return w.sees(key) ? page_of(jb.pool, jb.batch, w.s, key) : -1;
+    ChunkDeal deal;
+    Work w;
+    while (deal.next(jb, w, false)) {
+        if (!load_q(w, 0) || !load_q(w, 1)) return;
+        for (int j = 0; j <= w.n; j++) {
+            const uint32_t slot = kvn % kKvPairs, use = kvn / kKvPairs;  // (as many code stages as pair slots)
+            if (!ok_all(sbase + kCodeFull + 8u * slot, use & 1u)) return;
+            if (use > 0 && !ok_all(sbase + Smem::kv_free + 8u * slot, (use - 1u) & 1u)) return;
+            const uint32_t codes = sbase + kCodes + slot * 16384u, scales = sbase + kScales + slot * 1024u;
+            const uint32_t dst = sbase + Smem::kv + slot * 2u * kSlotBytes;
+            const int v0 = j > 0 ? w.key(j - 1) : 0, k0 = j < w.n ? w.key(j) : 0;
+            const bool v_whole = j > 0 && w.whole(v0), k_whole = j < w.n && w.whole(k0);
+#pragma unroll 2
+            for (int u = wid; u < 32; u += kW) {  // units 0-15: V(j-1), 16-31: K(j)
+                const bool is_k = u >= 16;
+                if (is_k ? j == w.n : j == 0) continue;
+                const int row = 8 * (u & 15) + r8;
+                uint4 c;
+                uint32_t sz;
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(c.x), "=r"(c.y), "=r"(c.z), "=r"(c.w) : "r"(codes + 512u * u + 16u * lane) : "memory");
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sz) : "r"(scales + 32u * u + 4u * r8) : "memory");
+                // A key that the item does not see counts as zeros whatever memory holds.
+                if (!(is_k ? k_whole : v_whole) && !w.sees((is_k ? k0 : v0) + row)) sz = 0u;
+                expand_unit(c, sz, piece_base(dst + (is_k ? kSlotBytes : 0u), row, q), q);
+            }
+            arrive(sbase + Smem::kv_full + 8u * slot);
+            if (lane == 0) mbar_arrive(sbase + kCodeFree + 8u * slot);  // (arrive() has met the warp: its reads are done)
+            kvn++;
+        }
+    }
+}
+
+// The codes: one lane per page box brings its rows of K(j) and of V(j-1) and their scales by bulk copies (a page holds them as one
+// run each).  Boxes of which the item sees nothing, and pages outside the pool, are left out: the expander zeroes what is not seen.
+FV_DEV void chunk_code_loader(const ChunkJob& jb, uint32_t sbase, int lane, const ChunkWait& wait) {
+    using namespace fvattn;
+    uint32_t kvn = 0;
+    auto ok_all = [&](uint32_t bar, uint32_t parity) { return __all_sync(fvpg::kFullWarp, wait(bar, parity)) != 0; };
+    const int boxes = kChunkTile / jb.box_rows;
+    auto box_row = [&](const Work& w, int k0) -> long long {  // pool row of this lane's box, -1: none
+        if (lane >= boxes) return -1;
+        const int a = k0 + lane * jb.box_rows, b = a + jb.box_rows;
+        if (!((a < w.span.hi && b > w.span.lo) || a < w.span.sink)) return -1;
+        const int page = page_of(jb.pool, jb.batch, w.s, a);
+        return page < 0 ? -1 : (long long)pool_row(jb.pool, page, w.head, a);
     };
     ChunkDeal deal;
-    Work w, nw;
+    Work w;
     bool ok = true;
-    bool have = deal.next(jb, w, false);
-    if (have) ok = load_q(w, 0) && load_q(w, 1);
-    while (ok && have) {
-        const bool more = deal.next(jb, nw, false);
-        if (more) ok = load_q(nw, 0);
-        CodeRow kc, vc;
-        int page = key_page(w, 0), ahead = w.n > 1 ? key_page(w, 1) : -1;
-        load_codes(kc, jb.pool.k, jb.pool.k_scale, jb, page, w.head, w.key(0) + row);
-        for (int j = 0; ok && j <= w.n; j++) {
+    while (ok && deal.next(jb, w, false)) {
+        long long row = box_row(w, w.key(0)), prev = -1;
+        for (int j = 0; j <= w.n; j++) {
+            const long long ahead = j + 1 < w.n ? box_row(w, w.key(j + 1)) : -1;  // (the look-up's latency runs under the wait)
             const uint32_t slot = kvn % kKvPairs, use = kvn / kKvPairs;
-            if (use > 0 && !ok_all(sbase + Smem::kv_free + 8u * slot, (use - 1u) & 1u)) { ok = false; break; }
-            const uint32_t dst = sbase + Smem::kv + slot * 2u * kSlotBytes;
-            // K(j) out of registers, then the loads of K(j + 1); V(j - 1) likewise, then those of V(j).
-            if (j < w.n) {
-                expand_row(kc, dst + kSlotBytes, row);
-                if (j + 1 < w.n) load_codes(kc, jb.pool.k, jb.pool.k_scale, jb, ahead, w.head, w.key(j + 1) + row);
+            if (use > 0 && !ok_all(sbase + kCodeFree + 8u * slot, (use - 1u) & 1u)) { ok = false; break; }
+            const bool k = j < w.n && row >= 0, v = j > 0 && prev >= 0;
+            const uint32_t tiles = __popc(__ballot_sync(fvpg::kFullWarp, k)) + __popc(__ballot_sync(fvpg::kFullWarp, v));
+            const uint32_t bar = sbase + kCodeFull + 8u * slot, code_bytes = (uint32_t)jb.box_rows * kQ4Bytes, scale_bytes = (uint32_t)jb.box_rows * 4;
+            if (lane == 0) mbar_expect_tx(bar, tiles * (code_bytes + scale_bytes));
+            __syncwarp();
+            const uint32_t codes = sbase + kCodes + slot * 16384u + lane * code_bytes, scales = sbase + kScales + slot * 1024u + lane * scale_bytes;
+            if (v) {
+                bulk_load(codes, jb.pool.v + prev * kQ4Bytes, code_bytes, bar);
+                bulk_load(scales, jb.pool.v_scale + prev, scale_bytes, bar);
             }
-            if (j > 0) expand_row(vc, dst, row);
-            arrive(sbase + Smem::kv_full + 8u * slot);
+            if (k) {
+                bulk_load(codes + 8192u, jb.pool.k + row * kQ4Bytes, code_bytes, bar);
+                bulk_load(scales + 512u, jb.pool.k_scale + row, scale_bytes, bar);
+            }
             kvn++;
-            if (j < w.n) {
-                load_codes(vc, jb.pool.v, jb.pool.v_scale, jb, page, w.head, w.key(j) + row);
-                page = ahead;
-                ahead = j + 2 < w.n ? key_page(w, j + 2) : -1;
-            }
+            prev = row;
+            row = ahead;
         }
-        if (ok && more) ok = load_q(nw, 1);
-        w = nw;
-        have = more;
+    }
+    __syncwarp();
+    if (lane == 0) {  // copies in flight must land before the CTA's shared memory goes away
+        for (uint32_t s = 0; s < (uint32_t)kKvPairs && s < kvn; s++) {
+            const uint32_t last = ((kvn - 1u - s) / kKvPairs) * kKvPairs + s;
+            mbar_drain(sbase + kCodeFull + 8u * s, (last / kKvPairs) & 1u);
+        }
     }
 }
 
@@ -621,8 +673,8 @@ FV_DEV void chunk_issuer(const ChunkJob& jb, uint32_t sbase, uint32_t tmem, cons
     Work w;
     bool ok = true;
     while (ok && deal.next(jb, w, false)) {
-        const uint32_t qa = qn % kQSlots, qb = (qn + 1u) % kQSlots;
-        const uint32_t qa_par = (qn / kQSlots) & 1u, qb_par = ((qn + 1u) / kQSlots) & 1u;
+        const uint32_t qa = qn % Roles<Q4>::kQ, qb = (qn + 1u) % Roles<Q4>::kQ;
+        const uint32_t qa_par = (qn / Roles<Q4>::kQ) & 1u, qb_par = ((qn + 1u) / Roles<Q4>::kQ) & 1u;
         qn += 2;
         const uint64_t qd_a = umma_desc_sw128(sbase + Smem::q + qa * kSlotBytes, 16, 1024);
         const uint64_t qd_b = umma_desc_sw128(sbase + Smem::q + qb * kSlotBytes, 16, 1024);
@@ -677,7 +729,7 @@ FV_DEV void chunk_persistent(const CUtensorMap* mq, const CUtensorMap* mk, const
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Smem::abort_flag);
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + Smem::tmem_slot);
     if (threadIdx.x == 0) {
-        const uint32_t producers = Q4 ? 4 : 1;  // the expander's four warps, or one transaction count
+        const uint32_t producers = Q4 ? R::kExpanders : 1;  // the expander's warps, or one transaction count
         for (int s = 0; s < kQSlots; s++) {
             mbar_init(sbase + Smem::q_full + 8u * s, producers);
             mbar_init(sbase + Smem::q_free + 8u * s, 1);
@@ -686,6 +738,8 @@ FV_DEV void chunk_persistent(const CUtensorMap* mq, const CUtensorMap* mk, const
             mbar_init(sbase + Smem::kv_full + 8u * s, producers);
             mbar_init(sbase + Smem::kv_free + 8u * s, Q4 ? 1 : 2);  // the issuer's commit (and the fixer)
             mbar_init(sbase + kVFixed + 8u * s, 1);
+            mbar_init(sbase + kCodeFull + 8u * s, 1);
+            mbar_init(sbase + kCodeFree + 8u * s, R::kExpanders);
         }
         for (int t = 0; t < 2; t++) {
             mbar_init(sbase + Smem::s_ready + 8u * t, 1);
@@ -719,7 +773,8 @@ FV_DEV void chunk_persistent(const CUtensorMap* mq, const CUtensorMap* mk, const
         if (warp == R::kIssuer) {
             if (lane == 0) chunk_issuer<Q4>(jb, sbase, tmem, waiter(2));
         } else if (Q4) {
-            if (warp >= R::kExpander) chunk_expander(jb, sbase, 32 * (warp - R::kExpander) + lane, lane, waiter(1));
+            if (warp >= R::kExpander) chunk_expander(jb, sbase, warp - R::kExpander, lane, waiter(6));
+            else if (warp == R::kLoader) chunk_code_loader(jb, sbase, lane, waiter(1));
         } else if (warp == R::kLoader) {
             chunk_loader(mq, mk, mv, jb, sbase, lane, waiter(1));
         } else if (warp == R::kFixer) {
