@@ -797,15 +797,64 @@ fv_paged_chunk_kernel(const __grid_constant__ CUtensorMap mq, const __grid_const
 #endif
 }
 
+// The items that the chunk kernel's runs cut: the part that begins the item lies with the CTA that `split` belongs to, the
+// others with the CTAs after it.  A warp a row, parts in their order.
+constexpr int kJoinBlocks = 8;  // of a split item's 256 rows
+__global__ void __launch_bounds__(kAttnThreads) fv_paged_join_kernel(const ChunkJob jb) {
+    const int lane = threadIdx.x & 31, c = blockIdx.x / kJoinBlocks, block = blockIdx.x - c * kJoinBlocks;
+    const ChunkSplit sp = jb.split[c];
+    if (!sp.valid) return;
+    constexpr int kRowsHere = 2 * kChunkRows / kJoinBlocks / kWarps;
+    for (int i = 0; i < kRowsHere; i++) {
+        const int r = (block * kRowsHere + i) * kWarps + (threadIdx.x >> 5), tile = r / kChunkRows, row = r - tile * kChunkRows;
+        const int row_tok = row / jb.group, tok = sp.tok0 + tile * jb.tile_tokens + row_tok;
+        if (row_tok >= jb.tile_tokens || tok >= sp.nq) continue;
+        // Walks the item's parts: slot of each, or -1 behind the last one.
+        auto part = [&](int& k) -> long long {
+            if (k == c) return 2ll * c + 1;
+            for (; k < sp.ctas; k++) {
+                const long long y = sp.total * k / sp.ctas - sp.start, y1 = sp.total * (k + 1) / sp.ctas - sp.start;
+                if (y >= sp.cost) break;
+                const int t0 = tile_behind((int)y, sp.tiles), t1 = tile_behind((int)min(y1, (long long)sp.cost), sp.tiles);
+                if (t0 >= sp.tiles) break;
+                if (t1 > t0) return 2ll * k;
+            }
+            return -1;
+        };
+        float top = neg_inf();
+        long long slot;
+        for (int k = c; (slot = part(k)) >= 0; k++) top = fmaxf(top, jb.part_lse[slot * 2 * kChunkRows + r]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+        if (top != neg_inf()) {
+            for (int k = c; (slot = part(k)) >= 0; k++) {
+                const float w = fvp::ex2(jb.part_lse[slot * 2 * kChunkRows + r] - top);
+                if (w == 0.f) continue;
+                const float4 x = *reinterpret_cast<const float4*>(jb.part_o + (slot * 2 * kChunkRows + r) * kD + 4 * lane);
+                sum += w;
+                acc.x = fmaf(w, x.x, acc.x);
+                acc.y = fmaf(w, x.y, acc.y);
+                acc.z = fmaf(w, x.z, acc.z);
+                acc.w = fmaf(w, x.w, acc.w);
+            }
+            const float inv = 1.f / sum;
+            acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
+        }
+        const size_t out = (size_t)(sp.q0 + tok) * jb.heads + sp.head * jb.group + (row - row_tok * jb.group);
+        *reinterpret_cast<uint2*>(jb.out + out * kD + 4 * lane) = make_uint2(fvp::pack_bf16x2(acc.x, acc.y), fvp::pack_bf16x2(acc.z, acc.w));
+    }
+}
+
 // ---- host --------------------------------------------------------------------------------------------------------------
 
 struct Shape {
     bool chunk;  // the tensor-core kernel for long chunks
     int splits, row_blocks, nt, tile_tokens;
     bool cluster;
+    int ctas;  // of the chunk kernel
 };
 // How a call is cut.  Few rows per kv head: blocks of 8 or 16 rows, and the keys in `splits` ranges so that all SMs have
-// work.  From kChunkFrom rows on: items of 2 x 128 rows, the keys cut where that evens out the waves.
+// work.  From kChunkFrom rows on: items of 2 x 128 rows, one CTA per SM.
 constexpr int kChunkFrom = 33;
 static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads, const Mask& m, int sms) {
     Shape s;
@@ -815,27 +864,13 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads,
     s.tile_tokens = s.chunk ? kChunkRows / group : 0;
     s.cluster = false;
     if (s.chunk) {
-        long long seen = b->max_kv;
-        if (m.block > 0 && m.window > 0) {
-            const long long some = ((long long)m.window + m.sink + 1) * m.block + 2 * s.tile_tokens;
-            seen = some < seen ? some : seen;
-        }
-        const int tiles = (int)((seen + kChunkTile - 1) / kChunkTile);
         s.nt = 0;
-        s.row_blocks = (b->max_q + 2 * s.tile_tokens - 1) / (2 * s.tile_tokens);
-        const long long items = (long long)b->seqs * kv->kv_heads * s.row_blocks;
-        // Time of a cut, in key tiles of a CTA: whole waves of equal items, each with a fixed cost of about four tiles,
-        // and the merge's traffic (a part is 516 bytes a row; a key tile takes about 1.5 us, 7.5 MB at 5 TB/s).
-        double best = 0;
         s.splits = 1;
-        for (int n = 1; n <= 16 && (n == 1 || tiles >= 4 * n); n++) {
-            const long long waves = (items * n + sms - 1) / sms;
-            const double cost = (double)waves * ((tiles + n - 1) / n + 4) + (n > 1 ? 2.0 + (double)b->max_q * b->seqs * heads * n * 1032.0 / 7.5e6 : 0.0);
-            if (n == 1 || cost < 0.95 * best) {
-                best = cost;
-                s.splits = n;
-            }
-        }
+        s.row_blocks = (b->max_q + 2 * s.tile_tokens - 1) / (2 * s.tile_tokens);
+        // (an upper bound of the line's length: with little work no more CTAs are launched than may find a run)
+        const long long longest = (long long)b->seqs * kv->kv_heads * s.row_blocks * ((b->max_kv + kChunkTile - 1) / kChunkTile + kItemCost);
+        const long long most = longest / kLeastRun;
+        s.ctas = (int)(most < 1 ? 1 : most < sms ? most : sms);
         return s;
     }
     s.nt = rows > 8 ? 2 : 1;
@@ -860,7 +895,13 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads,
     return s;
 }
 
-static int launch_chunk(cudaStream_t st, const fv_paged_kv* kv, const AttnArgs& a, const Shape& s, int dev, int sms) {
+// Scratch of a call: the parts of split rows (f32 and a log-sum-exp), for the chunk kernel two slots of 256 rows a CTA.
+static size_t workspace_of(const Shape& s, size_t rows) {
+    if (s.chunk) return (size_t)s.ctas * (2 * 2 * kChunkRows * (kD + 1) * sizeof(float) + sizeof(ChunkSplit));
+    return s.splits > 1 && !s.cluster ? s.splits * rows * (kD + 1) * sizeof(float) : 0;
+}
+
+static int launch_chunk(cudaStream_t st, const fv_paged_kv* kv, const AttnArgs& a, const Shape& s, int dev) {
     const bool q4 = kv->format == FV_PAGE_Q4;
     ChunkJob jb{};
     jb.pool = a.pool;
@@ -870,19 +911,19 @@ static int launch_chunk(cudaStream_t st, const fv_paged_kv* kv, const AttnArgs& 
     jb.q_tok = a.q_tok;
     jb.q_head = a.q_head;
     jb.out = a.out;
+    const size_t slots = 2 * (size_t)s.ctas * 2 * kChunkRows;  // rows of parts
     jb.part_o = a.part_o;
-    jb.part_lse = a.part_lse;
+    jb.part_lse = jb.part_o + slots * kD;
+    jb.split = reinterpret_cast<ChunkSplit*>(jb.part_lse + slots);
     jb.wait_status = a.batch.status - 1;
     jb.wait_cycles = FV_WAIT_CYCLES;
     jb.heads = a.heads;
     jb.group = a.group;
     jb.tile_tokens = s.tile_tokens;
-    jb.splits = s.splits;
-    jb.planes = a.batch.seqs * a.pool.kv_heads;
     jb.q_blocks = s.row_blocks;
-    const long long items = (long long)jb.planes * s.row_blocks * s.splits;
-    if (items > 0x3fffffffll) return FV_DECLINED;
-    jb.items = (int)items;
+    const long long groups = (long long)a.batch.seqs * s.row_blocks;
+    if (groups > 0x3fffffffll) return FV_DECLINED;
+    jb.groups = (int)groups;
     jb.box_rows = kv->page_rows < kChunkTile ? kv->page_rows : kChunkTile;
     jb.sl2 = a.sl2;
     CUtensorMap mq{}, mk{}, mv{};
@@ -910,12 +951,16 @@ static int launch_chunk(cudaStream_t st, const fv_paged_kv* kv, const AttnArgs& 
             attr_set[dev][q4] = true;
         }
     }
-    const unsigned grid = (unsigned)(items < sms ? items : sms);
+    const unsigned grid = (unsigned)s.ctas;
     if (q4) fv_paged_chunk_kernel<true><<<grid, Roles<true>::kThreads, kChunkSmem, st>>>(mq, mk, mv, jb);
     else fv_paged_chunk_kernel<false><<<grid, Roles<false>::kThreads, kChunkSmem, st>>>(mq, mk, mv, jb);
     FV_CUDA(cudaGetLastError());
-    fvrt::ran(fvrt::kLogPagedChunk, "paged attention: fv_paged_chunk_kernel<%s> (sm_100a tcgen05, persistent, %u CTAs) %d sequences x %d heads / %d, %d key ranges",
-              q4 ? "4 bits" : "bf16", grid, a.batch.seqs, a.heads, a.pool.kv_heads, s.splits);
+    if (grid > 1) {
+        fv_paged_join_kernel<<<grid * kJoinBlocks, kAttnThreads, 0, st>>>(jb);
+        FV_CUDA(cudaGetLastError());
+    }
+    fvrt::ran(fvrt::kLogPagedChunk, "paged attention: fv_paged_chunk_kernel<%s> (sm_100a tcgen05, persistent, %u CTAs) %d sequences x %d heads / %d",
+              q4 ? "4 bits" : "bf16", grid, a.batch.seqs, a.heads, a.pool.kv_heads);
     return FV_RAN;
 }
 
@@ -944,7 +989,7 @@ extern "C" size_t fv_paged_attn_workspace_bytes(const fv_paged_kv* kv, const fv_
         fvrt::sm_count(dev, &sms) != FV_RAN)
         return 0;
     const Shape s = shape_of(kv, b, heads, m, sms);
-    return s.splits > 1 && !s.cluster ? (size_t)s.splits * tokens * heads * (kD + 1) * sizeof(float) : 0;
+    return workspace_of(s, (size_t)tokens * heads);
 }
 
 extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* b, int tokens, const void* q, long long q_tok,
@@ -970,9 +1015,9 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
     if (rc != FV_RAN) return rc;
     const Shape s = shape_of(kv, b, heads, a.mask, sms);
     const size_t rows = (size_t)tokens * heads;
-    if (s.splits > 1 && !s.cluster && (!workspace || workspace_bytes < s.splits * rows * (kD + 1) * sizeof(float)))
-        return fvrt::fail(FV_ERR_INVALID, "paged attention: workspace of %zu bytes, %zu needed", workspace_bytes,
-                          s.splits * rows * (kD + 1) * sizeof(float));
+    const size_t need = workspace_of(s, rows);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fvrt::fail(FV_ERR_INVALID, "paged attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     a.q = (const uint16_t*)q;
     a.q_tok = q_tok;
     a.q_head = q_head;
@@ -990,13 +1035,7 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
     if (grid > 0x7fffffffll || (long long)rows > 0x7fffffffll) return FV_DECLINED;
     cudaStream_t st = (cudaStream_t)stream;
     if (s.chunk) {
-        rc = launch_chunk(st, kv, a, s, dev, sms);
-        if (rc != FV_RAN) return rc;
-        if (s.splits > 1) {
-            fv_paged_merge_kernel<<<(unsigned)((rows + kWarps - 1) / kWarps), kAttnThreads, 0, st>>>(a);
-            FV_CUDA(cudaGetLastError());
-        }
-        return FV_RAN;
+        return launch_chunk(st, kv, a, s, dev);
     }
     const bool q4 = kv->format == FV_PAGE_Q4;
     void (*fn)(AttnArgs);

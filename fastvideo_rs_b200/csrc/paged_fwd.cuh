@@ -1,10 +1,15 @@
 // Attention of long chunks over a paged K/V cache on the tensor cores (tcgen05), head dim 128.
 //
-// The skeleton is that of the dense kernel (attn_fwd.cuh): persistent CTAs, work items of two 128-row tiles dealt in snake
-// order, the K/V ring in pairs [V(j-1) | K(j)], one issuing thread, one query row per softmax thread, a softmax without a
-// maximum pass whose row sum guards the reference.  What differs:
-//   * A work item is (sequence, kv head, rows, key range).  A row tile holds 128 / g tokens of the g heads that share the
-//     kv head, so shared heads cost no extra pass over the keys; lengths, rows and the page table are read on the device.
+// The skeleton is that of the dense kernel (attn_fwd.cuh): persistent CTAs, work items of two 128-row tiles, the K/V ring in
+// pairs [V(j-1) | K(j)], one issuing thread, one query row per softmax thread, a softmax without a maximum pass whose row sum
+// guards the reference.  What differs:
+//   * A work item is (sequence, rows, kv head).  A row tile holds 128 / g tokens of the g heads that share the kv head, so
+//     shared heads cost no extra pass over the keys; lengths, rows and the page table are read on the device.
+//   * Items are of very different lengths (ragged sequences, causal rows) and seldom a multiple of the SMs.  So the items are
+//     laid end to end, each as long as its key tiles and kItemCost more, and every CTA takes an equal run of that line, which
+//     may begin and end inside an item.  Parts of an item go to a workspace with their log-sum-exp and one small kernel joins
+//     them, in order.  (Whole items dealt in snake order, cut in equal key ranges by a cost model, took 912 us for 4 680 rows x
+//     12 heads over 28 080 keys -- 228 items on 148 SMs -- and 512 us for three ragged chunks of 600 items.)
 //   * Key tiles are 128 keys at multiples of 128: those of the sinks, then those of the window.  Pages outside are not
 //     touched.
 //   * bf16 pages: one lane of the loader warp per page (or half a page of 256 rows) issues that page's TMA boxes; boxes
@@ -32,12 +37,26 @@ struct ChunkJob {
     const uint16_t* q;
     long long q_tok, q_head;
     uint16_t* out;
-    float *part_o, *part_lse;  // splits > 1: [splits, tokens * heads, 128] and [splits, tokens * heads]
+    float *part_o, *part_lse;  // [2 per CTA, 256 rows, 128] and [2 per CTA, 256]: a part that does not begin its item, one that does
+    struct ChunkSplit* split;  // [CTA]: the item that begins in the CTA's run and ends in another's
     int* wait_status;          // the first status word
     long long wait_cycles;
-    int heads, group, tile_tokens, splits, planes, q_blocks, items, box_rows;
+    int heads, group, tile_tokens, q_blocks, groups, box_rows;  // groups: sequences x row blocks
     float sl2;
 };
+constexpr int kItemCost = 4;   // what an item costs beside its key tiles, in key tiles: the pipeline fills and drains, the output
+constexpr int kLeastRun = 8;   // the shortest run worth a CTA
+struct ChunkSplit {
+    int valid, q0, nq, tok0, head, tiles, cost, ctas;
+    long long start, total;  // where the item begins on the line, and how long the line is
+};
+// The first key tile of an item that lies behind position y of its length: the fixed cost comes first, and no part is a
+// sliver of one tile.
+__host__ __device__ inline int tile_behind(int y, int tiles) {
+    if (y >= tiles + kItemCost) return tiles;
+    const int t = y - kItemCost;
+    return t < 2 ? 0 : tiles - t < 2 ? tiles : t;
+}
 
 #if defined(__CUDA_ARCH_FEAT_SM100_ALL) || defined(__CUDA_ARCH_FEAT_SM103_ALL) || !defined(__CUDA_ARCH__)
 
@@ -55,7 +74,9 @@ using namespace fvp;
 constexpr uint32_t kVFixed = Smem::total;
 constexpr uint32_t kCodeFull = kVFixed + 8 * fvattn::kKvPairs, kCodeFree = kCodeFull + 16;
 constexpr uint32_t kScales = (kCodeFree + 16 + 15) & ~15u;      // [stage][V | K][128 keys] (step, zero)
-constexpr uint32_t kChunkSmem = kScales + 2 * 1024;
+constexpr uint32_t kRun = kScales + 2 * 1024;  // this CTA's run
+constexpr uint32_t kScratch = kRun + 64;      // find_run's
+constexpr uint32_t kChunkSmem = kScratch + 256;
 constexpr uint32_t kCodes = Smem::q + 2 * fvattn::kSlotBytes;   // [stage][V | K][128 keys][64 bytes]
 static_assert(kVFixed % 8 == 0 && kChunkSmem <= 232448 && fvattn::kQSlots == 3 && fvattn::kSlotBytes == 32768, "shared memory");
 static_assert(fvattn::kKvPairs == 2 && fvattn::kEarlyKeys == 128, "the ring in pairs, P handed over whole");
@@ -73,8 +94,9 @@ struct Roles {
 struct Work {
     Seq seq;
     Span span;
-    int s, head, split, tok0;  // first token of the item inside the call's tokens of the sequence
-    int sinks, first, u0, n;   // its key tiles: number u0 + j of the row of sink tiles, then window tiles
+    int s, head, tok0;          // first token of the item inside the call's tokens of the sequence
+    int sinks, first, tiles;    // its key tiles: those of the sinks, then those of the window
+    int u0, n;                  // this CTA's part of them
     FV_DEV int pos0() const { return seq.len - seq.nq; }
     FV_DEV int key(int j) const {
         const int u = u0 + j;
@@ -82,38 +104,118 @@ struct Work {
     }
     FV_DEV bool sees(int j) const { return (j >= span.lo && j < span.hi) || j < span.sink; }
     FV_DEV bool whole(int k0) const { return (k0 >= span.lo && k0 + kChunkTile <= span.hi) || k0 + kChunkTile <= span.sink; }
+    FV_DEV bool begins() const { return u0 == 0; }
+    FV_DEV bool ends() const { return u0 + n == tiles; }
 };
-// False: item i has no rows.
-FV_DEV bool work_at(const ChunkJob& jb, int i, Work& w) {
-    const int per = jb.planes * jb.splits;
-    const int qb = jb.q_blocks - 1 - i / per, rest = i % per;  // (the last rows see the most keys: heaviest first)
-    w.split = rest % jb.splits;
-    const int plane = rest / jb.splits;
-    w.head = plane % jb.pool.kv_heads;
-    w.s = plane / jb.pool.kv_heads;
+// Group number i (a sequence's row block, an item for each of its kv heads): its rows and tiles, and the cost of one item;
+// 0 when there are no such rows.
+FV_DEV int group_at(const ChunkJob& jb, int i, Work& w) {
+    w.s = i / jb.q_blocks;
     w.seq = seq_of(jb.batch, w.s);
-    w.tok0 = qb * 2 * jb.tile_tokens;
-    if (w.tok0 >= w.seq.nq) return false;
+    w.tok0 = (i - w.s * jb.q_blocks) * 2 * jb.tile_tokens;
+    if (w.tok0 >= w.seq.nq) return 0;
     const int last = min(w.tok0 + 2 * jb.tile_tokens, w.seq.nq) - 1;
     w.span = span_of(jb.mask, w.pos0() + w.tok0, w.pos0() + last, w.seq.len);
     w.sinks = (w.span.sink + kChunkTile - 1) / kChunkTile;
     w.first = max(w.span.lo / kChunkTile, w.sinks);
-    const int count = w.sinks + max(0, (w.span.hi + kChunkTile - 1) / kChunkTile - w.first);
-    w.u0 = (int)((long long)count * w.split / jb.splits);
-    w.n = (int)((long long)count * (w.split + 1) / jb.splits) - w.u0;
-    return true;
+    w.tiles = w.sinks + max(0, (w.span.hi + kChunkTile - 1) / kChunkTile - w.first);
+    return w.tiles + kItemCost;
 }
-// The next item of this CTA that has rows (and, unless `empty` is allowed, keys).
-struct ChunkDeal {
-    int round = 0;
-    FV_DEV bool next(const ChunkJob& jb, Work& w, bool empty) {
-        const int g = (int)gridDim.x, c = (int)blockIdx.x;
-        for (;;) {
-            const int i = round * g + ((round & 1) ? g - 1 - c : c);
-            if (round * g >= jb.items) return false;
-            round++;
-            if (i < jb.items && work_at(jb, i, w) && (empty || w.n > 0)) return true;
+// This CTA's run of the line.
+struct Run {
+    long long total, from, to;
+    int ctas, group, head, off;  // CTAs that have runs; the item that `from` lies in and where in it
+};
+// Warp-inclusive sum.
+FV_DEV long long scan_warp(long long x, int lane) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(kFullWarp, x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+// The whole CTA adds up the line (a run of groups a thread) and finds its place on it.  `scratch`: 32 long longs.
+FV_DEV void find_run(const ChunkJob& jb, Run* run, long long* scratch) {
+    const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (int)blockDim.x >> 5;
+    const int per = (jb.groups + (int)blockDim.x - 1) / (int)blockDim.x;
+    const int g0 = min(tid * per, jb.groups), g1 = min(g0 + per, jb.groups);
+    long long mine = 0;
+    Work w;
+    for (int g = g0; g < g1; g++) mine += (long long)group_at(jb, g, w) * jb.pool.kv_heads;
+    const long long incl = scan_warp(mine, lane);
+    if (lane == 31) scratch[warp] = incl;
+    __syncthreads();
+    long long before = 0, total = 0;
+    for (int i = 0; i < warps; i++) {
+        if (i < warp) before += scratch[i];
+        total += scratch[i];
+    }
+    const long long excl = before + incl - mine;
+    const int ctas = (int)max(1ll, min((long long)gridDim.x, total / kLeastRun));
+    const bool idle = (int)blockIdx.x >= ctas;
+    const long long from = idle ? 0 : total * blockIdx.x / ctas, to = idle ? 0 : total * (blockIdx.x + 1) / ctas;
+    if (tid == 0) {
+        run->total = total;
+        run->from = from;
+        run->to = to;
+        run->ctas = ctas;
+    }
+    if (from < to && from >= excl && from < excl + mine) {
+        long long at = excl;
+        for (int g = g0; g < g1; g++) {
+            const int cost = group_at(jb, g, w);
+            const long long all = (long long)cost * jb.pool.kv_heads;
+            if (from < at + all) {
+                run->group = g;
+                run->head = (int)((from - at) / cost);
+                run->off = (int)((from - at) % cost);
+                break;
+            }
+            at += all;
         }
+    }
+    __syncthreads();
+}
+// The items of the run, in order.
+struct Walk {
+    Work g;  // the current group
+    int group, head, off, cost, left;
+    bool known;
+    FV_DEV explicit Walk(const Run& r) : group(r.group), head(r.head), off(r.off), cost(0), left((int)(r.to - r.from)), known(false) {}
+    // The next item with key tiles (`empty`: or with rows that see no key).  *ahead: what is left of the run from where this item
+    // began on the line.
+    FV_DEV bool next(const ChunkJob& jb, Work& w, bool empty, int* ahead = nullptr) {
+        while (left > 0 && group < jb.groups) {
+            if (!known) {
+                cost = group_at(jb, group, g);
+                known = true;
+            }
+            if (cost == 0) {
+                group++;
+                known = false;
+                continue;
+            }
+            const int end = min(cost, off + left);
+            const int t0 = tile_behind(off, g.tiles), t1 = tile_behind(end, g.tiles);
+            w = g;
+            w.head = head;
+            w.u0 = t0;
+            w.n = t1 - t0;
+            if (ahead) *ahead = left + off;
+            left -= end - off;
+            off = end;
+            if (end == cost) {
+                off = 0;
+                if (++head == jb.pool.kv_heads) {
+                    head = 0;
+                    group++;
+                    known = false;
+                }
+            }
+            if (w.n > 0 || (empty && w.tiles == 0 && end == cost)) return true;
+        }
+        return false;
     }
 };
 
@@ -302,7 +404,7 @@ static __device__ __noinline__ void chunk_write(void* base, uint32_t tO, float i
 }
 
 template <bool Q4>
-FV_DEV void chunk_softmax(const ChunkJob& jb, uint32_t sbase, uint32_t tmem, int warp, int lane, const ChunkWait& wait) {
+FV_DEV void chunk_softmax(const ChunkJob& jb, const Run& run, uint32_t sbase, uint32_t tmem, int warp, int lane, const ChunkWait& wait) {
     constexpr float kChunkGuard = Q4 ? 32768.f : fvattn::kGuard;  // a row sum of P above this could leave P's type
     constexpr float kBelow = Q4 ? 6.f : 0.f;                      // the reference starts 2^kBelow below the first maximum
     const int tile = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
@@ -312,9 +414,10 @@ FV_DEV void chunk_softmax(const ChunkJob& jb, uint32_t sbase, uint32_t tmem, int
     const float sl2 = jb.sl2;
     const int row_tok = row / jb.group, row_head = row - row_tok * jb.group;
     uint32_t s_count = 0, o_count = 0;
-    ChunkDeal deal;
+    Walk walk(run);
     Work w;
-    bool more = deal.next(jb, w, true);
+    int ahead = 0;
+    bool more = walk.next(jb, w, true, &ahead);
     while (more) {
         const int tok = w.tok0 + tile * jb.tile_tokens + row_tok;
         const bool live = row_tok < jb.tile_tokens && tok < w.seq.nq;
@@ -363,29 +466,30 @@ FV_DEV void chunk_softmax(const ChunkJob& jb, uint32_t sbase, uint32_t tmem, int
             }
             if (!hot) chunk_careful<Q4>(tS, tO, bt, cols, sl2, j > 0, lane, &rs);
         }
-        const bool have_o = w.n > 0;
-        const int split = w.split;
-        const int out_row = live ? (w.seq.q0 + tok) * jb.heads + w.head * jb.group + row_head : -1;
-        more = deal.next(jb, w, true);  // (looked up while the last product runs)
+        const bool have_o = w.n > 0, begins = w.begins(), part = !(begins && w.ends());
+        const int out_row = !live ? -1 : part ? tile * kChunkRows + row : (w.seq.q0 + tok) * jb.heads + w.head * jb.group + row_head;
+        if (begins && part && threadIdx.x == 0)
+            jb.split[blockIdx.x] = ChunkSplit{1, w.seq.q0, w.seq.nq, w.tok0, w.head, w.tiles, w.tiles + kItemCost, run.ctas, run.to - ahead, run.total};
+        more = walk.next(jb, w, true, &ahead);  // (looked up while the last product runs)
         if (have_o) {
             if (!__all_sync(kFullWarp, wait(bt + Smem::o_ready, o_count & 1u))) return;
             o_count++;
             tc_fence_after();
         }
         const float inv = rs.l > 0.f ? 1.f / rs.l : 0.f;
-        if (jb.splits == 1) {
+        if (!part) {
             chunk_write<Q4, false>(jb.out, tO, inv, out_row, have_o, lane);
         } else {
-            const size_t rows = (size_t)jb.batch.tokens * jb.heads;
-            chunk_write<Q4, true>(jb.part_o + (size_t)split * rows * kD, tO, inv, out_row, have_o, lane);
-            if (out_row >= 0) jb.part_lse[(size_t)split * rows + out_row] = rs.l > 0.f ? rs.m + log2f(rs.l) : neg_inf();
+            const size_t slot = 2 * (size_t)blockIdx.x + (begins ? 1 : 0);
+            chunk_write<Q4, true>(jb.part_o + slot * 2 * kChunkRows * kD, tO, inv, out_row, have_o, lane);
+            if (out_row >= 0) jb.part_lse[slot * 2 * kChunkRows + out_row] = rs.l > 0.f ? rs.m + log2f(rs.l) : neg_inf();
         }
     }
 }
 
 // --------------------------------------------------------------------------------- loader and fixer (bf16 pages)
-FV_DEV void chunk_loader(const CUtensorMap* mq, const CUtensorMap* mk, const CUtensorMap* mv, const ChunkJob& jb, uint32_t sbase,
-                         int lane, const ChunkWait& wait) {
+FV_DEV void chunk_loader(const CUtensorMap* mq, const CUtensorMap* mk, const CUtensorMap* mv, const ChunkJob& jb, const Run& run,
+                         uint32_t sbase, int lane, const ChunkWait& wait) {
     using namespace fvattn;
     uint32_t qn = 0, kvn = 0;
     if (lane == 0) {
@@ -423,13 +527,13 @@ FV_DEV void chunk_loader(const CUtensorMap* mq, const CUtensorMap* mk, const CUt
         tma_load4(at, map, bar, 0, row, head, page);
         tma_load4(at + kPanelBytes, map, bar, 64, row, head, page);
     };
-    ChunkDeal deal;
+    Walk walk(run);
     Work w, nw;
     bool ok = true;
-    bool have = deal.next(jb, w, false);
+    bool have = walk.next(jb, w, false);
     if (have) ok = load_q(w, 0) && load_q(w, 1);
     while (ok && have) {
-        const bool more = deal.next(jb, nw, false);
+        const bool more = walk.next(jb, nw, false);
         if (more) ok = load_q(nw, 0);
         int page = box_page(w, w.key(0)), prev = 0;
         for (int j = 0; ok && j <= w.n; j++) {
@@ -465,12 +569,12 @@ FV_DEV void chunk_loader(const CUtensorMap* mq, const CUtensorMap* mk, const CUt
 }
 
 // Follows the pairs one by one (it has a share in kv_free, so it can neither run ahead of a phase nor miss one).
-FV_DEV void chunk_fixer(const ChunkJob& jb, uint32_t sbase, int lane, const ChunkWait& wait) {
+FV_DEV void chunk_fixer(const ChunkJob& jb, const Run& run, uint32_t sbase, int lane, const ChunkWait& wait) {
     using namespace fvattn;
     uint32_t pn = 0;
-    ChunkDeal deal;
+    Walk walk(run);
     Work w;
-    while (deal.next(jb, w, false)) {
+    while (walk.next(jb, w, false)) {
         for (int j = 0; j <= w.n; j++) {
             const uint32_t slot = pn % kKvPairs;
             if (!__all_sync(fvpg::kFullWarp, wait(sbase + Smem::kv_full + 8u * slot, (pn / kKvPairs) & 1u))) return;
@@ -543,7 +647,7 @@ FV_DEV void expand_unit(uint4 c, uint32_t sz, uint32_t base, int q) {
 // Six warps, a pair's 32 units dealt in turn.  (With one key row a lane in four warps, page look-ups and loads of their own, the expansion
 // took as long as one and a half tiles' products: block of 4 680 rows x 12 heads over 28 080 keys 1 294 us against 958 us with bf16
 // pages; look-ups and loads are the loader's since.)
-FV_DEV void chunk_expander(const ChunkJob& jb, uint32_t sbase, int wid, int lane, const ChunkWait& wait) {
+FV_DEV void chunk_expander(const ChunkJob& jb, const Run& run, uint32_t sbase, int wid, int lane, const ChunkWait& wait) {
     using namespace fvattn;
     using R = Roles<true>;
     constexpr int kW = R::kExpanders;
@@ -578,9 +682,9 @@ FV_DEV void chunk_expander(const ChunkJob& jb, uint32_t sbase, int wid, int lane
         qn++;
         return true;
     };
-    ChunkDeal deal;
+    Walk walk(run);
     Work w;
-    while (deal.next(jb, w, false)) {
+    while (walk.next(jb, w, false)) {
         if (!load_q(w, 0) || !load_q(w, 1)) return;
         for (int j = 0; j <= w.n; j++) {
             const uint32_t slot = kvn % kKvPairs, use = kvn / kKvPairs;  // (as many code stages as pair slots)
@@ -612,7 +716,7 @@ FV_DEV void chunk_expander(const ChunkJob& jb, uint32_t sbase, int wid, int lane
 
 // The codes: one lane per page box brings its rows of K(j) and of V(j-1) and their scales by bulk copies (a page holds them as one
 // run each).  Boxes of which the item sees nothing, and pages outside the pool, are left out: the expander zeroes what is not seen.
-FV_DEV void chunk_code_loader(const ChunkJob& jb, uint32_t sbase, int lane, const ChunkWait& wait) {
+FV_DEV void chunk_code_loader(const ChunkJob& jb, const Run& run, uint32_t sbase, int lane, const ChunkWait& wait) {
     using namespace fvattn;
     uint32_t kvn = 0;
     auto ok_all = [&](uint32_t bar, uint32_t parity) { return __all_sync(fvpg::kFullWarp, wait(bar, parity)) != 0; };
@@ -624,10 +728,10 @@ FV_DEV void chunk_code_loader(const ChunkJob& jb, uint32_t sbase, int lane, cons
         const int page = page_of(jb.pool, jb.batch, w.s, a);
         return page < 0 ? -1 : (long long)pool_row(jb.pool, page, w.head, a);
     };
-    ChunkDeal deal;
+    Walk walk(run);
     Work w;
     bool ok = true;
-    while (ok && deal.next(jb, w, false)) {
+    while (ok && walk.next(jb, w, false)) {
         long long row = box_row(w, w.key(0)), prev = -1;
         for (int j = 0; j <= w.n; j++) {
             const long long ahead = j + 1 < w.n ? box_row(w, w.key(j + 1)) : -1;  // (the look-up's latency runs under the wait)
@@ -665,14 +769,14 @@ FV_DEV void chunk_code_loader(const ChunkJob& jb, uint32_t sbase, int lane, cons
 // Step j of an item: O_t += P_t(j-1) . V(j-1) for j > 0, then S_t = Q_t . K(j)^T for j < n, t = A then B, strictly in order
 // (fvattn::issuer_thread).
 template <bool Q4>
-FV_DEV void chunk_issuer(const ChunkJob& jb, uint32_t sbase, uint32_t tmem, const ChunkWait& wait) {
+FV_DEV void chunk_issuer(const ChunkJob& jb, const Run& run, uint32_t sbase, uint32_t tmem, const ChunkWait& wait) {
     using namespace fvattn;
     uint32_t qn = 0, pn = 0, pc = 0;
     uint32_t fixed[kKvPairs] = {};  // V tiles of each slot that the fixer had to touch so far
-    ChunkDeal deal;
+    Walk walk(run);
     Work w;
     bool ok = true;
-    while (ok && deal.next(jb, w, false)) {
+    while (ok && walk.next(jb, w, false)) {
         const uint32_t qa = qn % Roles<Q4>::kQ, qb = (qn + 1u) % Roles<Q4>::kQ;
         const uint32_t qa_par = (qn / Roles<Q4>::kQ) & 1u, qb_par = ((qn + 1u) / Roles<Q4>::kQ) & 1u;
         qn += 2;
@@ -728,7 +832,9 @@ FV_DEV void chunk_persistent(const CUtensorMap* mq, const CUtensorMap* mk, const
     const int warp = (int)(threadIdx.x >> 5), lane = (int)(threadIdx.x & 31);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Smem::abort_flag);
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + Smem::tmem_slot);
+    const Run& run = *reinterpret_cast<const Run*>(smem + kRun);
     if (threadIdx.x == 0) {
+        jb.split[blockIdx.x].valid = 0;
         const uint32_t producers = Q4 ? R::kExpanders : 1;  // the expander's warps, or one transaction count
         for (int s = 0; s < kQSlots; s++) {
             mbar_init(sbase + Smem::q_full + 8u * s, producers);
@@ -757,6 +863,8 @@ FV_DEV void chunk_persistent(const CUtensorMap* mq, const CUtensorMap* mk, const
     }
     __syncthreads();
     if (*abort_flag) return;  // CTA-uniform
+    find_run(jb, reinterpret_cast<Run*>(smem + kRun), reinterpret_cast<long long*>(smem + kScratch));
+    if (run.from == run.to) return;  // nothing on this CTA's part of the line
     if (warp == R::kIssuer) tmem_alloc(sbase + Smem::tmem_slot, 512);
     tc_fence_before();
     __syncthreads();
@@ -767,18 +875,18 @@ FV_DEV void chunk_persistent(const CUtensorMap* mq, const CUtensorMap* mk, const
     if (warp < kSoftmaxWarps) {
         if (Q4) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;" ::: "memory");
         else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;" ::: "memory");
-        chunk_softmax<Q4>(jb, sbase, tmem, warp, lane, waiter(3));
+        chunk_softmax<Q4>(jb, run, sbase, tmem, warp, lane, waiter(3));
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
         if (warp == R::kIssuer) {
-            if (lane == 0) chunk_issuer<Q4>(jb, sbase, tmem, waiter(2));
+            if (lane == 0) chunk_issuer<Q4>(jb, run, sbase, tmem, waiter(2));
         } else if (Q4) {
-            if (warp >= R::kExpander) chunk_expander(jb, sbase, warp - R::kExpander, lane, waiter(6));
-            else if (warp == R::kLoader) chunk_code_loader(jb, sbase, lane, waiter(1));
+            if (warp >= R::kExpander) chunk_expander(jb, run, sbase, warp - R::kExpander, lane, waiter(6));
+            else if (warp == R::kLoader) chunk_code_loader(jb, run, sbase, lane, waiter(1));
         } else if (warp == R::kLoader) {
-            chunk_loader(mq, mk, mv, jb, sbase, lane, waiter(1));
+            chunk_loader(mq, mk, mv, jb, run, sbase, lane, waiter(1));
         } else if (warp == R::kFixer) {
-            chunk_fixer(jb, sbase, lane, waiter(4));
+            chunk_fixer(jb, run, sbase, lane, waiter(4));
         }
         __syncwarp();
     }

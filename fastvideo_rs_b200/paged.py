@@ -119,7 +119,7 @@ class PagedBatch:
         if max_q < 0 or max_kv < 0:
             raise ValueError("PagedBatch: max_q and max_kv must not be negative")
         self.seqs, self.max_q, self.max_kv, self.device, self.index = seqs, int(max_q), int(max_kv), dev, page_table.get_device()
-        self._need = {}  # scratch bytes of a token by how the call is cut: a decode step asks for every layer
+        self._need = {}  # scratch bytes by the call's shape: a step asks for every layer
         self._c = _BatchC(page_table.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), seqs, width, self.max_q, self.max_kv)
         self._ref = ctypes.addressof(self._c)
 
@@ -253,14 +253,13 @@ def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[Block
         return out
     how = (1, mask.block_tokens, mask.window, mask.sink) if mask is not None else (0, 0, 0, 0)
     fns = _fns or _entries()
-    key = (how, heads, kv.kv_heads)
+    key = (how, heads, kv.kv_heads, tokens)
     need = batch._need.get(key)
     if need is None:
         need = 0
         if kv.index >= 0:
             with torch.cuda.device(kv.index):
-                need = batch._need[key] = fns[2](kv._ref, batch._ref, 1, heads, *how)
-    need *= tokens
+                need = batch._need[key] = fns[2](kv._ref, batch._ref, tokens, heads, *how)
     # (scratch of this call alone, from the stream's own pool: calls on other streams and captured graphs share nothing)
     ws = q.new_empty((need // 2,)) if need else None
     qt, qh = _strides(q)
