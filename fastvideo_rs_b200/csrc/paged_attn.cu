@@ -797,51 +797,69 @@ fv_paged_chunk_kernel(const __grid_constant__ CUtensorMap mq, const __grid_const
 #endif
 }
 
-// The items that the chunk kernel's runs cut: the part that begins the item lies with the CTA that `split` belongs to, the
-// others with the CTAs after it.  A warp a row, parts in their order.
-constexpr int kJoinBlocks = 8;  // of a split item's 256 rows
+// The items that the chunk kernel's runs cut: the part that begins the item lies with the run that `split` belongs to, the
+// others with the runs after it.  A warp a row; which parts there are is worked out once per block, a lane a run, and the
+// weights of a row a lane a part (one lane doing both for every row took 34 us for the 147 cuts of a launch, this 8).
+constexpr int kJoinBlocks = 16;  // of a split item's 256 rows
+constexpr int kMaxRuns = 1024;   // (kMaxPhases x SMs at most)
 __global__ void __launch_bounds__(kAttnThreads) fv_paged_join_kernel(const ChunkJob jb) {
-    const int lane = threadIdx.x & 31, c = blockIdx.x / kJoinBlocks, block = blockIdx.x - c * kJoinBlocks;
+    __shared__ int slots[kMaxRuns];
+    __shared__ int count;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x / kJoinBlocks, block = blockIdx.x - c * kJoinBlocks;
     const ChunkSplit sp = jb.split[c];
     if (!sp.valid) return;
+    if (warp == 0) {
+        int n = 1;
+        if (lane == 0) slots[0] = 2 * c + 1;
+        for (int k0 = c + 1; k0 < sp.runs; k0 += 32) {
+            const int k = k0 + lane;
+            bool mine = false, past = true;
+            if (k < sp.runs) {
+                const long long y = sp.total * k / sp.runs - sp.start, y1 = sp.total * (k + 1) / sp.runs - sp.start;
+                past = y >= sp.cost;
+                mine = !past && tile_behind((int)min(y1, (long long)sp.cost), sp.tiles) > tile_behind((int)y, sp.tiles);
+            }
+            const uint32_t have = __ballot_sync(kFullWarp, mine);
+            const int at = n + __popc(have & ((1u << lane) - 1u));
+            if (mine && at < kMaxRuns) slots[at] = 2 * k;
+            n = min(n + __popc(have), kMaxRuns);
+            if (__any_sync(kFullWarp, past)) break;
+        }
+        if (lane == 0) count = n;
+    }
+    __syncthreads();
+    const int n = count;
     constexpr int kRowsHere = 2 * kChunkRows / kJoinBlocks / kWarps;
+#pragma unroll 1
     for (int i = 0; i < kRowsHere; i++) {
-        const int r = (block * kRowsHere + i) * kWarps + (threadIdx.x >> 5), tile = r / kChunkRows, row = r - tile * kChunkRows;
+        const int r = (block * kRowsHere + i) * kWarps + warp, tile = r / kChunkRows, row = r - tile * kChunkRows;
         const int row_tok = row / jb.group, tok = sp.tok0 + tile * jb.tile_tokens + row_tok;
         if (row_tok >= jb.tile_tokens || tok >= sp.nq) continue;
-        // Walks the item's parts: slot of each, or -1 behind the last one.
-        auto part = [&](int& k) -> long long {
-            if (k == c) return 2ll * c + 1;
-            for (; k < sp.ctas; k++) {
-                const long long y = sp.total * k / sp.ctas - sp.start, y1 = sp.total * (k + 1) / sp.ctas - sp.start;
-                if (y >= sp.cost) break;
-                const int t0 = tile_behind((int)y, sp.tiles), t1 = tile_behind((int)min(y1, (long long)sp.cost), sp.tiles);
-                if (t0 >= sp.tiles) break;
-                if (t1 > t0) return 2ll * k;
-            }
-            return -1;
-        };
         float top = neg_inf();
-        long long slot;
-        for (int k = c; (slot = part(k)) >= 0; k++) top = fmaxf(top, jb.part_lse[slot * 2 * kChunkRows + r]);
+        for (int k = lane; k < n; k += 32) top = fmaxf(top, jb.part_lse[(size_t)slots[k] * 2 * kChunkRows + r]);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullWarp, top, d));
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         float sum = 0.f;
-        if (top != neg_inf()) {
-            for (int k = c; (slot = part(k)) >= 0; k++) {
-                const float w = fvp::ex2(jb.part_lse[slot * 2 * kChunkRows + r] - top);
-                if (w == 0.f) continue;
-                const float4 x = *reinterpret_cast<const float4*>(jb.part_o + (slot * 2 * kChunkRows + r) * kD + 4 * lane);
-                sum += w;
-                acc.x = fmaf(w, x.x, acc.x);
-                acc.y = fmaf(w, x.y, acc.y);
-                acc.z = fmaf(w, x.z, acc.z);
-                acc.w = fmaf(w, x.w, acc.w);
+        for (int k0 = 0; top != neg_inf() && k0 < n; k0 += 32) {
+            float w = 0.f;
+            if (k0 + lane < n) w = fvp::ex2(jb.part_lse[(size_t)slots[k0 + lane] * 2 * kChunkRows + r] - top);
+            const int here = min(32, n - k0);
+#pragma unroll 4
+            for (int k = 0; k < here; k++) {
+                const float wk = __shfl_sync(kFullWarp, w, k);
+                const float4 x = *reinterpret_cast<const float4*>(jb.part_o + ((size_t)slots[k0 + k] * 2 * kChunkRows + r) * kD + 4 * lane);
+                sum += wk;
+                acc.x = fmaf(wk, x.x, acc.x);
+                acc.y = fmaf(wk, x.y, acc.y);
+                acc.z = fmaf(wk, x.z, acc.z);
+                acc.w = fmaf(wk, x.w, acc.w);
             }
-            const float inv = 1.f / sum;
-            acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
         }
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
         const size_t out = (size_t)(sp.q0 + tok) * jb.heads + sp.head * jb.group + (row - row_tok * jb.group);
-        *reinterpret_cast<uint2*>(jb.out + out * kD + 4 * lane) = make_uint2(fvp::pack_bf16x2(acc.x, acc.y), fvp::pack_bf16x2(acc.z, acc.w));
+        *reinterpret_cast<uint2*>(jb.out + out * kD + 4 * lane) =
+            make_uint2(fvp::pack_bf16x2(acc.x * inv, acc.y * inv), fvp::pack_bf16x2(acc.z * inv, acc.w * inv));
     }
 }
 
@@ -851,11 +869,12 @@ struct Shape {
     bool chunk;  // the tensor-core kernel for long chunks
     int splits, row_blocks, nt, tile_tokens;
     bool cluster;
-    int ctas;  // of the chunk kernel
+    int ctas, phases;  // of the chunk kernel
 };
 // How a call is cut.  Few rows per kv head: blocks of 8 or 16 rows, and the keys in `splits` ranges so that all SMs have
 // work.  From kChunkFrom rows on: items of 2 x 128 rows, one CTA per SM.
 constexpr int kChunkFrom = 33;
+constexpr long long kL2Bytes = 126ll << 20;
 static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads, const Mask& m, int sms) {
     Shape s;
     const int group = heads / kv->kv_heads;
@@ -871,6 +890,16 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads,
         const long long longest = (long long)b->seqs * kv->kv_heads * s.row_blocks * ((b->max_kv + kChunkTile - 1) / kChunkTile + kItemCost);
         const long long most = longest / kLeastRun;
         s.ctas = (int)(most < 1 ? 1 : most < sms ? most : sms);
+        // Every CTA streams the keys of its items.  Where the keys of all items are more than L2 holds, the line is gone through in
+        // four phases, all CTAs on a quarter of it at a time (4 680 rows x 40 heads over 28 080 bf16 keys: 3 297 -> 2 901 us, 12 heads:
+        // 924 -> 827 us); where they fit that only makes more parts (1 501-token chunks over 69 MB of keys: 358 -> 422 us).
+        long long seen = b->max_kv;
+        if (m.block > 0 && m.window > 0) {
+            const long long some = ((long long)m.window + m.sink + 1) * m.block + b->max_q;
+            seen = some < seen ? some : seen;
+        }
+        const long long bytes = seen * b->seqs * kv->kv_heads * (kv->format == FV_PAGE_Q4 ? 2 * kQ4Bytes + 8 : 4 * kD);
+        s.phases = bytes > kL2Bytes && longest / ((long long)s.ctas * kMaxPhases) >= 32 ? kMaxPhases : 1;
         return s;
     }
     s.nt = rows > 8 ? 2 : 1;
@@ -897,7 +926,7 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads,
 
 // Scratch of a call: the parts of split rows (f32 and a log-sum-exp), for the chunk kernel two slots of 256 rows a CTA.
 static size_t workspace_of(const Shape& s, size_t rows) {
-    if (s.chunk) return (size_t)s.ctas * (2 * 2 * kChunkRows * (kD + 1) * sizeof(float) + sizeof(ChunkSplit));
+    if (s.chunk) return (size_t)s.ctas * s.phases * (2 * 2 * kChunkRows * (kD + 1) * sizeof(float) + sizeof(ChunkSplit));
     return s.splits > 1 && !s.cluster ? s.splits * rows * (kD + 1) * sizeof(float) : 0;
 }
 
@@ -911,7 +940,7 @@ static int launch_chunk(cudaStream_t st, const fv_paged_kv* kv, const AttnArgs& 
     jb.q_tok = a.q_tok;
     jb.q_head = a.q_head;
     jb.out = a.out;
-    const size_t slots = 2 * (size_t)s.ctas * 2 * kChunkRows;  // rows of parts
+    const size_t slots = 2 * (size_t)s.ctas * s.phases * 2 * kChunkRows;  // rows of parts
     jb.part_o = a.part_o;
     jb.part_lse = jb.part_o + slots * kD;
     jb.split = reinterpret_cast<ChunkSplit*>(jb.part_lse + slots);
@@ -921,9 +950,10 @@ static int launch_chunk(cudaStream_t st, const fv_paged_kv* kv, const AttnArgs& 
     jb.group = a.group;
     jb.tile_tokens = s.tile_tokens;
     jb.q_blocks = s.row_blocks;
-    const long long groups = (long long)a.batch.seqs * s.row_blocks;
-    if (groups > 0x3fffffffll) return FV_DECLINED;
-    jb.groups = (int)groups;
+    const long long items = (long long)a.batch.seqs * a.pool.kv_heads * s.row_blocks;
+    if (items > 0x3fffffffll) return FV_DECLINED;
+    jb.items = (int)items;
+    jb.phases = s.phases;
     jb.box_rows = kv->page_rows < kChunkTile ? kv->page_rows : kChunkTile;
     jb.sl2 = a.sl2;
     CUtensorMap mq{}, mk{}, mv{};
@@ -956,7 +986,7 @@ static int launch_chunk(cudaStream_t st, const fv_paged_kv* kv, const AttnArgs& 
     else fv_paged_chunk_kernel<false><<<grid, Roles<false>::kThreads, kChunkSmem, st>>>(mq, mk, mv, jb);
     FV_CUDA(cudaGetLastError());
     if (grid > 1) {
-        fv_paged_join_kernel<<<grid * kJoinBlocks, kAttnThreads, 0, st>>>(jb);
+        fv_paged_join_kernel<<<grid * s.phases * kJoinBlocks, kAttnThreads, 0, st>>>(jb);
         FV_CUDA(cudaGetLastError());
     }
     fvrt::ran(fvrt::kLogPagedChunk, "paged attention: fv_paged_chunk_kernel<%s> (sm_100a tcgen05, persistent, %u CTAs) %d sequences x %d heads / %d",

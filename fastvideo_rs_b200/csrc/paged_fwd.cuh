@@ -16,7 +16,7 @@
 //     of which the item sees nothing take a page coordinate past the pool, which reads as zeros.  In the few tiles that
 //     the item's visible keys only cover in part, one warp ("fixer") then zeroes V's rows that no row of the item sees: a P of
 //     zero times whatever memory holds there must be zero.
-//   * 4-bit pages: the loader brings the packed codes by bulk copies, six more warps expand them to f16 into the swizzled
+//   * 4-bit pages: the loader brings the packed codes by bulk copies, four more warps expand them to f16 into the swizzled
 //     tiles that TMA would have written, and bring Q as f16.  Both products then run in f16: a value zero + step code is rounded once, by
 //     2^-11 at most (in bf16 the roundings of K and V, 2^-8 each, would be of the size of the output's own), P by 2^-11.
 //     f16's range is the price: values beyond 65 504 saturate, below 2^-14 they lose relative precision.  Against that,
@@ -37,17 +37,18 @@ struct ChunkJob {
     const uint16_t* q;
     long long q_tok, q_head;
     uint16_t* out;
-    float *part_o, *part_lse;  // [2 per CTA, 256 rows, 128] and [2 per CTA, 256]: a part that does not begin its item, one that does
-    struct ChunkSplit* split;  // [CTA]: the item that begins in the CTA's run and ends in another's
+    float *part_o, *part_lse;  // [2 per run, 256 rows, 128] and [2 per run, 256]: a part that does not begin its item, one that does
+    struct ChunkSplit* split;  // [run]: the item that begins in the run and ends in another
     int* wait_status;          // the first status word
     long long wait_cycles;
-    int heads, group, tile_tokens, q_blocks, groups, box_rows;  // groups: sequences x row blocks
+    int heads, group, tile_tokens, q_blocks, items, box_rows;  // items: (sequence, kv head, row block), row blocks fastest
+    int phases;
     float sl2;
 };
 constexpr int kItemCost = 4;   // what an item costs beside its key tiles, in key tiles: the pipeline fills and drains, the output
 constexpr int kLeastRun = 8;   // the shortest run worth a CTA
 struct ChunkSplit {
-    int valid, q0, nq, tok0, head, tiles, cost, ctas;
+    int valid, q0, nq, tok0, head, tiles, cost, runs;
     long long start, total;  // where the item begins on the line, and how long the line is
 };
 // The first key tile of an item that lies behind position y of its length: the fixed cost comes first, and no part is a
@@ -75,7 +76,7 @@ constexpr uint32_t kVFixed = Smem::total;
 constexpr uint32_t kCodeFull = kVFixed + 8 * fvattn::kKvPairs, kCodeFree = kCodeFull + 16;
 constexpr uint32_t kScales = (kCodeFree + 16 + 15) & ~15u;      // [stage][V | K][128 keys] (step, zero)
 constexpr uint32_t kRun = kScales + 2 * 1024;  // this CTA's run
-constexpr uint32_t kScratch = kRun + 64;      // find_run's
+constexpr uint32_t kScratch = kRun + 128;     // find_run's
 constexpr uint32_t kChunkSmem = kScratch + 256;
 constexpr uint32_t kCodes = Smem::q + 2 * fvattn::kSlotBytes;   // [stage][V | K][128 keys][64 bytes]
 static_assert(kVFixed % 8 == 0 && kChunkSmem <= 232448 && fvattn::kQSlots == 3 && fvattn::kSlotBytes == 32768, "shared memory");
@@ -86,7 +87,7 @@ struct Roles {
     static constexpr int kWarps = Q4 ? 16 : 12;
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kLoader = 8, kIssuer = 9, kFixer = 10;  // (fixer: bf16)
-    static constexpr int kExpander = 10, kExpanders = 6;         // 4 bits: warps 10-15
+    static constexpr int kExpander = 12, kExpanders = 4;         // 4 bits: warps 12-15, one on each of the SM's schedulers
     static constexpr uint32_t kQ = Q4 ? 2 : fvattn::kQSlots;     // Q slots
 };
 
@@ -107,12 +108,14 @@ struct Work {
     FV_DEV bool begins() const { return u0 == 0; }
     FV_DEV bool ends() const { return u0 + n == tiles; }
 };
-// Group number i (a sequence's row block, an item for each of its kv heads): its rows and tiles, and the cost of one item;
-// 0 when there are no such rows.
-FV_DEV int group_at(const ChunkJob& jb, int i, Work& w) {
-    w.s = i / jb.q_blocks;
+// Item number i: its rows and tiles, and its cost; 0 when there are no such rows.
+FV_DEV int item_at(const ChunkJob& jb, int i, Work& w) {
+    const int plane = i / jb.q_blocks;
+    w.s = plane / jb.pool.kv_heads;
+    w.head = plane - w.s * jb.pool.kv_heads;
     w.seq = seq_of(jb.batch, w.s);
-    w.tok0 = (i - w.s * jb.q_blocks) * 2 * jb.tile_tokens;
+    w.tok0 = (i - plane * jb.q_blocks) * 2 * jb.tile_tokens;
+    w.tiles = 0;
     if (w.tok0 >= w.seq.nq) return 0;
     const int last = min(w.tok0 + 2 * jb.tile_tokens, w.seq.nq) - 1;
     w.span = span_of(jb.mask, w.pos0() + w.tok0, w.pos0() + last, w.seq.len);
@@ -121,10 +124,15 @@ FV_DEV int group_at(const ChunkJob& jb, int i, Work& w) {
     w.tiles = w.sinks + max(0, (w.span.hi + kChunkTile - 1) / kChunkTile - w.first);
     return w.tiles + kItemCost;
 }
-// This CTA's run of the line.
+// This CTA's runs of the line: number blockIdx + p gridDim of `runs` equal ones, p = 0 .. phases - 1.
+constexpr int kMaxPhases = 4;
 struct Run {
-    long long total, from, to;
-    int ctas, group, head, off;  // CTAs that have runs; the item that `from` lies in and where in it
+    long long total;
+    int runs;
+    struct Start {
+        int item, off, length;  // the item that the run begins in, where in it, and the run's length
+    } start[kMaxPhases];
+    FV_DEV long long edge(int v) const { return total * v / runs; }
 };
 // Warp-inclusive sum.
 FV_DEV long long scan_warp(long long x, int lane) {
@@ -135,14 +143,14 @@ FV_DEV long long scan_warp(long long x, int lane) {
     }
     return x;
 }
-// The whole CTA adds up the line (a run of groups a thread) and finds its place on it.  `scratch`: 32 long longs.
+// The whole CTA adds up the line (a run of items a thread) and finds its places on it.  `scratch`: 32 long longs.
 FV_DEV void find_run(const ChunkJob& jb, Run* run, long long* scratch) {
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (int)blockDim.x >> 5;
-    const int per = (jb.groups + (int)blockDim.x - 1) / (int)blockDim.x;
-    const int g0 = min(tid * per, jb.groups), g1 = min(g0 + per, jb.groups);
+    const int per = (jb.items + (int)blockDim.x - 1) / (int)blockDim.x;
+    const int i0 = min(tid * per, jb.items), i1 = min(i0 + per, jb.items);
     long long mine = 0;
     Work w;
-    for (int g = g0; g < g1; g++) mine += (long long)group_at(jb, g, w) * jb.pool.kv_heads;
+    for (int i = i0; i < i1; i++) mine += item_at(jb, i, w);
     const long long incl = scan_warp(mine, lane);
     if (lane == 31) scratch[warp] = incl;
     __syncthreads();
@@ -152,70 +160,62 @@ FV_DEV void find_run(const ChunkJob& jb, Run* run, long long* scratch) {
         total += scratch[i];
     }
     const long long excl = before + incl - mine;
-    const int ctas = (int)max(1ll, min((long long)gridDim.x, total / kLeastRun));
-    const bool idle = (int)blockIdx.x >= ctas;
-    const long long from = idle ? 0 : total * blockIdx.x / ctas, to = idle ? 0 : total * (blockIdx.x + 1) / ctas;
+    const int runs = (int)max(1ll, min((long long)gridDim.x * jb.phases, total / kLeastRun));
     if (tid == 0) {
         run->total = total;
-        run->from = from;
-        run->to = to;
-        run->ctas = ctas;
+        run->runs = runs;
     }
-    if (from < to && from >= excl && from < excl + mine) {
-        long long at = excl;
-        for (int g = g0; g < g1; g++) {
-            const int cost = group_at(jb, g, w);
-            const long long all = (long long)cost * jb.pool.kv_heads;
-            if (from < at + all) {
-                run->group = g;
-                run->head = (int)((from - at) / cost);
-                run->off = (int)((from - at) % cost);
-                break;
+    for (int p = 0; p < jb.phases; p++) {
+        const int v = (int)blockIdx.x + p * (int)gridDim.x;
+        const bool idle = v >= runs || total == 0;
+        const long long from = idle ? 0 : total * v / runs, to = idle ? 0 : total * (v + 1) / runs;
+        if (tid == 0) run->start[p].length = (int)(to - from);
+        if (from < to && from >= excl && from < excl + mine) {
+            long long at = excl;
+            for (int i = i0; i < i1; i++) {
+                const int cost = item_at(jb, i, w);
+                if (from < at + cost) {
+                    run->start[p].item = i;
+                    run->start[p].off = (int)(from - at);
+                    break;
+                }
+                at += cost;
             }
-            at += all;
         }
     }
     __syncthreads();
 }
-// The items of the run, in order.
+// The items of the CTA's runs, in order.
 struct Walk {
-    Work g;  // the current group
-    int group, head, off, cost, left;
-    bool known;
-    FV_DEV explicit Walk(const Run& r) : group(r.group), head(r.head), off(r.off), cost(0), left((int)(r.to - r.from)), known(false) {}
+    const Run& run;
+    int phase = -1, item = 0, off = 0, left = 0;
+    FV_DEV explicit Walk(const Run& r) : run(r) {}
+    FV_DEV int number() const { return (int)blockIdx.x + phase * (int)gridDim.x; }  // of the run
     // The next item with key tiles (`empty`: or with rows that see no key).  *ahead: what is left of the run from where this item
     // began on the line.
     FV_DEV bool next(const ChunkJob& jb, Work& w, bool empty, int* ahead = nullptr) {
-        while (left > 0 && group < jb.groups) {
-            if (!known) {
-                cost = group_at(jb, group, g);
-                known = true;
-            }
-            if (cost == 0) {
-                group++;
-                known = false;
+        for (;;) {
+            if (left <= 0 || item >= jb.items) {
+                if (++phase >= jb.phases) return false;
+                left = run.start[phase].length;
+                item = run.start[phase].item;
+                off = run.start[phase].off;
                 continue;
             }
+            const int cost = item_at(jb, item, w);
             const int end = min(cost, off + left);
-            const int t0 = tile_behind(off, g.tiles), t1 = tile_behind(end, g.tiles);
-            w = g;
-            w.head = head;
-            w.u0 = t0;
-            w.n = t1 - t0;
+            w.u0 = tile_behind(off, w.tiles);
+            w.n = tile_behind(end, w.tiles) - w.u0;
             if (ahead) *ahead = left + off;
             left -= end - off;
             off = end;
-            if (end == cost) {
+            const bool done = end == cost;
+            if (done) {
                 off = 0;
-                if (++head == jb.pool.kv_heads) {
-                    head = 0;
-                    group++;
-                    known = false;
-                }
+                item++;
             }
-            if (w.n > 0 || (empty && w.tiles == 0 && end == cost)) return true;
+            if (cost > 0 && (w.n > 0 || (empty && w.tiles == 0 && done))) return true;
         }
-        return false;
     }
 };
 
@@ -286,6 +286,9 @@ template <bool F16>
 FV_DEV uint32_t pack_p(float lo, float hi) {
     return F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
 }
+// A row sum of P above this could leave P's type.
+template <bool F16>
+constexpr float kChunkGuard = F16 ? 32768.f : fvattn::kGuard;
 // As fvattn::exp32: 2^(u sl2 + noff) of 32 columns to packed pairs, every fourth pair on the FMA pipe (POLY).
 template <bool F16, bool POLY>
 FV_DEV void chunk_exp32(const uint32_t (&u)[32], uint32_t* pw, uint64_t s2, uint64_t nf, uint64_t& acc0, uint64_t& acc1, float& top) {
@@ -307,12 +310,36 @@ FV_DEV void chunk_exp32(const uint32_t (&u)[32], uint32_t* pw, uint64_t s2, uint
     }
 }
 
-// A tile with invisible columns, or whose sum tripped the guard: exact maxima, the reference moved, O and the sum
-// rescaled (as fvattn::careful_tile, whose comment gives the reasons for keeping it out of line).
+// A tile with invisible columns, or whose sum tripped the guard (out of line for the reasons that fvattn::careful_tile
+// gives).  Where every row has a reference already, or sees nothing of the tile, one pass as in the hot path, the invisible
+// columns as -inf; else, or when that pass trips the guard, exact maxima first, the reference moved, O and the sum rescaled.
 template <bool F16>
 static __device__ __noinline__ void chunk_careful(uint32_t tS, uint32_t tO, uint32_t bt, Cols cols, float sl2, bool have_o, int lane,
                                                   RowState* rs) {
     float m = rs->m, l = rs->l;
+    // (bf16 only: in the 4-bit kernel, whose softmax threads have 184 registers, the longer function costs the loop around it more
+    // than the pass saves, 430 against 448 us for three ragged chunks.)
+    if (!F16 && __all_sync(kFullWarp, !cols.whole && (m != neg_inf() || (max(cols.lo, 0) >= cols.hi && cols.sink <= 0)))) {
+        const float ref = m == neg_inf() ? 0.f : -m;
+        const uint64_t s2 = pack_f32x2(sl2, sl2), nf = pack_f32x2(ref, ref);
+        uint64_t acc0 = pack_f32x2(0.f, 0.f), acc1 = acc0;
+        float top = 0.f;
+        uint32_t u[32], pw[64];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            fvattn::load_chunk(tS, c, u);
+            fvattn::land_chunk(u);
+            cols.hide(u, 32 * c);
+            chunk_exp32<F16, false>(u, pw + 16 * c, s2, nf, acc0, acc1, top);
+        }
+        const float sum = fvattn::part_sum<false>(acc0, acc1, top);
+        if (!__any_sync(kFullWarp, !(sum <= kChunkGuard<F16>))) {
+            fvattn::store_early(tS, pw);
+            fvattn::publish(bt + Smem::p_ready, lane);
+            rs->l = l + sum;
+            return;
+        }
+    }
     float mx = neg_inf();
 #pragma unroll 1
     for (int c = 0; c < 4; c++) {
@@ -405,7 +432,6 @@ static __device__ __noinline__ void chunk_write(void* base, uint32_t tO, float i
 
 template <bool Q4>
 FV_DEV void chunk_softmax(const ChunkJob& jb, const Run& run, uint32_t sbase, uint32_t tmem, int warp, int lane, const ChunkWait& wait) {
-    constexpr float kChunkGuard = Q4 ? 32768.f : fvattn::kGuard;  // a row sum of P above this could leave P's type
     constexpr float kBelow = Q4 ? 6.f : 0.f;                      // the reference starts 2^kBelow below the first maximum
     const int tile = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
@@ -456,7 +482,7 @@ FV_DEV void chunk_softmax(const ChunkJob& jb, const Run& run, uint32_t sbase, ui
                 fvattn::land_chunk(u1);
                 chunk_exp32<Q4, true>(u1, pw + 48, s2, nf, acc0, acc1, top);
                 const float sum = fvattn::part_sum<true>(acc0, acc1, top);
-                if (__any_sync(kFullWarp, live && !(sum <= kChunkGuard))) {
+                if (__any_sync(kFullWarp, live && !(sum <= kChunkGuard<Q4>))) {
                     hot = false;  // nothing of this tile is stored
                 } else {
                     fvattn::store_early(tS, pw);
@@ -466,10 +492,11 @@ FV_DEV void chunk_softmax(const ChunkJob& jb, const Run& run, uint32_t sbase, ui
             }
             if (!hot) chunk_careful<Q4>(tS, tO, bt, cols, sl2, j > 0, lane, &rs);
         }
+        const int number = walk.number();
         const bool have_o = w.n > 0, begins = w.begins(), part = !(begins && w.ends());
         const int out_row = !live ? -1 : part ? tile * kChunkRows + row : (w.seq.q0 + tok) * jb.heads + w.head * jb.group + row_head;
         if (begins && part && threadIdx.x == 0)
-            jb.split[blockIdx.x] = ChunkSplit{1, w.seq.q0, w.seq.nq, w.tok0, w.head, w.tiles, w.tiles + kItemCost, run.ctas, run.to - ahead, run.total};
+            jb.split[number] = ChunkSplit{1, w.seq.q0, w.seq.nq, w.tok0, w.head, w.tiles, w.tiles + kItemCost, run.runs, run.edge(number + 1) - ahead, run.total};
         more = walk.next(jb, w, true, &ahead);  // (looked up while the last product runs)
         if (have_o) {
             if (!__all_sync(kFullWarp, wait(bt + Smem::o_ready, o_count & 1u))) return;
@@ -480,7 +507,7 @@ FV_DEV void chunk_softmax(const ChunkJob& jb, const Run& run, uint32_t sbase, ui
         if (!part) {
             chunk_write<Q4, false>(jb.out, tO, inv, out_row, have_o, lane);
         } else {
-            const size_t slot = 2 * (size_t)blockIdx.x + (begins ? 1 : 0);
+            const size_t slot = 2 * (size_t)number + (begins ? 1 : 0);
             chunk_write<Q4, true>(jb.part_o + slot * 2 * kChunkRows * kD, tO, inv, out_row, have_o, lane);
             if (out_row >= 0) jb.part_lse[slot * 2 * kChunkRows + out_row] = rs.l > 0.f ? rs.m + log2f(rs.l) : neg_inf();
         }
@@ -644,9 +671,10 @@ FV_DEV void expand_unit(uint4 c, uint32_t sz, uint32_t base, int q) {
         store_piece(base ^ (16u * j), fma_f16x2(h0, s2, z2), fma_f16x2(h1, s2, z2), fma_f16x2(h2, s2, z2), fma_f16x2(h3, s2, z2));
     }
 }
-// Six warps, a pair's 32 units dealt in turn.  (With one key row a lane in four warps, page look-ups and loads of their own, the expansion
-// took as long as one and a half tiles' products: block of 4 680 rows x 12 heads over 28 080 keys 1 294 us against 958 us with bf16
-// pages; look-ups and loads are the loader's since.)
+// A pair's 32 units are dealt to the warps in turn.  Four warps, one per scheduler: their instructions come out of the softmax
+// warps' issue slots, and six (two schedulers with two of them) were slower, 430 against 412 us for three ragged chunks;
+// without the arithmetic of the expansion it would be 363.  (A first form with one key row a lane and page look-ups and loads of its
+// own took 709: look-ups and loads are the loader's since.)
 FV_DEV void chunk_expander(const ChunkJob& jb, const Run& run, uint32_t sbase, int wid, int lane, const ChunkWait& wait) {
     using namespace fvattn;
     using R = Roles<true>;
@@ -834,7 +862,7 @@ FV_DEV void chunk_persistent(const CUtensorMap* mq, const CUtensorMap* mk, const
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + Smem::tmem_slot);
     const Run& run = *reinterpret_cast<const Run*>(smem + kRun);
     if (threadIdx.x == 0) {
-        jb.split[blockIdx.x].valid = 0;
+        for (int p = 0; p < jb.phases; p++) jb.split[blockIdx.x + p * gridDim.x].valid = 0;
         const uint32_t producers = Q4 ? R::kExpanders : 1;  // the expander's warps, or one transaction count
         for (int s = 0; s < kQSlots; s++) {
             mbar_init(sbase + Smem::q_full + 8u * s, producers);
@@ -864,7 +892,7 @@ FV_DEV void chunk_persistent(const CUtensorMap* mq, const CUtensorMap* mk, const
     __syncthreads();
     if (*abort_flag) return;  // CTA-uniform
     find_run(jb, reinterpret_cast<Run*>(smem + kRun), reinterpret_cast<long long*>(smem + kScratch));
-    if (run.from == run.to) return;  // nothing on this CTA's part of the line
+    if (run.start[0].length == 0) return;  // nothing on this CTA's part of the line (a later run is never longer)
     if (warp == R::kIssuer) tmem_alloc(sbase + Smem::tmem_slot, 512);
     tc_fence_before();
     __syncthreads();
