@@ -722,15 +722,26 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_p
         }
         cluster.sync();
         for (int r = split; r < rows; r += a.splits) {
-            float top = neg_inf();
-            for (int i = 0; i < a.splits; i++) top = fmaxf(top, *cluster.map_shared_rank(&sh_m[0][r], i));
-            float acc = 0.f, sum = 0.f;
-            for (int i = 0; i < a.splits; i++) {
-                const float mi = *cluster.map_shared_rank(&sh_m[0][r], i);
-                const float f = mi == neg_inf() ? 0.f : fvp::ex2(mi - top);
-                if (f == 0.f) continue;
-                sum = fmaf(f, *cluster.map_shared_rank(&sh_l[0][r], i), sum);
-                acc = fmaf(f, *cluster.map_shared_rank(&sh_o[0][r][d], i), acc);
+            // (every load of the row on its way before the first is used: one after the other they took 2 us)
+            float mi[kMaxCluster], li[kMaxCluster], oi[kMaxCluster];
+#pragma unroll
+            for (int i = 0; i < kMaxCluster; i++) {
+                mi[i] = neg_inf();
+                li[i] = oi[i] = 0.f;
+                if (i < a.splits) {
+                    mi[i] = *cluster.map_shared_rank(&sh_m[0][r], i);
+                    li[i] = *cluster.map_shared_rank(&sh_l[0][r], i);
+                    oi[i] = *cluster.map_shared_rank(&sh_o[0][r][d], i);
+                }
+            }
+            float top = mi[0], acc = 0.f, sum = 0.f;
+#pragma unroll
+            for (int i = 1; i < kMaxCluster; i++) top = fmaxf(top, mi[i]);
+#pragma unroll
+            for (int i = 0; i < kMaxCluster; i++) {
+                const float f = mi[i] == neg_inf() ? 0.f : fvp::ex2(mi[i] - top);
+                sum = fmaf(f, li[i], sum);
+                if (f != 0.f) acc = fmaf(f, oi[i], acc);
             }
             a.out[out_row(r) * kD + d] = (uint16_t)fvp::pack_bf16x2(top == neg_inf() ? 0.f : acc / sum, 0.f);
         }

@@ -48,14 +48,19 @@ FV_DEV uint4 narrow8(const float* x) {
 FV_DEV float bf16_of(float x) {
     return __uint_as_float(fvp::pack_bf16x2(0.f, x) & 0xffff0000u);
 }
-FV_DEV float min_nan(float a, float b) {
+FV_DEV float min_nan(float a, float b, float c) {
     float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-FV_DEV float max_nan(float a, float b) {
+FV_DEV float max_nan(float a, float b, float c) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+FV_DEV float fma_sat(float a, float b, float c) {  // clamped to 0 .. 1
+    float r;
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
@@ -87,73 +92,99 @@ FV_DEV void rotate16(float (&x)[16], const float (&cs)[8], const float (&sn)[8])
         x[b] = __fadd_rn(__fmul_rn(xa, sn[i]), __fmul_rn(xb, cs[i]));
     }
 }
+// Four codes exactly as the rounded quotient gives them, where some lie near the middle h between two codes.  Without dividing:
+// d = y - step h is exact, and the quotient rounds to h itself (whose nearest integer is the even one) while |d| is at most
+// step times half a unit in h's last place, a quarter unit below a power of two.  Out of line.
+static __device__ __noinline__ uint32_t settle4(float a, float b, float c4, float d4, float zero, float step, float inv) {
+    const float x[4] = {a, b, c4, d4};
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float y = __fsub_rn(x[i], zero);
+        float c;
+        if (inv <= 3e38f) {
+            c = fminf(fmaxf(__fmul_rn(y, inv), -8.f), 7.f);
+            float r = rintf(c);
+            const float e = __fsub_rn(c, r);
+            if (fabsf(e) > 0.4999f) {
+                const float h = r + copysignf(0.5f, e), mag = fabsf(h);
+                const float d = copysignf(1.f, h) * __fmaf_rn(-step, h, y);  // > 0: farther from zero than h
+                const float unit = __uint_as_float(__float_as_uint(mag) & 0x7f800000u) * 0x1p-24f * step;
+                if (d > unit || d < (mag == 0.5f ? -0.5f * unit : -unit)) r = h + copysignf(0.5f, d * h);
+                else r = rintf(h);
+            }
+            c = r;
+        } else {  // (a step so small that its reciprocal overflows)
+            c = rintf(__fdiv_rn(y, step));
+        }
+        c = fminf(fmaxf(c, -8.f), 7.f);
+        w |= ((uint32_t)((int)c + 8) & 15u) << (4 * i);
+    }
+    return w;
+}
 // The same row in 4 bits: codes of this lane's 16 values as two words (8 values each), (step, zero) as one.  Collective
 // over the warp.  (A row of one value has step 0 and codes 0.  A row with a value that is not finite has a step that is
 // not: its codes say nothing, the row stands for NaN.)
 FV_DEV void quantize16(const float (&x)[16], uint32_t& lo, uint32_t& hi, uint32_t& scale) {
-    float mn = x[0], mx = x[0];
+    float mn = min_nan(x[0], x[1], x[2]), mx = max_nan(x[0], x[1], x[2]);
 #pragma unroll
-    for (int i = 1; i < 16; i++) {
-        mn = min_nan(mn, x[i]);
-        mx = max_nan(mx, x[i]);
+    for (int i = 3; i < 15; i += 2) {
+        mn = min_nan(mn, x[i], x[i + 1]);
+        mx = max_nan(mx, x[i], x[i + 1]);
     }
+    mn = min_nan(mn, x[15], x[15]);
+    mx = max_nan(mx, x[15], x[15]);
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) {
-        mn = min_nan(mn, __shfl_xor_sync(kFullWarp, mn, d));
-        mx = max_nan(mx, __shfl_xor_sync(kFullWarp, mx, d));
+        const float a = __shfl_xor_sync(kFullWarp, mn, d), b = __shfl_xor_sync(kFullWarp, mx, d);
+        mn = min_nan(mn, a, a);
+        mx = max_nan(mx, b, b);
     }
     const float step = bf16_of(__fdiv_rn(__fsub_rn(mx, mn), 15.f));
     const float zero = bf16_of(__fadd_rn(mn, __fmul_rn(8.f, step)));
     scale = fvp::pack_bf16x2(step, zero);
     lo = hi = 0x88888888u;
     if (!(step > 0.f)) return;
-    // A quotient by the reciprocal is off by a few units in the last place, which moves a code only where it lies at the
-    // middle between two: a lane that meets such a value (one in 10^4 lanes on ordinary data; a reciprocal that overflows is
-    // caught as well) takes true divisions.  Rounding to the nearest even code is the addition of 1.5 2^23 + 8, whose sum
-    // carries code + 8 in its lowest bits.
-    constexpr float kRound = 12582912.f + 8.f;
-    const float inv = __frcp_rn(step);
-    bool middle = !(inv <= 3e38f);
-    uint32_t n[16];
+    // code + 8 = 15 u, u = ((x - zero) / step + 8) / 15 clamped to 0 .. 1.  By the reciprocal 15 u is off by some 2^-20, which moves a
+    // code only where it lies at the middle between two: a lane that meets such a value settles it apart.  (True divisions there cost: values
+    // that came in as bf16 lie exactly in the middle often, in some row of every third warp.)  Adding 1.5 2^23 rounds to the nearest even
+    // integer; four codes are put together as one number in f32, which 16 bits fit exactly.
+    constexpr float kRound = 12582912.f;
+    const float inv = __frcp_rn(step), inv15 = inv * (1.f / 15.f);
+    uint32_t part[4];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const float raw = __fmul_rn(__fsub_rn(x[i], zero), inv);
-        const float c = fminf(fmaxf(raw, -8.f), 7.f);
-        const float t = __fadd_rn(c, kRound);
-        middle |= !(fabsf(__fsub_rn(c, __fsub_rn(t, kRound))) <= 0.49998f) || raw != raw;
-        n[i] = __float_as_uint(t) & 15u;
-    }
-    if (middle) {
+    for (int k = 0; k < 4; k++) {
+        float r[4], middle = inv <= 3e38f ? 0.f : 1.f;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], zero), step)), -8.f), 7.f);
-            n[i] = (uint32_t)((int)c + 8) & 15u;
+        for (int i = 0; i < 4; i++) {
+            const float u = fma_sat(__fsub_rn(x[4 * k + i], zero), inv15, 8.f / 15.f);
+            r[i] = __fsub_rn(__fmaf_rn(u, 15.f, kRound), kRound);
+            middle = fmaxf(middle, fabsf(__fmaf_rn(u, 15.f, -r[i])));
         }
+        const float four = __fmaf_rn(__fmaf_rn(__fmaf_rn(r[3], 16.f, r[2]), 16.f, r[1]), 16.f, r[0]);
+        part[k] = __float_as_uint(__fadd_rn(four, 8388608.f));  // its lowest 16 bits
+        if (middle > 0.49998f) part[k] = settle4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3], zero, step, inv);
     }
-    lo = hi = 0u;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        lo |= n[i] << (4 * i);
-        hi |= n[8 + i] << (4 * i);
-    }
+    lo = __byte_perm(part[0], part[1], 0x5410);
+    hi = __byte_perm(part[2], part[3], 0x5410);
 }
 
-// Rows of `count` heads from head `first` on, UNROLL at a time: raw bits in, `use(head, u0, u1)` gets 16 values.
+// Rows of heads first, first + step, .. below `last`, UNROLL at a time: raw bits in, `use(head, u0, u1)` gets 16 values.
 template <int UNROLL, class Use>
-FV_DEV void for_heads(const uint16_t* src, long long stride, int first, int last, const Use& use) {
+FV_DEV void for_heads(const uint16_t* src, long long stride, int first, int last, int step, const Use& use) {
     int h = first;
-    for (; h + UNROLL <= last; h += UNROLL) {
+    for (; h + (UNROLL - 1) * step < last; h += UNROLL * step) {
         uint4 u[UNROLL][2];
 #pragma unroll
         for (int i = 0; i < UNROLL; i++) {
-            const uint4* p = reinterpret_cast<const uint4*>(src + (long long)(h + i) * stride);
+            const uint4* p = reinterpret_cast<const uint4*>(src + (long long)(h + i * step) * stride);
             u[i][0] = __ldg(p);
             u[i][1] = __ldg(p + 8);
         }
 #pragma unroll
-        for (int i = 0; i < UNROLL; i++) use(h + i, u[i][0], u[i][1]);
+        for (int i = 0; i < UNROLL; i++) use(h + i * step, u[i][0], u[i][1]);
     }
-    for (; h < last; h++) {
+    for (; h < last; h += step) {
         const uint4* p = reinterpret_cast<const uint4*>(src + (long long)h * stride);
         use(h, __ldg(p), __ldg(p + 8));
     }
@@ -205,11 +236,12 @@ __global__ void __launch_bounds__(kThreads) fv_paged_append_kernel(const AppendA
             }
         }
     }
-    // This CTA's share of the token's rows: q's heads, then K's, then V's.
-    const int hk = a.pool.kv_heads, rows = a.q_heads + 2 * hk;
-    const int r0 = (int)((long long)rows * share / a.parts), r1 = (int)((long long)rows * (share + 1) / a.parts);
-    auto clip = [](int r, int n) { return min(max(r, 0), n); };
-    for_heads<4>(a.q + t * a.q_tok + 8 * part, a.q_head, clip(r0, a.q_heads), clip(r1, a.q_heads), [&](int h, uint4 u0, uint4 u1) {
+    // This CTA's share of the token's rows -- q's heads, then K's, then V's -- is every parts-th of them, so that each share has its
+    // part of the rows that are quantised (with runs of rows the last share had them all: 46 against 31 us for 4 142 tokens of
+    // 40 + 2 x 8 heads).
+    const int hk = a.pool.kv_heads, parts = a.parts;
+    auto first_of = [&](int before) { return (share + parts - before % parts) % parts; };  // `before` rows come before head 0
+    for_heads<4>(a.q + t * a.q_tok + 8 * part, a.q_head, share, a.q_heads, parts, [&](int h, uint4 u0, uint4 u1) {
         if (!mine) return;
         if (!placed) {
             u0 = u1 = make_uint4(0, 0, 0, 0);
@@ -254,11 +286,11 @@ __global__ void __launch_bounds__(kThreads) fv_paged_append_kernel(const AppendA
             o[8] = u1;
         };
     };
-    const int k0 = clip(r0 - a.q_heads, hk), k1 = clip(r1 - a.q_heads, hk);
-    if (turn) for_heads<Q4 ? 2 : 4>(a.k + t * a.k_tok + 8 * part, a.k_head, k0, k1, put(a.pool.k, a.pool.k_scale, true));
-    else for_heads<Q4 ? 2 : 4>(a.k + t * a.k_tok + 8 * part, a.k_head, k0, k1, put(a.pool.k, a.pool.k_scale, false));
-    for_heads<Q4 ? 2 : 4>(a.v + t * a.v_tok + 8 * part, a.v_head, clip(r0 - a.q_heads - hk, hk), clip(r1 - a.q_heads - hk, hk),
-                          put(a.pool.v, a.pool.v_scale, false));
+    constexpr int kUnroll = Q4 ? 2 : 4;
+    const int k0 = first_of(a.q_heads), v0 = first_of(a.q_heads + hk);
+    if (turn) for_heads<kUnroll>(a.k + t * a.k_tok + 8 * part, a.k_head, k0, hk, parts, put(a.pool.k, a.pool.k_scale, true));
+    else for_heads<kUnroll>(a.k + t * a.k_tok + 8 * part, a.k_head, k0, hk, parts, put(a.pool.k, a.pool.k_scale, false));
+    for_heads<kUnroll>(a.v + t * a.v_tok + 8 * part, a.v_head, v0, hk, parts, put(a.pool.v, a.pool.v_scale, false));
 }
 
 // Read: row r of the packed result is key first[s] + (r - cu_rows[s]) of sequence s, K and V, as bf16 (4-bit rows as the
@@ -388,11 +420,11 @@ int check_paged(const char* what, const fv_paged_kv* kv, const fv_paged_batch* b
     return FV_RAN;
 }
 
-// CTAs that share the heads of the same 16 tokens: as many as keep the GPU busy when there are few tokens, as few as
-// possible (one reads the tables' rows once for all heads) when there are many.
+// CTAs that share the heads of the same 16 tokens: about eight per SM with few tokens, as few as possible (one reads the tables'
+// rows once for all heads) with many.
 static int parts_for(int tokens, int rows, int sms) {
-    const int blocks = (tokens + kTokens - 1) / kTokens;
-    const long long want = (8ll * sms + blocks - 1) / blocks;
+    const long long blocks = (tokens + kTokens - 1) / kTokens;
+    const long long want = (8ll * sms + blocks / 2) / blocks;
     return (int)(want < 1 ? 1 : want > rows ? rows : want);
 }
 
