@@ -88,11 +88,12 @@ int take_spare_sms() {
 static thread_local char g_last_kernel[256] = "";
 static bool g_logged[kLogKeys];
 
-void ran(LogKey key, const char* fmt, ...) {
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(g_last_kernel, sizeof(g_last_kernel), fmt, ap);
-    va_end(ap);
+static thread_local struct {
+    const char *fmt, *text;
+    int v[6];
+} g_last_later;
+
+static void say_first(LogKey key) {
     bool first;
     {
         std::lock_guard<std::mutex> lk(g_mu);
@@ -101,8 +102,22 @@ void ran(LogKey key, const char* fmt, ...) {
     }
     if (first) {
         const char* e = getenv("FV_LOG");
-        if (!e || strcmp(e, "0") != 0) fprintf(stderr, "fvsdpa: %s\n", g_last_kernel);
+        if (!e || strcmp(e, "0") != 0) fprintf(stderr, "fvsdpa: %s\n", fv_last_kernel());
     }
+}
+
+void ran_later(LogKey key, const char* fmt, const char* text, int a, int b, int c, int d, int e, int f) {
+    g_last_later = {fmt, text, {a, b, c, d, e, f}};
+    say_first(key);
+}
+
+void ran(LogKey key, const char* fmt, ...) {
+    g_last_later.fmt = nullptr;
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_last_kernel, sizeof(g_last_kernel), fmt, ap);
+    va_end(ap);
+    say_first(key);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -177,7 +192,14 @@ int encode_map4_cached(CUtensorMap* map, const void* base, const uint64_t dims[4
 
 }  // namespace fvrt
 
-extern "C" const char* fv_last_kernel(void) { return fvrt::g_last_kernel; }
+extern "C" const char* fv_last_kernel(void) {
+    auto& l = fvrt::g_last_later;
+    if (l.fmt) {
+        snprintf(fvrt::g_last_kernel, sizeof(fvrt::g_last_kernel), l.fmt, l.text, l.v[0], l.v[1], l.v[2], l.v[3], l.v[4], l.v[5]);
+        l.fmt = nullptr;
+    }
+    return fvrt::g_last_kernel;
+}
 
 extern "C" int fv_hint_spare_sms(int sms) {
     fvrt::clear_error();

@@ -28,6 +28,9 @@ int take_spare_sms();
 // line of each thread is also kept for fv_last_kernel().
 enum LogKey { kLogDense = 0, kLogCausal, kLogSplitKv, kLogPrep, kLogVsa, kLogSp, kLogGlue, kLogPaged, kLogPagedAttn, kLogPagedChunk, kLogKeys };
 void ran(LogKey key, const char* fmt, ...);
+// The same for calls that take a few microseconds themselves: the line is put together when it is asked for (or the first time its
+// kind is seen).  `fmt` takes one string, then up to six ints; both strings are literals.
+void ran_later(LogKey key, const char* fmt, const char* text, int a = 0, int b = 0, int c = 0, int d = 0, int e = 0, int f = 0);
 
 // 4-D bf16 tensor map, dims innermost first, strides in bytes for dims 1..3,
 // box (64, box_rows, 1, 1), 128-byte swizzle, out-of-range reads as zero.

@@ -161,11 +161,13 @@ struct Values<false> {
         }
     }
     static FV_DEV size_t lane_offset(int g, int t) { return (size_t)(2 * t) * 256 + 16 * g; }
+    FV_DEV float step(int) const { return 1.f; }
 };
 template <>
 struct Values<true> {
     uint2 a[4];
     uint32_t s0, s1;
+    FV_DEV float step(int h) const { return __uint_as_float((h ? s1 : s0) << 16); }
 };
 
 // The ring of a warp (4 bits): a stage is a tile of 32 keys, K codes | V codes | K scales | V scales, brought by bulk copies (in
@@ -177,9 +179,9 @@ struct Ring {
     static constexpr int kStages = 3;
     static constexpr uint32_t kWarpBytes = kStages * kStageBytes;
 };
-template <bool Q4, int NT>
+template <bool Q4, int ROWS>
 struct DecodeSmem {
-    static constexpr uint32_t kJoin = kWarps * 8 * NT * (kD + 4) * 4 + 2 * kWarps * 8 * NT * 4;  // the warps' results side by side
+    static constexpr uint32_t kJoin = kWarps * ROWS * (kD + 4) * 4 + 2 * kWarps * ROWS * 4;  // the warps' results side by side
     static constexpr uint32_t kRing = Q4 ? kWarps * Ring::kWarpBytes : 0;                        // (the join comes after the ring)
     static constexpr uint32_t kBars = kRing > kJoin ? kRing : kJoin;
     static constexpr uint32_t kTotal = kBars + (Q4 ? kWarps * Ring::kStages * 8 : 0);
@@ -221,7 +223,7 @@ FV_DEV uint32_t lds32(uint32_t a) {
     return r;
 }
 
-// NT groups of 8 query rows.  The transposed products S^T = K . Q^T and O^T = V^T . P^T keep keys and head dim on the
+// Up to ROWS query rows (4 bits: 4, 8 or 16, bf16: 8 or 16).  The transposed products S^T = K . Q^T and O^T = V^T . P^T keep keys and head dim on the
 // 16-wide side of the matrix instruction and the (few) query rows on the 8-wide one; the sums of either product may run
 // in any order of d or key, so every lane's operands are whole 16-byte pieces as they lie in memory and no shared
 // memory is needed on the way.
@@ -230,11 +232,12 @@ FV_DEV uint32_t lds32(uint32_t a) {
 // bf16: a tile's K registers are loaded anew as soon as its scores are done and V's as soon as its product is, so that
 // memory is always being read while the warp computes.  4 bits: 16 keys are too few bytes for that (and the registers are
 // needed for more warps: expanding the codes is what bounds this form), so a ring in shared memory runs three stages ahead.
-template <bool Q4, int NT>
-__global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_paged_decode_kernel(const AttnArgs a) {
-    constexpr int kRows = 8 * NT;
+template <bool Q4, int ROWS>
+__global__ void __launch_bounds__(kAttnThreads, ROWS <= 8 ? 3 : 2) fv_paged_decode_kernel(const AttnArgs a) {
+    constexpr int kRows = ROWS, NT = (ROWS + 7) / 8;  // groups of 8 rows, the columns of a product
+    constexpr int EH = ROWS == 4 ? 1 : 2;             // columns of a product in a lane that stand for rows
     constexpr int SUB = kTile<Q4> / 16;  // products of 16 keys in a tile
-    using Sm = DecodeSmem<Q4, NT>;
+    using Sm = DecodeSmem<Q4, ROWS>;
     extern __shared__ __align__(128) unsigned char decode_smem[];
     float (*sh_o)[kRows][kD + 4] = reinterpret_cast<float (*)[kRows][kD + 4]>(decode_smem);
     float (*sh_m)[kRows] = reinterpret_cast<float (*)[kRows]>(decode_smem + kWarps * kRows * (kD + 4) * 4);
@@ -336,6 +339,9 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_p
         vt[0].load(lane_v, row);
     }
 
+    // The row of group n that column 2 t + e stands for.  With at most four rows (4 bits) they take the even columns: the odd ones of a
+    // lane then have no softmax.
+    auto row_of = [&](int n, int e) { return ROWS == 4 ? t : 8 * n + 2 * t + e; };
     // Q^T: column g of each group of 8 rows, in the order of d that the keys' lanes hold.  4 bits: as f16, scaled by a power
     // of two that brings the row's largest value to 2^8 .. 2^9 (what falls below f16's range is 2^-32 of that), which goes into
     // the row's softmax scale; qsum: the row's sum in the same units.
@@ -343,9 +349,9 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_p
     float qsum[NT][2], sl2[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const int r = row0 + 8 * n + g;
+        const int rq = ROWS == 4 ? ((g & 1) ? ROWS : g >> 1) : 8 * n + g, r = row0 + rq;
         uint4 u[4];
-        if (8 * n + g < rows) {
+        if (rq < rows) {
             const uint16_t* p = a.q + (size_t)(seq.q0 + r / a.group) * a.q_tok + (size_t)(head * a.group + r % a.group) * a.q_head;
 #pragma unroll
             for (int i = 0; i < 4; i++) u[i] = *reinterpret_cast<const uint4*>(p + (Q4 ? 32 * t + 8 * i : 32 * i + 8 * t));
@@ -395,7 +401,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_p
         }
     }
 
-    float o[NT][8][4];  // O^T: d by lane g and tile, rows 2 t and 2 t + 1
+    float o[NT][8][4];  // O^T: d by lane g and tile, rows row_of(n, 0) and row_of(n, 1)
     float m[NT][2], l[NT][2], z[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -437,7 +443,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_p
             next_row = __shfl_sync(kFullWarp, i0 + 1 < 32 ? cur.row[0] : nxt.row[0], (i0 + 1) & 31);
         }
 
-        // c0, c1: key g, rows 2 t and 2 t + 1; c2, c3: key g + 8.
+        // c0, c1: key g, rows row_of(n, 0) and (n, 1); c2, c3: key g + 8.
         float c[SUB][NT][4];
 #pragma unroll
         for (int i = 0; i < SUB; i++) {
@@ -467,10 +473,11 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_p
                 const float z0 = fmaf(-8.f, s0, hi_f(kt[i].s0)), z1 = fmaf(-8.f, s1, hi_f(kt[i].s1));
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    c[i][n][0] = fmaf(c[i][n][0], s0, z0 * qsum[n][0]);
-                    c[i][n][1] = fmaf(c[i][n][1], s0, z0 * qsum[n][1]);
-                    c[i][n][2] = fmaf(c[i][n][2], s1, z1 * qsum[n][0]);
-                    c[i][n][3] = fmaf(c[i][n][3], s1, z1 * qsum[n][1]);
+#pragma unroll
+                    for (int e = 0; e < EH; e++) {
+                        c[i][n][e] = fmaf(c[i][n][e], s0, z0 * qsum[n][e]);
+                        c[i][n][2 + e] = fmaf(c[i][n][2 + e], s1, z1 * qsum[n][e]);
+                    }
                 }
             }
             if constexpr (!Q4) {
@@ -491,8 +498,8 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_p
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int r = row0 + 8 * n + 2 * t + e, p = pos0 + r / a.group;
+                    for (int e = 0; e < EH; e++) {
+                        const int r = row0 + row_of(n, e), p = pos0 + r / a.group;
                         const Span sp = span_of(a.mask, p, p, seq.len);
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
@@ -521,15 +528,11 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_p
         constexpr float kGuard = Q4 ? 16384.f : 1099511627776.f, kGuardP = 1.2676506e30f;  // 2^100
         float p[SUB][NT][4] = {}, ps[SUB][NT][4], sum = 0.f, sum_s = 0.f;
         auto weigh = [&vt, &p, &ps](int i, int n) {
-            if constexpr (Q4) {
-                const float s0 = lo_f(vt[i].s0), s1 = lo_f(vt[i].s1);
-                ps[i][n][0] = p[i][n][0] * s0;
-                ps[i][n][1] = p[i][n][1] * s0;
-                ps[i][n][2] = p[i][n][2] * s1;
-                ps[i][n][3] = p[i][n][3] * s1;
-            } else {
+            ps[i][n][1] = ps[i][n][3] = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; e++) ps[i][n][e] = p[i][n][e];
+            for (int e = 0; e < EH; e++) {
+                ps[i][n][e] = Q4 ? p[i][n][e] * vt[i].step(0) : p[i][n][e];
+                ps[i][n][2 + e] = Q4 ? p[i][n][2 + e] * vt[i].step(1) : p[i][n][2 + e];
             }
         };
 #pragma unroll
@@ -537,7 +540,10 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_p
 #pragma unroll
             for (int n = 0; n < NT; n++) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) p[i][n][e] = fvp::ex2(fmaf(c[i][n][e], sl2[n][e & 1], -m[n][e & 1]));
+                for (int e = 0; e < EH; e++) {
+                    p[i][n][e] = fvp::ex2(fmaf(c[i][n][e], sl2[n][e], -m[n][e]));
+                    p[i][n][2 + e] = fvp::ex2(fmaf(c[i][n][2 + e], sl2[n][e], -m[n][e]));
+                }
                 weigh(i, n);
                 if (Q4) sum += (p[i][n][0] + p[i][n][1]) + (p[i][n][2] + p[i][n][3]);
                 sum_s += (ps[i][n][0] + ps[i][n][1]) + (ps[i][n][2] + ps[i][n][3]);
@@ -547,7 +553,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_p
 #pragma unroll
             for (int n = 0; n < NT; n++) {
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
+                for (int e = 0; e < EH; e++) {
                     float mx = neg_inf();
 #pragma unroll
                     for (int i = 0; i < SUB; i++) {
@@ -589,12 +595,13 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_p
             uint32_t pb[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                l[n][0] += p[i][n][0] + p[i][n][2];
-                l[n][1] += p[i][n][1] + p[i][n][3];
-                if constexpr (Q4) {
-                    const float z0 = fmaf(-8.f, lo_f(vt[i].s0), hi_f(vt[i].s0)), z1 = fmaf(-8.f, lo_f(vt[i].s1), hi_f(vt[i].s1));
-                    z[n][0] = fmaf(p[i][n][0], z0, fmaf(p[i][n][2], z1, z[n][0]));
-                    z[n][1] = fmaf(p[i][n][1], z0, fmaf(p[i][n][3], z1, z[n][1]));
+#pragma unroll
+                for (int e = 0; e < EH; e++) {
+                    l[n][e] += p[i][n][e] + p[i][n][2 + e];
+                    if constexpr (Q4) {
+                        const float z0 = fmaf(-8.f, vt[i].step(0), hi_f(vt[i].s0)), z1 = fmaf(-8.f, vt[i].step(1), hi_f(vt[i].s1));
+                        z[n][e] = fmaf(p[i][n][e], z0, fmaf(p[i][n][2 + e], z1, z[n][e]));
+                    }
                 }
                 pb[n][0] = transpose8(pack_p<Q4>(ps[i][n][0], ps[i][n][1]));
                 pb[n][1] = transpose8(pack_p<Q4>(ps[i][n][2], ps[i][n][3]));
@@ -644,7 +651,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_p
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
+                    for (int e = 0; e < EH; e++) {
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) z[n][e] += __shfl_xor_sync(kFullWarp, z[n][e], d);
 #pragma unroll
@@ -664,13 +671,13 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? (Q4 ? 4 : 3) : 2) fv_p
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
+        for (int e = 0; e < EH; e++) {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) {
                 l[n][e] += __shfl_xor_sync(kFullWarp, l[n][e], d);
                 z[n][e] += __shfl_xor_sync(kFullWarp, z[n][e], d);
             }
-            const int r = 8 * n + 2 * t + e;
+            const int r = row_of(n, e);
             if (g == 0) {
                 sh_m[warp][r] = m[n][e];
                 sh_l[warp][r] = l[n][e];
@@ -878,7 +885,7 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_join_kernel(const Chunk
 
 struct Shape {
     bool chunk;  // the tensor-core kernel for long chunks
-    int splits, row_blocks, nt, tile_tokens;
+    int splits, row_blocks, block_rows, tile_tokens;
     bool cluster;
     int ctas, phases;  // of the chunk kernel
 };
@@ -894,7 +901,7 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads,
     s.tile_tokens = s.chunk ? kChunkRows / group : 0;
     s.cluster = false;
     if (s.chunk) {
-        s.nt = 0;
+        s.block_rows = 0;
         s.splits = 1;
         s.row_blocks = (b->max_q + 2 * s.tile_tokens - 1) / (2 * s.tile_tokens);
         // (an upper bound of the line's length: with little work no more CTAs are launched than may find a run)
@@ -913,8 +920,8 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads,
         s.phases = bytes > kL2Bytes && longest / ((long long)s.ctas * kMaxPhases) >= 32 ? kMaxPhases : 1;
         return s;
     }
-    s.nt = rows > 8 ? 2 : 1;
-    s.row_blocks = (int)((rows + 8 * s.nt - 1) / (8 * s.nt));
+    s.block_rows = rows > 8 ? 16 : rows <= 4 && kv->format == FV_PAGE_Q4 ? 4 : 8;
+    s.row_blocks = (int)((rows + s.block_rows - 1) / s.block_rows);
     long long keys = b->max_kv;
     if (m.block > 0 && m.window > 0) {  // rows of one block see window blocks and the sinks, max_q rows a little more
         const long long most = ((long long)m.window + m.sink + 1) * m.block + b->max_q;
@@ -924,7 +931,7 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads,
     // Key ranges: as many as fill the SMs once; where the rows alone nearly do, three times over, so that ragged ends even
     // out.  Up to kMaxCluster ranges are one cluster, which joins its parts itself; the merge kernel behind more of them takes
     // about 5 us, so more need enough tiles a warp (0.75 us each) to be worth it.
-    const int resident = sms * (s.nt == 1 ? (kv->format == FV_PAGE_Q4 ? 4 : 3) : 2);  // CTAs that run at a time
+    const int resident = sms * (s.block_rows <= 8 ? 3 : 2);  // CTAs that run at a time
     const long long tiles = (keys + 15) / 16, most = (tiles + 2 * kWarps - 1) / (2 * kWarps);  // at least 32 keys per warp
     long long n = resident / ctas;
     if (n < 2) n = (3ll * resident + ctas - 1) / ctas;
@@ -1000,8 +1007,8 @@ static int launch_chunk(cudaStream_t st, const fv_paged_kv* kv, const AttnArgs& 
         fv_paged_join_kernel<<<grid * s.phases * kJoinBlocks, kAttnThreads, 0, st>>>(jb);
         FV_CUDA(cudaGetLastError());
     }
-    fvrt::ran(fvrt::kLogPagedChunk, "paged attention: fv_paged_chunk_kernel<%s> (sm_100a tcgen05, persistent, %u CTAs) %d sequences x %d heads / %d",
-              q4 ? "4 bits" : "bf16", grid, a.batch.seqs, a.heads, a.pool.kv_heads);
+    fvrt::ran_later(fvrt::kLogPagedChunk, "paged attention: fv_paged_chunk_kernel<%s> (sm_100a tcgen05, persistent, %d CTAs) %d sequences x %d heads / %d",
+              q4 ? "4 bits" : "bf16", (int)grid, a.batch.seqs, a.heads, a.pool.kv_heads);
     return FV_RAN;
 }
 
@@ -1085,17 +1092,18 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
         fn = f;
         smem = bytes;
     };
-    if (q4 && s.nt == 1) pick(fv_paged_decode_kernel<true, 1>, DecodeSmem<true, 1>::kTotal);
-    else if (q4) pick(fv_paged_decode_kernel<true, 2>, DecodeSmem<true, 2>::kTotal);
-    else if (s.nt == 1) pick(fv_paged_decode_kernel<false, 1>, DecodeSmem<false, 1>::kTotal);
-    else pick(fv_paged_decode_kernel<false, 2>, DecodeSmem<false, 2>::kTotal);
+    if (q4 && s.block_rows == 4) pick(fv_paged_decode_kernel<true, 4>, DecodeSmem<true, 4>::kTotal);
+    else if (q4 && s.block_rows == 8) pick(fv_paged_decode_kernel<true, 8>, DecodeSmem<true, 8>::kTotal);
+    else if (q4) pick(fv_paged_decode_kernel<true, 16>, DecodeSmem<true, 16>::kTotal);
+    else if (s.block_rows == 8) pick(fv_paged_decode_kernel<false, 8>, DecodeSmem<false, 8>::kTotal);
+    else pick(fv_paged_decode_kernel<false, 16>, DecodeSmem<false, 16>::kTotal);
     if (q4) {  // (more shared memory than a launch gets unasked)
-        static bool attr_set[64][3] = {};
+        static bool attr_set[64][17] = {};
         static std::mutex attr_mu;
         std::lock_guard<std::mutex> lock(attr_mu);
-        if (!attr_set[dev][s.nt]) {
+        if (!attr_set[dev][s.block_rows]) {
             FV_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-            attr_set[dev][s.nt] = true;
+            attr_set[dev][s.block_rows] = true;
         }
     }
     cudaLaunchConfig_t cfg{};
@@ -1114,7 +1122,7 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
         fv_paged_merge_kernel<<<(unsigned)((rows + kWarps - 1) / kWarps), kAttnThreads, 0, st>>>(a);
         FV_CUDA(cudaGetLastError());
     }
-    fvrt::ran(fvrt::kLogPagedAttn, "paged attention: fv_paged_decode_kernel<%s, %d rows> %d sequences x %d heads / %d, %d key ranges",
-              q4 ? "4 bits" : "bf16", 8 * s.nt, b->seqs, heads, kv->kv_heads, s.splits);
+    fvrt::ran_later(fvrt::kLogPagedAttn, "paged attention: fv_paged_decode_kernel<%s, %d rows> %d sequences x %d heads / %d, %d key ranges",
+              q4 ? "4 bits" : "bf16", s.block_rows, b->seqs, heads, kv->kv_heads, s.splits);
     return FV_RAN;
 }

@@ -472,7 +472,7 @@ extern "C" int fv_paged_append_bf16(void* stream, const fv_paged_kv* kv, const f
                        : (half ? fv_paged_append_kernel<false, true> : fv_paged_append_kernel<false, false>);
     fn<<<(unsigned)grid, kThreads, 0, (cudaStream_t)stream>>>(a);
     FV_CUDA(cudaGetLastError());
-    fvrt::ran(fvrt::kLogPaged, "paged append: fv_paged_append_kernel<%s> %d tokens x (%d + 2 x %d) heads", q4 ? "4 bits" : "bf16",
+    fvrt::ran_later(fvrt::kLogPaged, "paged append: fv_paged_append_kernel<%s> %d tokens x (%d + 2 x %d) heads", q4 ? "4 bits" : "bf16",
               tokens, a.q_heads, kv->kv_heads);
     return FV_RAN;
 }
@@ -502,7 +502,7 @@ extern "C" int fv_paged_read_bf16(void* stream, const fv_paged_kv* kv, const fv_
     if (kv->format == FV_PAGE_Q4) fv_paged_read_kernel<true><<<(unsigned)grid, kThreads, 0, (cudaStream_t)stream>>>(a);
     else fv_paged_read_kernel<false><<<(unsigned)grid, kThreads, 0, (cudaStream_t)stream>>>(a);
     FV_CUDA(cudaGetLastError());
-    fvrt::ran(fvrt::kLogPaged, "paged read: fv_paged_read_kernel<%s> %d rows x 2 x %d heads", kv->format == FV_PAGE_Q4 ? "4 bits" : "bf16", rows,
+    fvrt::ran_later(fvrt::kLogPaged, "paged read: fv_paged_read_kernel<%s> %d rows x 2 x %d heads", kv->format == FV_PAGE_Q4 ? "4 bits" : "bf16", rows,
               kv->kv_heads);
     return FV_RAN;
 }

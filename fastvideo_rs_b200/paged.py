@@ -127,22 +127,33 @@ class PagedBatch:
 _bf16, _f32, _SCALE = torch.bfloat16, torch.float32, D ** -0.5
 
 
-def _heads_in(name: str, t: torch.Tensor, tokens: int, heads: int, index: int) -> None:
-    """t is bf16 [tokens, heads, 128] on device `index` (-1: any number of tokens or heads)."""
-    shape = t.shape
+def _refuse(name: str, t: torch.Tensor, index: int, tokens: int = -1, heads: int = -1) -> None:
+    """Says why t is not bf16 [tokens, heads, 128] on device `index` (-1: any number of tokens or heads)."""
     if t.get_device() != index:
         raise ValueError(f"{name} must be a CUDA tensor on cuda:{index}: this package has no CPU path")
-    if t.dtype != _bf16 or len(shape) != 3 or shape[2] != D or (t.stride(2) != 1 and t.numel() > 0):
+    if t.dtype != _bf16 or t.dim() != 3 or t.shape[2] != D or (t.stride(2) != 1 and t.numel() > 0):
         raise ValueError(f"{name} must be bfloat16 [tokens, heads, 128] with adjacent values")
-    if (tokens >= 0 and shape[0] != tokens) or (heads >= 0 and shape[1] != heads):
-        raise ValueError(f"{name} is {list(shape)}: {tokens} tokens of {heads} heads are wanted")
+    raise ValueError(f"{name} is {list(t.shape)}: {tokens} tokens of {heads} heads are wanted")
 
 
-def _strides(t: torch.Tensor) -> Tuple[int, int]:
-    """Strides of tokens and heads; those of an extent of one mean nothing and count as a row's."""
-    a, b, _ = t.stride()
-    n, h, _ = t.shape
-    return (a if n > 1 else D), (b if h > 1 else D)
+def _heads_in(name: str, t: torch.Tensor, index: int, tokens: int = -1, heads: int = -1) -> Tuple[int, int, int, int]:
+    """(tokens, heads, their strides) of a bf16 [tokens, heads, 128] tensor; the stride of an extent of one means nothing and
+    counts as a row's.  (Reads each property once: a decode step passes here for every layer, and the time between two
+    launches is what it costs.)"""
+    shape = t.shape
+    if len(shape) != 3 or t.dtype is not _bf16 or t.get_device() != index:
+        _refuse(name, t, index)
+    n, h, d = shape
+    a, b, c = t.stride()
+    if d != D or (c != 1 and n * h) or (tokens >= 0 and n != tokens) or (heads >= 0 and h != heads):
+        _refuse(name, t, index, tokens, heads)
+    return n, h, a if n > 1 else D, b if h > 1 else D
+
+
+def _rows_like(q: torch.Tensor, n: int, h: int) -> torch.Tensor:
+    """A contiguous [n, h, 128] result beside q."""
+    out = torch.empty_like(q)  # (keeps q's order of extents, which is nearly always this one)
+    return out if out.is_contiguous() else q.new_empty((n, h, D))
 
 
 def _call(kv: PagedKv, batch: PagedBatch, what: str, fn, *args) -> None:
@@ -167,17 +178,18 @@ def append(kv: PagedKv, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, *, 
     given: token t with row positions[t] (int32), by default its position in its sequence.  pairing "interleaved": values
     2 i and 2 i + 1 (the tables of wan.wan_rope_tables), "half": values i and i + 64.  q [tokens, heads, 128], if given, is
     rotated too and returned as [tokens, heads, 128].  Two tokens of a call must not fall on the same cache row."""
-    tokens, index = k.shape[0], kv.index
-    _heads_in("append: k", k, -1, kv.kv_heads, index)
-    _heads_in("append: v", v, tokens, kv.kv_heads, index)
+    index = kv.index
+    tokens, _, kt, kh = _heads_in("append: k", k, index, -1, kv.kv_heads)
+    _, _, vt, vh = _heads_in("append: v", v, index, tokens, kv.kv_heads)
     if pairing not in PAIRINGS:
         raise ValueError(f"append: unknown pairing {pairing!r} {tuple(PAIRINGS)}")
     cp = sp = pp = None
     rows = 0
     if cos is not None and sin is not None:
-        rows = cos.shape[0]
+        shape = cos.shape
+        rows = shape[0] if len(shape) == 2 else 0
         for name, t in (("cos", cos), ("sin", sin)):
-            if t.dtype != _f32 or t.get_device() != index or not t.is_contiguous() or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != D:
+            if t.shape != (rows, D) or t.dtype is not _f32 or t.get_device() != index or not t.is_contiguous():
                 raise ValueError(f"append: {name} must be a contiguous CUDA float32 [rows, 128] tensor on cuda:{index}")
         cp, sp = cos.data_ptr(), sin.data_ptr()
         if positions is not None:
@@ -187,23 +199,19 @@ def append(kv: PagedKv, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, *, 
     heads = qt = qh = 0
     qp = op = None
     if q is not None:
-        _heads_in("append: q", q, tokens, -1, index)
-        heads, qp, (qt, qh) = q.shape[1], q.data_ptr(), _strides(q)
+        _, heads, qt, qh = _heads_in("append: q", q, index, tokens)
         if q_out is None:
-            q_out = q.new_empty((tokens, heads, D))
+            q_out = _rows_like(q, tokens, heads)
         else:
-            _heads_in("append: q_out", q_out, tokens, heads, index)
+            _heads_in("append: q_out", q_out, index, tokens, heads)
             if not q_out.is_contiguous():
                 raise ValueError("append: q_out must be contiguous")
-        op = q_out.data_ptr()
-        if heads == 0:
-            qp = op = None
+        if heads:
+            qp, op = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("append: q_out without q")
     if tokens == 0 or batch.seqs == 0 or batch.max_q == 0:
         return q_out
-    kt, kh = _strides(k)
-    vt, vh = _strides(v)
     _call(kv, batch, "paged append", (_fns or _entries())[0], tokens, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, qp, qt, qh, heads, op,
           cp, sp, rows, pp, PAIRINGS[pairing])
     return q_out
@@ -239,14 +247,13 @@ def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[Block
     by token, a window of `window` tokens, the first `sink` tokens always visible; block_tokens of a frame: the streaming
     form of the block-causal mask.  A row that sees no key is zero.  Pages of which no row sees a key need not exist.
     With `out`, rows that belong to no sequence keep what they hold."""
-    _heads_in("attend: q", q, -1, -1, kv.index)
-    tokens, heads, _ = q.shape
+    tokens, heads, qt, qh = _heads_in("attend: q", q, kv.index)
     if heads < 1 or heads % kv.kv_heads:
         raise ValueError(f"attend: {heads} heads over {kv.kv_heads} K/V heads")
     if out is None:
-        out = q.new_empty((tokens, heads, D))
+        out = _rows_like(q, tokens, heads)
     else:
-        _heads_in("attend: out", out, tokens, heads, kv.index)
+        _heads_in("attend: out", out, kv.index, tokens, heads)
         if not out.is_contiguous():
             raise ValueError("attend: out must be contiguous")
     if tokens == 0 or batch.seqs == 0 or batch.max_q == 0:
@@ -262,7 +269,6 @@ def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[Block
                 need = batch._need[key] = fns[2](kv._ref, batch._ref, tokens, heads, *how)
     # (scratch of this call alone, from the stream's own pool: calls on other streams and captured graphs share nothing)
     ws = q.new_empty((need // 2,)) if need else None
-    qt, qh = _strides(q)
     _call(kv, batch, "paged attention", fns[3], tokens, q.data_ptr(), qt, qh, heads, *how, _SCALE if scale is None else float(scale),
           out.data_ptr(), ws.data_ptr() if need else None, need)
     return out
