@@ -11,6 +11,7 @@
 #include <cooperative_groups.h>
 #include <math.h>
 #include <stdlib.h>
+#include <string.h>
 #include <mutex>
 
 namespace fvpg {
@@ -819,7 +820,7 @@ fv_paged_chunk_kernel(const __grid_constant__ CUtensorMap mq, const __grid_const
 // others with the runs after it.  A warp a row; which parts there are is worked out once per block, a lane a run, and the
 // weights of a row a lane a part (one lane doing both for every row took 34 us for the 147 cuts of a launch, this 8).
 constexpr int kJoinBlocks = 16;  // of a split item's 256 rows
-constexpr int kMaxRuns = 1024;   // (kMaxPhases x SMs at most)
+constexpr int kMaxRuns = 1024;   // of a launch
 __global__ void __launch_bounds__(kAttnThreads) fv_paged_join_kernel(const ChunkJob jb) {
     __shared__ int slots[kMaxRuns];
     __shared__ int count;
@@ -889,15 +890,33 @@ struct Shape {
     bool cluster;
     int ctas, phases;  // of the chunk kernel
 };
-// How a call is cut.  Few rows per kv head: blocks of 8 or 16 rows, and the keys in `splits` ranges so that all SMs have
-// work.  From kChunkFrom rows on: items of 2 x 128 rows, one CTA per SM.
-constexpr int kChunkFrom = 33;
+// How a call is cut.  Few rows per kv head: blocks of up to 16 rows, and the keys in `splits` ranges so that all SMs have
+// work.  Many: items of 2 x 128 rows, one CTA per SM.  Which of the two: an estimate of both in us, fitted to sweeps over 16 to 160
+// rows, 1 to 32 sequences of 2 000 to 20 011 keys and both page formats (e.g. 8 sequences of 20 011 bf16 keys, 32 heads on 8: 16 rows
+// 112 us in blocks of 16 and 123 us in items, 24 rows 197 and 125; one sequence of 20 011: 64 rows 56 and 62, 96 rows 126 and 62;
+// one of 2 000: 160 rows 22 and 35).  FV_PAGED_KERNEL=rows or items (kept for A/B) takes the choice away.
 constexpr long long kL2Bytes = 126ll << 20;
+static bool take_items(long long planes, long long rows, long long keys, bool q4) {
+    const char* e = getenv("FV_PAGED_KERNEL");
+    if (e && strcmp(e, "items") == 0) return true;
+    if ((e && strcmp(e, "rows") == 0) || rows <= 16) return false;
+    const double work = (double)planes * keys, blocks = (double)((rows + 15) / 16), items = (double)((rows + 255) / 256);
+    const double stream = work * (q4 ? 2 * kQ4Bytes + 8 : 4 * kD) / 5.9e6, compute = work * blocks * (q4 ? 4.5e-5 : 7e-5);
+    const double in_rows = 10.0 + (stream > compute ? stream : compute);
+    const double in_items = 35.0 + items * (work / kChunkTile + planes * kItemCost) * 0.0142;
+    return in_items < in_rows;
+}
 static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads, const Mask& m, int sms) {
     Shape s;
     const int group = heads / kv->kv_heads;
     const long long rows = (long long)b->max_q * group;
-    s.chunk = rows >= kChunkFrom && group <= kChunkRows;
+    long long keys = b->max_kv;
+    if (m.block > 0 && m.window > 0) {  // rows of one block see window blocks and the sinks, max_q rows a little more
+        const long long most = ((long long)m.window + m.sink + 1) * m.block + b->max_q;
+        keys = most < keys ? most : keys;
+    }
+    const bool q4 = kv->format == FV_PAGE_Q4;
+    s.chunk = group <= kChunkRows && take_items((long long)b->seqs * kv->kv_heads, rows, keys, q4);
     s.tile_tokens = s.chunk ? kChunkRows / group : 0;
     s.cluster = false;
     if (s.chunk) {
@@ -911,22 +930,12 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads,
         // Every CTA streams the keys of its items.  Where the keys of all items are more than L2 holds, the line is gone through in
         // four phases, all CTAs on a quarter of it at a time (4 680 rows x 40 heads over 28 080 bf16 keys: 3 297 -> 2 901 us, 12 heads:
         // 924 -> 827 us); where they fit that only makes more parts (1 501-token chunks over 69 MB of keys: 358 -> 422 us).
-        long long seen = b->max_kv;
-        if (m.block > 0 && m.window > 0) {
-            const long long some = ((long long)m.window + m.sink + 1) * m.block + b->max_q;
-            seen = some < seen ? some : seen;
-        }
-        const long long bytes = seen * b->seqs * kv->kv_heads * (kv->format == FV_PAGE_Q4 ? 2 * kQ4Bytes + 8 : 4 * kD);
-        s.phases = bytes > kL2Bytes && longest / ((long long)s.ctas * kMaxPhases) >= 32 ? kMaxPhases : 1;
+        const long long bytes = keys * b->seqs * kv->kv_heads * (q4 ? 2 * kQ4Bytes + 8 : 4 * kD);
+        s.phases = bytes > kL2Bytes && longest / ((long long)s.ctas * kMaxPhases) >= 32 && s.ctas * kMaxPhases <= kMaxRuns ? kMaxPhases : 1;
         return s;
     }
-    s.block_rows = rows > 8 ? 16 : rows <= 4 && kv->format == FV_PAGE_Q4 ? 4 : 8;
+    s.block_rows = rows > 8 ? 16 : rows <= 4 && q4 ? 4 : 8;
     s.row_blocks = (int)((rows + s.block_rows - 1) / s.block_rows);
-    long long keys = b->max_kv;
-    if (m.block > 0 && m.window > 0) {  // rows of one block see window blocks and the sinks, max_q rows a little more
-        const long long most = ((long long)m.window + m.sink + 1) * m.block + b->max_q;
-        keys = most < keys ? most : keys;
-    }
     const long long ctas = (long long)b->seqs * kv->kv_heads * s.row_blocks;
     // Key ranges: as many as fill the SMs once; where the rows alone nearly do, three times over, so that ragged ends even
     // out.  Up to kMaxCluster ranges are one cluster, which joins its parts itself; the merge kernel behind more of them takes

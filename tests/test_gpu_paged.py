@@ -12,6 +12,13 @@ pytestmark = pytest.mark.gpu
 FMTS = ["bf16", "q4"]
 
 
+@pytest.fixture(params=["rows", "items"])
+def kernel(request, monkeypatch):
+    """Either of the two attention kernels, whichever the sizes would choose."""
+    monkeypatch.setenv("FV_PAGED_KERNEL", request.param)
+    return request.param
+
+
 def check(got, want, bound, what):
     assert torch.isfinite(got).all(), what
     err = (got.double().cpu() - want).abs()
@@ -55,7 +62,7 @@ ATTEND = [
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("i", range(len(ATTEND)))
-def test_attend_matches_the_formula(fvlib, fmt, i):
+def test_attend_matches_the_formula(fvlib, kernel, fmt, i):
     from fastvideo_rs_b200 import paged, sdpa
     kv_len, nq, heads, hk, rows, mask = ATTEND[i]
     case = Case(fmt, kv_len, nq, heads, hk, rows, seed=100 + i)
@@ -67,9 +74,43 @@ def test_attend_matches_the_formula(fvlib, fmt, i):
     assert torch.equal(out, paged.attend(kv, batch, q, mask_of(mask)))  # the same bits again
 
 
+# Work for the long-chunk kernel: ragged, cut across CTAs, parts joined.
+LARGE = [
+    ([3000, 1111], [600, 300], 4, 2, 64, (1, 0, 0)),
+    ([4000], [700], 5, 1, 16, (1, 1500, 6)),
+    ([2600, 90, 2000], [500, 90, 1], 6, 2, 128, (40, 9, 1)),
+    ([6000], [1300], 2, 2, 32, None),
+]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("i", range(len(LARGE)))
+def test_long_chunks_cut_and_joined(fvlib, fmt, i, monkeypatch):
+    from fastvideo_rs_b200 import _lib, paged, sdpa
+    monkeypatch.setenv("FV_PAGED_KERNEL", "items")
+    kv_len, nq, heads, hk, rows, mask = LARGE[i]
+    case = Case(fmt, kv_len, nq, heads, hk, rows, seed=200 + i)
+    kv, batch, q = case.device()
+    out = paged.attend(kv, batch, q, mask_of(mask))
+    assert "fv_paged_chunk_kernel" in _lib.last_kernel()
+    assert sdpa.device_status() == 0
+    want, bound = case.expect(mask)
+    check(out, want, bound, f"{fmt} {LARGE[i]}")
+    assert torch.equal(out, paged.attend(kv, batch, q, mask_of(mask)))
+
+
+def test_which_kernel_runs(fvlib):
+    from fastvideo_rs_b200 import _lib, paged
+    for fmt in FMTS:
+        for kv_len, nq, name in (([300], [1], "decode"), ([300], [60], "decode"), ([6000], [1300], "chunk")):
+            kv, batch, q = Case(fmt, kv_len, nq, 4, 2, 64).device()
+            paged.attend(kv, batch, q, mask_of((1, 0, 0)))
+            assert f"fv_paged_{name}_kernel<{'4 bits' if fmt == 'q4' else 'bf16'}" in _lib.last_kernel()
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("i", [2, 3, 7, 8, 12, 16, 19])
-def test_memory_that_no_row_sees_has_no_influence(fvlib, fmt, i):
+def test_memory_that_no_row_sees_has_no_influence(fvlib, kernel, fmt, i):
     """Rows behind the sequences, unused pages and pages outside of the window hold NaN or are given back."""
     from fastvideo_rs_b200 import paged, sdpa
     kv_len, nq, heads, hk, rows, mask = ATTEND[i]
@@ -90,7 +131,7 @@ def test_memory_that_no_row_sees_has_no_influence(fvlib, fmt, i):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("nq,heads", [(1, 8), (200, 4)])
-def test_large_scores_move_the_reference(fvlib, fmt, nq, heads):
+def test_large_scores_move_the_reference(fvlib, kernel, fmt, nq, heads):
     """Scores that grow along the keys by far more than the softmax's guard: every tile outgrows the reference."""
     from fastvideo_rs_b200 import paged
     case = Case(fmt, [400], [nq], heads, 2, 16, seed=7)
@@ -103,7 +144,7 @@ def test_large_scores_move_the_reference(fvlib, fmt, nq, heads):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("nq", [3, 150])
-def test_rows_before_the_sequence_are_zero(fvlib, fmt, nq):
+def test_rows_before_the_sequence_are_zero(fvlib, kernel, fmt, nq):
     """More new tokens than the sequence holds: the first rows have no position and see nothing."""
     from fastvideo_rs_b200 import paged, sdpa
     case = Case(fmt, [2], [nq], 4, 2, 16, seed=3)
@@ -119,7 +160,7 @@ def test_rows_before_the_sequence_are_zero(fvlib, fmt, nq):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("nq", [1, 170])
-def test_padded_batch_strides_stream_and_out(fvlib, fmt, nq):
+def test_padded_batch_strides_stream_and_out(fvlib, kernel, fmt, nq):
     from fastvideo_rs_b200 import paged, sdpa
     case = Case(fmt, [500, 300], [nq, 1], 4, 2, 16, seed=5, pad=7)
     kv, batch, q = case.device()
@@ -141,7 +182,7 @@ def test_padded_batch_strides_stream_and_out(fvlib, fmt, nq):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
-def test_scale_argument(fvlib, fmt):
+def test_scale_argument(fvlib, kernel, fmt):
     from fastvideo_rs_b200 import paged
     case = Case(fmt, [333], [20], 4, 2, 16, seed=6)
     kv, batch, q = case.device()
@@ -151,7 +192,7 @@ def test_scale_argument(fvlib, fmt):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("nq", [1, 140])
-def test_captured_call_follows_the_tables(fvlib, fmt, nq):
+def test_captured_call_follows_the_tables(fvlib, kernel, fmt, nq):
     """A captured call reads lengths, rows and tables anew at every replay, within the bounds it was captured with."""
     from fastvideo_rs_b200 import paged, sdpa
     a = Case(fmt, [900, 450], [nq, 1], 4, 2, 16, seed=8)
@@ -294,7 +335,7 @@ def test_reading_whole_sequences_and_ranges(fvlib, fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
-def test_streaming_run_equals_one_chunk(fvlib, fmt):
+def test_streaming_run_equals_one_chunk(fvlib, kernel, fmt):
     """A prompt and then single tokens, appended and attended to step by step under a sliding window with sinks whose pages
     are given back as it slides, against the formula over everything that was appended."""
     from fastvideo_rs_b200 import paged, sdpa
@@ -336,7 +377,7 @@ def test_streaming_run_equals_one_chunk(fvlib, fmt):
     check(got, want, room, fmt)
 
 
-def test_rows_past_four_gigabytes(fvlib):
+def test_rows_past_four_gigabytes(fvlib, kernel):
     """Pages whose byte offsets pass 32 bits."""
     from fastvideo_rs_b200 import paged, sdpa
     pages, rows = 70000, 256
@@ -354,7 +395,7 @@ def test_rows_past_four_gigabytes(fvlib):
 
 
 @pytest.mark.parametrize("nq", [1, 150])
-def test_broken_tables_are_reported_and_not_followed(fvlib, nq):
+def test_broken_tables_are_reported_and_not_followed(fvlib, kernel, nq):
     from fastvideo_rs_b200 import FvError, paged, sdpa
     mask = mask_of((1, 0, 0))
     case = Case("bf16", [400, 200], [nq, 1], 4, 2, 16, seed=11)
