@@ -9,5 +9,6 @@ are the host-side mirror of the reference interface over torch tensors:
     wan        rope tables, q/k RMSNorm + RoPE prologue, WanSelfAttention
     sp         shard_ranges and the sequence-parallel attention
     vsa        TilePlan and video sparse attention
+    paged      a paged K/V cache in bf16 or 4 bits: append with rotation, read back, attention with window and sinks
 """
 from ._lib import Declined, FvError  # noqa: F401

@@ -1067,7 +1067,10 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
     if (!q || !out) return fvrt::fail(FV_ERR_INVALID, "paged attention: null operand");
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15)
         return fvrt::fail(FV_ERR_INVALID, "paged attention: operands must be 16-byte aligned");
-    if ((q_tok | q_head) & 7) return fvrt::fail(FV_ERR_INVALID, "paged attention: strides must be multiples of 8 values");
+    if (tokens == 1) q_tok = kD;  // (the stride of an extent of one means nothing)
+    if (heads == 1) q_head = kD;
+    if (((q_tok | q_head) & 7) || q_tok <= 0 || q_head <= 0)
+        return fvrt::fail(FV_ERR_INVALID, "paged attention: strides must be positive multiples of 8 values");
     rc = fvrt::sm_count(dev, &sms);
     if (rc != FV_RAN) return rc;
     const Shape s = shape_of(kv, b, heads, a.mask, sms);

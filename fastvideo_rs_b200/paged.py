@@ -116,8 +116,8 @@ class PagedBatch:
         self.page_table = _index("PagedBatch: page_table", page_table, (seqs, width), dev)
         self.kv_len = _index("PagedBatch: kv_len", kv_len, (seqs,), dev)
         self.cu_q = _index("PagedBatch: cu_q", cu_q, (seqs + 1,), dev)
-        if max_q < 0 or max_kv < 0:
-            raise ValueError("PagedBatch: max_q and max_kv must not be negative")
+        if not 0 <= max_q < 1 << 30 or not 0 <= max_kv < 1 << 30:
+            raise ValueError("PagedBatch: max_q and max_kv must be 0 .. 2^30 - 1")
         self.seqs, self.max_q, self.max_kv, self.device, self.index = seqs, int(max_q), int(max_kv), dev, page_table.get_device()
         self._need = {}  # scratch bytes by the call's shape: a step asks for every layer
         self._c = _BatchC(page_table.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), seqs, width, self.max_q, self.max_kv)
@@ -245,7 +245,9 @@ def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[Block
     mask None: every key of the sequence.  BlockCausal(block_tokens, window, sink): key j is visible to position p iff
     t_j <= t_p and (window == 0 or t_p - t_j < window or t_j < sink), t = index // block_tokens -- block_tokens 1: causal
     by token, a window of `window` tokens, the first `sink` tokens always visible; block_tokens of a frame: the streaming
-    form of the block-causal mask.  A row that sees no key is zero.  Pages of which no row sees a key need not exist.
+    form of the block-causal mask.  A row that sees no key is zero.  Pages of which no row sees a key need not exist.  Sums and softmax statistics are f32,
+    probabilities are rounded to the type of the products: bf16, over 4-bit pages f16 (there long chunks also take q and the
+    cached values through f16: what is beyond 65 504 saturates, what is below 2^-14 loses relative precision).
     With `out`, rows that belong to no sequence keep what they hold."""
     tokens, heads, qt, qh = _heads_in("attend: q", q, kv.index)
     if heads < 1 or heads % kv.kv_heads:
@@ -263,6 +265,8 @@ def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[Block
     key = (how, heads, kv.kv_heads, tokens)
     need = batch._need.get(key)
     if need is None:
+        if max(how) > 0x7fffffff or min(how) < 0:
+            raise ValueError(f"attend: {mask} is out of range")
         need = 0
         if kv.index >= 0:
             with torch.cuda.device(kv.index):

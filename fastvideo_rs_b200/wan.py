@@ -117,6 +117,21 @@ class WanSelfAttention:
         plan = Plan.block_causal(scale, self.causal) if self.causal is not None else Plan.dense(scale)
         return sdpa(q, k, v, plan)
 
+    def forward_paged(self, qkv: torch.Tensor, kv, batch, *, positions: Optional[torch.Tensor] = None,
+                      scale: Optional[float] = None) -> torch.Tensor:
+        """forward_self over a paged K/V cache (paged.PagedKv, paged.PagedBatch), for streaming rollouts of any number and length:
+        qkv [1, tokens, 3 * dim] bf16 holds the batch's tokens packed one sequence after the other.  q and k are normalised,
+        rotated with the table rows of their positions in their sequences (or of `positions`, int32 [tokens]) while K and V
+        are appended, and the queries attend to the cache under this layer's block-causal mask (all keys without one).
+        Returns [tokens, heads, 128], the merged heads of every token.  (q and k are rounded to bf16 between norm and
+        rotation, which forward_self is not.)"""
+        from . import paged
+        if qkv.dim() != 3 or qkv.shape[0] != 1:
+            raise ValueError("forward_paged: qkv must be [1, tokens, 3 * dim], the sequences packed")
+        q, k, v = (t[0].transpose(0, 1) for t in qk_prep(qkv, self.wq, self.wk, None, None, self.heads, eps=self.eps))
+        q = paged.append(kv, batch, k, v, q=q, cos=self.cos, sin=self.sin, positions=positions)
+        return paged.attend(kv, batch, q, self.causal, scale=scale)
+
     def attend_vsa(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, gate_proj: torch.Tensor) -> torch.Tensor:
         """attend_vsa (wan/transformer.rs:354-390): q, k normed and roped, v split, BHSD; the gate is the gate
         projection split into heads with no norm and no rotation (wan/transformer.rs:336-347), linear."""

@@ -302,7 +302,10 @@ FV_API int fv_sdpa_window_bf16(void* stream, const void* q, const void* k_cache,
  *   t_j < sink), t = index / block_tokens: block_tokens 1 is causal by token.  (The mask of fv_sdpa_dense_bf16 but that the
  *   sinks stay causal too: what a cache can hold.)  Rows that see no key give zeros.  Keys that no row of a tile of rows may see have
  *   no influence whatever their memory holds; a key that some row sees must be finite (a NaN in it may reach other
- *   rows of the call).  The workspace is scratch of this call alone (fv_paged_attn_workspace_bytes, may be 0; same arguments).
+ *   rows of the call).  f32 sums and statistics; probabilities are rounded to the products' type, bf16, over 4-bit pages f16
+ *   (where long chunks take q and the cached values through f16 too: beyond 65 504 they saturate, below 2^-14 they lose
+ *   relative precision).  Strides are positive.  FV_PAGED_KERNEL=rows or items (kept for A/B) fixes which of the two kernels runs.
+ *   The workspace is scratch of this call alone (fv_paged_attn_workspace_bytes, may be 0; same arguments).
  * Declines: empty batches, more than 2^31 - 1 blocks of work. */
 #define FV_PAGE_BF16 0
 #define FV_PAGE_Q4 1

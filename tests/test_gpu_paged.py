@@ -377,6 +377,54 @@ def test_streaming_run_equals_one_chunk(fvlib, kernel, fmt):
     check(got, want, room, fmt)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+def test_wan_layer_streams_over_pages(fvlib, fmt):
+    """WanSelfAttention.forward_paged block by block of frames, two rollouts of different lengths packed, under a window of
+    blocks with a sink block, against norm, rotation and attention in 64 bits on what the cache was given."""
+    from fastvideo_rs_b200 import paged, sdpa, wan
+    from fastvideo_rs_b200.sdpa import BlockCausal
+    heads, frame, frames = 3, 20, 7
+    mask = (frame, 3, 1)
+    g = torch.Generator().manual_seed(12)
+    w = [1 + 0.1 * torch.randn(heads * D, generator=g) for _ in range(2)]
+    layer = wan.WanSelfAttention((frames, 4, 5), heads, w[0].cuda(), w[1].cuda(), causal=BlockCausal(*mask))
+    cos, sin = layer.cos.cpu().double(), layer.sin.cpu().double()
+    qkv = torch.randn(2, frames * frame, 3 * heads * D, generator=g).to(torch.bfloat16)
+    kv = paged.PagedKv.empty(24, 16, heads, fmt)
+    table = torch.randperm(24, generator=g).to(torch.int32)[:18].view(2, 9).contiguous()
+    have, seen = [0, 0], [[], []]
+    for step in range(frames):
+        new = [frame, frame if step % 2 == 0 else 0]  # the second rollout advances every other step
+        rows = [qkv[s, have[s]:have[s] + new[s]] for s in range(2)]
+        have = [a + b for a, b in zip(have, new)]
+        cu = torch.tensor([0, new[0], new[0] + new[1]], dtype=torch.int32)
+        batch = paged.PagedBatch(table.cuda(), torch.tensor(have, dtype=torch.int32).cuda(), cu.cuda(), max_q=frame, max_kv=max(have))
+        out = layer.forward_paged(torch.cat(rows)[None].cuda(), kv, batch)
+        assert out.shape == (sum(new), heads, D)
+        kr, vr = (t.double().cpu() for t in paged.read(kv, batch, rows=sum(new)))
+        for s in range(2):
+            if not new[s]:
+                continue
+            part = slice(int(cu[s]), int(cu[s + 1]))
+            x = rows[s].double().view(new[s], 3, heads * D)
+            norm = [(y / torch.sqrt(y.pow(2).mean(-1, keepdim=True) + 1e-6) * w[i].double()).view(-1, heads, D) for i, y in ((0, x[:, 0]), (1, x[:, 1]))]
+            at = slice(have[s] - new[s], have[s])
+            c, sn = cos[at][:, None], sin[at][:, None]
+            q64, k64 = (rotate64(y, c, sn, "interleaved") for y in norm)
+            if fmt == "bf16":  # two roundings to bf16, of values no larger than sqrt(2) of a pair's larger one
+                assert float((kr[part] - k64).abs().max()) <= 2.0 * math.sqrt(2.0) * BF16_HALF * float(norm[1].abs().max())
+                assert torch.equal(vr[part], x[:, 2].view(-1, heads, D))
+            seen[s].append((kr[part], vr[part]))
+            ks, vs = (torch.cat([t[i] for t in seen[s]]) for i in range(2))
+            want, mag = attend64(q64, ks, vs, mask)
+            # q is off by two roundings as well: each score by at most 2 sqrt(2) 2^-8 |q| |k| / sqrt(128), P by as much relatively;
+            # 4 bits: read() rounds K and V to bf16 once more, and P's products' zeros come on top (|zero| <= 1.5)
+            off = 2.0 * math.sqrt(2.0) * BF16_HALF * float(q64.norm(dim=-1).max() * ks.norm(dim=-1).max()) / math.sqrt(D)
+            off = off * (1.0 if fmt == "bf16" else 2.0)
+            check(out[part], want, BF16_HALF * want.abs() + (2 * BF16_HALF + off) * (mag + (1.5 if fmt == "q4" else 0.0)), f"{fmt} step {step} rollout {s}")
+    assert sdpa.device_status() == 0
+
+
 def test_rows_past_four_gigabytes(fvlib, kernel):
     """Pages whose byte offsets pass 32 bits."""
     from fastvideo_rs_b200 import paged, sdpa
@@ -446,8 +494,12 @@ def test_refusals(fvlib):
         paged.attend(kv, batch, q, scale=-1.0)
     with pytest.raises(FvError, match="block_tokens"):
         paged.attend(kv, batch, q, BlockCausal(0, 1, 1))
-    with pytest.raises(FvError, match="block_tokens"):
+    with pytest.raises(ValueError, match="range"):
         paged.attend(kv, batch, q, BlockCausal(1, -1, 1))
+    with pytest.raises(ValueError, match="range"):
+        paged.attend(kv, batch, q, BlockCausal(1, 1 << 31, 1))
+    with pytest.raises(FvError, match="positive"):
+        paged.attend(kv, batch, q[:1].expand(4, 4, D))
     with pytest.raises(FvError, match="aligned|multiples"):
         paged.attend(kv, batch, torch.zeros(4 * 4 * 132 + 4, dtype=torch.bfloat16, device="cuda")[4:].view(4, 4, 132)[..., :128])
     with pytest.raises(ValueError, match="out must be"):

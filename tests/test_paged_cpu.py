@@ -31,6 +31,14 @@ def test_handles_refuse_what_is_not_a_cache(fvlib):
         paged.PagedBatch(torch.zeros(4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), max_q=1, max_kv=1)
 
 
+def test_batch_bounds(fvlib):
+    from fastvideo_rs_b200 import paged
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    for kw in (dict(max_q=-1, max_kv=1), dict(max_q=1, max_kv=1 << 30), dict(max_q=1 << 32, max_kv=1)):
+        with pytest.raises(ValueError, match="2\\^30|int32"):
+            paged.PagedBatch(z(1, 4), z(1), z(2), **kw)
+
+
 def _c(**kw):
     from fastvideo_rs_b200 import paged
     kv = dict(k=16, v=16, k_scale=None, v_scale=None, format=0, pages=4, page_rows=16, kv_heads=2)
