@@ -1021,41 +1021,42 @@ static int launch_chunk(cudaStream_t st, const fv_paged_kv* kv, const AttnArgs& 
     return FV_RAN;
 }
 
-static int check_mask(int mask_mode, int block_tokens, int window, int sink, Mask* m) {
-    if (mask_mode == FV_MASK_NONE) {
+static int check_mask(const fv_paged_query& x, Mask* m) {
+    if (x.mask_mode == FV_MASK_NONE) {
         *m = Mask{0, 0, 0};
         return FV_RAN;
     }
-    if (mask_mode != FV_MASK_BLOCK_CAUSAL) return fvrt::fail(FV_ERR_INVALID, "paged attention: unknown mask mode %d", mask_mode);
-    if (block_tokens < 1 || window < 0 || sink < 0)
+    if (x.mask_mode != FV_MASK_BLOCK_CAUSAL) return fvrt::fail(FV_ERR_INVALID, "paged attention: unknown mask mode %d", x.mask_mode);
+    if (x.block_tokens < 1 || x.window < 0 || x.sink < 0)
         return fvrt::fail(FV_ERR_INVALID, "paged attention: block-causal needs block_tokens >= 1, window, sink >= 0");
-    *m = Mask{block_tokens, window, sink};
+    *m = Mask{x.block_tokens, x.window, x.sink};
     return FV_RAN;
 }
 
 }  // namespace fvpg
 
-extern "C" size_t fv_paged_attn_workspace_bytes(const fv_paged_kv* kv, const fv_paged_batch* b, int tokens, int heads, int mask_mode,
-                                                int block_tokens, int window, int sink) {
+extern "C" size_t fv_paged_attn_workspace_bytes(const fv_paged_kv* kv, const fv_paged_batch* b, const fv_paged_query* x) {
     using namespace fvpg;
     fvrt::clear_error();
     Mask m;
     int dev, sms;
-    if (!kv || !b || kv->kv_heads < 1 || heads < 1 || heads % kv->kv_heads || b->seqs < 1 || tokens < 1 || b->max_q < 1 ||
-        check_mask(mask_mode, block_tokens, window, sink, &m) != FV_RAN || fvrt::require_sm100(&dev) != FV_RAN ||
+    if (!kv || !b || !x || kv->kv_heads < 1 || x->heads < 1 || x->heads % kv->kv_heads || b->seqs < 1 || x->tokens < 1 || b->max_q < 1 ||
+        check_mask(*x, &m) != FV_RAN || fvrt::require_sm100(&dev) != FV_RAN ||
         fvrt::sm_count(dev, &sms) != FV_RAN)
         return 0;
-    const Shape s = shape_of(kv, b, heads, m, sms);
-    return workspace_of(s, (size_t)tokens * heads);
+    return workspace_of(shape_of(kv, b, x->heads, m, sms), (size_t)x->tokens * x->heads);
 }
 
-extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* b, int tokens, const void* q, long long q_tok,
-                                  long long q_head, int heads, int mask_mode, int block_tokens, int window, int sink, float scale,
-                                  void* out, void* workspace, size_t workspace_bytes) {
+extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* b, const fv_paged_query* x) {
     using namespace fvpg;
     fvrt::clear_error();
+    if (!x) return fvrt::fail(FV_ERR_INVALID, "paged attention: null operand");
+    const int tokens = x->tokens, heads = x->heads;
+    const void* q = x->q;
+    void *out = x->out, *workspace = x->workspace;
+    const float scale = x->scale;
     AttnArgs a{};
-    int rc = check_mask(mask_mode, block_tokens, window, sink, &a.mask);
+    int rc = check_mask(*x, &a.mask);
     if (rc != FV_RAN) return rc;
     if (heads < 1 || (kv && kv->kv_heads > 0 && heads % kv->kv_heads))
         return fvrt::fail(FV_ERR_INVALID, "paged attention: %d heads over %d K/V heads", heads, kv ? kv->kv_heads : 0);
@@ -1067,8 +1068,7 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
     if (!q || !out) return fvrt::fail(FV_ERR_INVALID, "paged attention: null operand");
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15)
         return fvrt::fail(FV_ERR_INVALID, "paged attention: operands must be 16-byte aligned");
-    if (tokens == 1) q_tok = kD;  // (the stride of an extent of one means nothing)
-    if (heads == 1) q_head = kD;
+    const long long q_tok = tokens == 1 ? kD : x->q_tok, q_head = heads == 1 ? kD : x->q_head;  // (that of an extent of one means nothing)
     if (((q_tok | q_head) & 7) || q_tok <= 0 || q_head <= 0)
         return fvrt::fail(FV_ERR_INVALID, "paged attention: strides must be positive multiples of 8 values");
     rc = fvrt::sm_count(dev, &sms);
@@ -1076,8 +1076,8 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
     const Shape s = shape_of(kv, b, heads, a.mask, sms);
     const size_t rows = (size_t)tokens * heads;
     const size_t need = workspace_of(s, rows);
-    if (need > 0 && (!workspace || workspace_bytes < need))
-        return fvrt::fail(FV_ERR_INVALID, "paged attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (need > 0 && (!workspace || x->workspace_bytes < need))
+        return fvrt::fail(FV_ERR_INVALID, "paged attention: workspace of %zu bytes, %zu needed", x->workspace_bytes, need);
     a.q = (const uint16_t*)q;
     a.q_tok = q_tok;
     a.q_head = q_head;

@@ -431,12 +431,14 @@ static int parts_for(int tokens, int rows, int sms) {
 
 }  // namespace fvpg
 
-extern "C" int fv_paged_append_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* b, int tokens, const void* k, long long k_tok,
-                                    long long k_head, const void* v, long long v_tok, long long v_head, const void* q,
-                                    long long q_tok, long long q_head, int q_heads, void* q_out, const float* cosv,
-                                    const float* sinv, int table_rows, const int* positions, int pairing) {
+extern "C" int fv_paged_append_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* b, const fv_paged_rows* x) {
     using namespace fvpg;
     fvrt::clear_error();
+    if (!x) return fvrt::fail(FV_ERR_INVALID, "paged append: null operand");
+    const void *k = x->k, *v = x->v, *q = x->q;
+    void* q_out = x->q_out;
+    const float *cosv = x->cosv, *sinv = x->sinv;
+    const int tokens = x->tokens, q_heads = x->q_heads, table_rows = x->table_rows, pairing = x->pairing;
     AppendArgs a{};
     int dev;
     const int rc = check_paged("paged append", kv, b, tokens, &a.pool, &a.batch, &dev);
@@ -444,22 +446,22 @@ extern "C" int fv_paged_append_bf16(void* stream, const fv_paged_kv* kv, const f
     if (!k || !v) return fvrt::fail(FV_ERR_INVALID, "paged append: null operand");
     if ((q != nullptr) != (q_out != nullptr) || (q && q_heads < 1) || q_heads > 4096)
         return fvrt::fail(FV_ERR_INVALID, "paged append: q, q_out and q_heads go together");
-    if ((cosv != nullptr) != (sinv != nullptr) || (cosv && table_rows < 1) || (positions && !cosv))
+    if ((cosv != nullptr) != (sinv != nullptr) || (cosv && table_rows < 1) || (x->positions && !cosv))
         return fvrt::fail(FV_ERR_INVALID, "paged append: cos, sin, their rows and positions go together");
     if (pairing != FV_ROPE_INTERLEAVED && pairing != FV_ROPE_HALF)
         return fvrt::fail(FV_ERR_INVALID, "paged append: unknown pairing %d", pairing);
     if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)q_out | (uintptr_t)cosv | (uintptr_t)sinv) & 15)
         return fvrt::fail(FV_ERR_INVALID, "paged append: operands must be 16-byte aligned");
-    if ((k_tok | k_head | v_tok | v_head | (q ? q_tok | q_head : 0)) & 7)
+    if ((x->k_tok | x->k_head | x->v_tok | x->v_head | (q ? x->q_tok | x->q_head : 0)) & 7)
         return fvrt::fail(FV_ERR_INVALID, "paged append: strides must be multiples of 8 values");
     a.q = (const uint16_t*)q;
     a.k = (const uint16_t*)k;
     a.v = (const uint16_t*)v;
     a.q_out = (uint16_t*)q_out;
-    a.q_tok = q_tok; a.q_head = q_head; a.k_tok = k_tok; a.k_head = k_head; a.v_tok = v_tok; a.v_head = v_head;
+    a.q_tok = x->q_tok; a.q_head = x->q_head; a.k_tok = x->k_tok; a.k_head = x->k_head; a.v_tok = x->v_tok; a.v_head = x->v_head;
     a.cosv = cosv;
     a.sinv = sinv;
-    a.positions = positions;
+    a.positions = x->positions;
     a.table_rows = table_rows;
     a.q_heads = q ? q_heads : 0;
     int sms;

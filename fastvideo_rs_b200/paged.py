@@ -8,6 +8,7 @@ the sequences of a call lie in it and serves every layer that uses the same tabl
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -18,7 +19,10 @@ from .sdpa import BlockCausal
 FORMATS = ("bf16", "q4")
 PAIRINGS = {"interleaved": 0, "half": 1}
 D = 128
-_vp, _ll, _int = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
+_vp, _int = ctypes.c_void_p, ctypes.c_int
+# fv_paged_rows and fv_paged_query, packed: one bytes object is a fifth of what twenty ctypes arguments cost a call.
+_rows_struct = struct.Struct("@7P6q4i")
+_query_struct = struct.Struct("@3PN2q6if")
 
 
 class _KvC(ctypes.Structure):
@@ -42,13 +46,11 @@ def _entries():
     global _fns
     if _fns is None:
         L = _lib.lib()
-        L.fv_paged_append_bf16.argtypes = [_vp, _vp, _vp, _int, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _int, _vp, _vp, _vp,
-                                           _int, _vp, _int]
+        L.fv_paged_append_bf16.argtypes = [_vp, _vp, _vp, _vp]
         L.fv_paged_read_bf16.argtypes = [_vp, _vp, _vp, _vp, _vp, _int, _vp, _vp]
-        L.fv_paged_attn_workspace_bytes.argtypes = [_vp, _vp, _int, _int, _int, _int, _int, _int]
+        L.fv_paged_attn_workspace_bytes.argtypes = [_vp, _vp, _vp]
         L.fv_paged_attn_workspace_bytes.restype = ctypes.c_size_t
-        L.fv_paged_attn_bf16.argtypes = [_vp, _vp, _vp, _int, _vp, _ll, _ll, _int, _int, _int, _int, _int, ctypes.c_float, _vp, _vp,
-                                         ctypes.c_size_t]
+        L.fv_paged_attn_bf16.argtypes = [_vp, _vp, _vp, _vp]
         _fns = (L.fv_paged_append_bf16, L.fv_paged_read_bf16, L.fv_paged_attn_workspace_bytes, L.fv_paged_attn_bf16)
     return _fns
 
@@ -183,8 +185,7 @@ def append(kv: PagedKv, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, *, 
     _, _, vt, vh = _heads_in("append: v", v, index, tokens, kv.kv_heads)
     if pairing not in PAIRINGS:
         raise ValueError(f"append: unknown pairing {pairing!r} {tuple(PAIRINGS)}")
-    cp = sp = pp = None
-    rows = 0
+    cp = sp = pp = rows = 0
     if cos is not None and sin is not None:
         shape = cos.shape
         rows = shape[0] if len(shape) == 2 else 0
@@ -197,7 +198,7 @@ def append(kv: PagedKv, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, *, 
     elif cos is not None or sin is not None or positions is not None:
         raise ValueError("append: cos, sin and positions go together")
     heads = qt = qh = 0
-    qp = op = None
+    qp = op = 0
     if q is not None:
         _, heads, qt, qh = _heads_in("append: q", q, index, tokens)
         if q_out is None:
@@ -212,8 +213,8 @@ def append(kv: PagedKv, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, *, 
         raise ValueError("append: q_out without q")
     if tokens == 0 or batch.seqs == 0 or batch.max_q == 0:
         return q_out
-    _call(kv, batch, "paged append", (_fns or _entries())[0], tokens, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, qp, qt, qh, heads, op,
-          cp, sp, rows, pp, PAIRINGS[pairing])
+    _call(kv, batch, "paged append", (_fns or _entries())[0],
+          _rows_struct.pack(k.data_ptr(), v.data_ptr(), qp, op, cp, sp, pp, kt, kh, vt, vh, qt, qh, tokens, heads, rows, PAIRINGS[pairing]))
     return q_out
 
 
@@ -270,9 +271,10 @@ def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[Block
         need = 0
         if kv.index >= 0:
             with torch.cuda.device(kv.index):
-                need = batch._need[key] = fns[2](kv._ref, batch._ref, tokens, heads, *how)
+                need = batch._need[key] = fns[2](kv._ref, batch._ref, _query_struct.pack(0, 0, 0, 0, 0, 0, tokens, heads, *how, 0.0))
     # (scratch of this call alone, from the stream's own pool: calls on other streams and captured graphs share nothing)
     ws = q.new_empty((need // 2,)) if need else None
-    _call(kv, batch, "paged attention", fns[3], tokens, q.data_ptr(), qt, qh, heads, *how, _SCALE if scale is None else float(scale),
-          out.data_ptr(), ws.data_ptr() if need else None, need)
+    _call(kv, batch, "paged attention", fns[3],
+          _query_struct.pack(q.data_ptr(), out.data_ptr(), ws.data_ptr() if need else 0, need, qt, qh, tokens, heads, *how,
+                             _SCALE if scale is None else float(scale)))
     return out

@@ -284,7 +284,7 @@ FV_API int fv_sdpa_window_bf16(void* stream, const void* q, const void* k_cache,
  *   with broken numbers counts as empty) and fv_device_status answers FV_ERR_DEVICE_STATUS with code 200 (page), 201 (batch)
  *   or 202 (position).
  *
- * fv_paged_append_bf16: k, v [tokens, kv_heads, 128] bf16 and, unless null, q [tokens, q_heads, 128]; *_tok and *_head are
+ * fv_paged_append_bf16: k, v [tokens, kv_heads, 128] bf16 and, unless null, q [tokens, q_heads, 128] (null: q_heads 0); *_tok and *_head are
  *   strides in values (multiples of 8), so slices of a fused projection are read in place.  cosv, sinv (both or neither)
  *   f32 [table_rows, 128]: token t is rotated with row positions[t] (i32; null: its position in the sequence), pairing
  *   FV_ROPE_INTERLEAVED (values 2 i, 2 i + 1; each factor stored twice, as fv_wan_rope_tables writes them) or FV_ROPE_HALF
@@ -305,7 +305,8 @@ FV_API int fv_sdpa_window_bf16(void* stream, const void* q, const void* k_cache,
  *   rows of the call).  f32 sums and statistics; probabilities are rounded to the products' type, bf16, over 4-bit pages f16
  *   (where long chunks take q and the cached values through f16 too: beyond 65 504 they saturate, below 2^-14 they lose
  *   relative precision).  Strides are positive.  FV_PAGED_KERNEL=rows or items (kept for A/B) fixes which of the two kernels runs.
- *   The workspace is scratch of this call alone (fv_paged_attn_workspace_bytes, may be 0; same arguments).
+ *   The workspace is scratch of this call alone (fv_paged_attn_workspace_bytes of the same query, may be 0; it reads
+ *   neither pointers nor strides nor scale).
  * Declines: empty batches, more than 2^31 - 1 blocks of work. */
 #define FV_PAGE_BF16 0
 #define FV_PAGE_Q4 1
@@ -320,17 +321,27 @@ typedef struct fv_paged_batch {
     const int *page_table, *kv_len, *cu_q;
     int seqs, table_width, max_q, max_kv;
 } fv_paged_batch;
-FV_API int fv_paged_append_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* batch, int tokens, const void* k, long long k_tok,
-                                long long k_head, const void* v, long long v_tok, long long v_head, const void* q,
-                                long long q_tok, long long q_head, int q_heads, void* q_out, const float* cosv,
-                                const float* sinv, int table_rows, const int* positions, int pairing);
+typedef struct fv_paged_rows {
+    const void *k, *v, *q;
+    void* q_out;
+    const float *cosv, *sinv;
+    const int* positions;
+    long long k_tok, k_head, v_tok, v_head, q_tok, q_head;
+    int tokens, q_heads, table_rows, pairing;
+} fv_paged_rows;
+typedef struct fv_paged_query {
+    const void* q;
+    void *out, *workspace;
+    size_t workspace_bytes;
+    long long q_tok, q_head;
+    int tokens, heads, mask_mode, block_tokens, window, sink;
+    float scale;
+} fv_paged_query;
+FV_API int fv_paged_append_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* batch, const fv_paged_rows* rows);
 FV_API int fv_paged_read_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* batch, const int* cu_rows,
                               const int* first, int rows, void* k_out, void* v_out);
-FV_API size_t fv_paged_attn_workspace_bytes(const fv_paged_kv* kv, const fv_paged_batch* batch, int tokens, int heads, int mask_mode,
-                                            int block_tokens, int window, int sink);
-FV_API int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* batch, int tokens, const void* q, long long q_tok,
-                              long long q_head, int heads, int mask_mode, int block_tokens, int window, int sink,
-                              float scale, void* out, void* workspace, size_t workspace_bytes);
+FV_API size_t fv_paged_attn_workspace_bytes(const fv_paged_kv* kv, const fv_paged_batch* batch, const fv_paged_query* query);
+FV_API int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* batch, const fv_paged_query* query);
 
 /* ---- operand rounding for f32-stored activations ------------------------------------------------
  * The reference rounds q, k, v to bf16 before its attention kernels under bf16 activations and rounds the

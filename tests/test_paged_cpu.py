@@ -48,6 +48,21 @@ def _c(**kw):
     return paged._KvC(*kv.values()), paged._BatchC(*b.values())
 
 
+def _rows(**kw):
+    from fastvideo_rs_b200 import paged
+    x = dict(k=16, v=16, q=0, q_out=0, cos=0, sin=0, positions=0, k_tok=256, k_head=128, v_tok=256, v_head=128, q_tok=0, q_head=0,
+             tokens=1, q_heads=0, table_rows=0, pairing=0)
+    x.update(kw)
+    return paged._rows_struct.pack(*x.values())
+
+
+def _query(**kw):
+    from fastvideo_rs_b200 import paged
+    x = dict(q=16, out=16, workspace=0, workspace_bytes=0, q_tok=512, q_head=128, tokens=1, heads=4, mode=1, block=1, window=0, sink=0, scale=0.1)
+    x.update(kw)
+    return paged._query_struct.pack(*x.values())
+
+
 @pytest.mark.parametrize("kw,text", [(dict(format=2), b"format"), (dict(pages=0), b"pool"), (dict(kv_heads=0), b"pool"),
                                      (dict(page_rows=8), b"rows"), (dict(page_rows=48), b"rows"), (dict(page_rows=512), b"rows"),
                                      (dict(max_kv=65), b"does not hold"), (dict(seqs=-1), b"negative"), (dict(max_q=-1), b"negative")])
@@ -56,11 +71,10 @@ def test_c_entries_refuse_bad_sizes_before_any_device(fvlib, kw, text):
     append, read, need, attn = paged._entries()
     kv, b = _c(**kw)
     kr, br = ctypes.addressof(kv), ctypes.addressof(b)
-    assert append(None, kr, br, 1, 16, 256, 128, 16, 256, 128, None, 0, 0, 0, None, None, None, 0, None, 0) == -1
+    assert append(None, kr, br, _rows()) == -1
     assert text in fvlib.fv_last_error()
     assert read(None, kr, br, 16, None, 1, 16, 16) == -1 and text in fvlib.fv_last_error()
-    rc = attn(None, kr, br, 1, 16, 512, 128, 4, 1, 1, 0, 0, 0.1, 16, None, 0)
-    assert rc == -1
+    assert attn(None, kr, br, _query()) == -1
 
 
 def test_c_entries_refuse_and_decline(fvlib):
@@ -68,19 +82,16 @@ def test_c_entries_refuse_and_decline(fvlib):
     append, read, need, attn = paged._entries()
     kv, b = _c()
     kr, br = ctypes.addressof(kv), ctypes.addressof(b)
-    assert append(None, None, br, 1, 16, 256, 128, 16, 256, 128, None, 0, 0, 0, None, None, None, 0, None, 0) == -1
+    assert append(None, None, br, _rows()) == -1 and append(None, kr, br, None) == -1 and attn(None, kr, br, None) == -1
     for bad in (dict(heads=3), dict(scale=0.0), dict(scale=math.inf), dict(mode=7), dict(block=0), dict(window=-1), dict(sink=-1)):
-        a = dict(heads=4, mode=1, block=1, window=0, sink=0, scale=0.1)
-        a.update(bad)
-        rc = attn(None, kr, br, 1, 16, 512, 128, a["heads"], a["mode"], a["block"], a["window"], a["sink"], a["scale"], 16, None, 0)
-        assert rc == -1, bad
+        assert attn(None, kr, br, _query(**bad)) == -1, bad
     # empty calls are declined before a device is asked for
-    assert attn(None, kr, br, 0, 16, 512, 128, 4, 1, 1, 0, 0, 0.1, 16, None, 0) == 1
-    assert append(None, kr, br, 0, 16, 256, 128, 16, 256, 128, None, 0, 0, 0, None, None, None, 0, None, 0) == 1
+    assert attn(None, kr, br, _query(tokens=0)) == 1
+    assert append(None, kr, br, _rows(tokens=0)) == 1
     assert read(None, kr, br, 16, None, 0, 16, 16) == 1
     if not torch.cuda.is_available():  # no CPU path
-        assert attn(None, kr, br, 1, 16, 512, 128, 4, 1, 1, 0, 0, 0.1, 16, None, 0) == -3
-        assert need(kr, br, 1, 4, 1, 1, 0, 0) == 0
+        assert attn(None, kr, br, _query()) == -3 and append(None, kr, br, _rows()) == -3
+        assert need(kr, br, _query()) == 0
 
 
 @pytest.mark.parametrize("mask", [(1, 0, 0), (1, 5, 0), (1, 5, 3), (4, 2, 1), (7, 0, 0), (3, 1, 2)])
