@@ -1,6 +1,7 @@
 // Attention of a ragged batch's queries over a paged K/V cache: block-causal with a sliding window and sinks, shared
 // K/V heads, pages of bf16 or of 4 bits.  This file: the kernel for few query rows per K/V head (decode steps, short
-// chunks), the merge of key ranges, and the C entry.
+// chunks), the kernels that join parts, the choice between this kernel and the one for long chunks (paged_fwd.cuh), and the C
+// entries.
 //
 // Row r of a (sequence, kv head) is token r / g, head r % g of the heads that share that K/V head (g = heads /
 // kv_heads): one pass over the keys serves all of them.
@@ -39,7 +40,6 @@ struct AttnArgs {
     float sl2;
     long long wait_cycles;
 };
-
 
 using fvattn::neg_inf;
 
@@ -93,8 +93,8 @@ FV_DEV uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(
 // The eight codes of a word as four f16 pairs, pair i from nibbles i and i + 4: a nibble n at bits 0-3 of a half word is the
 // f16 number n 2^-24 as it stands (below f16's normal numbers, which the matrix unit multiplies exactly), at bits 4-7
 // 16 n 2^-24.  One shift and four masks a word and nothing else: expanding the codes is what bounds this kernel (with the
-// codes or-ed into 1024's mantissa and the 1024 taken off again by an addition it took 160 instead of 112 us for 32 sequences of
-// 20 011 keys).  The factors, and the 8 between n and the code, are taken out of the products' results.
+// codes or-ed into 1024's mantissa and the 1024 taken off again by an addition it took 160 instead of 129 us for 32 sequences of
+// 20 011 keys; as bytes for the 8-bit matrix instruction, q in two parts, 137).  The factors, and the 8 between n and the code, are taken out of the products' results.
 FV_DEV void codes_f16(uint32_t w, uint32_t (&h)[4]) {
     const uint32_t v = w >> 8;
     h[0] = w & 0x000f000fu;
@@ -224,15 +224,17 @@ FV_DEV uint32_t lds32(uint32_t a) {
     return r;
 }
 
-// Up to ROWS query rows (4 bits: 4, 8 or 16, bf16: 8 or 16).  The transposed products S^T = K . Q^T and O^T = V^T . P^T keep keys and head dim on the
-// 16-wide side of the matrix instruction and the (few) query rows on the 8-wide one; the sums of either product may run
-// in any order of d or key, so every lane's operands are whole 16-byte pieces as they lie in memory and no shared
-// memory is needed on the way.
+// Up to ROWS query rows (4 bits: 4, 8 or 16, bf16: 8 or 16).  The transposed products S^T = K . Q^T and O^T = V^T . P^T keep
+// keys and head dim on the 16-wide side of the matrix instruction and the (few) query rows on the 8-wide one; the sums of
+// either product may run in any order of d or key, so every lane's operands are whole 16-byte pieces as they lie in memory.
 //
 // A warp takes a run of tiles of its own.  Their pool rows are looked up 32 at a time, one tile a lane, a batch ahead.
-// bf16: a tile's K registers are loaded anew as soon as its scores are done and V's as soon as its product is, so that
-// memory is always being read while the warp computes.  4 bits: 16 keys are too few bytes for that (and the registers are
-// needed for more warps: expanding the codes is what bounds this form), so a ring in shared memory runs three stages ahead.
+// bf16, bound by HBM: a tile's K registers are loaded anew as soon as its scores are done and V's as soon as its product is, so
+// that memory is always being read while the warp computes, straight into registers: 32 ragged sequences of up to 9 001 keys, 32
+// heads on 8, 140 us = 5.97 TB/s, 0.91 of the measured copy bandwidth; 6 windows of 8 190 keys, 40 heads on 8, 36 us = 5.6 TB/s.
+// 4 bits, bound by the logic pipe: 32 keys are 4.3 KB, so a ring in shared memory runs three stages ahead: 32 sequences of up to
+// 20 011 keys 116 us = 4.3 TB/s (loads into registers: 173).  Three CTAs an SM: with a fourth the registers no longer suffice,
+// 128 against 123 us.  At most four rows stand on every other column of the products, which leaves half of the softmax: 123 -> 116 us.
 template <bool Q4, int ROWS>
 __global__ void __launch_bounds__(kAttnThreads, ROWS <= 8 ? 3 : 2) fv_paged_decode_kernel(const AttnArgs a) {
     constexpr int kRows = ROWS, NT = (ROWS + 7) / 8;  // groups of 8 rows, the columns of a product

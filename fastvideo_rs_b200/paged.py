@@ -229,7 +229,7 @@ def read(kv: PagedKv, batch: PagedBatch, *, rows: int, cu_rows: Optional[torch.T
     cu = batch.cu_q if cu_rows is None else _index("read: cu_rows", cu_rows, (batch.seqs + 1,), kv.device)
     if first is not None:
         _index("read: first", first, (batch.seqs,), kv.device)
-    k, v = torch.empty((2, rows, kv.kv_heads, D), dtype=_bf16, device=kv.device).unbind(0)
+    k, v = (kv.k if kv.k_scale is None else kv.k_scale).new_empty((2, rows, kv.kv_heads, D)).unbind(0)  # (either is bf16)
     if rows == 0:
         return k, v
     if batch.seqs == 0:
