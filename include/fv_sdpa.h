@@ -307,6 +307,7 @@ FV_API int fv_sdpa_window_bf16(void* stream, const void* q, const void* k_cache,
  *   relative precision).  Strides are positive.  FV_PAGED_KERNEL=rows or items (kept for A/B) fixes which of the two kernels runs.
  *   The workspace is scratch of this call alone (fv_paged_attn_workspace_bytes of the same query, may be 0; it reads
  *   neither pointers nor strides nor scale).
+ * Each call may be captured in a graph; make the first call of its kind in a process before that, so that its kernel is loaded.
  * Declines: empty batches, more than 2^31 - 1 blocks of work. */
 #define FV_PAGE_BF16 0
 #define FV_PAGE_Q4 1
