@@ -680,6 +680,7 @@ __global__ void __launch_bounds__(kAttnThreads, ROWS <= 8 ? 3 : 2) fv_paged_deco
                 l[n][e] += __shfl_xor_sync(kFullWarp, l[n][e], d);
                 z[n][e] += __shfl_xor_sync(kFullWarp, z[n][e], d);
             }
+            if (!(l[n][e] >= 0.f)) m[n][e] = -neg_inf();  // a score that is not a number: the row comes out as one that is not
             const int r = row_of(n, e);
             if (g == 0) {
                 sh_m[warp][r] = m[n][e];
@@ -770,7 +771,7 @@ __global__ void __launch_bounds__(kAttnThreads, ROWS <= 8 ? 3 : 2) fv_paged_deco
         } else {
             const size_t pi = (size_t)split * a.batch.tokens * a.heads + oi;
             a.part_o[pi * kD + d] = acc;
-            if (d == 0) a.part_lse[pi] = top == neg_inf() ? neg_inf() : top + log2f(sum);
+            if (d == 0) a.part_lse[pi] = sum > 0.f ? top + log2f(sum) : top;  // (no key: -inf; not a number: +inf)
         }
     }
 }
@@ -908,13 +909,13 @@ static bool take_items(long long planes, long long rows, long long keys, bool q4
     const double in_items = 35.0 + items * (work / kChunkTile + planes * kItemCost) * 0.0142;
     return in_items < in_rows;
 }
-static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads, const Mask& m, int sms) {
+static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int tokens, int heads, const Mask& m, int sms) {
     Shape s;
-    const int group = heads / kv->kv_heads;
-    const long long rows = (long long)b->max_q * group;
+    const int group = heads / kv->kv_heads, max_q = b->max_q < tokens ? b->max_q : tokens;
+    const long long rows = (long long)max_q * group;
     long long keys = b->max_kv;
     if (m.block > 0 && m.window > 0) {  // rows of one block see window blocks and the sinks, max_q rows a little more
-        const long long most = ((long long)m.window + m.sink + 1) * m.block + b->max_q;
+        const long long most = ((long long)m.window + m.sink + 1) * m.block + max_q;
         keys = most < keys ? most : keys;
     }
     const bool q4 = kv->format == FV_PAGE_Q4;
@@ -924,7 +925,7 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int heads,
     if (s.chunk) {
         s.block_rows = 0;
         s.splits = 1;
-        s.row_blocks = (b->max_q + 2 * s.tile_tokens - 1) / (2 * s.tile_tokens);
+        s.row_blocks = (max_q + 2 * s.tile_tokens - 1) / (2 * s.tile_tokens);
         // (an upper bound of the line's length: with little work no more CTAs are launched than may find a run)
         const long long longest = (long long)b->seqs * kv->kv_heads * s.row_blocks * ((b->max_kv + kChunkTile - 1) / kChunkTile + kItemCost);
         const long long most = longest / kLeastRun;
@@ -1046,7 +1047,7 @@ extern "C" size_t fv_paged_attn_workspace_bytes(const fv_paged_kv* kv, const fv_
         check_mask(*x, &m) != FV_RAN || fvrt::require_sm100(&dev) != FV_RAN ||
         fvrt::sm_count(dev, &sms) != FV_RAN)
         return 0;
-    return workspace_of(shape_of(kv, b, x->heads, m, sms), (size_t)x->tokens * x->heads);
+    return workspace_of(shape_of(kv, b, x->tokens, x->heads, m, sms), (size_t)x->tokens * x->heads);
 }
 
 extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_paged_batch* b, const fv_paged_query* x) {
@@ -1075,8 +1076,9 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
         return fvrt::fail(FV_ERR_INVALID, "paged attention: strides must be positive multiples of 8 values");
     rc = fvrt::sm_count(dev, &sms);
     if (rc != FV_RAN) return rc;
-    const Shape s = shape_of(kv, b, heads, a.mask, sms);
     const size_t rows = (size_t)tokens * heads;
+    if (rows > 0x7fffffffull) return FV_DECLINED;
+    const Shape s = shape_of(kv, b, tokens, heads, a.mask, sms);
     const size_t need = workspace_of(s, rows);
     if (need > 0 && (!workspace || x->workspace_bytes < need))
         return fvrt::fail(FV_ERR_INVALID, "paged attention: workspace of %zu bytes, %zu needed", x->workspace_bytes, need);
@@ -1094,7 +1096,7 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
     a.sl2 = scale * 1.4426950408889634f;
     a.wait_cycles = FV_WAIT_CYCLES;
     const long long grid = (long long)b->seqs * kv->kv_heads * s.row_blocks * s.splits;
-    if (grid > 0x7fffffffll || (long long)rows > 0x7fffffffll) return FV_DECLINED;
+    if (grid > 0x7fffffffll) return FV_DECLINED;
     cudaStream_t st = (cudaStream_t)stream;
     if (s.chunk) {
         return launch_chunk(st, kv, a, s, dev);

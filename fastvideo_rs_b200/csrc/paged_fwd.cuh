@@ -515,7 +515,8 @@ FV_DEV void chunk_softmax(const ChunkJob& jb, const Run& run, uint32_t sbase, ui
         } else {
             const size_t slot = 2 * (size_t)number + (begins ? 1 : 0);
             chunk_write<Q4, true>(jb.part_o + slot * 2 * kChunkRows * kD, tO, inv, out_row, have_o, lane);
-            if (out_row >= 0) jb.part_lse[slot * 2 * kChunkRows + out_row] = rs.l > 0.f ? rs.m + log2f(rs.l) : neg_inf();
+            if (out_row >= 0)
+                jb.part_lse[slot * 2 * kChunkRows + out_row] = rs.l > 0.f ? rs.m + log2f(rs.l) : rs.l == 0.f ? neg_inf() : -neg_inf();  // (+inf: not a number)
         }
     }
 }

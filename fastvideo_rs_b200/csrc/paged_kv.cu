@@ -396,8 +396,8 @@ int check_paged(const char* what, const fv_paged_kv* kv, const fv_paged_batch* b
         return fvrt::fail(FV_ERR_INVALID, "%s: negative size in the batch", what);
     if ((long long)b->table_width * kv->page_rows < b->max_kv)
         return fvrt::fail(FV_ERR_INVALID, "%s: a table of %d pages of %d rows does not hold %d keys", what, b->table_width, kv->page_rows, b->max_kv);
-    if (b->max_kv > 0x3fffffff || b->max_q > 0x3fffffff)
-        return fvrt::fail(FV_ERR_INVALID, "%s: sequences of %d keys, %d of them new", what, b->max_kv, b->max_q);
+    if (b->max_kv > 0x3fffffff || b->max_q > 0x3fffffff || rows > 0x3fffffff)
+        return fvrt::fail(FV_ERR_INVALID, "%s: sequences of %d keys, %d of them new, %d rows", what, b->max_kv, b->max_q, rows);
     if ((long long)kv->pages * kv->kv_heads * kv->page_rows > 0xfffffff0ll)  // (the kernels number the pool's rows in 32 bits)
         return fvrt::fail(FV_ERR_INVALID, "%s: a pool of %d pages x %d heads x %d rows", what, kv->pages, kv->kv_heads, kv->page_rows);
     if (b->seqs == 0 || rows == 0) return FV_DECLINED;

@@ -179,7 +179,7 @@ def append(kv: PagedKv, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, *, 
     multiples of 8: slices of a fused projection are read in place), K rotated on the way when cos / sin f32 [rows, 128] are
     given: token t with row positions[t] (int32), by default its position in its sequence.  pairing "interleaved": values
     2 i and 2 i + 1 (the tables of wan.wan_rope_tables), "half": values i and i + 64.  q [tokens, heads, 128], if given, is
-    rotated too and returned as [tokens, heads, 128].  Two tokens of a call must not fall on the same cache row."""
+    rotated too and returned as [tokens, heads, 128] (in q_out, which may be q itself).  Two tokens of a call must not fall on the same cache row."""
     index = kv.index
     tokens, _, kt, kh = _heads_in("append: k", k, index, -1, kv.kv_heads)
     _, _, vt, vh = _heads_in("append: v", v, index, tokens, kv.kv_heads)
@@ -241,15 +241,16 @@ def read(kv: PagedKv, batch: PagedBatch, *, rows: int, cu_rows: Optional[torch.T
 
 def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[BlockCausal] = None, *,
            scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Attention of q [tokens, heads, 128] bf16 (the batch's tokens, rotated; strides as in append) over the cache, in place:
+    """Attention of q [tokens, heads, 128] bf16 (the batch's tokens, rotated; strides as in append, but none 0) over the cache, in place:
     returns [tokens, heads, 128] bf16.  heads is a multiple of kv_heads; head h reads K/V head h // (heads // kv_heads).
     mask None: every key of the sequence.  BlockCausal(block_tokens, window, sink): key j is visible to position p iff
     t_j <= t_p and (window == 0 or t_p - t_j < window or t_j < sink), t = index // block_tokens -- block_tokens 1: causal
     by token, a window of `window` tokens, the first `sink` tokens always visible; block_tokens of a frame: the streaming
-    form of the block-causal mask.  A row that sees no key is zero.  Pages of which no row sees a key need not exist.  Sums and softmax statistics are f32,
-    probabilities are rounded to the type of the products: bf16, over 4-bit pages f16 (there long chunks also take q and the
+    form of the block-causal mask.  A row that sees no key is zero.  Pages of which no row sees a key need not exist; what
+    memory holds where no row of the call sees it has no influence, but a key that some row sees must be finite (a NaN may reach
+    other rows of the call; one in q reaches only its own row).  Sums and softmax statistics are f32, probabilities are rounded to the type of the products: bf16, over 4-bit pages f16 (there long chunks also take q and the
     cached values through f16: what is beyond 65 504 saturates, what is below 2^-14 loses relative precision).
-    With `out`, rows that belong to no sequence keep what they hold."""
+    With `out` (which may be q itself), rows that belong to no sequence keep what they hold."""
     tokens, heads, qt, qh = _heads_in("attend: q", q, kv.index)
     if heads < 1 or heads % kv.kv_heads:
         raise ValueError(f"attend: {heads} heads over {kv.kv_heads} K/V heads")
@@ -263,7 +264,7 @@ def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[Block
         return out
     how = (1, mask.block_tokens, mask.window, mask.sink) if mask is not None else (0, 0, 0, 0)
     fns = _fns or _entries()
-    key = (how, heads, kv.kv_heads, tokens)
+    key = (how, heads, kv.kv_heads, tokens, kv.format)
     need = batch._need.get(key)
     if need is None:
         if max(how) > 0x7fffffff or min(how) < 0:

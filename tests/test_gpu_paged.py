@@ -477,6 +477,124 @@ def test_broken_tables_are_reported_and_not_followed(fvlib, kernel, nq):
     assert torch.equal(paged.attend(kv, batch, q, mask)[nq], good[nq])
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("nq", [1, 150])
+@pytest.mark.parametrize("kv_len", [400, 9000])
+def test_a_query_that_is_not_a_number_stays_one(fvlib, kernel, fmt, nq, kv_len):
+    """A NaN in q reaches its own row and no other, however many parts the row's keys are cut into."""
+    from fastvideo_rs_b200 import paged
+    case = Case(fmt, [kv_len], [nq], 4, 2, 64, seed=12)
+    kv, batch, q = case.device()
+    want, bound = case.expect((1, 0, 0))
+    q[nq // 2, 1] = math.nan
+    q[nq - 1, 2, 5] = math.nan
+    out = paged.attend(kv, batch, q, mask_of((1, 0, 0)))
+    bad = torch.zeros(nq, 4, dtype=torch.bool, device="cuda")
+    bad[nq // 2, 1] = bad[nq - 1, 2] = True
+    assert bool(out[bad].isnan().all())
+    good = ~bad.cpu()
+    check(out[~bad], want[good], bound[good], fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("nq", [1, 150])
+@pytest.mark.parametrize("kv_len", [700, 9000])
+def test_out_may_be_q(fvlib, kernel, fmt, nq, kv_len):
+    from fastvideo_rs_b200 import paged
+    case = Case(fmt, [kv_len, 300], [nq, 3], 8, 2, 32, seed=13)
+    kv, batch, q = case.device()
+    cos, sin = (t.cuda() for t in tables(kv_len, "half"))
+    k = torch.randn(case.tokens, 2, D, device="cuda").to(torch.bfloat16)
+    want_q = paged.append(kv, batch, k, k, q=q, cos=cos, sin=sin, pairing="half")
+    want = paged.attend(kv, batch, want_q, mask_of((1, 0, 0)))
+    assert paged.append(kv, batch, k, k, q=q, cos=cos, sin=sin, pairing="half", q_out=q) is q
+    assert torch.equal(q, want_q)
+    assert paged.attend(kv, batch, q, mask_of((1, 0, 0)), out=q) is q
+    assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("nq", [1, 150])
+def test_one_batch_serves_pools_of_both_formats(fvlib, kernel, nq):
+    """Layers of both formats in turn, whose calls need scratch of different sizes, and bounds far above what the call holds."""
+    from fastvideo_rs_b200 import paged
+    b, c = (Case(fmt, [20011], [nq], 4, 1, 64, seed=14) for fmt in FMTS)
+    kv, batch, q = b.device()
+    kv4, batch4, q4 = c.device()
+    wants = paged.attend(kv, batch, q, mask_of((1, 0, 0))), paged.attend(kv4, batch4, q4, mask_of((1, 0, 0)))
+    batch4.page_table.copy_(batch.page_table)  # (both pools are laid out alike)
+    assert torch.equal(b.table, c.table)
+    wide = paged.PagedBatch(batch.page_table, batch.kv_len, batch.cu_q, max_q=(1 << 30) - 1, max_kv=20011)
+    for shared in (batch, wide):
+        for _ in range(2):
+            assert torch.equal(paged.attend(kv, shared, q, mask_of((1, 0, 0))), wants[0])
+            assert torch.equal(paged.attend(kv4, shared, q4, mask_of((1, 0, 0))), wants[1])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_two_streams_at_once(fvlib, kernel, fmt):
+    """Calls in flight side by side share no scratch."""
+    from fastvideo_rs_b200 import paged, sdpa
+    cases = [Case(fmt, [9000, 400], [nq, 2], 8, 2, 64, seed=15 + nq) for nq in (1, 200)]
+    on = [c.device() for c in cases]
+    wants = [paged.attend(kv, batch, q, mask_of((1, 0, 0))) for kv, batch, q in on]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in on]
+    outs = [[], []]
+    for _ in range(10):
+        for i, (kv, batch, q) in enumerate(on):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(paged.attend(kv, batch, q, mask_of((1, 0, 0))))
+    torch.cuda.synchronize()
+    assert sdpa.device_status() == 0
+    for want, got in zip(wants, outs):
+        assert all(torch.equal(want, x) for x in got)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_captured_steps_of_append_and_attend(fvlib, kernel, fmt):
+    """A step of two layers -- append, attend, twice -- captured once and replayed for token after token, beside a second graph of the
+    same step, equals the calls made one by one."""
+    from fastvideo_rs_b200 import paged, sdpa
+    heads, hk, rows, total, mask = 8, 2, 16, 40, mask_of((1, 20, 3))
+    g = torch.Generator().manual_seed(16)
+    proj = torch.randn(2, total, heads + 2 * hk, D, generator=g).to(torch.bfloat16).cuda()
+    cos, sin = (t.cuda() for t in tables(total, "interleaved"))
+    table = torch.arange((total + rows - 1) // rows, dtype=torch.int32, device="cuda")[None]
+    mk = lambda: [paged.PagedKv.empty(table.shape[1], rows, hk, fmt) for _ in range(2)]
+    batch = paged.PagedBatch(table, torch.zeros(1, dtype=torch.int32, device="cuda"), torch.tensor([0, 1], dtype=torch.int32, device="cuda"),
+                             max_q=1, max_kv=total)
+    token = torch.empty(2, 1, heads + 2 * hk, D, dtype=torch.bfloat16, device="cuda")
+
+    def step(pools):
+        outs = []
+        for kv, x in zip(pools, token):
+            q, k, v = x.split([heads, hk, hk], 1)
+            outs.append(paged.attend(kv, batch, paged.append(kv, batch, k, v, q=q, cos=cos, sin=sin), mask))
+        return torch.stack(outs)
+
+    plain = mk()
+    want = []
+    for t in range(total):
+        batch.kv_len.fill_(t + 1)
+        token.copy_(proj[:, t:t + 1])
+        want.append(step(plain))
+    graphs = []
+    for _ in range(2):
+        pools, graph = mk(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(pools)
+        graphs.append((pools, graph, out))
+    for t in range(total):
+        batch.kv_len.fill_(t + 1)
+        token.copy_(proj[:, t:t + 1])
+        for pools, graph, out in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for pools, graph, out in graphs:
+            assert torch.equal(out, want[t])
+    assert sdpa.device_status() == 0
+
+
 def test_refusals(fvlib):
     from fastvideo_rs_b200 import FvError, paged
     from fastvideo_rs_b200.sdpa import BlockCausal

@@ -85,6 +85,7 @@ def test_c_entries_refuse_and_decline(fvlib):
     assert append(None, None, br, _rows()) == -1 and append(None, kr, br, None) == -1 and attn(None, kr, br, None) == -1
     for bad in (dict(heads=3), dict(scale=0.0), dict(scale=math.inf), dict(mode=7), dict(block=0), dict(window=-1), dict(sink=-1)):
         assert attn(None, kr, br, _query(**bad)) == -1, bad
+    assert append(None, kr, br, _rows(tokens=1 << 30)) == -1 and read(None, kr, br, 16, None, 1 << 30, 16, 16) == -1
     # empty calls are declined before a device is asked for
     assert attn(None, kr, br, _query(tokens=0)) == 1
     assert append(None, kr, br, _rows(tokens=0)) == 1
