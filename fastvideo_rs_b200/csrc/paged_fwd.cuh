@@ -50,7 +50,7 @@ struct ChunkJob {
     float sl2;
 };
 constexpr int kItemCost = 4;   // what an item costs beside its key tiles, in key tiles: the pipeline fills and drains, the output
-constexpr int kLeastRun = 8;   // the shortest run worth a CTA
+constexpr int kLeastRun = 4;   // the shortest run worth a CTA (8: 23 against 16 us for 16 items of two tiles)
 struct ChunkSplit {
     int valid, q0, nq, tok0, head, tiles, cost, runs;
     long long start, total;  // where the item begins on the line, and how long the line is
@@ -317,6 +317,16 @@ FV_DEV void chunk_exp32(const uint32_t (&u)[32], uint32_t* pw, uint64_t s2, uint
     }
 }
 
+// Bit c: the row sees column c0 + c of the tile.  (Three comparisons a column instead took more than the exponentials.)
+FV_DEV uint32_t seen_bits(const Cols& k, int c0) {
+    auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
+    return (below(k.hi - c0) & ~below(k.lo - c0)) | below(k.sink - c0);
+}
+FV_DEV void hide_columns(uint32_t (&u)[32], uint32_t seen) {
+#pragma unroll
+    for (int c = 0; c < 32; c++) u[c] = (seen & (1u << c)) ? u[c] : as_u(neg_inf());
+}
+
 // A tile with invisible columns, or whose sum tripped the guard (out of line for the reasons that fvattn::careful_tile
 // gives).  Where every row has a reference already, or sees nothing of the tile, one pass as in the hot path, the invisible
 // columns as -inf; else, or when that pass trips the guard, exact maxima first, the reference moved, O and the sum rescaled.
@@ -334,10 +344,16 @@ static __device__ __noinline__ void chunk_careful(uint32_t tS, uint32_t tO, uint
         uint32_t u[32], pw[64];
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-            fvattn::load_chunk(tS, c, u);
-            fvattn::land_chunk(u);
-            cols.hide(u, 32 * c);
-            chunk_exp32<F16, false>(u, pw + 16 * c, s2, nf, acc0, acc1, top);
+            const uint32_t seen = seen_bits(cols, 32 * c);
+            if (__any_sync(kFullWarp, seen != 0u)) {
+                fvattn::load_chunk(tS, c, u);
+                fvattn::land_chunk(u);
+                hide_columns(u, seen);
+                chunk_exp32<F16, false>(u, pw + 16 * c, s2, nf, acc0, acc1, top);
+            } else {
+#pragma unroll
+                for (int w = 0; w < 16; w++) pw[16 * c + w] = 0u;
+            }
         }
         const float sum = fvattn::part_sum<false>(acc0, acc1, top);
         if (!__any_sync(kFullWarp, !(sum <= kChunkGuard<F16>))) {
@@ -350,10 +366,12 @@ static __device__ __noinline__ void chunk_careful(uint32_t tS, uint32_t tO, uint
     float mx = neg_inf();
 #pragma unroll 1
     for (int c = 0; c < 4; c++) {
+        const uint32_t seen = seen_bits(cols, 32 * c);
+        if (!__any_sync(kFullWarp, seen != 0u)) continue;
         uint32_t u[32];
         fvattn::load_chunk(tS, c, u);
         fvattn::land_chunk(u);
-        cols.hide(u, 32 * c);
+        hide_columns(u, seen);
         mx = fmaxf(mx, fvattn::max32(u));
     }
     const float cand = mx * sl2;
@@ -380,13 +398,19 @@ static __device__ __noinline__ void chunk_careful(uint32_t tS, uint32_t tO, uint
 #pragma unroll 1
     for (int c = 0; c < 4; c++) {
         uint32_t u[32], pw[16];
-        fvattn::load_chunk(tS, c, u);
-        fvattn::land_chunk(u);
-        cols.hide(u, 32 * c);
-        uint64_t acc0 = pack_f32x2(0.f, 0.f), acc1 = acc0;
-        float top = 0.f;
-        chunk_exp32<F16, false>(u, pw, s2, nf, acc0, acc1, top);
-        l += fvattn::part_sum<false>(acc0, acc1, top);
+        const uint32_t seen = seen_bits(cols, 32 * c);
+        if (__any_sync(kFullWarp, seen != 0u)) {
+            fvattn::load_chunk(tS, c, u);
+            fvattn::land_chunk(u);
+            hide_columns(u, seen);
+            uint64_t acc0 = pack_f32x2(0.f, 0.f), acc1 = acc0;
+            float top = 0.f;
+            chunk_exp32<F16, false>(u, pw, s2, nf, acc0, acc1, top);
+            l += fvattn::part_sum<false>(acc0, acc1, top);
+        } else {
+#pragma unroll
+            for (int w = 0; w < 16; w++) pw[w] = 0u;
+        }
         tmem_st16(tS + 16u * (uint32_t)c, pw);
     }
     fvattn::publish(bt + Smem::p_ready, lane);
