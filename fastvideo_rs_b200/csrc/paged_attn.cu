@@ -787,21 +787,36 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_merge_kernel(const Attn
     if (s >= a.batch.seqs) return;
     const Seq seq = seq_of(a.batch, s);
     if (tok < seq.q0 || tok >= seq.q0 + seq.nq) return;
+    // (a lane a weight, and the loads of eight parts on their way before the first is used: one sequence of 20 011 keys, 8 heads on 1, 64
+    // parts, 17 us for both kernels; one part after the other 27)
     float top = neg_inf();
-    for (int i = 0; i < a.splits; i++) top = fmaxf(top, a.part_lse[(size_t)i * rows + row]);
+    for (int i = lane; i < a.splits; i += 32) top = fmaxf(top, a.part_lse[(size_t)i * rows + row]);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullWarp, top, d));
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
-    if (top != neg_inf()) {
-        for (int i = 0; i < a.splits; i++) {
-            const float w = fvp::ex2(a.part_lse[(size_t)i * rows + row] - top);
-            if (w == 0.f) continue;
-            const float4 x = *reinterpret_cast<const float4*>(a.part_o + ((size_t)i * rows + row) * kD + 4 * lane);
-            sum += w;
-            acc.x = fmaf(w, x.x, acc.x);
-            acc.y = fmaf(w, x.y, acc.y);
-            acc.z = fmaf(w, x.z, acc.z);
-            acc.w = fmaf(w, x.w, acc.w);
+    for (int i0 = 0; i0 < a.splits && top != neg_inf(); i0 += 32) {
+        const float w = i0 + lane < a.splits ? fvp::ex2(a.part_lse[(size_t)(i0 + lane) * rows + row] - top) : 0.f;
+        const int here = min(32, a.splits - i0);
+        constexpr int kAhead = 8;
+        for (int i = 0; i < here; i += kAhead) {
+            float4 x[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; j++)
+                x[j] = __ldcg(reinterpret_cast<const float4*>(a.part_o + ((size_t)(i0 + min(i + j, here - 1)) * rows + row) * kD + 4 * lane));
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                const float wj = __shfl_sync(kFullWarp, w, (i + j) & 31);
+                if (i + j >= here || wj == 0.f) continue;
+                sum += wj;
+                acc.x = fmaf(wj, x[j].x, acc.x);
+                acc.y = fmaf(wj, x[j].y, acc.y);
+                acc.z = fmaf(wj, x[j].z, acc.z);
+                acc.w = fmaf(wj, x[j].w, acc.w);
+            }
         }
+    }
+    if (top != neg_inf()) {
         const float inv = 1.f / sum;
         acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
     }
@@ -851,37 +866,75 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_join_kernel(const Chunk
     }
     __syncthreads();
     const int n = count;
+    // The warp's rows go together, so that the loads of all of them are in flight at a time (one after the other: 34 against 15 us
+    // under the profiler for 88 runs over 6 items of 40 rows, 12 against 7.4 for 148 over 40 of 256).
     constexpr int kRowsHere = 2 * kChunkRows / kJoinBlocks / kWarps;
-#pragma unroll 1
-    for (int i = 0; i < kRowsHere; i++) {
-        const int r = (block * kRowsHere + i) * kWarps + warp, tile = r / kChunkRows, row = r - tile * kChunkRows;
-        const int row_tok = row / jb.group, tok = sp.tok0 + tile * jb.tile_tokens + row_tok;
-        if (row_tok >= jb.tile_tokens || tok >= sp.nq) continue;
-        float top = neg_inf();
-        for (int k = lane; k < n; k += 32) top = fmaxf(top, jb.part_lse[(size_t)slots[k] * 2 * kChunkRows + r]);
+    const int r0 = block * kRowsHere * kWarps + warp;  // its rows: r0 + kWarps i
+    long long out[kRowsHere];  // -1: none
+    bool any = false;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullWarp, top, d));
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float sum = 0.f;
-        for (int k0 = 0; top != neg_inf() && k0 < n; k0 += 32) {
-            float w = 0.f;
-            if (k0 + lane < n) w = fvp::ex2(jb.part_lse[(size_t)slots[k0 + lane] * 2 * kChunkRows + r] - top);
-            const int here = min(32, n - k0);
-#pragma unroll 4
-            for (int k = 0; k < here; k++) {
-                const float wk = __shfl_sync(kFullWarp, w, k);
-                const float4 x = *reinterpret_cast<const float4*>(jb.part_o + ((size_t)slots[k0 + k] * 2 * kChunkRows + r) * kD + 4 * lane);
-                sum += wk;
-                acc.x = fmaf(wk, x.x, acc.x);
-                acc.y = fmaf(wk, x.y, acc.y);
-                acc.z = fmaf(wk, x.z, acc.z);
-                acc.w = fmaf(wk, x.w, acc.w);
+    for (int i = 0; i < kRowsHere; i++) {
+        const int r = r0 + kWarps * i, tile = r / kChunkRows, row = r - tile * kChunkRows;
+        const int row_tok = row / jb.group, tok = sp.tok0 + tile * jb.tile_tokens + row_tok;
+        const bool live = row_tok < jb.tile_tokens && tok < sp.nq;
+        out[i] = live ? (long long)(sp.q0 + tok) * jb.heads + sp.head * jb.group + (row - row_tok * jb.group) : -1;
+        any |= live;
+    }
+    if (!any) return;
+    float top[kRowsHere], sum[kRowsHere];
+    float4 acc[kRowsHere];
+#pragma unroll
+    for (int i = 0; i < kRowsHere; i++) {
+        top[i] = neg_inf();
+        sum[i] = 0.f;
+        acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    auto lse = [&](int k, int i) { return jb.part_lse[(size_t)slots[k] * 2 * kChunkRows + r0 + kWarps * i]; };
+    for (int k = lane; k < n; k += 32) {
+#pragma unroll
+        for (int i = 0; i < kRowsHere; i++)
+            if (out[i] >= 0) top[i] = fmaxf(top[i], lse(k, i));
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsHere; i++) {
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(kFullWarp, top[i], d));
+    }
+    for (int k0 = 0; k0 < n; k0 += 32) {
+        float w[kRowsHere];
+#pragma unroll
+        for (int i = 0; i < kRowsHere; i++) w[i] = k0 + lane < n && top[i] != neg_inf() ? fvp::ex2(lse(k0 + lane, i) - top[i]) : 0.f;
+        const int here = min(32, n - k0);
+        constexpr int kAhead = 4;  // parts whose loads are on their way before the first is used
+        for (int k = 0; k < here; k += kAhead) {
+            float4 x[kAhead][kRowsHere];
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {  // (also of rows that are none: their sums are not stored)
+                const float* part = jb.part_o + ((size_t)slots[k0 + min(k + j, here - 1)] * 2 * kChunkRows + r0) * kD + 4 * lane;
+#pragma unroll
+                for (int i = 0; i < kRowsHere; i++) x[j][i] = __ldcg(reinterpret_cast<const float4*>(part + (size_t)kWarps * i * kD));
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                if (k + j >= here) break;
+#pragma unroll
+                for (int i = 0; i < kRowsHere; i++) {
+                    const float wk = __shfl_sync(kFullWarp, w[i], k + j);
+                    sum[i] += wk;
+                    acc[i].x = fmaf(wk, x[j][i].x, acc[i].x);
+                    acc[i].y = fmaf(wk, x[j][i].y, acc[i].y);
+                    acc[i].z = fmaf(wk, x[j][i].z, acc[i].z);
+                    acc[i].w = fmaf(wk, x[j][i].w, acc[i].w);
+                }
             }
         }
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
-        const size_t out = (size_t)(sp.q0 + tok) * jb.heads + sp.head * jb.group + (row - row_tok * jb.group);
-        *reinterpret_cast<uint2*>(jb.out + out * kD + 4 * lane) =
-            make_uint2(fvp::pack_bf16x2(acc.x * inv, acc.y * inv), fvp::pack_bf16x2(acc.z * inv, acc.w * inv));
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsHere; i++) {
+        if (out[i] < 0) continue;
+        const float inv = sum[i] > 0.f ? 1.f / sum[i] : 0.f;
+        *reinterpret_cast<uint2*>(jb.out + (size_t)out[i] * kD + 4 * lane) =
+            make_uint2(fvp::pack_bf16x2(acc[i].x * inv, acc[i].y * inv), fvp::pack_bf16x2(acc[i].z * inv, acc[i].w * inv));
     }
 }
 
@@ -893,20 +946,41 @@ struct Shape {
     bool cluster;
     int ctas, phases;  // of the chunk kernel
 };
-// How a call is cut.  Few rows per kv head: blocks of up to 16 rows, and the keys in `splits` ranges so that all SMs have
-// work.  Many: items of 2 x 128 rows, one CTA per SM.  Which of the two: an estimate of both in us, fitted to sweeps over 16 to 160
-// rows, 1 to 32 sequences of 2 000 to 20 011 keys and both page formats (e.g. 8 sequences of 20 011 bf16 keys, 32 heads on 8: 16 rows
-// 112 us in blocks of 16 and 123 us in items, 24 rows 197 and 125; one sequence of 20 011: 64 rows 56 and 62, 96 rows 126 and 62;
-// one of 2 000: 160 rows 22 and 35).  FV_PAGED_KERNEL=rows or items (kept for A/B) takes the choice away.
 constexpr long long kL2Bytes = 126ll << 20;
-static bool take_items(long long planes, long long rows, long long keys, bool q4) {
+// Key ranges: as many as fill the SMs once; where the rows alone nearly do, three times over, so that ragged ends even
+// out.  Up to kMaxCluster ranges are one cluster, which joins its parts itself.  More need the merge kernel, which costs about 4 us: they
+// are taken where they shorten a warp's run of tiles (0.72 us for 16 keys of bf16, 0.34 us of 4 bits) by more than that, with at least
+// four of them left to it; of 4 bits, bound by the SMs' own pipes, two CTAs an SM are enough.  (One sequence of 20 011 keys, 32 heads on 8:
+// 25 us in 55 ranges of bf16, 48 in 8; 16 us in 32 ranges of 4 bits, 20 in 8.  Of 4 001 keys: 14 and 12; 12 and 9.)
+// `ctas` blocks of rows, of which `resident` run at a time.
+static int key_ranges(long long ctas, int resident, long long keys, bool q4, int sms) {
+    const long long tiles = (keys + 15) / 16, most = (tiles + 2 * kWarps - 1) / (2 * kWarps);  // at least 32 keys per warp
+    long long n = resident / ctas;
+    if (n < 2) n = (3ll * resident + ctas - 1) / ctas;
+    if (n > kMaxCluster) {
+        const long long full = q4 ? 2ll * sms / ctas : n, whole = tiles / (4 * kWarps);
+        n = full < whole ? full : whole;
+        if (n <= kMaxCluster || (q4 ? 0.34 : 0.72) * (double)(tiles / kWarps) * (1.0 / kMaxCluster - 1.0 / (double)n) < 4.0) n = kMaxCluster;
+    }
+    n = n < most ? n : most;
+    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+// How a call is cut.  Few rows per kv head: blocks of up to 16 rows, and the keys in ranges.  Many: items of 2 x 128 rows, one CTA
+// per SM.  Which of the two: an estimate of both in us, fitted to 326 calls of 20 to 800 rows, 1 to 16 sequences of 200 to 20 011 keys, 1 and 8
+// kv heads, both page formats, over which the choice costs 1.2 % more than the better kernel would.  E.g. 8 kv heads, bf16: one sequence of
+// 20 011 keys 20 rows 35 us in blocks of rows and 53 in items, 96 rows 77 and 53; sixteen of 200 keys 48 rows 28 and 20.
+// FV_PAGED_KERNEL=rows or items (kept for A/B) takes the choice away.
+static bool take_items(long long planes, long long rows, long long keys, bool q4, int sms) {
     const char* e = getenv("FV_PAGED_KERNEL");
     if (e && strcmp(e, "items") == 0) return true;
     if ((e && strcmp(e, "rows") == 0) || rows <= 16) return false;
-    const double work = (double)planes * keys, blocks = (double)((rows + 15) / 16), items = (double)((rows + 255) / 256);
-    const double stream = work * (q4 ? 2 * kQ4Bytes + 8 : 4 * kD) / 5.9e6, compute = work * blocks * (q4 ? 4.5e-5 : 7e-5);
-    const double in_rows = 10.0 + (stream > compute ? stream : compute);
-    const double in_items = 35.0 + items * (work / kChunkTile + planes * kItemCost) * 0.0142;
+    const long long ctas = planes * ((rows + 15) / 16);
+    const int resident = 2 * sms, n = key_ranges(ctas, resident, keys, q4, sms);
+    const double load = (double)ctas * n / resident, waves = load <= 1.0 ? 1.0 : 0.5 * (load + ceil(load));  // (their CTAs end at different times)
+    const double in_rows = 6.2 + waves * ((q4 ? 7.2 : 5.4) + (q4 ? 0.50 : 0.86) * (double)keys / (16.0 * kWarps * n)) + (n > kMaxCluster ? 4.0 : 0.0);
+    const double items = (double)planes * (double)((rows + 255) / 256), line = items * (double)((keys + kChunkTile - 1) / kChunkTile + kItemCost);
+    const double runs = line < (double)kLeastRun * sms ? line / kLeastRun : (double)sms, parts = runs / items;
+    const double in_items = (q4 ? 7.0 + 1.83 * line / runs : 4.7 + 1.72 * line / runs) + (parts > 1.0 ? 9.0 + 0.65 * (parts - 1.0) : 0.0);
     return in_items < in_rows;
 }
 static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int tokens, int heads, const Mask& m, int sms) {
@@ -919,7 +993,7 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int tokens
         keys = most < keys ? most : keys;
     }
     const bool q4 = kv->format == FV_PAGE_Q4;
-    s.chunk = group <= kChunkRows && take_items((long long)b->seqs * kv->kv_heads, rows, keys, q4);
+    s.chunk = group <= kChunkRows && take_items((long long)b->seqs * kv->kv_heads, rows, keys, q4, sms);
     s.tile_tokens = s.chunk ? kChunkRows / group : 0;
     s.cluster = false;
     if (s.chunk) {
@@ -940,16 +1014,7 @@ static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int tokens
     s.block_rows = rows > 8 ? 16 : rows <= 4 && q4 ? 4 : 8;
     s.row_blocks = (int)((rows + s.block_rows - 1) / s.block_rows);
     const long long ctas = (long long)b->seqs * kv->kv_heads * s.row_blocks;
-    // Key ranges: as many as fill the SMs once; where the rows alone nearly do, three times over, so that ragged ends even
-    // out.  Up to kMaxCluster ranges are one cluster, which joins its parts itself; the merge kernel behind more of them takes
-    // about 5 us, so more need enough tiles a warp (0.75 us each) to be worth it.
-    const int resident = sms * (s.block_rows <= 8 ? 3 : 2);  // CTAs that run at a time
-    const long long tiles = (keys + 15) / 16, most = (tiles + 2 * kWarps - 1) / (2 * kWarps);  // at least 32 keys per warp
-    long long n = resident / ctas;
-    if (n < 2) n = (3ll * resident + ctas - 1) / ctas;
-    if (n > kMaxCluster && (n < 16 || tiles < 16 * kWarps * kMaxCluster)) n = kMaxCluster;
-    n = n < most ? n : most;
-    s.splits = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+    s.splits = key_ranges(ctas, sms * (s.block_rows <= 8 ? 3 : 2), keys, q4, sms);
     s.cluster = s.splits > 1 && s.splits <= kMaxCluster;
     return s;
 }
