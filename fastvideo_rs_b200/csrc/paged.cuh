@@ -79,10 +79,26 @@ FV_DEV size_t pool_row(const Pool& p, int page, int head, int key) {
     return ((((size_t)page * p.kv_heads + head) << p.log_rows) + (size_t)(key & ((1 << p.log_rows) - 1)));
 }
 
+// A divisor known on the host: quotients of 0 .. 2^31 - 1 by a multiplication (Granlund and Montgomery, Division by Invariant
+// Integers using Multiplication, 1994).  The kernels' indices and masks divide a dozen times before anything is read; each division that is not
+// one of these is a chain of some twenty instructions.
+struct Div {
+    uint32_t d, mul;
+    int shift;
+    static Div of(int d) {
+        Div v{(uint32_t)d, 0, 0};
+        while ((1ull << v.shift) < v.d) v.shift++;
+        v.mul = (uint32_t)((((1ull << v.shift) - v.d) << 32) / v.d + 1);
+        return v;
+    }
+};
+FV_DEV int operator/(int n, const Div& v) { return (int)((__umulhi((uint32_t)n, v.mul) + (uint32_t)n) >> v.shift); }
+
 // The mask: key j is visible to position p iff t_j <= t_p and (window == 0 or t_p - t_j < window or t_j < sink), with
 // t = index / block; block == 0: every key below the sequence's length.
 struct Mask {
     int block, window, sink;
+    Div by_block;
 };
 // Keys that positions first .. last see between them: [0, sink) U [lo, hi), sink <= lo.
 struct Span {
@@ -96,11 +112,11 @@ FV_DEV Span span_of(const Mask& m, int first, int last, int len) {
     if (m.block == 0) return Span{0, 0, len};
     if (last < 0) return Span{0, 0, 0};
     Span s;
-    s.hi = min(len, mul_sat(last / m.block + 1, m.block));
+    s.hi = min(len, mul_sat(last / m.by_block + 1, m.block));
     s.lo = 0;
     s.sink = 0;
     if (m.window > 0) {
-        s.lo = mul_sat(max(0, max(first, 0) / m.block - m.window + 1), m.block);
+        s.lo = mul_sat(max(0, max(first, 0) / m.by_block - m.window + 1), m.block);
         s.sink = min(mul_sat(m.sink, m.block), s.hi);
         if (s.sink >= s.lo) s.lo = s.sink = 0;
     }

@@ -35,7 +35,8 @@ struct AttnArgs {
     uint16_t* out;            // [tokens, heads, 128]
     float* part_o;            // [splits, tokens * heads, 128] normalised, when splits > 1
     float* part_lse;          // [splits, tokens * heads], base 2
-    int heads, group, splits, row_blocks;
+    int heads, group, splits;
+    Div by_group, by_splits, by_blocks, by_heads;  // blocks of rows of a (sequence, kv head); kv heads
     int cluster;              // the key ranges of a block of rows are one cluster, which joins them itself
     float sl2;
     long long wait_cycles;
@@ -247,16 +248,14 @@ __global__ void __launch_bounds__(kAttnThreads, ROWS <= 8 ? 3 : 2) fv_paged_deco
     float (*sh_l)[kRows] = sh_m + kWarps;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     int b = blockIdx.x;
-    const int split = b % a.splits;
-    b /= a.splits;
-    const int rb = b % a.row_blocks;
-    b /= a.row_blocks;
-    const int head = b % a.pool.kv_heads, s = b / a.pool.kv_heads;
+    const int ranges = b / a.by_splits, split = b - ranges * a.splits;
+    b = ranges / a.by_blocks;
+    const int rb = ranges - b * (int)a.by_blocks.d, s = b / a.by_heads, head = b - s * a.pool.kv_heads;
     const Seq seq = seq_of(a.batch, s);
     const int row0 = rb * kRows, rows = min(kRows, seq.nq * a.group - row0);
     if (rows <= 0) return;  // (the same for all key ranges of these rows)
     const int pos0 = seq.len - seq.nq;  // position of the sequence's first token of this call
-    const int first = pos0 + row0 / a.group, last = pos0 + (row0 + rows - 1) / a.group;
+    const int first = pos0 + row0 / a.by_group, last = pos0 + (row0 + rows - 1) / a.by_group;
     const Span span = span_of(a.mask, first, last, seq.len);
     const Tiles<kTile<Q4>> tiles(span);
     const int u0 = (int)((long long)tiles.count * split / a.splits), u1 = (int)((long long)tiles.count * (split + 1) / a.splits);
@@ -355,7 +354,8 @@ __global__ void __launch_bounds__(kAttnThreads, ROWS <= 8 ? 3 : 2) fv_paged_deco
         const int rq = ROWS == 4 ? ((g & 1) ? ROWS : g >> 1) : 8 * n + g, r = row0 + rq;
         uint4 u[4];
         if (rq < rows) {
-            const uint16_t* p = a.q + (size_t)(seq.q0 + r / a.group) * a.q_tok + (size_t)(head * a.group + r % a.group) * a.q_head;
+            const int tok = r / a.by_group;
+            const uint16_t* p = a.q + (size_t)(seq.q0 + tok) * a.q_tok + (size_t)(head * a.group + r - tok * a.group) * a.q_head;
 #pragma unroll
             for (int i = 0; i < 4; i++) u[i] = *reinterpret_cast<const uint4*>(p + (Q4 ? 32 * t + 8 * i : 32 * i + 8 * t));
         } else {
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kAttnThreads, ROWS <= 8 ? 3 : 2) fv_paged_deco
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
                     for (int e = 0; e < EH; e++) {
-                        const int r = row0 + row_of(n, e), p = pos0 + r / a.group;
+                        const int r = row0 + row_of(n, e), p = pos0 + r / a.by_group;
                         const Span sp = span_of(a.mask, p, p, seq.len);
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
@@ -695,83 +695,96 @@ __global__ void __launch_bounds__(kAttnThreads, ROWS <= 8 ? 3 : 2) fv_paged_deco
         }
     }
     __syncthreads();
-    const int d = threadIdx.x;  // kAttnThreads == kD
-    auto out_row = [&](int r) { return (size_t)(seq.q0 + (row0 + r) / a.group) * a.heads + head * a.group + (row0 + r) % a.group; };
-    // Row r of this CTA: value d against the row's reference, and the sum of P.
-    auto join = [&](int r, float& top, float& sum) {
-        top = sh_m[0][r];
-#pragma unroll
-        for (int w = 1; w < kWarps; w++) top = fmaxf(top, sh_m[w][r]);
-        float acc = 0.f;
-        sum = 0.f;
-        if (top != neg_inf()) {
-#pragma unroll
-            for (int w = 0; w < kWarps; w++) {
-                const float f = fvp::ex2(sh_m[w][r] - top);
-                sum = fmaf(f, sh_l[w][r], sum);
-                if (f != 0.f) acc = fmaf(f, sh_o[w][r][d], acc);
-            }
-        }
-        return acc;
+    // A warp takes whole rows, warp + 4 i, four values a lane, all of them at a time (a value a thread, row after row, took 5 us of 16 rows).
+    auto out_row = [&](int r) {
+        const int tok = (row0 + r) / a.by_group;
+        return (size_t)(seq.q0 + tok) * a.heads + head * a.group + (row0 + r - tok * a.group);
     };
+    auto add = [](float4& acc, float f, const float4& x) {  // (what has no weight may hold anything)
+        if (f == 0.f) return;
+        acc.x = fmaf(f, x.x, acc.x);
+        acc.y = fmaf(f, x.y, acc.y);
+        acc.z = fmaf(f, x.z, acc.z);
+        acc.w = fmaf(f, x.w, acc.w);
+    };
+    auto pack = [](const float4& x, float by) {
+        return make_uint2(fvp::pack_bf16x2(x.x * by, x.y * by), fvp::pack_bf16x2(x.z * by, x.w * by));
+    };
+    constexpr int kMine = kRows / kWarps;
+    float top[kMine], sum[kMine];  // the reference of a row, and the sum of P against it
+    float4 acc[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; i++) {
+        const int r = warp + kWarps * i;
+        top[i] = sh_m[0][r];
+#pragma unroll
+        for (int w = 1; w < kWarps; w++) top[i] = fmaxf(top[i], sh_m[w][r]);
+        sum[i] = 0.f;
+        acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            const float f = sh_m[w][r] == neg_inf() ? 0.f : fvp::ex2(sh_m[w][r] - top[i]);
+            sum[i] = fmaf(f, sh_l[w][r], sum[i]);
+            add(acc[i], f, *reinterpret_cast<const float4*>(&sh_o[w][r][4 * lane]));
+        }
+    }
     if (a.cluster) {
-        // The key ranges of these rows are the CTAs of one cluster: each joins its own warps, then the rows are dealt to
+        // The key ranges of these rows are the CTAs of one cluster: each has joined its own warps, then the rows are dealt to
         // the CTAs, which read each other's parts over distributed shared memory, in the order of the ranges.
         cg::cluster_group cluster = cg::this_cluster();
-        float part[kRows], tops[kRows], sums[kRows];
+        __syncwarp();
 #pragma unroll
-        for (int r = 0; r < kRows; r++) part[r] = r < rows ? join(r, tops[r], sums[r]) : 0.f;
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < kRows; r++) {
-            if (r >= rows) break;
-            sh_o[0][r][d] = part[r];
-            if (d == 0) {
-                sh_m[0][r] = tops[r];
-                sh_l[0][r] = sums[r];
+        for (int i = 0; i < kMine; i++) {  // (rows of this warp's own)
+            const int r = warp + kWarps * i;
+            *reinterpret_cast<float4*>(&sh_o[0][r][4 * lane]) = acc[i];
+            if (lane == 0) {
+                sh_m[0][r] = top[i];
+                sh_l[0][r] = sum[i];
             }
         }
         cluster.sync();
-        for (int r = split; r < rows; r += a.splits) {
+        for (int r = split + a.splits * warp; r < rows; r += a.splits * kWarps) {
             // (every load of the row on its way before the first is used: one after the other they took 2 us)
-            float mi[kMaxCluster], li[kMaxCluster], oi[kMaxCluster];
+            float mi[kMaxCluster], li[kMaxCluster];
+            float4 oi[kMaxCluster];
 #pragma unroll
             for (int i = 0; i < kMaxCluster; i++) {
                 mi[i] = neg_inf();
-                li[i] = oi[i] = 0.f;
+                li[i] = 0.f;
+                oi[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (i < a.splits) {
                     mi[i] = *cluster.map_shared_rank(&sh_m[0][r], i);
                     li[i] = *cluster.map_shared_rank(&sh_l[0][r], i);
-                    oi[i] = *cluster.map_shared_rank(&sh_o[0][r][d], i);
+                    oi[i] = *cluster.map_shared_rank(reinterpret_cast<float4*>(&sh_o[0][r][4 * lane]), i);
                 }
             }
-            float top = mi[0], acc = 0.f, sum = 0.f;
+            float m_all = mi[0], l_all = 0.f;
+            float4 o_all = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int i = 1; i < kMaxCluster; i++) top = fmaxf(top, mi[i]);
+            for (int i = 1; i < kMaxCluster; i++) m_all = fmaxf(m_all, mi[i]);
 #pragma unroll
             for (int i = 0; i < kMaxCluster; i++) {
-                const float f = mi[i] == neg_inf() ? 0.f : fvp::ex2(mi[i] - top);
-                sum = fmaf(f, li[i], sum);
-                if (f != 0.f) acc = fmaf(f, oi[i], acc);
+                const float f = mi[i] == neg_inf() ? 0.f : fvp::ex2(mi[i] - m_all);
+                l_all = fmaf(f, li[i], l_all);
+                add(o_all, f, oi[i]);
             }
-            a.out[out_row(r) * kD + d] = (uint16_t)fvp::pack_bf16x2(top == neg_inf() ? 0.f : acc / sum, 0.f);
+            *reinterpret_cast<uint2*>(a.out + out_row(r) * kD + 4 * lane) = pack(o_all, m_all == neg_inf() ? 0.f : 1.f / l_all);
         }
         cluster.sync();  // (no CTA leaves while another one still reads its part)
         return;
     }
 #pragma unroll
-    for (int r = 0; r < kRows; r++) {
+    for (int i = 0; i < kMine; i++) {
+        const int r = warp + kWarps * i;
         if (r >= rows) break;
-        float top, sum;
-        float acc = join(r, top, sum);
-        if (top != neg_inf()) acc /= sum;
+        const float by = top[i] == neg_inf() ? 0.f : 1.f / sum[i];
         const size_t oi = out_row(r);
         if (a.splits == 1) {
-            a.out[oi * kD + d] = (uint16_t)fvp::pack_bf16x2(acc, 0.f);
+            *reinterpret_cast<uint2*>(a.out + oi * kD + 4 * lane) = pack(acc[i], by);
         } else {
             const size_t pi = (size_t)split * a.batch.tokens * a.heads + oi;
-            a.part_o[pi * kD + d] = acc;
-            if (d == 0) a.part_lse[pi] = sum > 0.f ? top + log2f(sum) : top;  // (no key: -inf; not a number: +inf)
+            *reinterpret_cast<float4*>(a.part_o + pi * kD + 4 * lane) = make_float4(acc[i].x * by, acc[i].y * by, acc[i].z * by, acc[i].w * by);
+            if (lane == 0) a.part_lse[pi] = sum[i] > 0.f ? top[i] + log2f(sum[i]) : top[i];  // (no key: -inf; not a number: +inf)
         }
     }
 }
@@ -875,7 +888,7 @@ __global__ void __launch_bounds__(kAttnThreads) fv_paged_join_kernel(const Chunk
 #pragma unroll
     for (int i = 0; i < kRowsHere; i++) {
         const int r = r0 + kWarps * i, tile = r / kChunkRows, row = r - tile * kChunkRows;
-        const int row_tok = row / jb.group, tok = sp.tok0 + tile * jb.tile_tokens + row_tok;
+        const int row_tok = row / jb.by_group, tok = sp.tok0 + tile * jb.tile_tokens + row_tok;
         const bool live = row_tok < jb.tile_tokens && tok < sp.nq;
         out[i] = live ? (long long)(sp.q0 + tok) * jb.heads + sp.head * jb.group + (row - row_tok * jb.group) : -1;
         any |= live;
@@ -1044,7 +1057,9 @@ static int launch_chunk(cudaStream_t st, const fv_paged_kv* kv, const AttnArgs& 
     jb.heads = a.heads;
     jb.group = a.group;
     jb.tile_tokens = s.tile_tokens;
-    jb.q_blocks = s.row_blocks;
+    jb.by_group = a.by_group;
+    jb.by_blocks = a.by_blocks;
+    jb.by_heads = a.by_heads;
     const long long items = (long long)a.batch.seqs * a.pool.kv_heads * s.row_blocks;
     if (items > 0x3fffffffll) return FV_DECLINED;
     jb.items = (int)items;
@@ -1091,13 +1106,13 @@ static int launch_chunk(cudaStream_t st, const fv_paged_kv* kv, const AttnArgs& 
 
 static int check_mask(const fv_paged_query& x, Mask* m) {
     if (x.mask_mode == FV_MASK_NONE) {
-        *m = Mask{0, 0, 0};
+        *m = Mask{};
         return FV_RAN;
     }
     if (x.mask_mode != FV_MASK_BLOCK_CAUSAL) return fvrt::fail(FV_ERR_INVALID, "paged attention: unknown mask mode %d", x.mask_mode);
     if (x.block_tokens < 1 || x.window < 0 || x.sink < 0)
         return fvrt::fail(FV_ERR_INVALID, "paged attention: block-causal needs block_tokens >= 1, window, sink >= 0");
-    *m = Mask{x.block_tokens, x.window, x.sink};
+    *m = Mask{x.block_tokens, x.window, x.sink, Div::of(x.block_tokens)};
     return FV_RAN;
 }
 
@@ -1156,7 +1171,10 @@ extern "C" int fv_paged_attn_bf16(void* stream, const fv_paged_kv* kv, const fv_
     a.heads = heads;
     a.group = heads / kv->kv_heads;
     a.splits = s.splits;
-    a.row_blocks = s.row_blocks;
+    a.by_group = Div::of(a.group);
+    a.by_splits = Div::of(s.splits);
+    a.by_blocks = Div::of(s.row_blocks);
+    a.by_heads = Div::of(kv->kv_heads);
     a.cluster = s.cluster;
     a.sl2 = scale * 1.4426950408889634f;
     a.wait_cycles = FV_WAIT_CYCLES;

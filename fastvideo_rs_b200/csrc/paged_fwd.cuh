@@ -45,8 +45,9 @@ struct ChunkJob {
     struct ChunkSplit* split;  // [run]: the item that begins in the run and ends in another
     int* wait_status;          // the first status word
     long long wait_cycles;
-    int heads, group, tile_tokens, q_blocks, items, box_rows;  // items: (sequence, kv head, row block), row blocks fastest
+    int heads, group, tile_tokens, items, box_rows;  // items: (sequence, kv head, row block), row blocks fastest
     int phases;
+    Div by_group, by_blocks, by_heads;  // row blocks of a plane; kv heads
     float sl2;
 };
 constexpr int kItemCost = 4;   // what an item costs beside its key tiles, in key tiles: the pipeline fills and drains, the output
@@ -114,11 +115,11 @@ struct Work {
 };
 // Item number i: its rows and tiles, and its cost; 0 when there are no such rows.
 FV_DEV int item_at(const ChunkJob& jb, int i, Work& w) {
-    const int plane = i / jb.q_blocks;
-    w.s = plane / jb.pool.kv_heads;
+    const int plane = i / jb.by_blocks;
+    w.s = plane / jb.by_heads;
     w.head = plane - w.s * jb.pool.kv_heads;
     w.seq = seq_of(jb.batch, w.s);
-    w.tok0 = (i - plane * jb.q_blocks) * 2 * jb.tile_tokens;
+    w.tok0 = (i - plane * (int)jb.by_blocks.d) * 2 * jb.tile_tokens;
     w.tiles = 0;
     if (w.tok0 >= w.seq.nq) return 0;
     const int last = min(w.tok0 + 2 * jb.tile_tokens, w.seq.nq) - 1;
@@ -468,7 +469,7 @@ FV_DEV void chunk_softmax(const ChunkJob& jb, const Run& run, uint32_t sbase, ui
     const uint32_t tS = lanes + fvattn::tmem_scores((uint32_t)tile), tO = lanes + fvattn::tmem_output((uint32_t)tile);
     const uint32_t bt = sbase + 8u * (uint32_t)tile;
     const float sl2 = jb.sl2;
-    const int row_tok = row / jb.group, row_head = row - row_tok * jb.group;
+    const int row_tok = row / jb.by_group, row_head = row - row_tok * jb.group;
     uint32_t s_count = 0, o_count = 0;
     Walk walk(run);
     Work w;
@@ -723,7 +724,7 @@ FV_DEV void chunk_expander(const ChunkJob& jb, const Run& run, uint32_t sbase, i
         const uint32_t dst = sbase + Smem::q + slot * kSlotBytes;
 #pragma unroll 1
         for (int u = wid; u < 16; u += kW) {
-            const int row = 8 * u + r8, row_tok = row / jb.group, tok = w.tok0 + tile * jb.tile_tokens + row_tok;
+            const int row = 8 * u + r8, row_tok = row / jb.by_group, tok = w.tok0 + tile * jb.tile_tokens + row_tok;
             const bool live = row_tok < jb.tile_tokens && tok < w.seq.nq;
             const uint16_t* p = jb.q + (long long)(w.seq.q0 + (live ? tok : 0)) * jb.q_tok +
                                 (long long)(w.head * jb.group + (live ? row - row_tok * jb.group : 0)) * jb.q_head + 32 * q;
