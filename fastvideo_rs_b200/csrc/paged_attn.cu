@@ -984,8 +984,8 @@ static int key_ranges(long long ctas, int resident, long long keys, bool q4, int
 }
 // How a call is cut.  Few rows per kv head: blocks of up to 16 rows, and the keys in ranges.  Many: items of 2 x 128 rows, one CTA
 // per SM.  Which of the two: an estimate of both in us, fitted to 326 calls of 20 to 800 rows, 1 to 16 sequences of 200 to 20 011 keys, 1 and 8
-// kv heads, both page formats, over which the choice costs 1.2 % more than the better kernel would.  E.g. 8 kv heads, bf16: one sequence of
-// 20 011 keys 20 rows 35 us in blocks of rows and 53 in items, 96 rows 77 and 53; sixteen of 200 keys 48 rows 28 and 20.
+// kv heads, both page formats, over which the choice costs 0.6 % more than the better kernel would.  E.g. 8 kv heads, bf16: one sequence of
+// 20 011 keys 20 rows 31 us in blocks of rows and 43 in items, 96 rows 116 and 43; sixteen of 200 keys 48 rows 17 and 19, 400 rows 51 and 27.
 // FV_PAGED_KERNEL=rows or items (kept for A/B) takes the choice away.
 static bool take_items(long long planes, long long rows, long long keys, bool q4, int sms) {
     const char* e = getenv("FV_PAGED_KERNEL");
@@ -994,10 +994,10 @@ static bool take_items(long long planes, long long rows, long long keys, bool q4
     const long long ctas = planes * ((rows + 15) / 16);
     const int resident = 2 * sms, n = key_ranges(ctas, resident, keys, q4, sms);
     const double load = (double)ctas * n / resident, waves = load <= 1.0 ? 1.0 : 0.5 * (load + ceil(load));  // (their CTAs end at different times)
-    const double in_rows = 6.2 + waves * ((q4 ? 7.2 : 5.4) + (q4 ? 0.50 : 0.86) * (double)keys / (16.0 * kWarps * n)) + (n > kMaxCluster ? 4.0 : 0.0);
+    const double in_rows = 5.0 + waves * ((q4 ? 3.8 : 2.2) + (q4 ? 0.49 : 0.85) * (double)keys / (16.0 * kWarps * n)) + (n > kMaxCluster ? 4.0 : 0.0);
     const double items = (double)planes * (double)((rows + 255) / 256), line = items * (double)((keys + kChunkTile - 1) / kChunkTile + kItemCost);
     const double runs = line < (double)kLeastRun * sms ? line / kLeastRun : (double)sms, parts = runs / items;
-    const double in_items = (q4 ? 7.0 + 1.83 * line / runs : 4.7 + 1.72 * line / runs) + (parts > 1.0 ? 9.0 + 0.65 * (parts - 1.0) : 0.0);
+    const double in_items = (q4 ? 4.9 + 1.83 * line / runs : 4.3 + 1.66 * line / runs) + (parts > 1.0 ? 8.8 + 0.64 * (parts - 1.0) : 0.0);
     return in_items < in_rows;
 }
 static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int tokens, int heads, const Mask& m, int sms) {

@@ -10,8 +10,8 @@
 //     may begin and end inside an item.  Parts of an item go to a workspace with their log-sum-exp and one small kernel joins
 //     them, in order.  (Whole items dealt in snake order, cut in equal key ranges by a cost model, took 912 us for 4 680 rows x
 //     12 heads over 28 080 keys -- 228 items on 148 SMs -- and 512 us for three ragged chunks of 600 items.)
-//   * Key tiles are 128 keys at multiples of 128: those of the sinks, then those of the window.  Pages outside are not
-//     touched.
+//   * Key tiles are 128 keys at multiples of 128: those of the window, then those of the sinks (a reference taken from a few sinks would
+//     not hold for long: 460 against 404 us for three ragged chunks over 4-bit pages).  Pages outside are not touched.
 //   * bf16 pages: one lane of the loader warp per page (or half a page of 256 rows) issues that page's TMA boxes; boxes
 //     of which the item sees nothing take a page coordinate past the pool, which reads as zeros.  In the few tiles that
 //     the item's visible keys only cover in part, one warp ("fixer") then zeroes V's rows that no row of the item sees: a P of
@@ -101,12 +101,12 @@ struct Work {
     Seq seq;
     Span span;
     int s, head, tok0;          // first token of the item inside the call's tokens of the sequence
-    int sinks, first, tiles;    // its key tiles: those of the sinks, then those of the window
+    int sinks, first, tiles;    // its key tiles: those of the window, then those of the sinks
     int u0, n;                  // this CTA's part of them
     FV_DEV int pos0() const { return seq.len - seq.nq; }
     FV_DEV int key(int j) const {
         const int u = u0 + j;
-        return (u < sinks ? u : first + (u - sinks)) * kChunkTile;
+        return (u < tiles - sinks ? first + u : u - (tiles - sinks)) * kChunkTile;
     }
     FV_DEV bool sees(int j) const { return (j >= span.lo && j < span.hi) || j < span.sink; }
     FV_DEV bool whole(int k0) const { return (k0 >= span.lo && k0 + kChunkTile <= span.hi) || k0 + kChunkTile <= span.sink; }
@@ -328,86 +328,96 @@ FV_DEV void hide_columns(uint32_t (&u)[32], uint32_t seen) {
     for (int c = 0; c < 32; c++) u[c] = (seen & (1u << c)) ? u[c] : as_u(neg_inf());
 }
 
+template <bool F16>
+FV_DEV void unpack_p(uint32_t w, float& lo, float& hi) {
+    if (F16) {
+        asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(lo), "=f"(hi) : "r"(w));
+    } else {
+        lo = as_f(w << 16);
+        hi = as_f(w & 0xffff0000u);
+    }
+}
+// The reference of this lane's row moves for chunk c of the tile: to `below` the chunk's largest where there was none, else by a
+// whole power of two, so that the P stored already (chunks 0 .. c - 1) stay exact.  O, the sum and that P are rescaled.
+template <bool F16>
+FV_DEV void move_reference(uint32_t tS, uint32_t tO, int c, float cand, bool have_o, float& m, float& l) {
+    float a = 1.f;
+    if (cand > m + 7.f) {  // (32 columns above a quarter of the guard have one above 2^8)
+        const float want = cand - kChunkBelow<F16>;
+        if (m == neg_inf()) {
+            a = 0.f;
+            m = want;
+        } else {
+            const float k = ceilf(want - m);
+            a = ex2(-k);
+            m += k;
+        }
+        l *= a;
+    }
+    if (!__any_sync(kFullWarp, a != 1.f)) return;
+    auto rescale = [&](uint32_t at, bool packed) {
+        uint32_t o[32];
+        tmem_ld32_issue(at, o);
+        tmem_ld_wait();
+        tmem_pin(o);
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            float x = as_f(o[i]), y;
+            if (packed) {
+                unpack_p<F16>(o[i], x, y);
+                o[i] = pack_p<F16>(x * a, y * a);
+            } else {
+                o[i] = as_u(x * a);
+            }
+        }
+        tmem_st32(at, o);
+    };
+    if (have_o) {
+#pragma unroll 1
+        for (int q = 0; q < 4; q++) rescale(tO + 32u * q, false);
+    }
+    if (c > 0) {  // (16 columns a chunk; those behind them in the last 32 hold scores that are done with)
+        tmem_st_wait();
+#pragma unroll 1
+        for (int q = 0; 2 * q < c; q++) rescale(tS + 32u * q, true);
+    }
+}
+
 // A tile with invisible columns, or whose sum tripped the guard (out of line for the reasons that fvattn::careful_tile
-// gives).  Where every row has a reference already, or sees nothing of the tile, one pass as in the hot path, the invisible
-// columns as -inf; else, or when that pass trips the guard, exact maxima first, the reference moved, O and the sum rescaled.
+// gives).  In one pass of four chunks of 32 columns, the invisible ones as -inf: P of a chunk (16 columns) takes the place of scores
+// that have been read.  Where a row has no reference yet, or a chunk's sum is above a quarter of the guard (so that a tile that the hot path
+// gave up always moves its reference), the reference moves there.  (With a pass
+// for the maxima first: two sequences of 2 048 tokens, 32 heads on 8, 83 against 80 us, 4 bits 107 against 104.)
 template <bool F16>
 static __device__ __noinline__ void chunk_careful(uint32_t tS, uint32_t tO, uint32_t bt, Cols cols, float sl2, bool have_o, int lane,
                                                   RowState* rs) {
     float m = rs->m, l = rs->l;
-    // (bf16 only: in the 4-bit kernel, whose softmax threads have 184 registers, the longer function costs the loop around it more
-    // than the pass saves, 430 against 448 us for three ragged chunks.)
-    if (!F16 && __all_sync(kFullWarp, !cols.whole && (m != neg_inf() || (max(cols.lo, 0) >= cols.hi && cols.sink <= 0)))) {
-        const float ref = m == neg_inf() ? 0.f : -m;
-        const uint64_t s2 = pack_f32x2(sl2, sl2), nf = pack_f32x2(ref, ref);
-        uint64_t acc0 = pack_f32x2(0.f, 0.f), acc1 = acc0;
-        float top = 0.f;
-        uint32_t u[32], pw[64];
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const uint32_t seen = seen_bits(cols, 32 * c);
-            if (__any_sync(kFullWarp, seen != 0u)) {
+    const uint64_t s2 = pack_f32x2(sl2, sl2);
+#pragma unroll 1
+    for (int c = 0; c < 4; c++) {
+        uint32_t pw[16];
+        const uint32_t seen = seen_bits(cols, 32 * c);
+        if (__any_sync(kFullWarp, seen != 0u)) {
+            for (bool moved = false;; moved = true) {
+                uint32_t u[32];
                 fvattn::load_chunk(tS, c, u);
                 fvattn::land_chunk(u);
                 hide_columns(u, seen);
-                chunk_exp32<F16, false>(u, pw + 16 * c, s2, nf, acc0, acc1, top);
-            } else {
-#pragma unroll
-                for (int w = 0; w < 16; w++) pw[16 * c + w] = 0u;
+                const float noff = m == neg_inf() ? 0.f : -m;
+                const uint64_t nf = pack_f32x2(noff, noff);
+                uint64_t acc0 = pack_f32x2(0.f, 0.f), acc1 = acc0;
+                float top = 0.f;
+                const bool none = __any_sync(kFullWarp, m == neg_inf() && seen != 0u);
+                if (moved || !none) {
+                    chunk_exp32<F16, false>(u, pw, s2, nf, acc0, acc1, top);
+                    const float sum = fvattn::part_sum<false>(acc0, acc1, top);
+                    if (moved || !__any_sync(kFullWarp, !(sum <= 0.25f * kChunkGuard<F16>))) {
+                        l += sum;
+                        break;
+                    }
+                }
+                move_reference<F16>(tS, tO, c, fvattn::max32(u) * sl2, have_o, m, l);
             }
-        }
-        const float sum = fvattn::part_sum<false>(acc0, acc1, top);
-        if (!__any_sync(kFullWarp, !(sum <= kChunkGuard<F16>))) {
-            fvattn::store_early(tS, pw);
-            fvattn::publish(bt + Smem::p_ready, lane);
-            rs->l = l + sum;
-            return;
-        }
-    }
-    float mx = neg_inf();
-#pragma unroll 1
-    for (int c = 0; c < 4; c++) {
-        const uint32_t seen = seen_bits(cols, 32 * c);
-        if (!__any_sync(kFullWarp, seen != 0u)) continue;
-        uint32_t u[32];
-        fvattn::load_chunk(tS, c, u);
-        fvattn::land_chunk(u);
-        hide_columns(u, seen);
-        mx = fmaxf(mx, fvattn::max32(u));
-    }
-    const float cand = mx * sl2;
-    float a = 1.f;
-    if (cand > m + 8.f) {
-        a = ex2(m - (cand - kChunkBelow<F16>));
-        m = cand - kChunkBelow<F16>;
-        l *= a;
-    }
-    if (have_o && __any_sync(kFullWarp, a != 1.f)) {
-#pragma unroll 1
-        for (int q = 0; q < 4; q++) {
-            uint32_t o[32];
-            tmem_ld32_issue(tO + 32u * q, o);
-            tmem_ld_wait();
-            tmem_pin(o);
-#pragma unroll
-            for (int c = 0; c < 32; c++) o[c] = as_u(as_f(o[c]) * a);
-            tmem_st32(tO + 32u * q, o);
-        }
-    }
-    const float noff = (m == neg_inf()) ? 0.f : -m;
-    const uint64_t s2 = pack_f32x2(sl2, sl2), nf = pack_f32x2(noff, noff);
-#pragma unroll 1
-    for (int c = 0; c < 4; c++) {
-        uint32_t u[32], pw[16];
-        const uint32_t seen = seen_bits(cols, 32 * c);
-        if (__any_sync(kFullWarp, seen != 0u)) {
-            fvattn::load_chunk(tS, c, u);
-            fvattn::land_chunk(u);
-            hide_columns(u, seen);
-            uint64_t acc0 = pack_f32x2(0.f, 0.f), acc1 = acc0;
-            float top = 0.f;
-            chunk_exp32<F16, false>(u, pw, s2, nf, acc0, acc1, top);
-            l += fvattn::part_sum<false>(acc0, acc1, top);
         } else {
 #pragma unroll
             for (int w = 0; w < 16; w++) pw[w] = 0u;
