@@ -232,9 +232,9 @@ FV_DEV uint32_t lds32(uint32_t a) {
 // A warp takes a run of tiles of its own.  Their pool rows are looked up 32 at a time, one tile a lane, a batch ahead.
 // bf16, bound by HBM: a tile's K registers are loaded anew as soon as its scores are done and V's as soon as its product is, so
 // that memory is always being read while the warp computes, straight into registers: 32 ragged sequences of up to 9 001 keys, 32
-// heads on 8, 140 us = 5.97 TB/s, 0.91 of the measured copy bandwidth; 6 windows of 8 190 keys, 40 heads on 8, 36 us = 5.6 TB/s.
+// heads on 8, 137 us = 6.10 TB/s, 0.93 of the measured copy bandwidth; 6 windows of 8 190 keys, 40 heads on 8, 34.5 us = 5.8 TB/s.
 // 4 bits, bound by the logic pipe: 32 keys are 4.3 KB, so a ring in shared memory runs three stages ahead: 32 sequences of up to
-// 20 011 keys 116 us = 4.3 TB/s (loads into registers: 173).  Three CTAs an SM: with a fourth the registers no longer suffice,
+// 20 011 keys 110 us = 4.5 TB/s (loads into registers: 173).  Three CTAs an SM: with a fourth the registers no longer suffice,
 // 128 against 123 us.  At most four rows stand on every other column of the products, which leaves half of the softmax: 123 -> 116 us.
 template <bool Q4, int ROWS>
 __global__ void __launch_bounds__(kAttnThreads, ROWS <= 8 ? 3 : 2) fv_paged_decode_kernel(const AttnArgs a) {

@@ -22,9 +22,9 @@
 //     f16's range is the price: values beyond 65 504 saturate, below 2^-14 they lose relative precision.  Against that,
 //     P's reference is set 2^6 below the maximum that it is taken from: P up to 2^15 fits, and P is zero only 2^30 below it.
 // Bound by the tensor pipe and by what feeds it (128 x 128 x 16 products from shared memory take all of its bandwidth): 4 680 rows x
-// 12 heads over 28 080 bf16 keys 722 us under the profiler = 1 119 TFLOP/s, tensor pipe 62 % of the active cycles (787-840 us in a
-// loop at the power cap); three ragged chunks of up to 1 501 tokens, 40 heads on 8, windows of 4 100 keys (35 tiles an item, five of
-// them cut by the mask) 345 us with bf16 pages, 51 %, and 405 us with 4-bit pages, 43 %.
+// 12 heads over 28 080 bf16 keys 710 us under the profiler = 1 137 TFLOP/s, tensor pipe 62 % of the active cycles (690-830 us in a
+// loop, at the power cap); three ragged chunks of up to 1 501 tokens, 40 heads on 8, windows of 4 100 keys (35 tiles an item, five of
+// them cut by the mask) 326 us with bf16 pages, 56 %, and 394 us with 4-bit pages, 46 %.
 #pragma once
 #include "attn_fwd.cuh"
 #include "paged.cuh"

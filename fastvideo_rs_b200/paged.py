@@ -229,7 +229,8 @@ def read(kv: PagedKv, batch: PagedBatch, *, rows: int, cu_rows: Optional[torch.T
     cu = batch.cu_q if cu_rows is None else _index("read: cu_rows", cu_rows, (batch.seqs + 1,), kv.device)
     if first is not None:
         _index("read: first", first, (batch.seqs,), kv.device)
-    k, v = (kv.k if kv.k_scale is None else kv.k_scale).new_empty((2, rows, kv.kv_heads, D)).unbind(0)  # (either is bf16)
+    k = (kv.k if kv.k_scale is None else kv.k_scale).new_empty((rows, kv.kv_heads, D))  # (either is bf16)
+    v = torch.empty_like(k)  # (cheaper than two views of one tensor)
     if rows == 0:
         return k, v
     if batch.seqs == 0:
