@@ -603,15 +603,20 @@ __global__ void __launch_bounds__(kAttnThreads, ROWS <= 8 ? 3 : 2) fv_paged_deco
 #pragma unroll
             for (int n = 0; n < NT; n++) {
 #pragma unroll
-                for (int e = 0; e < EH; e++) {
-                    l[n][e] += p[i][n][e] + p[i][n][2 + e];
-                    if constexpr (Q4) {
-                        const float z0 = fmaf(-8.f, vt[i].step(0), hi_f(vt[i].s0)), z1 = fmaf(-8.f, vt[i].step(1), hi_f(vt[i].s1));
-                        z[n][e] = fmaf(p[i][n][e], z0, fmaf(p[i][n][2 + e], z1, z[n][e]));
-                    }
+                for (int e = 0; e < EH; e++) l[n][e] += p[i][n][e] + p[i][n][2 + e];
+                const uint32_t pk0 = pack_p<Q4>(ps[i][n][0], ps[i][n][1]), pk1 = pack_p<Q4>(ps[i][n][2], ps[i][n][3]);
+                if constexpr (Q4) {
+                    // P zero - 8 (P step), the latter as the product takes it: its rounding then meets the code, not the 8 as well
+                    // (which could be a hundred times the value).
+                    float r[4];
+                    unpack_p<true>(pk0, r[0], r[1]);
+                    unpack_p<true>(pk1, r[2], r[3]);
+#pragma unroll
+                    for (int e = 0; e < EH; e++)
+                        z[n][e] = fmaf(-8.f, r[e] + r[2 + e], fmaf(p[i][n][e], hi_f(vt[i].s0), fmaf(p[i][n][2 + e], hi_f(vt[i].s1), z[n][e])));
                 }
-                pb[n][0] = transpose8(pack_p<Q4>(ps[i][n][0], ps[i][n][1]));
-                pb[n][1] = transpose8(pack_p<Q4>(ps[i][n][2], ps[i][n][3]));
+                pb[n][0] = transpose8(pk0);
+                pb[n][1] = transpose8(pk1);
             }
             // O^T += V^T . P^T: the pair of one d and two neighbouring keys comes out of two keys' words.
             if constexpr (Q4) {

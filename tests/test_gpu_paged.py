@@ -143,6 +143,17 @@ def test_large_scores_move_the_reference(fvlib, kernel, fmt, nq, heads):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+def test_small_values_of_few_keys(fvlib, kernel, fmt):
+    """Two and three keys: here single values near zero meet weights of one half, and nothing averages an error out."""
+    from fastvideo_rs_b200 import paged
+    for seed in range(40):
+        case = Case(fmt, [15, 2, 3, 3], [15, 2, 3, 3], 8, 1, 64, seed=1000 + seed)
+        kv, batch, q = case.device()
+        want, bound = case.expect(None)
+        check(paged.attend(kv, batch, q), want, bound, f"{fmt} {seed}")
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("nq", [3, 150])
 def test_rows_before_the_sequence_are_zero(fvlib, kernel, fmt, nq):
     """More new tokens than the sequence holds: the first rows have no position and see nothing."""
