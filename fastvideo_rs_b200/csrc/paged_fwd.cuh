@@ -297,7 +297,8 @@ constexpr float kChunkGuard = F16 ? 32768.f : fvattn::kGuard;
 // A reference is set 2^this below the maximum that it is taken from.
 template <bool F16>
 constexpr float kChunkBelow = F16 ? 6.f : 0.f;
-// As fvattn::exp32: 2^(u sl2 + noff) of 32 columns to packed pairs, every fourth pair on the FMA pipe (POLY).
+// As fvattn::exp32: 2^(u sl2 + noff) of 32 columns to packed pairs, every fourth pair on the FMA pipe (POLY: bf16 pages; with 4-bit
+// ones the expander wants the issue slots that this takes, three ragged chunks 388 with and 377 us without).
 template <bool F16, bool POLY>
 FV_DEV void chunk_exp32(const uint32_t (&u)[32], uint32_t* pw, uint64_t s2, uint64_t nf, uint64_t& acc0, uint64_t& acc1, float& top) {
 #pragma unroll
@@ -513,16 +514,16 @@ FV_DEV void chunk_softmax(const ChunkJob& jb, const Run& run, uint32_t sbase, ui
                 uint64_t acc0 = pack_f32x2(0.f, 0.f), acc1 = acc0;
                 float top = 0.f;
                 fvattn::load_chunk(tS, 1, u1);
-                chunk_exp32<Q4, true>(u0, pw, s2, nf, acc0, acc1, top);
+                chunk_exp32<Q4, !Q4>(u0, pw, s2, nf, acc0, acc1, top);
                 fvattn::land_chunk(u1);
                 fvattn::load_chunk(tS, 2, u0);
-                chunk_exp32<Q4, true>(u1, pw + 16, s2, nf, acc0, acc1, top);
+                chunk_exp32<Q4, !Q4>(u1, pw + 16, s2, nf, acc0, acc1, top);
                 fvattn::land_chunk(u0);
                 fvattn::load_chunk(tS, 3, u1);
-                chunk_exp32<Q4, true>(u0, pw + 32, s2, nf, acc0, acc1, top);
+                chunk_exp32<Q4, !Q4>(u0, pw + 32, s2, nf, acc0, acc1, top);
                 fvattn::land_chunk(u1);
-                chunk_exp32<Q4, true>(u1, pw + 48, s2, nf, acc0, acc1, top);
-                const float sum = fvattn::part_sum<true>(acc0, acc1, top);
+                chunk_exp32<Q4, !Q4>(u1, pw + 48, s2, nf, acc0, acc1, top);
+                const float sum = fvattn::part_sum<!Q4>(acc0, acc1, top);
                 if (__any_sync(kFullWarp, live && !(sum <= kChunkGuard<Q4>))) {
                     hot = false;  // nothing of this tile is stored
                 } else {
