@@ -24,7 +24,7 @@
 // Bound by the tensor pipe and by what feeds it (128 x 128 x 16 products from shared memory take all of its bandwidth): 4 680 rows x
 // 12 heads over 28 080 bf16 keys 710 us under the profiler = 1 137 TFLOP/s, tensor pipe 62 % of the active cycles (690-830 us in a
 // loop, at the power cap); three ragged chunks of up to 1 501 tokens, 40 heads on 8, windows of 4 100 keys (35 tiles an item, five of
-// them cut by the mask) 326 us with bf16 pages, 56 %, and 394 us with 4-bit pages, 46 %.
+// them cut by the mask) 326 us with bf16 pages, 56 %, and 392 us with 4-bit pages, 46 %.
 #pragma once
 #include "attn_fwd.cuh"
 #include "paged.cuh"
