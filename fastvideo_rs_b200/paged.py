@@ -121,7 +121,7 @@ class PagedBatch:
         if not 0 <= max_q < 1 << 30 or not 0 <= max_kv < 1 << 30:
             raise ValueError("PagedBatch: max_q and max_kv must be 0 .. 2^30 - 1")
         self.seqs, self.max_q, self.max_kv, self.device, self.index = seqs, int(max_q), int(max_kv), dev, page_table.get_device()
-        self._need = {}  # scratch bytes by the call's shape: a step asks for every layer
+        self._need = {}  # scratch bytes by the call's shape: a step asks for every layer (FV_PAGED_KERNEL is set before the first)
         self._c = _BatchC(page_table.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), seqs, width, self.max_q, self.max_kv)
         self._ref = ctypes.addressof(self._c)
 
