@@ -98,7 +98,23 @@ class WanSelfAttention:
                  theta: float = 10000.0, causal: Optional[BlockCausal] = None, device="cuda", vsa=None):
         self.grid, self.heads, self.eps, self.causal, self.vsa = tuple(grid), heads, eps, causal, vsa
         self.wq, self.wk = wq, wk
+        self.theta = theta
         self.cos, self.sin = wan_rope_tables(grid, 128, theta, 0, device)
+        self._longer = []  # forward_paged: the same tables over more frames, the longest last
+
+    def _tables(self, rows: int):
+        """cos, sin of at least `rows` positions: the grid's, or, beyond them, the same rows followed by those of later frames.  Each
+        time they grow they at least double, and the shorter ones stay: a captured call reads the tables that it was captured with."""
+        have = self._longer[-1] if self._longer and self.cos.shape[0] < rows else (self.cos, self.sin)
+        if rows > have[0].shape[0]:
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                raise ValueError(f"forward_paged: the rotation tables hold {have[0].shape[0]} positions, the batch's max_kv is {rows}; they "
+                                 "cannot grow while a graph is captured: make one call with these bounds before the capture")
+            frame = self.grid[1] * self.grid[2]
+            frames = max(-(-rows // frame), 2 * have[0].shape[0] // frame)
+            have = wan_rope_tables((frames, *self.grid[1:]), 128, self.theta, 0, self.cos.device)
+            self._longer.append(have)
+        return have
 
     def forward_self(self, qkv: torch.Tensor, scale: Optional[float] = None, gate: Optional[torch.Tensor] = None,
                      merged: bool = False) -> torch.Tensor:
@@ -124,12 +140,17 @@ class WanSelfAttention:
         rotated with the table rows of their positions in their sequences (or of `positions`, int32 [tokens]) while K and V
         are appended, and the queries attend to the cache under this layer's block-causal mask (all keys without one).
         Returns [tokens, heads, 128], the merged heads of every token.  (q and k are rounded to bf16 between norm and
-        rotation, which forward_self is not.)"""
+        rotation, which forward_self is not.)
+
+        Where batch.max_kv passes the grid, the layer makes longer tables (1 KB a position), before a capture if there is one.  With
+        `positions` it does not: they are rows of the grid's tables, and one outside of them is reported by device_status (202) and
+        neither stored nor rotated."""
         from . import paged
         if qkv.dim() != 3 or qkv.shape[0] != 1:
             raise ValueError("forward_paged: qkv must be [1, tokens, 3 * dim], the sequences packed")
+        cos, sin = self._tables(batch.max_kv if positions is None else 0)
         q, k, v = (t[0].transpose(0, 1) for t in qk_prep(qkv, self.wq, self.wk, None, None, self.heads, eps=self.eps))
-        q = paged.append(kv, batch, k, v, q=q, cos=self.cos, sin=self.sin, positions=positions)
+        q = paged.append(kv, batch, k, v, q=q, cos=cos, sin=sin, positions=positions)
         return paged.attend(kv, batch, q, self.causal, scale=scale)
 
     def attend_vsa(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, gate_proj: torch.Tensor) -> torch.Tensor:
