@@ -138,7 +138,8 @@ class WanSelfAttention:
         """forward_self over a paged K/V cache (paged.PagedKv, paged.PagedBatch), for streaming rollouts of any number and length:
         qkv [1, tokens, 3 * dim] bf16 holds the batch's tokens packed one sequence after the other.  q and k are normalised,
         rotated with the table rows of their positions in their sequences (or of `positions`, int32 [tokens]) while K and V
-        are appended, and the queries attend to the cache under this layer's block-causal mask (all keys without one).
+        are appended, and the queries attend to the cache under this layer's block-causal mask (all keys without one; a layer with a VSA
+        context is refused).
         Returns [tokens, heads, 128], the merged heads of every token.  (q and k are rounded to bf16 between norm and
         rotation, which forward_self is not.)
 
@@ -146,6 +147,8 @@ class WanSelfAttention:
         `positions` it does not: they are rows of the grid's tables, and one outside of them is reported by device_status (202) and
         neither stored nor rotated."""
         from . import paged
+        if self.vsa is not None:
+            raise ValueError("forward_paged: no VSA route over pages (its tiles are those of the whole grid); use forward_self")
         if qkv.dim() != 3 or qkv.shape[0] != 1:
             raise ValueError("forward_paged: qkv must be [1, tokens, 3 * dim], the sequences packed")
         cos, sin = self._tables(batch.max_kv if positions is None else 0)

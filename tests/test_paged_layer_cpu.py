@@ -1,4 +1,4 @@
-"""WanSelfAttention.forward_paged without a device: its rotation tables."""
+"""WanSelfAttention.forward_paged without a device: its rotation tables and what it refuses."""
 import pytest
 import torch
 
@@ -21,3 +21,12 @@ def test_tables_go_on_behind_the_grid(fvlib):
         kept.append(cos)
     assert kept[0] is kept[1] and kept[3] is kept[4] and kept[5] is layer.cos  # (once made they stay)
     assert len(layer._longer) == 3 and len(layer.cos) == 40
+
+
+def test_a_layer_with_a_vsa_context_is_refused(fvlib):
+    """forward_self takes the VSA route there; dense attention in its place would be another result without a word."""
+    from fastvideo_rs_b200 import wan
+    w = torch.ones(2 * 128)
+    layer = wan.WanSelfAttention((2, 4, 5), 2, w, w, device="cpu", vsa=object())
+    with pytest.raises(ValueError, match="VSA"):
+        layer.forward_paged(torch.zeros(1, 4, 768, dtype=torch.bfloat16), None, None)
