@@ -6,8 +6,11 @@
 // token's row of its sequence's page, in bf16 or in 4 bits; q goes to a packed tensor.  Rotation arithmetic is that of the
 // BHSD rope kernel: f32, products and sums rounded separately, one rounding to bf16.  4 bits, per row of 128 values x:
 //     step = bf16((max x - min x) / 15), zero = bf16(min x + 8 step), code = clamp(rint((x - zero) / step), -8, 7),
-// stored as code + 8 (even value in the low half of a byte): a row stands for zero + step * code.  K is quantised from
-// the f32 rotation, not from its bf16 rounding.  One scale for the whole row because its factor then leaves the
+// stored as code + 8 (even value in the low half of a byte): a row stands for zero + step * code.  Where zero's rounding moved it by
+// more than a quarter of a step (an offset of some 64 steps and more), step is the smallest bf16 whose codes still span the row:
+//     step = max((max x - zero) / 7, (zero - min x) / 8), rounded up.
+// So no value is more than half a step off: at the ends the codes fall short by a quarter of a step and 15 times step's rounding,
+// 0.31 of it, or by nothing.  K is quantised from the f32 rotation, not from its bf16 rounding.  One scale for the whole row because its factor then leaves the
 // attention's products (q . k = step (q . code) + zero sum(q)), so that these run on exact codes.
 //
 // HBM-bound: 8 lanes hold one row of one head (16 values a lane), a warp the same head of 4 neighbouring tokens, a CTA
@@ -125,7 +128,7 @@ static __device__ __noinline__ uint32_t settle4(float a, float b, float c4, floa
     return w;
 }
 // The same row in 4 bits: codes of this lane's 16 values as two words (8 values each), (step, zero) as one.  Collective
-// over the warp.  (A row of one value has step 0 and codes 0.  A row with a value that is not finite has a step that is
+// over the warp.  (A row of one bf16 value has step 0 and codes 0.  A row with a value that is not finite has a step that is
 // not: its codes say nothing, the row stands for NaN.)
 FV_DEV void quantize16(const float (&x)[16], uint32_t& lo, uint32_t& hi, uint32_t& scale) {
     float mn = min_nan(x[0], x[1], x[2]), mx = max_nan(x[0], x[1], x[2]);
@@ -142,8 +145,12 @@ FV_DEV void quantize16(const float (&x)[16], uint32_t& lo, uint32_t& hi, uint32_
         mn = min_nan(mn, a, a);
         mx = max_nan(mx, b, b);
     }
-    const float step = bf16_of(__fdiv_rn(__fsub_rn(mx, mn), 15.f));
-    const float zero = bf16_of(__fadd_rn(mn, __fmul_rn(8.f, step)));
+    float step = bf16_of(__fdiv_rn(__fsub_rn(mx, mn), 15.f));
+    const float mid = __fadd_rn(mn, __fmul_rn(8.f, step)), zero = bf16_of(mid);
+    if (fabsf(zero - mid) > 0.25f * step) {
+        const float wide = fmaxf(__fdiv_rn(__fsub_rn(mx, zero), 7.f), 0.125f * __fsub_rn(zero, mn));
+        step = __uint_as_float((__float_as_uint(wide) + 0xffffu) & 0xffff0000u);  // up to the next bf16
+    }
     scale = fvp::pack_bf16x2(step, zero);
     lo = hi = 0x88888888u;
     if (!(step > 0.f)) return;

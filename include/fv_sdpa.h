@@ -290,7 +290,9 @@ FV_API int fv_sdpa_window_bf16(void* stream, const void* q, const void* k_cache,
  *   FV_ROPE_INTERLEAVED (values 2 i, 2 i + 1; each factor stored twice, as fv_wan_rope_tables writes them) or FV_ROPE_HALF
  *   (values i, i + 64; factors i and i + 64 equal).  K, rotated, and V go to the tokens' rows in the pages; q, rotated, to
  *   q_out [tokens, q_heads, 128].  f32 arithmetic, products and sums rounded separately, one rounding to bf16 (or from f32
- *   to 4 bits: step = bf16((max - min) / 15), zero = bf16(min + 8 step), code = clamp(rint((x - zero) / step), -8, 7)).
+ *   to 4 bits: step = bf16((max - min) / 15), zero = bf16(min + 8 step), code = clamp(rint((x - zero) / step), -8, 7); where
+ *   |zero - (min + 8 step)| > step / 4, step = max((max - zero) / 7, (zero - min) / 8) rounded up to bf16.  A value is at most
+ *   half a step off, which for rows with an offset far above their range is a share of zero's rounding, 2^-8 |x| / 14, not of the range).
  *   Tokens before the start of their sequence (nq > kv_len) are stored nowhere and their q_out is zero.  Two tokens of one
  *   call must not fall on the same row.
  * fv_paged_read_bf16: rows first[s] .. first[s] + (cu_rows[s + 1] - cu_rows[s]) of each sequence as packed

@@ -86,3 +86,65 @@ def test_longer_tables_are_not_made_while_a_graph_is_captured(fvlib):
         got = layer_ready.forward_paged(qkv, kv, batch)
     graph.replay()
     assert torch.equal(got, want)
+
+
+# ---- the 4-bit format -------------------------------------------------------------------------------------------------
+
+def quantize_rows(x):
+    """(codes 0..15 uint8, (step, zero) bf16) of f32 rows, with the step widened where the rounding of zero asks for it."""
+    lo, hi = x.amin(-1), x.amax(-1)
+    step = ((hi - lo) / torch.full_like(hi, 15.0)).to(torch.bfloat16).float()
+    mid = lo + 8.0 * step
+    zero = mid.to(torch.bfloat16).float()
+    wide = torch.maximum((hi - zero) / torch.full_like(hi, 7.0), (zero - lo) * 0.125)
+    wide = ((wide.view(torch.int32) + 0xffff) & -65536).view(torch.float32)  # up to the next bf16
+    step = torch.where((zero - mid).abs() > 0.25 * step, wide, step)
+    c = torch.round((x - zero[..., None]) / step[..., None]).clamp(-8, 7)
+    c = torch.where(step[..., None] > 0, c, torch.zeros_like(c))
+    return (c + 8).to(torch.uint8), torch.stack([step, zero], -1).to(torch.bfloat16)
+
+
+def _offset_rows():
+    g = torch.Generator().manual_seed(30)
+    rows = [torch.tensor([1000.0, 1004.0] * 64), torch.tensor([1000.0, 1004.0, 1008.0, 1000.0] * 32),
+            torch.tensor([-1000.0] * 127 + [-996.0]), torch.full((D,), 1000.0), torch.zeros(D), torch.tensor([256.0, 258.0] * 64)]
+    for _ in range(500):  # an offset of up to 2^14 ranges, either sign
+        span, off = 2.0 ** float(torch.rand((), generator=g) * 20 - 10), 2.0 ** float(torch.rand((), generator=g) * 14)
+        rows.append(span * (torch.randn(D, generator=g) + (off if len(rows) % 2 else -off)))
+    for _ in range(100):
+        rows.append(torch.randn(D, generator=g))
+    return torch.stack(rows).to(torch.bfloat16)
+
+
+def test_four_bit_rows_with_an_offset_read_back_within_half_a_step(fvlib):
+    """The codes span the row whatever its offset is: no value is more than half a step off, and the step is no larger than the
+    range and the roundings of zero and step make it."""
+    from fastvideo_rs_b200 import paged
+    x = _offset_rows()
+    n = len(x)
+    kv = paged.PagedKv.empty((n + 15) // 16, 16, 1, "q4")
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    batch = paged.PagedBatch(torch.arange((n + 15) // 16, dtype=torch.int32, device="cuda")[None], i32(n), i32(0, n), max_q=n, max_kv=n)
+    # K through a rotation whose f32 results are no bf16 values, V as it is
+    turn = torch.linspace(0, 3, n)[:, None] * torch.ones(D)
+    cos, sin = turn.cos(), turn.sin()
+    paged.append(kv, batch, x.cuda()[:, None], x.cuda()[:, None], cos=cos.cuda(), sin=sin.cuda())
+    turned = torch.empty(n, D)
+    xf = x.float()
+    turned[:, 0::2] = xf[:, 0::2] * cos[:, 0::2] - xf[:, 1::2] * sin[:, 0::2]
+    turned[:, 1::2] = xf[:, 0::2] * sin[:, 0::2] + xf[:, 1::2] * cos[:, 0::2]
+    for name, rows in (("v", xf), ("k", turned)):
+        codes = unpack(getattr(kv, name).cpu()[:, 0].flatten(0, 1)[:n])
+        scale = getattr(kv, name + "_scale").cpu()[:, 0].flatten(0, 1)[:n]
+        want_codes, want_scale = quantize_rows(rows)
+        assert torch.equal(scale, want_scale) and torch.equal(codes, want_codes), name
+        step, zero = scale[:, :1].double(), scale[:, 1:].double()
+        r = rows.double()
+        off = (zero + step * (codes.double() - 8.0) - r).abs()
+        # half a step; f32: the subtraction of zero 2^-24 of the difference, the quotient 2^-24 of up to 8 steps
+        assert bool((off <= step * (0.5 + 2.0 ** -19)).all()), (name, float((off / step.clamp(min=1e-30)).max()))
+        span, most = r.amax(-1) - r.amin(-1), r.abs().amax(-1)
+        # (zero is 2^-8 of at most max |x| + a step off; step is rounded once, or up: 2^-7; three f32 roundings)
+        assert bool((step[:, 0] <= (1 + 2.0 ** -6) * (span / 15 + BF16_HALF * (most + span / 15) / 7) + 1e-30).all()), name
+    k, v = paged.read(kv, batch, rows=n)
+    assert torch.isfinite(k).all() and torch.isfinite(v).all()
