@@ -19,7 +19,10 @@
 //   * 4-bit pages: the loader brings the packed codes by bulk copies, four more warps expand them to f16 into the swizzled
 //     tiles that TMA would have written, and bring Q as f16.  Both products then run in f16: a value zero + step code is rounded
 //     once, by 2^-11 at most (in bf16 the roundings of K and V, 2^-8 each, would be of the size of the output's own), P by 2^-11.
-//     f16's range is the price: values beyond 65 504 saturate, below 2^-14 they lose relative precision.  Against that,
+//     f16's range stays out of it: K and V of an item and every row of q are brought to the upper end of f16 by powers of two,
+//     which go into the row's softmax scale and the output's.  Two warps survey the scales of an item's keys while the item before is
+//     at work.  Values down to 2^-26 of the largest of their item keep their 11 bits.  (A factor a tile instead, worked out when its
+//     scales come: 400 -> 436 us for three ragged chunks, most of it a wait and a load a tile in the softmax.)
 //     P's reference is set 2^6 below the maximum that it is taken from: P up to 2^15 fits, and P is zero only 2^30 below it.
 // Bound by the tensor pipe and by what feeds it (128 x 128 x 16 products from shared memory take all of its bandwidth): 4 680 rows x
 // 12 heads over 28 080 bf16 keys 710 us under the profiler = 1 137 TFLOP/s, tensor pipe 62 % of the active cycles (690-830 us in a
@@ -79,10 +82,15 @@ using namespace fvp;
 // their barriers and scales come last.
 constexpr uint32_t kVFixed = Smem::total;
 constexpr uint32_t kCodeFull = kVFixed + 8 * fvattn::kKvPairs, kCodeFree = kCodeFull + 16;
-constexpr uint32_t kScales = (kCodeFree + 16 + 15) & ~15u;      // [stage][V | K][128 keys] (step, zero)
-constexpr uint32_t kRun = kScales + 2 * 1024;  // this CTA's run
-constexpr uint32_t kScratch = kRun + 128;     // find_run's
-constexpr uint32_t kChunkSmem = kScratch + 256;
+// Of item i, in slot i & 1: K's and V's sizes are there; the rows' sizes are too; all of them have been read.
+constexpr uint32_t kSurveyed = kCodeFree + 16, kItemReady = kSurveyed + 16, kItemFree = kItemReady + 16;
+constexpr uint32_t kFirstDone = kItemFree + 16, kFirstTop = kFirstDone + 16;  // [K | V]: the softmax warps' share of a run's first survey
+constexpr uint32_t kSizes = (kFirstTop + 8 + 15) & ~15u;         // [item & 1][K | V]: Size
+constexpr uint32_t kScales = kSizes + 32;                        // [stage][V | K][128 keys] (step, zero)
+constexpr uint32_t kRowSizes = kScales + 2 * 1024;               // [item & 1][row tile][128 rows] exponents, a byte each
+constexpr uint32_t kScratch = kRowSizes;                         // find_run's, before there are any
+constexpr uint32_t kRun = kRowSizes + 4 * kChunkRows;            // this CTA's run
+constexpr uint32_t kChunkSmem = kRun + 64;
 constexpr uint32_t kCodes = Smem::q + 2 * fvattn::kSlotBytes;   // [stage][V | K][128 keys][64 bytes]
 static_assert(kVFixed % 8 == 0 && kChunkSmem <= 232448 && fvattn::kQSlots == 3 && fvattn::kSlotBytes == 32768, "shared memory");
 static_assert(fvattn::kKvPairs == 2 && fvattn::kEarlyKeys == 128, "the ring in pairs, P handed over whole");
@@ -92,6 +100,7 @@ struct Roles {
     static constexpr int kWarps = Q4 ? 16 : 12;
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kLoader = 8, kIssuer = 9, kFixer = 10;  // (fixer: bf16)
+    static constexpr int kSurveyor = 10;                         // 4 bits: warps 10 (K) and 11 (V)
     static constexpr int kExpander = 12, kExpanders = 4;         // 4 bits: warps 12-15, one on each of the SM's schedulers
     static constexpr uint32_t kQ = Q4 ? 2 : fvattn::kQSlots;     // Q slots
 };
@@ -139,6 +148,7 @@ struct Run {
     } start[kMaxPhases];
     FV_DEV long long edge(int v) const { return total * v / runs; }
 };
+static_assert(sizeof(Run) <= 64 && kRun % 8 == 0, "shared memory");
 // Warp-inclusive sum.
 FV_DEV long long scan_warp(long long x, int lane) {
 #pragma unroll
@@ -279,6 +289,98 @@ FV_DEV void chunk_output(uint32_t tO, uint32_t tP, uint64_t vd, bool fresh) {
         "}"
         ::"r"(tO), "r"(tP), "l"(vd), "r"(idesc), "r"(fresh ? 1u : 0u)
         : "memory");
+}
+
+// ---------------------------------------------------------------------------------------- sizes (4-bit pages)
+// The power of two that numbers of which the largest has the biased exponent e are divided by for f16: what is left is below 2^13, values
+// zero + step code (twice the larger of |zero| and 8 |step| at most) below 2^14.  Limited so that the factors stay normal numbers.
+FV_DEV int size_of(int e) { return min(max(e, 24), 250) - 139; }
+FV_DEV float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
+FV_DEV int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23); }  // x >= 0
+// The larger magnitudes of two pairs of bf16 (their signs mean nothing; a NaN gives way to a number).
+FV_DEV uint32_t larger_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+FV_DEV uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+FV_DEV uint32_t twice_bf16(int e) { return 0x00010001u * ((uint32_t)(127 + e) << 7); }  // 2^e, two of it
+
+// A survey: the largest |zero| or 8 |step| of the keys that an item sees, of K or V, as the bits of an f32.  Tiles first, first + stride, ..;
+// all of a warp, and each lane gets the result.  Pages are looked up a box a lane, for up to 32 boxes at a time; of a tile's scales
+// a lane holds four keys, four tiles are in flight (eight: more code in all, 404 -> 412 us for three ragged chunks).
+FV_DEV uint32_t survey(const ChunkJob& jb, const Work& w, int which, int first, int stride, int lane) {
+    constexpr int kAhead = 4;
+    constexpr uint32_t kNone = 0xffffffffu;
+    const uint32_t* scales = which ? jb.pool.v_scale : jb.pool.k_scale;
+    const int log_box = min(jb.pool.log_rows, 7), log_boxes = 7 - log_box, per = 32 >> log_boxes;  // boxes of a tile, tiles of a look-up
+    const int tiles = (w.n - first + stride - 1) / stride;                                        // (of this warp; may be less than one)
+    uint32_t top_step = 0, top_zero = 0;
+#pragma unroll 1
+    for (int j0 = 0; j0 < tiles; j0 += per) {
+        uint32_t row = kNone;
+        if (j0 + (lane >> log_boxes) < tiles) {
+            const int a = w.key(first + stride * (j0 + (lane >> log_boxes))) + ((lane << log_box) & (kChunkTile - 1)), b = a + (1 << log_box);
+            if ((a < w.span.hi && b > w.span.lo) || a < w.span.sink) {
+                const int page = page_of(jb.pool, jb.batch, w.s, a);
+                if (page >= 0) row = (uint32_t)pool_row(jb.pool, page, w.head, a);
+            }
+        }
+        const int end = min(per, tiles - j0);
+#pragma unroll 1
+        for (int t0 = 0; t0 < end; t0 += kAhead) {
+            uint4 x[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) {
+                const uint32_t r = __shfl_sync(fvpg::kFullWarp, row, ((t0 + i) << log_boxes) + ((4 * lane) >> log_box));
+                x[i] = make_uint4(0, 0, 0, 0);
+                if (t0 + i < end && r != kNone) x[i] = __ldg(reinterpret_cast<const uint4*>(scales + r + ((4 * lane) & ((1 << log_box) - 1))));
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) {
+                const int key = t0 + i < end ? w.key(first + stride * (j0 + t0 + i)) : 0;
+                if (!w.whole(key)) {
+                    if (!w.sees(key + 4 * lane)) x[i].x = 0;
+                    if (!w.sees(key + 4 * lane + 1)) x[i].y = 0;
+                    if (!w.sees(key + 4 * lane + 2)) x[i].z = 0;
+                    if (!w.sees(key + 4 * lane + 3)) x[i].w = 0;
+                }
+                const uint32_t pair[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t step = pair[k] << 17, zero = pair[k] & 0x7fff0000u;  // (step: a bit further up)
+                    if (step < 0xff000000u && zero < 0x7f800000u) {                     // (a row that is not finite has no say)
+                        top_step = max(top_step, step);
+                        top_zero = max(top_zero, zero);
+                    }
+                }
+            }
+        }
+    }
+    const float top = fmaxf(8.f * __uint_as_float(top_step >> 1), __uint_as_float(top_zero));
+    return __reduce_max_sync(fvpg::kFullWarp, __float_as_uint(top));
+}
+// A run's first item has nothing to hide its survey behind: the softmax warps, which wait anyway, take four fifths of it.  (220 tiles
+// of 28 080 keys would else take 23 us.)
+constexpr int kFirstSurvey = 1 + fvattn::kSoftmaxWarps / 2;  // warps of each of K and V
+struct Size {
+    float by;     // 2^size
+    uint32_t up;  // 2^-size as two bf16
+};
+static __device__ __noinline__ void first_survey(const ChunkJob& jb, const Run& run, uint32_t sbase, int warp, int lane) {
+    const int which = warp & 1;
+    Walk walk(run);
+    Work w;
+    if (!walk.next(jb, w, false)) return;
+    const uint32_t top = survey(jb, w, which, 1 + (warp >> 1), kFirstSurvey, lane);
+    if (lane == 0) {
+        asm volatile("red.shared.max.u32 [%0], %1;" ::"r"(sbase + kFirstTop + 4u * which), "r"(top) : "memory");
+        mbar_arrive(sbase + kFirstDone + 8u * which);
+    }
 }
 
 // -------------------------------------------------------------------------------------------------- softmax
@@ -479,9 +581,10 @@ FV_DEV void chunk_softmax(const ChunkJob& jb, const Run& run, uint32_t sbase, ui
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
     const uint32_t tS = lanes + fvattn::tmem_scores((uint32_t)tile), tO = lanes + fvattn::tmem_output((uint32_t)tile);
     const uint32_t bt = sbase + 8u * (uint32_t)tile;
-    const float sl2 = jb.sl2;
+    float sl2 = jb.sl2;
     const int row_tok = row / jb.by_group, row_head = row - row_tok * jb.group;
-    uint32_t s_count = 0, o_count = 0;
+    uint32_t s_count = 0, o_count = 0, item = 0;  // (item: those with key tiles)
+    if (Q4) first_survey(jb, run, sbase, warp, lane);
     Walk walk(run);
     Work w;
     int ahead = 0;
@@ -492,6 +595,15 @@ FV_DEV void chunk_softmax(const ChunkJob& jb, const Run& run, uint32_t sbase, ui
         const int pos = w.pos0() + tok;
         const Span rsp = span_of(jb.mask, pos, pos, w.seq.len);
         RowState rs{neg_inf(), 0.f};
+        if (Q4 && w.n > 0) {  // the row's softmax scale, with the sizes of its q and of the item's K
+            if (!__all_sync(kFullWarp, wait(sbase + kItemReady + 8u * (item & 1u), (item >> 1) & 1u))) return;
+            uint32_t e;
+            float k;
+            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(e) : "r"(sbase + kRowSizes + 2 * kChunkRows * (item & 1u) + threadIdx.x) : "memory");
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(k) : "r"(sbase + kSizes + 16u * (item & 1u)) : "memory");
+            // (a row of q with an infinity has scores that are not numbers)
+            sl2 = e == 255u ? __int_as_float(0x7fffffff) : jb.sl2 * power_of_two(size_of((int)e)) * k;
+        }
         for (int j = 0; j < w.n; j++) {
             if (!__all_sync(kFullWarp, wait(bt + Smem::s_ready, s_count & 1u))) return;
             s_count++;
@@ -545,7 +657,14 @@ FV_DEV void chunk_softmax(const ChunkJob& jb, const Run& run, uint32_t sbase, ui
             o_count++;
             tc_fence_after();
         }
-        const float inv = rs.l > 0.f ? 1.f / rs.l : 0.f;
+        float inv = rs.l > 0.f ? 1.f / rs.l : 0.f;
+        if (Q4 && have_o) {
+            float v;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(sbase + kSizes + 16u * (item & 1u) + 8u) : "memory");
+            inv *= v;
+            fvattn::warp_arrive(sbase + kItemFree + 8u * (item & 1u), lane);
+            item++;
+        }
         if (!part) {
             chunk_write<Q4, false>(jb.out, tO, inv, out_row, have_o, lane);
         } else {
@@ -679,6 +798,11 @@ FV_DEV uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
+FV_DEV uint32_t pack_f16x2_inf(float lo, float hi) {  // (a row that is not finite stays one)
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 FV_DEV uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
     uint32_t r;
     asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
@@ -695,11 +819,12 @@ FV_DEV uint32_t piece_base(uint32_t tile, int row, int q) {
 }
 // Eight values of a word stand in a piece in the order 0 4 1 5 2 6 3 7: the pairs that one mask gives.  Q's pieces get the
 // same order (the sum over d does not care), and the output's columns are put back when they are stored.
-// f16 values zero + step code: a nibble is or-ed into 1024's mantissa (unit 1) where it lies, 1024 + n or 1024 + 16 n, an
+// f16 values (zero + step code) up, `up` a power of two as two bf16: a nibble is or-ed into 1024's mantissa (unit 1) where it lies, 1024 + n or 1024 + 16 n, an
 // addition or multiply-add makes it n - 8 exactly, and one more multiply-add rounds once.
-FV_DEV void expand_unit(uint4 c, uint32_t sz, uint32_t base, int q) {
-    const float step = __uint_as_float(sz << 16), zero = __uint_as_float(sz & 0xffff0000u);
-    const uint32_t s2 = pack_f16x2(step, step), z2 = pack_f16x2(zero, zero);
+FV_DEV void expand_unit(uint4 c, uint32_t sz, uint32_t up, uint32_t base, int q) {
+    sz = mul_bf16x2(sz, up);
+    const uint32_t sz16 = pack_f16x2_inf(__uint_as_float(sz << 16), __uint_as_float(sz & 0xffff0000u));
+    const uint32_t s2 = __byte_perm(sz16, 0, 0x1010), z2 = __byte_perm(sz16, 0, 0x3232);
     // (Quarters 0 and 2, 1 and 3 meet in the same banks, in different panels: the upper two take their words in the order 2 3 0 1.)
     const bool swap = q >= 2;
     const uint32_t word[4] = {swap ? c.z : c.x, swap ? c.w : c.y, swap ? c.x : c.z, swap ? c.y : c.w};
@@ -722,7 +847,7 @@ FV_DEV void chunk_expander(const ChunkJob& jb, const Run& run, uint32_t sbase, i
     using namespace fvattn;
     using R = Roles<true>;
     constexpr int kW = R::kExpanders;
-    uint32_t qn = 0, kvn = 0;
+    uint32_t qn = 0, kvn = 0, item = 0;
     const int r8 = lane >> 2, q = lane & 3;  // this lane's row of a unit and its quarter
     auto ok_all = [&](uint32_t bar, uint32_t parity) { return __all_sync(fvpg::kFullWarp, wait(bar, parity)) != 0; };
     auto arrive = [&](uint32_t bar) {
@@ -740,13 +865,25 @@ FV_DEV void chunk_expander(const ChunkJob& jb, const Run& run, uint32_t sbase, i
             const uint16_t* p = jb.q + (long long)(w.seq.q0 + (live ? tok : 0)) * jb.q_tok +
                                 (long long)(w.head * jb.group + (live ? row - row_tok * jb.group : 0)) * jb.q_head + 32 * q;
             const uint32_t base = piece_base(dst, row, q);
+            uint4 x[4];
+            uint32_t top = 0;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (live) x = __ldg(reinterpret_cast<const uint4*>(p) + j);
-                auto low = [](uint32_t a, uint32_t b) { return pack_f16x2(__uint_as_float(a << 16), __uint_as_float(b << 16)); };
-                auto high = [](uint32_t a, uint32_t b) { return pack_f16x2(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u)); };
-                store_piece(base ^ (16u * j), low(x.x, x.z), high(x.x, x.z), low(x.y, x.w), high(x.y, x.w));
+                x[j] = live ? __ldg(reinterpret_cast<const uint4*>(p) + j) : make_uint4(0, 0, 0, 0);
+                top = larger_bf16x2(larger_bf16x2(top, larger_bf16x2(x[j].x, x[j].y)), larger_bf16x2(x[j].z, x[j].w));
+            }
+            top = larger_bf16x2(top, __shfl_xor_sync(fvpg::kFullWarp, top, 1));
+            top = larger_bf16x2(top, __shfl_xor_sync(fvpg::kFullWarp, top, 2)) & 0x7fff7fffu;
+            const int e = (int)(max(top & 0xffffu, top >> 16) >> 7);
+            if (q == 0)
+                asm volatile("st.shared.u8 [%0], %1;" ::"r"(sbase + kRowSizes + kChunkRows * (2 * (item & 1u) + tile) + row), "r"(e) : "memory");
+            const uint32_t up = twice_bf16(-size_of(e));
+            auto low = [](uint32_t a, uint32_t b) { return pack_f16x2(__uint_as_float(a << 16), __uint_as_float(b << 16)); };
+            auto high = [](uint32_t a, uint32_t b) { return pack_f16x2(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u)); };
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t a = mul_bf16x2(x[j].x, up), b = mul_bf16x2(x[j].y, up), c = mul_bf16x2(x[j].z, up), d = mul_bf16x2(x[j].w, up);
+                store_piece(base ^ (16u * j), low(a, c), high(a, c), low(b, d), high(b, d));
             }
         }
         arrive(sbase + Smem::q_full + 8u * slot);
@@ -757,6 +894,12 @@ FV_DEV void chunk_expander(const ChunkJob& jb, const Run& run, uint32_t sbase, i
     Work w;
     while (walk.next(jb, w, false)) {
         if (!load_q(w, 0) || !load_q(w, 1)) return;
+        if (!ok_all(sbase + kSurveyed + 8u * (item & 1u), (item >> 1) & 1u)) return;
+        uint32_t up_k, up_v;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(up_k) : "r"(sbase + kSizes + 16u * (item & 1u) + 4u) : "memory");
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(up_v) : "r"(sbase + kSizes + 16u * (item & 1u) + 12u) : "memory");
+        warp_arrive(sbase + kItemReady + 8u * (item & 1u), lane);
+        item++;
         for (int j = 0; j <= w.n; j++) {
             const uint32_t slot = kvn % kKvPairs, use = kvn / kKvPairs;  // (as many code stages as pair slots)
             if (!ok_all(sbase + kCodeFull + 8u * slot, use & 1u)) return;
@@ -776,12 +919,37 @@ FV_DEV void chunk_expander(const ChunkJob& jb, const Run& run, uint32_t sbase, i
                 asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sz) : "r"(scales + 32u * u + 4u * r8) : "memory");
                 // A key that the item does not see counts as zeros whatever memory holds.
                 if (!(is_k ? k_whole : v_whole) && !w.sees((is_k ? k0 : v0) + row)) sz = 0u;
-                expand_unit(c, sz, piece_base(dst + (is_k ? kSlotBytes : 0u), row, q), q);
+                expand_unit(c, sz, is_k ? up_k : up_v, piece_base(dst + (is_k ? kSlotBytes : 0u), row, q), q);
             }
             arrive(sbase + Smem::kv_full + 8u * slot);
             if (lane == 0) mbar_arrive(sbase + kCodeFree + 8u * slot);  // (arrive() has met the warp: its reads are done)
             kvn++;
         }
+    }
+}
+
+// The sizes of an item's K or V, an item ahead of the expander (which is what the tensor cores wait for).
+FV_DEV void chunk_surveyor(const ChunkJob& jb, const Run& run, uint32_t sbase, int which, int lane, const ChunkWait& wait) {
+    uint32_t item = 0;
+    Walk walk(run);
+    Work w;
+    while (walk.next(jb, w, false)) {
+        uint32_t top = survey(jb, w, which, 0, item == 0 ? kFirstSurvey : 1, lane);
+        const uint32_t slot = item & 1u;
+        if (item == 0) {
+            if (!__all_sync(fvpg::kFullWarp, wait(sbase + kFirstDone + 8u * which, 0))) return;
+            uint32_t others;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(others) : "r"(sbase + kFirstTop + 4u * which) : "memory");
+            top = max(top, others);
+        } else if (item > 1 && !__all_sync(fvpg::kFullWarp, wait(sbase + kItemFree + 8u * slot, ((item >> 1) - 1u) & 1u))) {
+            return;
+        }
+        const int size = size_of((int)(top >> 23));
+        if (lane == 0) {
+            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(sbase + kSizes + 16u * slot + 8u * which), "r"(__float_as_uint(power_of_two(size))), "r"(twice_bf16(-size)) : "memory");
+            mbar_arrive(sbase + kSurveyed + 8u * slot);
+        }
+        item++;
     }
 }
 
@@ -918,12 +1086,19 @@ FV_DEV void chunk_persistent(const CUtensorMap* mq, const CUtensorMap* mk, const
             mbar_init(sbase + kCodeFull + 8u * s, 1);
             mbar_init(sbase + kCodeFree + 8u * s, R::kExpanders);
         }
+        for (int s = 0; s < 2; s++) {
+            mbar_init(sbase + kFirstDone + 8u * s, kFirstSurvey - 1);
+            mbar_init(sbase + kSurveyed + 8u * s, 2);
+            mbar_init(sbase + kItemReady + 8u * s, R::kExpanders);
+            mbar_init(sbase + kItemFree + 8u * s, kSoftmaxWarps);
+        }
         for (int t = 0; t < 2; t++) {
             mbar_init(sbase + Smem::s_ready + 8u * t, 1);
             mbar_init(sbase + Smem::p_ready + 8u * t, 4);
             mbar_init(sbase + Smem::o_ready + 8u * t, 1);
         }
         mbar_init(sbase + Smem::drain, 1);
+        *reinterpret_cast<volatile uint32_t*>(smem + kFirstTop) = *reinterpret_cast<volatile uint32_t*>(smem + kFirstTop + 4) = 0u;
         int bad = (*(volatile int*)jb.wait_status != FV_ST_OK) ? 1 : 0;  // a CTA that starts after another one gave up does nothing
         if (sbase & 1023u) {
             atomicCAS(jb.wait_status, FV_ST_OK, FV_ST_BAD_SMEM);
@@ -953,6 +1128,7 @@ FV_DEV void chunk_persistent(const CUtensorMap* mq, const CUtensorMap* mk, const
             if (lane == 0) chunk_issuer<Q4>(jb, run, sbase, tmem, waiter(2));
         } else if (Q4) {
             if (warp >= R::kExpander) chunk_expander(jb, run, sbase, warp - R::kExpander, lane, waiter(6));
+            else if (warp >= R::kSurveyor) chunk_surveyor(jb, run, sbase, warp - R::kSurveyor, lane, waiter(4));
             else if (warp == R::kLoader) chunk_code_loader(jb, run, sbase, lane, waiter(1));
         } else if (warp == R::kLoader) {
             chunk_loader(mq, mk, mv, jb, run, sbase, lane, waiter(1));

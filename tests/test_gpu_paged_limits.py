@@ -148,3 +148,86 @@ def test_four_bit_rows_with_an_offset_read_back_within_half_a_step(fvlib):
         assert bool((step[:, 0] <= (1 + 2.0 ** -6) * (span / 15 + BF16_HALF * (most + span / 15) / 7) + 1e-30).all()), name
     k, v = paged.read(kv, batch, rows=n)
     assert torch.isfinite(k).all() and torch.isfinite(v).all()
+
+
+# ---- 4-bit values far from one ----------------------------------------------------------------------------------------
+
+def _scaled(case, name, power):
+    """Every row of `name` times 2^power[s][j] (power: a number, or per sequence and key), exactly."""
+    for s, n in enumerate(case.kv_len):
+        p = power if not torch.is_tensor(power) else power[:n]
+        f = 2.0 ** (p * torch.ones(n, dtype=torch.float64))
+        case.rows[name][s] = case.rows[name][s] * f[:, None, None]
+        j = torch.arange(n)
+        page, row = case.table[s].long()[j // case.page_rows], j % case.page_rows
+        case.scales[name][page, :, row] = (case.scales[name][page, :, row].double() * f[:, None, None]).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("powers", [(0, 0, -24), (0, 0, 18), (0, 0, -60), (0, 0, 100), (20, -20, 0), (-18, 18, 0), (-40, 40, 30), (60, -60, -40), (-20, 0, -20)])
+@pytest.mark.parametrize("nq,kv_len,mask", [(1, 700, (1, 0, 0)), (150, 700, (1, 0, 0)), (150, 1500, (1, 300, 5)), (40, 333, None)])
+def test_four_bit_values_of_any_size(fvlib, kernel, powers, nq, kv_len, mask):
+    """q, K and V times powers of two: what the f16 products of long chunks hold is a matter of the kernel, not of the caller."""
+    from fastvideo_rs_b200 import paged, sdpa
+    case = Case("q4", [kv_len, 90], [nq, 5], 4, 2, 16, seed=40)
+    pq, pk, pv = powers
+    case.q = (case.q.double() * 2.0 ** pq).to(torch.bfloat16)
+    _scaled(case, "k", pk)
+    _scaled(case, "v", pv)
+    kv, batch, q = case.device()
+    out = paged.attend(kv, batch, q, mask_of(mask))
+    assert sdpa.device_status() == 0
+    want, bound = case.expect(mask)
+    check(out, want, bound, f"{powers} {nq} {kv_len}")
+
+
+def test_four_bit_values_of_every_size_in_one_call(fvlib, kernel):
+    """Keys whose V is of another size every 128 keys, from 2^-40 to 2^40."""
+    from fastvideo_rs_b200 import paged, sdpa
+    for seed, runs in enumerate(([0, -40, 40], [40, 0, -40, 0], [-12, 12, -7, 7, 17, -20], [3, -3])):
+        n = 1400
+        case = Case("q4", [n, 600], [200, 3], 4, 2, 32, seed=50 + seed)
+        p = torch.tensor(runs, dtype=torch.float64).repeat_interleave(128).repeat(n)[:n]
+        _scaled(case, "v", p)
+        kv, batch, q = case.device()
+        want, bound = case.expect((1, 0, 0))
+        # (Case's bound adds the largest |zero| of all keys to the terms: here of the keys that carry the row's weights)
+        per = []
+        for s, (m, nq) in enumerate(zip(case.kv_len, case.nq)):
+            qs = case.q[case.cu[s]:case.cu[s + 1]].double()
+            j = torch.arange(m)
+            page, row = case.table[s].long()[j // 32], j % 32
+            sc = case.scales["v"][page, :, row].double()
+            top = (sc[..., 1].abs() + 8 * sc[..., 0].abs())[..., None].expand(m, 2, D)
+            per.append(attend64(qs, case.rows["k"][s], top, (1, 0, 0))[0])
+        bound = BF16_HALF * want.abs() + (BF16_HALF + 2.0 ** -10) * torch.cat(per) + 1e-30
+        out = paged.attend(kv, batch, q, mask_of((1, 0, 0)))
+        assert sdpa.device_status() == 0
+        check(out, want, bound, f"{runs}")
+
+
+def test_rows_of_q_of_every_size(fvlib, kernel):
+    from fastvideo_rs_b200 import paged
+    case = Case("q4", [500], [140], 4, 2, 16, seed=60)
+    p = torch.tensor([0, -30, 3, -9, 40, 0, -60, 1], dtype=torch.float64).repeat(70)
+    case.q = case.q.double() * 2.0 ** torch.minimum(p, torch.tensor(1.0, dtype=torch.float64)).view(140, 4, 1)
+    case.q = case.q.to(torch.bfloat16)
+    kv, batch, q = case.device()
+    want, bound = case.expect((1, 0, 0))
+    check(paged.attend(kv, batch, q, mask_of((1, 0, 0))), want, bound, "rows")
+
+
+def test_a_four_bit_row_that_is_not_finite_stands_for_nan(fvlib, kernel):
+    """A row with an infinity was appended: whoever sees it gets what is not a number, other sequences nothing of it."""
+    from fastvideo_rs_b200 import paged
+    for which in ("k", "v"):
+        for bad in (math.inf, -math.inf, math.nan):
+            case = Case("q4", [300, 200], [140, 3], 4, 2, 16, seed=62)
+            kv, batch, q = case.device()
+            clean = paged.attend(kv, batch, q, mask_of((1, 0, 0)))
+            x = torch.randn(case.tokens, 2, D, device="cuda").to(torch.bfloat16)
+            y = x.clone()
+            y[0, 1, 3] = bad  # the first token of the first sequence: key 160, which all 140 rows see
+            paged.append(kv, batch, y if which == "k" else x, y if which == "v" else x)
+            out = paged.attend(kv, batch, q, mask_of((1, 0, 0)))
+            assert bool(out[:140, 2:].isnan().all()), (which, bad)
+            assert not bool(out[140:].isnan().any()) and not bool(clean.isnan().any())
