@@ -392,7 +392,8 @@ __global__ void __launch_bounds__(kAttnThreads, ROWS <= 8 ? 3 : 2) fv_paged_deco
                 qf[n][4 * i + 2] = pack_f16x2(lo_f(u[n][i].y) * up, lo_f(u[n][i].w) * up);
                 qf[n][4 * i + 3] = pack_f16x2(hi_f(u[n][i].y) * up16, hi_f(u[n][i].w) * up16);
             }
-            const float scaled = sum * up * (1.f / kCodeUnit), back = a.sl2 * down * kCodeUnit;
+            // (an infinity in q: the scores are not numbers, where f16's largest value and zero * sum(q) would give something finite)
+            const float scaled = sum * up * (1.f / kCodeUnit), back = top < -neg_inf() ? a.sl2 * down * kCodeUnit : __int_as_float(0x7fffffff);
             qsum[n][0] = __shfl_sync(kFullWarp, scaled, 8 * t);      // of row 2 t, which the lanes 4 (2 t) .. hold
             qsum[n][1] = __shfl_sync(kFullWarp, scaled, 8 * t + 4);  // of row 2 t + 1
             sl2[n][0] = __shfl_sync(kFullWarp, back, 8 * t);

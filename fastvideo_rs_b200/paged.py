@@ -249,7 +249,7 @@ def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[Block
     by token, a window of `window` tokens, the first `sink` tokens always visible; block_tokens of a frame: the streaming
     form of the block-causal mask.  A row that sees no key is zero.  Pages of which no row sees a key need not exist; what
     memory holds where no row of the call sees it has no influence, but a key that some row sees must be finite (a NaN may reach
-    other rows of the call; one in q reaches only its own row).  Sums and softmax statistics are f32, probabilities are rounded to the type of the products: bf16, over 4-bit pages f16 (there long
+    other rows of the call; one in q reaches only its own row, as an infinity does).  Sums and softmax statistics are f32, probabilities are rounded to the type of the products: bf16, over 4-bit pages f16 (there long
     chunks also take q and the cached values through f16, scaled to its upper end: a value that is 2^-26 and less of the largest that the
     same 256 rows see in its sequence and head loses relative precision).
     With `out` (which may be q itself), rows that belong to no sequence keep what they hold."""

@@ -216,6 +216,24 @@ def test_rows_of_q_of_every_size(fvlib, kernel):
     check(paged.attend(kv, batch, q, mask_of((1, 0, 0))), want, bound, "rows")
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("nq", [1, 150])
+def test_an_infinite_query_is_not_a_number(fvlib, kernel, fmt, nq):
+    """An infinity in q: the row is not a number (its scores are infinities of both signs), and no other row changes."""
+    from fastvideo_rs_b200 import paged
+    case = Case(fmt, [700], [nq], 4, 2, 64, seed=61)
+    kv, batch, q = case.device()
+    want, bound = case.expect((1, 0, 0))
+    q[nq // 2, 1, 7] = math.inf
+    q[nq - 1, 2, 5] = -math.inf
+    out = paged.attend(kv, batch, q, mask_of((1, 0, 0)))
+    bad = torch.zeros(nq, 4, dtype=torch.bool, device="cuda")
+    bad[nq // 2, 1] = bad[nq - 1, 2] = True
+    assert bool(out[bad].isnan().all())
+    good = ~bad.cpu()
+    check(out[~bad], want[good], bound[good], fmt)
+
+
 def test_a_four_bit_row_that_is_not_finite_stands_for_nan(fvlib, kernel):
     """A row with an infinity was appended: whoever sees it gets what is not a number, other sequences nothing of it."""
     from fastvideo_rs_b200 import paged
