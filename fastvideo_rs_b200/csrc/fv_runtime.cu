@@ -221,12 +221,13 @@ extern "C" int fv_device_status(void* stream, int* code_out) {
     int words[2] = {0, 0};
     FV_CUDA(cudaMemcpyAsync(words, w, sizeof(words), cudaMemcpyDeviceToHost, (cudaStream_t)stream));
     FV_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
-    const int code = words[0] ? words[0] : words[1];
+    const int which = words[0] ? 0 : 1, code = words[which];
     if (code_out) *code_out = code;
     if (code != 0) {
-        FV_CUDA(cudaMemsetAsync(w, 0, sizeof(words), (cudaStream_t)stream));
+        // (only the word that is told of: when both are set the next call tells of the other)
+        FV_CUDA(cudaMemsetAsync(w + which, 0, sizeof(int), (cudaStream_t)stream));
         FV_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
-        if (words[0] == 0)
+        if (which == 1)
             return fvrt::fail(FV_ERR_DEVICE_STATUS, "paged cache: %s (status %d)",
                               code == 200   ? "a page that a call needed lies outside the pool or the table"
                               : code == 201 ? "cu_q or the lengths of a batch are outside its bounds"

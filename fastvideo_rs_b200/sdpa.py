@@ -256,8 +256,9 @@ def splitkv_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, splits: int, 
 
 
 def device_status() -> int:
-    """Synchronises the current stream and returns the kernels' status word (0 = every bounded wait
-    completed); raises FvError when a kernel gave up."""
+    """Synchronises the current stream and returns the kernels' status (0 = every bounded wait completed and no paged call met
+    tables that lead outside of its cache); raises FvError when a kernel gave up a wait (100 + role), or met such tables (200 .. 202).
+    What is told is cleared; when both happened this call tells of the wait and the next one of the tables."""
     code = ctypes.c_int(0)
     rc = _lib.lib().fv_device_status(_stream_ptr(), ctypes.byref(code))
     _lib.check(rc, "device_status")

@@ -55,7 +55,8 @@ FV_API const char* fv_version(void);
 /* Reads and clears the current device's kernel status.  Synchronises `stream`.
  * Returns FV_RAN when every kernel finished its waits, FV_ERR_DEVICE_STATUS when one
  * gave up (code in *code_out: 100 + role) or met tables of a paged cache that lead outside of it (200 .. 202, see there;
- * unlike a wait that ran out these do not keep later launches from running), FV_ERR_CUDA on a CUDA error.
+ * unlike a wait that ran out these do not keep later launches from running), FV_ERR_CUDA on a CUDA error.  When both happened the
+ * wait is told first and the tables by the next call.
  * The word is part of the library's module image (a file-scope __device__ array, zero at load): every
  * kernel of the library reports there, the two-pass call on built-in scratch included, and neither this
  * call nor any launch allocates for it. */

@@ -249,3 +249,21 @@ def test_a_four_bit_row_that_is_not_finite_stands_for_nan(fvlib, kernel):
             out = paged.attend(kv, batch, q, mask_of((1, 0, 0)))
             assert bool(out[:140, 2:].isnan().all()), (which, bad)
             assert not bool(out[140:].isnan().any()) and not bool(clean.isnan().any())
+
+
+# ---- what is refused, reported and kept -------------------------------------------------------------------------------
+
+def test_a_wait_that_ran_out_and_a_bad_page_are_both_told(fvlib):
+    """One status read tells of the wait, the next one of the page."""
+    from fastvideo_rs_b200 import FvError, paged, sdpa
+    case = Case("bf16", [40], [1], 4, 2, 16, seed=1)
+    kv, batch, q = case.device()
+    batch.page_table[0, 1] = -1
+    paged.attend(kv, batch, q, mask_of((1, 0, 0)))
+    fvlib.fv_selftest_wait_timeout.argtypes = [ctypes.c_void_p, ctypes.c_longlong]
+    assert fvlib.fv_selftest_wait_timeout(ctypes.c_void_p(torch.cuda.current_stream().cuda_stream), 100000) == 0
+    with pytest.raises(FvError, match="wait"):
+        sdpa.device_status()
+    with pytest.raises(FvError, match="status 200"):
+        sdpa.device_status()
+    assert sdpa.device_status() == 0
