@@ -158,6 +158,20 @@ def _rows_like(q: torch.Tensor, n: int, h: int) -> torch.Tensor:
     return out if out.is_contiguous() else q.new_empty((n, h, D))
 
 
+def _keep_apart(name: str, out: torch.Tensor, other: str, t: torch.Tensor, n: int, h: int, nt: int, nh: int, in_place: bool = False) -> None:
+    """Refuses a result (contiguous) that shares memory with rows of an operand t [n, h, 128] (strides nt, nh), which other blocks may
+    still have to read; in_place: but for one that is the operand itself."""
+    at = (out.data_ptr() - t.data_ptr()) // 2  # in values, of the first byte of out
+    size = out.numel()
+    if at >= (n - 1) * nt + (h - 1) * nh + D or at + size <= 0 or size == 0 or n * h == 0:
+        return
+    if in_place and at == 0 and size == n * h * D and (h == 1 or nh == D) and (n == 1 or nt == h * D):
+        return
+    first = (torch.arange(n)[:, None] * nt + torch.arange(h) * nh).flatten()  # (out may lie in a gap between the rows)
+    if bool(((first < at + size) & (first + D > at)).any()):
+        raise ValueError(f"{name} overlaps {other}" + (", of which it may only be the whole" if in_place else ""))
+
+
 def _call(kv: PagedKv, batch: PagedBatch, what: str, fn, *args) -> None:
     """One C entry on the current stream of the cache's device."""
     index = kv.index
@@ -179,7 +193,7 @@ def append(kv: PagedKv, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, *, 
     multiples of 8: slices of a fused projection are read in place), K rotated on the way when cos / sin f32 [rows, 128] are
     given: token t with row positions[t] (int32), by default its position in its sequence.  pairing "interleaved": values
     2 i and 2 i + 1 (the tables of wan.wan_rope_tables), "half": values i and i + 64.  q [tokens, heads, 128], if given, is
-    rotated too and returned as [tokens, heads, 128] (in q_out, which may be q itself).  Two tokens of a call must not fall on the same cache row."""
+    rotated too and returned as [tokens, heads, 128] (in q_out, which may be q itself, and else shares no memory with q, k and v).  Two tokens of a call must not fall on the same cache row."""
     index = kv.index
     tokens, _, kt, kh = _heads_in("append: k", k, index, -1, kv.kv_heads)
     _, _, vt, vh = _heads_in("append: v", v, index, tokens, kv.kv_heads)
@@ -207,6 +221,9 @@ def append(kv: PagedKv, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, *, 
             _heads_in("append: q_out", q_out, index, tokens, heads)
             if not q_out.is_contiguous():
                 raise ValueError("append: q_out must be contiguous")
+            _keep_apart("append: q_out", q_out, "q", q, tokens, heads, qt, qh, in_place=True)
+            _keep_apart("append: q_out", q_out, "k", k, tokens, kv.kv_heads, kt, kh)
+            _keep_apart("append: q_out", q_out, "v", v, tokens, kv.kv_heads, vt, vh)
         if heads:
             qp, op = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
@@ -252,7 +269,7 @@ def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[Block
     other rows of the call; one in q reaches only its own row, as an infinity does).  Sums and softmax statistics are f32, probabilities are rounded to the type of the products: bf16, over 4-bit pages f16 (there long
     chunks also take q and the cached values through f16, scaled to its upper end: a value that is 2^-26 and less of the largest that the
     same 256 rows see in its sequence and head loses relative precision).
-    With `out` (which may be q itself), rows that belong to no sequence keep what they hold."""
+    With `out` (which may be q itself, and else shares no memory with it), rows that belong to no sequence keep what they hold."""
     tokens, heads, qt, qh = _heads_in("attend: q", q, kv.index)
     if heads < 1 or heads % kv.kv_heads:
         raise ValueError(f"attend: {heads} heads over {kv.kv_heads} K/V heads")
@@ -262,6 +279,7 @@ def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[Block
         _heads_in("attend: out", out, kv.index, tokens, heads)
         if not out.is_contiguous():
             raise ValueError("attend: out must be contiguous")
+        _keep_apart("attend: out", out, "q", q, tokens, heads, qt, qh, in_place=True)
     if tokens == 0 or batch.seqs == 0 or batch.max_q == 0:
         return out
     how = (1, mask.block_tokens, mask.window, mask.sink) if mask is not None else (0, 0, 0, 0)

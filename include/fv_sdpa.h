@@ -307,7 +307,8 @@ FV_API int fv_sdpa_window_bf16(void* stream, const void* q, const void* k_cache,
  *   no influence whatever their memory holds; a key that some row sees must be finite (a NaN in it may reach other
  *   rows of the call).  f32 sums and statistics; probabilities are rounded to the products' type, bf16, over 4-bit pages f16
  *   (where long chunks take q and the cached values through f16 too, scaled to its upper end: a value that is 2^-26 and less of the
- *   largest that the same 256 rows see in its sequence and head loses relative precision).  Strides are positive.  FV_PAGED_KERNEL=rows or items (kept for A/B) fixes which of the two kernels runs.
+ *   largest that the same 256 rows see in its sequence and head loses relative precision).  Strides are positive.
+ *   out may be q itself (contiguous), as q_out may be above; else results share no memory with operands.  FV_PAGED_KERNEL=rows or items (kept for A/B) fixes which of the two kernels runs.
  *   The workspace is scratch of this call alone (fv_paged_attn_workspace_bytes of the same query, may be 0; it reads
  *   neither pointers nor strides nor scale).
  * Each call may be captured in a graph; make the first call of its kind in a process before that, so that its kernel is loaded.

@@ -267,3 +267,29 @@ def test_a_wait_that_ran_out_and_a_bad_page_are_both_told(fvlib):
     with pytest.raises(FvError, match="status 200"):
         sdpa.device_status()
     assert sdpa.device_status() == 0
+
+
+def test_results_that_overlap_operands_are_refused(fvlib):
+    """out may be q itself; anything in between would be read after it was written."""
+    from fastvideo_rs_b200 import paged
+    n, heads, hk = 20, 4, 2
+    case = Case("bf16", [60], [n], heads, hk, 16, seed=2)
+    kv, batch, _ = case.device()
+    room = torch.randn(2 * n * 8 * D, device="cuda").to(torch.bfloat16)
+    q = room[:n * heads * D].view(n, heads, D)
+    late = room[8 * D:8 * D + n * heads * D].view(n, heads, D)
+    fused = room[:n * 8 * D].view(n, 8, D)
+    k = room[n * heads * D:][:n * hk * D].view(n, hk, D)
+    with pytest.raises(ValueError, match="overlap"):
+        paged.attend(kv, batch, q, out=late)
+    with pytest.raises(ValueError, match="overlap"):
+        paged.attend(kv, batch, fused[:, :heads], out=q)
+    with pytest.raises(ValueError, match="overlap"):
+        paged.append(kv, batch, k, k, q=q, q_out=late)
+    with pytest.raises(ValueError, match="overlap"):
+        paged.append(kv, batch, k, k, q=q.clone(), q_out=room[n * heads * D:2 * n * heads * D].view(n, heads, D))
+    # side by side, and in place
+    want = paged.attend(kv, batch, q, mask_of((1, 0, 0)))
+    beside = room[n * heads * D:2 * n * heads * D].view(n, heads, D)
+    assert torch.equal(paged.attend(kv, batch, q, mask_of((1, 0, 0)), out=beside), want)
+    assert torch.equal(paged.attend(kv, batch, q, mask_of((1, 0, 0)), out=q), want)
