@@ -152,6 +152,22 @@ def _heads_in(name: str, t: torch.Tensor, index: int, tokens: int = -1, heads: i
     return n, h, a if n > 1 else D, b if h > 1 else D
 
 
+_KEPT = 64  # shapes that a batch remembers
+
+
+def _scratch_bytes(kv: "PagedKv", batch: "PagedBatch", mask: Optional[BlockCausal], key) -> int:
+    """Scratch of an attention call of this shape; the batch remembers it."""
+    how, heads, _, tokens, _ = key
+    if max(how) > 0x7fffffff or min(how) < 0:
+        raise ValueError(f"attend: {mask} is out of range")
+    with torch.cuda.device(kv.index):
+        need = (_fns or _entries())[2](kv._ref, batch._ref, _query_struct.pack(0, 0, 0, 0, 0, 0, tokens, heads, *how, 0.0))
+    if len(batch._need) >= _KEPT:  # (a program whose number of packed rows never comes again)
+        batch._need.clear()
+    batch._need[key] = need
+    return need
+
+
 def _rows_like(q: torch.Tensor, n: int, h: int) -> torch.Tensor:
     """A contiguous [n, h, 128] result beside q."""
     out = torch.empty_like(q)  # (keeps q's order of extents, which is nearly always this one)
@@ -287,15 +303,10 @@ def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[Block
     key = (how, heads, kv.kv_heads, tokens, kv.format)
     need = batch._need.get(key)
     if need is None:
-        if max(how) > 0x7fffffff or min(how) < 0:
-            raise ValueError(f"attend: {mask} is out of range")
-        need = 0
-        if kv.index >= 0:
-            with torch.cuda.device(kv.index):
-                need = batch._need[key] = fns[2](kv._ref, batch._ref, _query_struct.pack(0, 0, 0, 0, 0, 0, tokens, heads, *how, 0.0))
+        need = _scratch_bytes(kv, batch, mask, key)
     # (scratch of this call alone, from the stream's own pool: calls on other streams and captured graphs share nothing)
     ws = q.new_empty((need // 2,)) if need else None
+    scale = _SCALE if scale is None else float(scale)
     _call(kv, batch, "paged attention", fns[3],
-          _query_struct.pack(q.data_ptr(), out.data_ptr(), ws.data_ptr() if need else 0, need, qt, qh, tokens, heads, *how,
-                             _SCALE if scale is None else float(scale)))
+          _query_struct.pack(q.data_ptr(), out.data_ptr(), ws.data_ptr() if need else 0, need, qt, qh, tokens, heads, *how, scale))
     return out

@@ -293,3 +293,14 @@ def test_results_that_overlap_operands_are_refused(fvlib):
     beside = room[n * heads * D:2 * n * heads * D].view(n, heads, D)
     assert torch.equal(paged.attend(kv, batch, q, mask_of((1, 0, 0)), out=beside), want)
     assert torch.equal(paged.attend(kv, batch, q, mask_of((1, 0, 0)), out=q), want)
+
+
+def test_what_a_batch_keeps_does_not_grow(fvlib):
+    """One batch with another number of packed rows at every call."""
+    from fastvideo_rs_b200 import paged
+    case = Case("bf16", [40], [1], 4, 2, 16, seed=4, pad=400)
+    kv, batch, q = case.device()
+    want = paged.attend(kv, batch, q)[:1]
+    for n in range(1, 400):
+        assert torch.equal(paged.attend(kv, batch, q[:n])[:1], want)
+    assert len(batch._need) <= 64
