@@ -121,7 +121,7 @@ class PagedBatch:
         if not 0 <= max_q < 1 << 30 or not 0 <= max_kv < 1 << 30:
             raise ValueError("PagedBatch: max_q and max_kv must be 0 .. 2^30 - 1")
         self.seqs, self.max_q, self.max_kv, self.device, self.index = seqs, int(max_q), int(max_kv), dev, page_table.get_device()
-        self._need = {}  # scratch bytes by the call's shape: a step asks for every layer (FV_PAGED_KERNEL is set before the first)
+        self._need = {}  # scratch bytes by the call's shape: a step asks for every layer
         self._c = _BatchC(page_table.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), seqs, width, self.max_q, self.max_kv)
         self._ref = ctypes.addressof(self._c)
 
@@ -307,6 +307,14 @@ def attend(kv: PagedKv, batch: PagedBatch, q: torch.Tensor, mask: Optional[Block
     # (scratch of this call alone, from the stream's own pool: calls on other streams and captured graphs share nothing)
     ws = q.new_empty((need // 2,)) if need else None
     scale = _SCALE if scale is None else float(scale)
-    _call(kv, batch, "paged attention", fns[3],
-          _query_struct.pack(q.data_ptr(), out.data_ptr(), ws.data_ptr() if need else 0, need, qt, qh, tokens, heads, *how, scale))
+    try:
+        _call(kv, batch, "paged attention", fns[3],
+              _query_struct.pack(q.data_ptr(), out.data_ptr(), ws.data_ptr() if need else 0, need, qt, qh, tokens, heads, *how, scale))
+    except _lib.FvError:  # (FV_PAGED_KERNEL may have changed since this shape was first asked for: refused before anything ran)
+        fresh = _scratch_bytes(kv, batch, mask, key)
+        if fresh <= need:
+            raise
+        ws = q.new_empty((fresh // 2,))
+        _call(kv, batch, "paged attention", fns[3],
+              _query_struct.pack(q.data_ptr(), out.data_ptr(), ws.data_ptr(), fresh, qt, qh, tokens, heads, *how, scale))
     return out

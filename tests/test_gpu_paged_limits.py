@@ -295,6 +295,17 @@ def test_results_that_overlap_operands_are_refused(fvlib):
     assert torch.equal(paged.attend(kv, batch, q, mask_of((1, 0, 0)), out=q), want)
 
 
+def test_the_kernel_switch_may_change_under_a_batch(fvlib, monkeypatch):
+    """FV_PAGED_KERNEL changes what scratch a call needs, also of a batch that has been asked before."""
+    from fastvideo_rs_b200 import paged
+    case = Case("q4", [9000], [30], 4, 1, 64, seed=3)
+    kv, batch, q = case.device()
+    want, bound = case.expect((1, 0, 0))
+    for name in ("rows", "items", "rows", "items"):
+        monkeypatch.setenv("FV_PAGED_KERNEL", name)
+        check(paged.attend(kv, batch, q, mask_of((1, 0, 0))), want, bound, name)
+
+
 def test_what_a_batch_keeps_does_not_grow(fvlib):
     """One batch with another number of packed rows at every call."""
     from fastvideo_rs_b200 import paged
