@@ -461,6 +461,7 @@ extern "C" int fv_paged_append_bf16(void* stream, const fv_paged_kv* kv, const f
         return fvrt::fail(FV_ERR_INVALID, "paged append: unknown pairing %d", pairing);
     if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)q_out | (uintptr_t)cosv | (uintptr_t)sinv) & 15)
         return fvrt::fail(FV_ERR_INVALID, "paged append: operands must be 16-byte aligned");
+    if ((uintptr_t)x->positions & 3) return fvrt::fail(FV_ERR_INVALID, "paged append: positions must be 4-byte aligned");
     if ((x->k_tok | x->k_head | x->v_tok | x->v_head | (q ? x->q_tok | x->q_head : 0)) & 7)
         return fvrt::fail(FV_ERR_INVALID, "paged append: strides must be multiples of 8 values");
     a.q = (const uint16_t*)q;

@@ -315,3 +315,15 @@ def test_what_a_batch_keeps_does_not_grow(fvlib):
     for n in range(1, 400):
         assert torch.equal(paged.attend(kv, batch, q[:n])[:1], want)
     assert len(batch._need) <= 64
+
+
+def test_positions_must_be_aligned(fvlib):
+    from fastvideo_rs_b200 import paged
+    append = paged._entries()[0]
+    case = Case("bf16", [40], [2], 1, 1, 16, seed=5)
+    kv, batch, q = case.device()
+    x = torch.zeros(2, 1, D, dtype=torch.bfloat16, device="cuda")
+    table = torch.ones(40, D, device="cuda")
+    where = torch.zeros(8, dtype=torch.int32, device="cuda")
+    rows = paged._rows_struct.pack(x.data_ptr(), x.data_ptr(), 0, 0, table.data_ptr(), table.data_ptr(), where.data_ptr() + 2, D, D, D, D, 0, 0, 2, 0, 40, 0)
+    assert append(None, kv._ref, batch._ref, rows) == -1 and b"aligned" in fvlib.fv_last_error()
