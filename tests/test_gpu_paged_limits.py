@@ -251,6 +251,113 @@ def test_a_four_bit_row_that_is_not_finite_stands_for_nan(fvlib, kernel):
             assert not bool(out[140:].isnan().any()) and not bool(clean.isnan().any())
 
 
+# ---- probabilities and masks, counted ---------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("heads", [2, 16])
+def test_four_bit_probabilities_are_rounded_at_eleven_bits(fvlib, kernel, heads):
+    """Scores and values that every product holds exactly, and outputs that nearly cancel: what is left is P's rounding, 2^-11."""
+    from fastvideo_rs_b200 import paged
+    g = torch.Generator().manual_seed(70)
+    for n, nq in ((5, 5), (37, 20), (200, 70)):
+        case = Case("q4", [n], [nq], heads, 1, 16, seed=70)
+        codes = {"k": torch.full((n, 1, D), 8), "v": torch.randint(0, 16, (n, 1, D), generator=g)}
+        codes["k"][:, 0, 0] = torch.randint(0, 16, (n,), generator=g)
+        codes["v"][1::2] = (16 - codes["v"][0::2][: n // 2]).clamp(max=15)  # nearly the negative of the key before
+        q = torch.zeros(nq, heads, D)
+        q[..., 0] = torch.randint(1, 256, (nq, heads), generator=g) / 64.0
+        case.q = q.to(torch.bfloat16)
+        j = torch.arange(n)
+        page, row = case.table[0].long()[j // 16], j % 16
+        for name in ("k", "v"):
+            case.pool[name][page, :, row] = pack(codes[name]).to(torch.uint8)
+            case.scales[name][page, :, row] = torch.tensor([0.25, 0.0]).to(torch.bfloat16)
+            case.rows[name] = [0.25 * (codes[name].double() - 8.0)]
+        kv, batch, qd = case.device()
+        out = paged.attend(kv, batch, qd, mask_of((1, 0, 0)))
+        want, mag = attend64(case.q.double(), case.rows["k"][0], case.rows["v"][0], (1, 0, 0))
+        # P: half a step of f16, 2^-11; the exponential and the f32 sums (scores up to 16: 2^-24 of them in the exponent, ex2 2^-22): 2^-15
+        bound = BF16_HALF * want.abs() + (F16_HALF + 2.0 ** -15) * mag + 1e-30
+        check(out, want, bound, f"{n}")
+
+
+COUNTED = [([400], [1], (1, 0, 0)), ([400], [1], (1, 257, 0)), ([1031], [1], (1, 300, 5)), ([1031], [260], (1, 300, 5)), ([900], [333], (1, 129, 0)),
+           ([777], [777], (1, 0, 0)), ([640], [160], (160, 2, 1)), ([1000], [129], (100, 2, 2)), ([515, 64], [3, 64], (7, 20, 3)), ([4100], [40], (1, 1000, 130))]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("i", range(len(COUNTED)))
+def test_every_visible_key_counts_once(fvlib, kernel, fmt, i):
+    """q of zeros: every visible key has the same weight.  V marks key j in column j % 128, so an output is a count of a few keys
+    over the number of visible ones: a key too many or too few, anywhere, is far outside the roundings."""
+    from fastvideo_rs_b200 import paged, sdpa
+    kv_len, nq, mask = COUNTED[i]
+    case = Case(fmt, kv_len, nq, 2, 1, 32, seed=80 + i)
+    case.q = torch.zeros_like(case.q)
+    for s, n in enumerate(kv_len):
+        j = torch.arange(n)
+        page, row = case.table[s].long()[j // 32], j % 32
+        mark = torch.zeros(n, 1, D)
+        mark[j, 0, j % D] = 1.0
+        case.rows["v"][s] = mark.double()
+        if fmt == "bf16":
+            case.pool["v"][page, :, row] = mark.to(torch.bfloat16)
+        else:
+            case.pool["v"][page, :, row] = pack((8 + mark).to(torch.uint8))
+            case.scales["v"][page, :, row] = torch.tensor([1.0, 0.0]).to(torch.bfloat16)
+    kv, batch, q = case.device()
+    out = paged.attend(kv, batch, q, mask_of(mask))
+    assert sdpa.device_status() == 0
+    want = torch.cat([attend64(case.q[case.cu[s]:case.cu[s + 1]].double(), case.rows["k"][s], case.rows["v"][s], mask)[0] for s in range(len(kv_len))])
+    # P is a power of two or one, sums of up to 4 100 of them are exact in f32; the quotient and the parts' joins 2^-20; bf16
+    check(out, want, (BF16_HALF + 2.0 ** -18) * want + 1e-30, f"{fmt} {COUNTED[i]}")
+
+
+# ---- the Wan layer against its contiguous form ------------------------------------------------------------------------
+
+def test_paged_layer_agrees_with_the_contiguous_one(fvlib):
+    """One chunk-causal pass over a whole clip: forward_paged over bf16 pages against forward_self on the same projection."""
+    from fastvideo_rs_b200 import paged, wan
+    from fastvideo_rs_b200.sdpa import BlockCausal
+    heads, frame, frames = 3, 20, 6
+    g = torch.Generator().manual_seed(90)
+    w = [(1 + 0.1 * torch.randn(heads * D, generator=g)).cuda() for _ in range(2)]
+    qkv = torch.randn(1, frames * frame, 3 * heads * D, generator=g).to(torch.bfloat16).cuda()
+    layer = wan.WanSelfAttention((frames, 4, 5), heads, *w, causal=BlockCausal(frame, 0, 0))
+    want = layer.forward_self(qkv)[0].transpose(0, 1).double().cpu()
+    got = _stream(layer, qkv, frame, "bf16", heads)
+    q, k, v = (t[0].transpose(0, 1).double().cpu() for t in wan.qk_prep(qkv, *w, layer.cos, layer.sin, heads))
+    o, mag = attend64(q, k, v, (frame, 0, 0))
+    # q and k are off by one more rounding to bf16 (2^-8 of a pair's values, sqrt(2) of it after the rotation): each score by at
+    # most 2 sqrt(2) 2^-8 |q| |k| / sqrt(128) -- by Cauchy -- and P by twice that; both sides round P and the result
+    off = 2 * 2.0 * math.sqrt(2.0) * BF16_HALF * float(q.norm(dim=-1).max() * k.norm(dim=-1).max()) / math.sqrt(D)
+    check(got, want, 2 * BF16_HALF * o.abs() + (2 * BF16_HALF + 2.0 ** -9 + off) * mag, "layer")
+    # and no further from the 64-bit result than that
+    check(got, o, BF16_HALF * o.abs() + (BF16_HALF + 2.0 ** -10 + off) * mag, "64 bits")
+
+
+def test_sinks_move_on_by_appending_them_again(fvlib):
+    """The rows of the sinks get the rotation of later positions by appending their raw keys once more with `positions`."""
+    from fastvideo_rs_b200 import paged, sdpa, wan
+    cos, sin = wan.wan_rope_tables((6, 4, 5))
+    n, sink = 100, 20
+    g = torch.Generator().manual_seed(91)
+    k, v = (torch.randn(n, 2, D, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    kv = paged.PagedKv.empty(8, 16, 2)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    table = torch.arange(7, dtype=torch.int32, device="cuda")[None]
+    whole = paged.PagedBatch(table, i32(n), i32(0, n), max_q=n, max_kv=n)
+    paged.append(kv, whole, k, v, cos=cos, sin=sin)
+    before = paged.read(kv, whole, rows=n)
+    head = paged.PagedBatch(table, i32(sink), i32(0, sink), max_q=sink, max_kv=sink)
+    where = torch.arange(40, 40 + sink, dtype=torch.int32, device="cuda")
+    paged.append(kv, head, k[:sink], v[:sink], cos=cos, sin=sin, positions=where)
+    after = paged.read(kv, whole, rows=n)
+    assert sdpa.device_status() == 0
+    assert torch.equal(after[0][sink:], before[0][sink:]) and torch.equal(after[1], before[1])
+    want = rotate64(k[:sink].double().cpu(), cos[where.long()].double().cpu()[:, None], sin[where.long()].double().cpu()[:, None], "interleaved")
+    assert bool(((after[0][:sink].double().cpu() - want).abs() <= BF16_HALF * want.abs() + 2.0 ** -21 * k.abs().max().item()).all())
+
+
 # ---- what is refused, reported and kept -------------------------------------------------------------------------------
 
 def test_a_wait_that_ran_out_and_a_bad_page_are_both_told(fvlib):
