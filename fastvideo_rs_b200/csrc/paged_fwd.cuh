@@ -931,6 +931,7 @@ FV_DEV void chunk_expander(const ChunkJob& jb, const Run& run, uint32_t sbase, i
 // The sizes of an item's K or V, an item ahead of the expander (which is what the tensor cores wait for).
 FV_DEV void chunk_surveyor(const ChunkJob& jb, const Run& run, uint32_t sbase, int which, int lane, const ChunkWait& wait) {
     uint32_t item = 0;
+    int before[2] = {0, 0};  // key tiles of the last two items
     Walk walk(run);
     Work w;
     while (walk.next(jb, w, false)) {
@@ -941,9 +942,13 @@ FV_DEV void chunk_surveyor(const ChunkJob& jb, const Run& run, uint32_t sbase, i
             uint32_t others;
             asm volatile("ld.shared.u32 %0, [%1];" : "=r"(others) : "r"(sbase + kFirstTop + 4u * which) : "memory");
             top = max(top, others);
-        } else if (item > 1 && !__all_sync(fvpg::kFullWarp, wait(sbase + kItemFree + 8u * slot, ((item >> 1) - 1u) & 1u))) {
-            return;
+        } else if (item > 1) {  // (the only wait that lasts for a whole item: some 3 500 cycles a tile)
+            ChunkWait patient = wait;
+            patient.cycles += 16384ll * (before[0] + before[1]);
+            if (!__all_sync(fvpg::kFullWarp, patient(sbase + kItemFree + 8u * slot, ((item >> 1) - 1u) & 1u))) return;
         }
+        before[0] = before[1];
+        before[1] = w.n;
         const int size = size_of((int)(top >> 23));
         if (lane == 0) {
             asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(sbase + kSizes + 16u * slot + 8u * which), "r"(__float_as_uint(power_of_two(size))), "r"(twice_bf16(-size)) : "memory");

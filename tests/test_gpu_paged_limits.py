@@ -434,3 +434,46 @@ def test_positions_must_be_aligned(fvlib):
     where = torch.zeros(8, dtype=torch.int32, device="cuda")
     rows = paged._rows_struct.pack(x.data_ptr(), x.data_ptr(), 0, 0, table.data_ptr(), table.data_ptr(), where.data_ptr() + 2, D, D, D, D, 0, 0, 2, 0, 40, 0)
     assert append(None, kv._ref, batch._ref, rows) == -1 and b"aligned" in fvlib.fv_last_error()
+
+
+# ---- many items a CTA -------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fmt,heads,nq,n", [("q4", 40, 1030, 28100), ("bf16", 12, 2060, 24000)])
+def test_keys_beyond_l2_in_phases(fvlib, fmt, heads, nq, n):
+    """More keys than L2 holds: the long-chunk kernel goes through its line of items in four phases, several runs a CTA.  Against 64
+    bits on a few rows of every head, at the ends of the row blocks and inside them."""
+    from fastvideo_rs_b200 import _lib, paged, sdpa
+    rows, mask = 128, (1, n - 600, 9)
+    pages = (n + rows - 1) // rows
+    g = torch.Generator(device="cuda").manual_seed(100)
+    if fmt == "q4":
+        pools = [torch.randint(0, 256, (pages, heads, rows, 64), generator=g, device="cuda", dtype=torch.uint8) for _ in range(2)]
+        scales = [torch.stack([0.2 + 0.2 * torch.rand(pages, heads, rows, generator=g, device="cuda"),
+                               0.3 * torch.randn(pages, heads, rows, generator=g, device="cuda")], -1).to(torch.bfloat16) for _ in range(2)]
+        kv = paged.PagedKv(*pools, *scales)
+    else:
+        pools = [torch.randn(pages, heads, rows, D, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+        kv = paged.PagedKv(*pools)
+    table = torch.randperm(pages, device="cuda", generator=g).to(torch.int32)[None].contiguous()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    batch = paged.PagedBatch(table, i32(n), i32(0, nq), max_q=nq, max_kv=n)
+    q = torch.randn(nq, heads, D, generator=g, device="cuda", dtype=torch.bfloat16)
+    out = paged.attend(kv, batch, q, mask_of(mask))
+    assert "fv_paged_chunk_kernel" in _lib.last_kernel() and sdpa.device_status() == 0
+    assert torch.equal(out, paged.attend(kv, batch, q, mask_of(mask)))
+    k, v = (t.double() for t in paged.read(kv, batch, rows=n, cu_rows=i32(0, n), first=i32(0)))
+    if fmt == "q4":
+        at = lambda t: t[table[0].long()].transpose(1, 2).flatten(0, 1)[:n]
+        k, v = (at(s)[..., 1:].double() + at(s)[..., :1].double() * (torch.stack([at(p) & 15, at(p) >> 4], -1).flatten(-2).double() - 8.0)
+                for p, s in zip(pools, scales))
+    pick = torch.tensor([0, 1, 127, 128, 255, 256, 511, 700, 1023, 1024, nq - 1], device="cuda")
+    p, j = pick[:, None] + n - nq, torch.arange(n, device="cuda")
+    seen = (j <= p) & ((p - j < mask[1]) | (j < mask[2]))
+    for h in range(heads):
+        s = (q[pick, h].double() @ k[:, h].T / math.sqrt(D)).masked_fill(~seen, -math.inf)
+        w = torch.softmax(s, -1)
+        want, mag = w @ v[:, h], w @ v[:, h].abs()
+        if fmt == "q4":
+            mag = mag + 1.5
+        err = (out[pick, h].double() - want).abs()
+        assert bool((err <= BF16_HALF * want.abs() + (BF16_HALF + 2.0 ** -10) * mag).all()), (h, float(err.max()))
