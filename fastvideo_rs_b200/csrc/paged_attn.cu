@@ -1003,7 +1003,7 @@ static bool take_items(long long planes, long long rows, long long keys, bool q4
     const double in_rows = 5.0 + waves * ((q4 ? 3.8 : 2.2) + (q4 ? 0.49 : 0.85) * (double)keys / (16.0 * kWarps * n)) + (n > kMaxCluster ? 4.0 : 0.0);
     const double items = (double)planes * (double)((rows + 255) / 256), line = items * (double)((keys + kChunkTile - 1) / kChunkTile + kItemCost);
     const double runs = line < (double)kLeastRun * sms ? line / kLeastRun : (double)sms, parts = runs / items;
-    const double in_items = (q4 ? 6.2 + 1.83 * line / runs : 4.3 + 1.66 * line / runs) + (parts > 1.0 ? 8.8 + 0.64 * (parts - 1.0) : 0.0);
+    const double in_items = (q4 ? 4.9 + 1.83 * line / runs : 4.3 + 1.66 * line / runs) + (parts > 1.0 ? 8.8 + 0.64 * (parts - 1.0) : 0.0);
     return in_items < in_rows;
 }
 static Shape shape_of(const fv_paged_kv* kv, const fv_paged_batch* b, int tokens, int heads, const Mask& m, int sms) {
