@@ -233,9 +233,9 @@ FV_DEV uint32_t lds32(uint32_t a) {
 // bf16, bound by HBM: a tile's K registers are loaded anew as soon as its scores are done and V's as soon as its product is, so
 // that memory is always being read while the warp computes, straight into registers: 32 ragged sequences of up to 9 001 keys, 32
 // heads on 8, 137 us = 6.10 TB/s, 0.93 of the measured copy bandwidth; 6 windows of 8 190 keys, 40 heads on 8, 34.5 us = 5.8 TB/s.
-// 4 bits, bound by the logic pipe: 32 keys are 4.3 KB, so a ring in shared memory runs three stages ahead: 32 sequences of up to
-// 20 011 keys 110 us = 4.5 TB/s (loads into registers: 173).  Three CTAs an SM: with a fourth the registers no longer suffice,
-// 128 against 123 us.  At most four rows stand on every other column of the products, which leaves half of the softmax: 123 -> 116 us.
+// 4 bits, bound by latency (issue slots 50 %, logic pipe 52 %, DRAM 53 %: nothing is full with 12 warps an SM): 32 keys are 4.3 KB, so a
+// ring in shared memory runs three stages ahead: 32 sequences of up to 20 011 keys 110 us = 4.5 TB/s (loads into registers: 173).  Three
+// CTAs an SM: with a fourth the registers no longer suffice, 128 against 123 us.  At most four rows stand on every other column of the products, which leaves half of the softmax: 123 -> 116 us.
 template <bool Q4, int ROWS>
 __global__ void __launch_bounds__(kAttnThreads, ROWS <= 8 ? 3 : 2) fv_paged_decode_kernel(const AttnArgs a) {
     constexpr int kRows = ROWS, NT = (ROWS + 7) / 8;  // groups of 8 rows, the columns of a product
@@ -990,7 +990,8 @@ static int key_ranges(long long ctas, int resident, long long keys, bool q4, int
 }
 // How a call is cut.  Few rows per kv head: blocks of up to 16 rows, and the keys in ranges.  Many: items of 2 x 128 rows, one CTA
 // per SM.  Which of the two: an estimate of both in us, fitted to 326 calls of 20 to 800 rows, 1 to 16 sequences of 200 to 20 011 keys, 1 and 8
-// kv heads, both page formats, over which the choice costs 0.6 % more than the better kernel would.  E.g. 8 kv heads, bf16: one sequence of
+// kv heads, both page formats, over which the choice costs 0.7 % more than the better kernel would, at worst half as much again (96 rows over
+// 20 011 4-bit keys of 8 kv heads).  E.g. 8 kv heads, bf16: one sequence of
 // 20 011 keys 20 rows 31 us in blocks of rows and 43 in items, 96 rows 116 and 43; sixteen of 200 keys 48 rows 17 and 19, 400 rows 51 and 27.
 // FV_PAGED_KERNEL=rows or items (kept for A/B) takes the choice away.
 static bool take_items(long long planes, long long rows, long long keys, bool q4, int sms) {

@@ -27,7 +27,8 @@
 // Bound by the tensor pipe and by what feeds it (128 x 128 x 16 products from shared memory take all of its bandwidth): 4 680 rows x
 // 12 heads over 28 080 bf16 keys 710 us under the profiler = 1 137 TFLOP/s, tensor pipe 62 % of the active cycles (690-830 us in a
 // loop, at the power cap); three ragged chunks of up to 1 501 tokens, 40 heads on 8, windows of 4 100 keys (35 tiles an item, five of
-// them cut by the mask) 326 us with bf16 pages, 56 %, and 392 us with 4-bit pages, 46 %.
+// them cut by the mask) 326 us with bf16 pages, 56 %, and 402 us with 4-bit pages, 45 % (in a graph, with the join, 306-345 and 365-390).
+// ptxas spills 56 bytes a thread over bf16 pages and 88 over 4-bit ones.
 #pragma once
 #include "attn_fwd.cuh"
 #include "paged.cuh"
@@ -840,8 +841,8 @@ FV_DEV void expand_unit(uint4 c, uint32_t sz, uint32_t up, uint32_t base, int q)
     }
 }
 // A pair's 32 units are dealt to the warps in turn.  Four warps, one per scheduler: their instructions come out of the softmax
-// warps' issue slots, and six (two schedulers with two of them) were slower, 430 against 412 us for three ragged chunks;
-// without the arithmetic of the expansion it would be 363.  (A first form with one key row a lane and page look-ups and loads of its
+// warps' issue slots, and six (two schedulers with two of them) were slower, 430 against 412 us for three ragged chunks
+// when that was the kernel's time; without the arithmetic of the expansion it would have been 363.  (A first form with one key row a lane and page look-ups and loads of its
 // own took 709: look-ups and loads are the loader's since.)
 FV_DEV void chunk_expander(const ChunkJob& jb, const Run& run, uint32_t sbase, int wid, int lane, const ChunkWait& wait) {
     using namespace fvattn;

@@ -16,8 +16,9 @@
 // HBM-bound: 8 lanes hold one row of one head (16 values a lane), a warp the same head of 4 neighbouring tokens, a CTA
 // of 16: their rows lie side by side in a page, each lane keeps its token's cosines and sines in registers over all heads,
 // and q's, K's and V's heads are loops of their own without a branch inside, four rows in flight per lane.  4 680 tokens x 3 x 40
-// heads to bf16 pages: 50-52 us = 5.6-5.8 TB/s, 0.86 of the measured copy bandwidth (a token a CTA: 87).  To 4 bits the quantisation
-// bounds it: 5 016 tokens x (40 + 2 x 8) heads 31 us, of which the bytes are 16.
+// heads to bf16 pages: 50-52 us = 5.6-5.8 TB/s, 0.86 of the measured copy bandwidth (a token a CTA: 87).  To 4 bits: 5 016
+// tokens x (40 + 2 x 8) heads 31 us, of which the bytes are 16: some 250 instructions a lane and row in 1.41 waves of CTAs (six run at a time
+// on an SM), which leaves the issue slots 44 % busy.
 #include "fv_runtime.h"
 #include "paged.cuh"
 #include "paged_host.h"

@@ -108,7 +108,9 @@ class PagedBatch:
     that the call does not need may be -1).  kv_len [seqs] int32: tokens of each sequence, those of this call included.
     cu_q [seqs + 1] int32, ascending from 0: rows cu_q[s] .. cu_q[s + 1] of the packed operands are the last tokens of
     sequence s.  max_q and max_kv bound the tokens and lengths; the tensors may change under a captured graph as long as they
-    keep to them.  Rows of an operand from cu_q[seqs] on belong to no sequence: outputs leave them as they were."""
+    keep to them (but bounds far above what a call holds cost time, since they are what its kernel is chosen and laid out by: one token of each
+    of 16 sequences of 4 000 keys, 32 heads on 8, bf16, 39 us with max_q 1, 65 with 256, 143 with 4 096).  Rows of an operand from cu_q[seqs] on
+    belong to no sequence: outputs leave them as they were (an output that the call allocates holds anything there)."""
 
     def __init__(self, page_table: torch.Tensor, kv_len: torch.Tensor, cu_q: torch.Tensor, *, max_q: int, max_kv: int):
         if page_table.dim() != 2:
