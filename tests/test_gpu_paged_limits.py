@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from _paged import D, BF16_HALF, Case, attend64, pack, rotate64, seen_matrix, unpack
+from _paged import D, BF16_HALF, Case, attend64, pack, rotate64, unpack
 
 pytestmark = pytest.mark.gpu
 
